@@ -44,8 +44,14 @@ class Weight(C.Structure):
                 ("ry", C.c_void_p), ("K", C.c_int32), ("N", C.c_int32), ("dtype", C.c_int32)]
 
 
+class Ssm(C.Structure):
+    """struct frhip_ssm"""
+    _fields_ = [("A", C.c_void_p), ("D", C.c_void_p), ("dt_bias", C.c_void_p), ("channels", C.c_int32), ("states", C.c_int32),
+                ("groups", C.c_int32), ("dt_softplus", C.c_int32)]
+
+
 _vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
-_WP = C.POINTER(Weight)
+_WP, _SP = C.POINTER(Weight), C.POINTER(Ssm)
 
 _SIGS = {
     "frhip_abi_version": (_i, []),
@@ -110,6 +116,12 @@ _SIGS = {
     "frhip_gemm_few_tile": (_i, [_i, _i, _i, _vp, _i, _vp]),
     "frhip_seq_gemm_form": (_i, [_i, _i, _i, _vp, _i, _i, _vp]),
     "frhip_seq_codes_way": (_i, [_i, _i, _i, _vp, _i, _i, _vp]),
+    "frhip_conv_one": (_i, [_i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp]),
+    "frhip_conv_seq": (_i, [_i, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp]),
+    "frhip_ssm_one": (_i, [_SP, _i] + [_vp, _i] * 5 + [_vp, _vp, _vp, _i, _i, _vp]),
+    "frhip_ssm_workspace_bytes": (_sz, [_SP, _i, _i]),
+    "frhip_ssm_seq": (_i, [_SP, _i, _vp] + [_vp, _i] * 5 + [_vp, _vp, _vp, _i, _i, _vp, _vp]),
+    "frhip_ssm_cut": (_i, [_SP, _i, _vp, _i, _vp]),
     "frhip_copy_probe": (_i, [_vp, _vp, _sz, _vp]),
     "frhip_read_probe": (_i, [_vp, _sz, _vp, _vp]),
     "frhip_mfma_probe": (_i, [_i, _i, _vp, _vp, _vp, _vp]),

@@ -1,0 +1,782 @@
+// Operators of a selective state space layer: the short causal convolution and the scan whose decay depends on the input.
+//
+// The scan of a channel d with states n is linear in h,
+//   h_t = a_t h_{t-1} + b_t,   a_t = exp(dt_t A[n]),   b_t = dt_t x_t B_t[n],
+// and its decay over a stretch of time is exp(A[n] * (sum of dt_t)): a stretch is summed up by that sum, one number a channel, and
+// by the state that it ends in from an empty one.  So a prompt is cut into chunks of time:
+//   1. every chunk but a prompt's last is scanned from an empty state -> its end state and its sum of dt;
+//   2. every chunk folds the chunks before it into its true start state and is scanned again, with outputs.
+// One token is the formula itself.
+#include <climits>
+#include <cstring>
+#include <initializer_list>
+
+#include "device_utils.h"
+#include "frhip_internal.h"
+
+#pragma clang fp contract(off)
+
+namespace frhip {
+
+constexpr int kSeqTable = 128;  // prompts of a launch; more go out in several
+struct SeqTable {
+  int start[kSeqTable + 1];  // first row
+  int chunk[kSeqTable + 1];  // first chunk (every prompt has one at least)
+};
+
+// The prompt that chunk `j` belongs to: the last i with first(i) <= j.  `first` does not descend.
+template <class F>
+__device__ __forceinline__ int find_seq(int nseq, int j, F first) {
+  int lo = 0, hi = nseq - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (first(mid) <= j) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|); log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, with atanh(s) / s as a polynomial
+// in s^2 (Chebyshev fit over [0, 1/9], 8e-9 relative), so that small values keep their relative accuracy.  FINE: the rounding of
+// -|v| log2(e), which exp2 would scale by |v|, is made good.
+template <bool FINE>
+__device__ __forceinline__ float softplus_f(float v) {
+  const float m = __builtin_fabsf(v), t = m * -kLog2e;
+  float e = __builtin_amdgcn_exp2f(t);
+  if constexpr (FINE) {
+    // m log2(e) = -t + r, log2(e) = kLog2e + 1.925963033500752e-8
+    const float r = __builtin_fmaf(m, 1.925963033500752e-8f, __builtin_fmaf(m, kLog2e, t));
+    e = __builtin_fmaf(e, -r * 0.693147180559945f, e);
+    e = m < 80.f ? e : expf(-m);  // beyond, r is no small number of an infinite m, and e is below what exp2 keeps
+  }
+  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+  float p = __builtin_fmaf(q, 0.1408732831478119f, 0.1398070901632309f);
+  p = __builtin_fmaf(p, q, 0.20012426376342773f);
+  p = __builtin_fmaf(p, q, 0.3333315849304199f);
+  p = __builtin_fmaf(p, q, 1.0f);
+  return __builtin_fmaxf(v, 0.f) + 2.0f * s * p;  // a NaN stays one through s
+}
+
+template <class T>
+__device__ __forceinline__ float silu_f(float v) {
+  if constexpr (sizeof(T) == 4) return v / (1.0f + expf(-v));
+  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -kLog2e));
+}
+
+// ---------------------------------------------------------------------------
+// Short causal convolution.  Bound by memory: every element once in and once out.  A thread has 16 bytes of channels and walks a tile
+// of rows with the last W rows in registers.
+// ---------------------------------------------------------------------------
+template <class T>
+struct ConvArgs {
+  const T *x, *state;
+  T *state_out, *y;
+  const float *w, *bias;
+  int ldx, ldy, C, silu;
+  int nseq, tile;  // conv_seq: rows of a tile
+  int rows, ncv;   // conv_one
+};
+
+template <class T>
+constexpr int kConvLanes = 16 / sizeof(T);  // channels of a thread
+
+// Up to V elements at any address of one, the first n of them; the same instruction as for aligned 16 bytes if there are V
+template <class T, int V>
+__device__ __forceinline__ void load_group(float (&v)[V], const T* p, int n) {
+  typedef T any __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  if (n >= V) {
+    const any t = *reinterpret_cast<const any*>(p);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = (float)t[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = i < n ? (float)p[i] : 0.f;
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_group(T* p, const float (&v)[V], int n) {
+  typedef T any __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  if (n >= V) {
+    any t;
+#pragma unroll
+    for (int i = 0; i < V; i++) t[i] = (T)v[i];
+    *reinterpret_cast<any*>(p) = t;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++)
+      if (i < n) p[i] = (T)v[i];
+  }
+}
+
+template <class T, int W>
+struct ConvTaps {
+  static constexpr int V = kConvLanes<T>;
+  float w[W][V], b[V];
+  __device__ __forceinline__ void load(const ConvArgs<T>& a, int c, int n) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const int ci = c + (i < n ? i : 0);
+      b[i] = a.bias ? a.bias[ci] : 0.f;
+#pragma unroll
+      for (int j = 0; j < W; j++) w[j][i] = a.w[(size_t)ci * W + j];
+    }
+  }
+  // past: the last W rows, oldest first
+  __device__ __forceinline__ void apply(const float (&past)[W][V], float (&y)[V], int silu) const {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      float s = b[i];
+#pragma unroll
+      for (int j = 0; j < W; j++) s = __builtin_fmaf(w[j][i], past[j][i], s);
+      y[i] = silu ? silu_f<T>(s) : s;
+    }
+  }
+};
+
+template <class T, int W>
+__global__ __launch_bounds__(256) void conv_one_kernel(ConvArgs<T> a) {
+  constexpr int V = kConvLanes<T>;
+  const size_t item = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int row = (int)(item / a.ncv), c = (int)(item % a.ncv) * V, n = a.C - c;
+  if (row >= a.rows) return;
+  float past[W][V], y[V];
+  const size_t st = (size_t)row * (W - 1) * a.C + c;
+#pragma unroll
+  for (int j = 0; j < W - 1; j++) load_group<T, V>(past[j], a.state + st + (size_t)j * a.C, n);
+  load_group<T, V>(past[W - 1], a.x + (size_t)row * a.ldx + c, n);
+  ConvTaps<T, W> taps;
+  taps.load(a, c, n);
+  taps.apply(past, y, a.silu);
+  store_group<T, V>(a.y + (size_t)row * a.ldy + c, y, n);
+#pragma unroll
+  for (int j = 0; j < W - 1; j++) store_group<T, V>(a.state_out + st + (size_t)j * a.C, past[j + 1], n);
+}
+
+// blockIdx.x: a tile of rows of one prompt, blockIdx.y: a block of channels.  The threads of a prompt's first tile read its state and
+// write the new one, so that the two may be the same memory.
+template <class T, int W>
+__global__ __launch_bounds__(256) void conv_seq_kernel(ConvArgs<T> a, SeqTable tab) {
+  constexpr int V = kConvLanes<T>;
+  const int j0 = blockIdx.x, i = find_seq(a.nseq, j0, [&](int k) { return tab.chunk[k]; });
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V, n = a.C - c;
+  if (n <= 0) return;
+  const int first = tab.start[i], end = tab.start[i + 1], t0 = first + (j0 - tab.chunk[i]) * a.tile;
+  const int t1 = end - t0 < a.tile ? end : t0 + a.tile;
+  ConvTaps<T, W> taps;
+  taps.load(a, c, n);
+  float past[W][V];
+  const T* x = a.x + c;
+  if (t0 == first) {
+    const size_t st = (size_t)i * (W - 1) * a.C + c;
+    float old[W - 1][V];
+#pragma unroll
+    for (int j = 0; j < W - 1; j++) {
+      load_group<T, V>(old[j], a.state + st + (size_t)j * a.C, n);
+#pragma unroll
+      for (int v = 0; v < V; v++) past[j + 1][v] = old[j][v];
+    }
+    const int len = end - first;
+#pragma unroll
+    for (int j = 0; j < W - 1; j++) {  // the input W - 1 - j tokens ahead of the end, or what the old state holds of it
+      float v[V];
+      const int t = end - (W - 1) + j;
+      if (t >= first) {
+        load_group<T, V>(v, x + (size_t)t * a.ldx, n);
+      } else {
+#pragma unroll
+        for (int k = 0; k < W - 1; k++)
+          if (k == j + len) {
+#pragma unroll
+            for (int q = 0; q < V; q++) v[q] = old[k][q];
+          }
+      }
+      store_group<T, V>(a.state_out + st + (size_t)j * a.C, v, n);
+    }
+  } else {  // a tile has W - 1 rows at least
+#pragma unroll
+    for (int j = 1; j < W; j++) load_group<T, V>(past[j], x + (size_t)(t0 - W + j) * a.ldx, n);
+  }
+  for (int t = t0; t < t1; t++) {
+    float y[V];
+#pragma unroll
+    for (int j = 0; j < W - 1; j++)
+#pragma unroll
+      for (int v = 0; v < V; v++) past[j][v] = past[j + 1][v];
+    load_group<T, V>(past[W - 1], x + (size_t)t * a.ldx, n);
+    taps.apply(past, y, a.silu);
+    store_group<T, V>(a.y + (size_t)t * a.ldy + c, y, n);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Selective scan
+// ---------------------------------------------------------------------------
+template <class T>
+struct SsmArgs {
+  const T *x, *dt, *B, *C, *z;
+  T* y;
+  const float *A, *D, *dt_bias, *state;
+  float* state_out;
+  float *ends, *sums;  // of the chunks that are not a prompt's last: [local chunks, then prompts][N][D], [local chunks][D]
+  int ldx, lddt, ldb, ldc, ldz, ldy;
+  int D_, N, cpg, softplus;  // channels, states, channels of a group
+  int nblk;                  // workgroups of a group's channels
+  int chunk, nlocal;         // rows of a chunk; chunks that are not a prompt's last
+  int nseq, rows;            // prompts of the launch; scan of one token: rows
+};
+
+constexpr int kScanRows = 8;  // rows that go through LDS and registers together
+
+// Waves of a workgroup: NW of them share a channel's states, NPL each, and there are four or NW in all.
+constexpr int scan_waves(int nw) { return nw < 4 ? 4 : nw; }
+
+// LOCAL: step 1 of the scan, otherwise step 2.  A lane has one channel and NPL of its states in registers; B and C of kScanRows rows go
+// through LDS as fp32, where every lane reads the same address.
+template <class T, int NPL, int NW, bool LOCAL>
+__global__ __launch_bounds__(scan_waves(NW) * 64) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
+  constexpr int WAVES = scan_waves(NW), CW = WAVES / NW, NT = NPL * NW, TB = kScanRows, STAGE = (TB * 2 * NT + WAVES * 64 - 1) / (WAVES * 64);
+  __shared__ __attribute__((aligned(16))) float bc[2][TB][2][NT];
+  __shared__ float part[NW > 1 ? WAVES : 1][NW > 1 ? TB : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cw = wave / NW, nw = wave % NW;
+  const int j0 = blockIdx.y;
+  const int i = LOCAL ? find_seq(a.nseq, j0, [&](int k) { return tab.chunk[k] - k; })
+                      : find_seq(a.nseq, j0, [&](int k) { return tab.chunk[k]; });
+  const int nchunk = tab.chunk[i + 1] - tab.chunk[i], ci = j0 - tab.chunk[i] + (LOCAL ? i : 0), local0 = tab.chunk[i] - i;
+  const int end = tab.start[i + 1], t0 = tab.start[i] + ci * a.chunk, t1 = end - t0 < a.chunk ? end : t0 + a.chunk;
+  const int g = blockIdx.x / a.nblk, cg = (blockIdx.x - g * a.nblk) * (CW * 64) + cw * 64 + lane;
+  const bool mine = cg < a.cpg;
+  const int d = g * a.cpg + (mine ? cg : a.cpg - 1), n0 = nw * NPL;
+
+  float A2[NPL], h[NPL];
+#pragma unroll
+  for (int k = 0; k < NPL; k++) {
+    const bool ok = n0 + k < a.N;
+    A2[k] = ok ? a.A[(size_t)d * a.N + n0 + k] * kLog2e : 0.f;
+    h[k] = 0.f;
+  }
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
+  const size_t ND = (size_t)a.N * a.D_;
+  if constexpr (LOCAL) {
+    if (ci == 0 && mine) {  // step 2 reads it here: its last chunk may overwrite the state
+#pragma unroll
+      for (int k = 0; k < NPL; k++)
+        if (n0 + k < a.N) a.ends[(size_t)(a.nlocal + local0) * ND + (size_t)(n0 + k) * a.D_ + d] = a.state[((size_t)i * a.D_ + d) * a.N + n0 + k];
+    }
+  } else if (nchunk == 1) {
+#pragma unroll
+    for (int k = 0; k < NPL; k++)
+      if (n0 + k < a.N) h[k] = a.state[((size_t)i * a.D_ + d) * a.N + n0 + k];
+  } else {
+#pragma unroll
+    for (int k = 0; k < NPL; k++)
+      if (n0 + k < a.N) h[k] = a.ends[(size_t)(a.nlocal + local0) * ND + (size_t)(n0 + k) * a.D_ + d];
+    for (int p = 0; p < ci; p++) {
+      const float s = a.sums[(size_t)(local0 + p) * a.D_ + d];
+      const float* e = a.ends + (size_t)(local0 + p) * ND + d;
+#pragma unroll
+      for (int k = 0; k < NPL; k++)
+        if (n0 + k < a.N) h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A2[k]), h[k], e[(size_t)(n0 + k) * a.D_]);
+    }
+  }
+
+  const T* const Bg = a.B + (size_t)g * a.N;
+  const T* const Cg = a.C + (size_t)g * a.N;
+  const float skip = !LOCAL && a.D ? a.D[d] : 0.f;
+  float sum = 0.f, xr[TB], dr[TB], zr[TB], st[STAGE];
+  auto request = [&](int t) {  // rows past the chunk repeat its last one
+#pragma unroll
+    for (int r = 0; r < TB; r++) {
+      const int row = t + r < t1 ? t + r : t1 - 1;
+      xr[r] = (float)a.x[(size_t)row * a.ldx + d];
+      dr[r] = (float)a.dt[(size_t)row * a.lddt + d];
+      if constexpr (!LOCAL) zr[r] = a.z ? (float)a.z[(size_t)row * a.ldz + d] : 0.f;
+    }
+#pragma unroll
+    for (int q = 0; q < STAGE; q++) {
+      const int e = threadIdx.x + q * (WAVES * 64), r = e / (2 * NT), c = (e / NT) & 1, n = e % NT;
+      st[q] = e < TB * 2 * NT && t + r < t1 && n < a.N ? (float)(c ? Cg + (size_t)(t + r) * a.ldc : Bg + (size_t)(t + r) * a.ldb)[n] : 0.f;
+    }
+  };
+  if (t0 < t1) request(t0);
+  int buf = 0;
+  for (int t = t0; t < t1; t += TB, buf ^= 1) {
+    float x[TB], dt[TB], z[TB];
+#pragma unroll
+    for (int q = 0; q < STAGE; q++) {
+      const int e = threadIdx.x + q * (WAVES * 64);
+      if (e < TB * 2 * NT) (&bc[buf][0][0][0])[e] = st[q];
+    }
+#pragma unroll
+    for (int r = 0; r < TB; r++) {
+      const float v = dr[r] + bias;
+      const bool live = t + r < t1;
+      dt[r] = live ? (a.softplus ? softplus_f<sizeof(T) == 4>(v) : v) : 0.f;
+      x[r] = live ? xr[r] : 0.f;
+      z[r] = zr[r];
+    }
+    __syncthreads();
+    if (t + TB < t1) request(t + TB);
+#pragma unroll
+    for (int r = 0; r < TB; r++) {
+      const float u = dt[r] * x[r];
+      float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+      for (int k = 0; k < NPL; k++) {
+        const float decay = __builtin_amdgcn_exp2f(dt[r] * A2[k]);
+        h[k] = __builtin_fmaf(decay, h[k], u * bc[buf][r][0][n0 + k]);
+        if constexpr (!LOCAL) {
+          float& y = k & 1 ? y1 : y0;
+          y = __builtin_fmaf(bc[buf][r][1][n0 + k], h[k], y);
+        }
+      }
+      if constexpr (LOCAL) {
+        sum += dt[r];
+      } else if constexpr (NW == 1) {
+        const float y = __builtin_fmaf(skip, x[r], y0 + y1);
+        if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<T>(z[r]) : y);
+      } else {
+        part[wave][r][lane] = y0 + y1;
+      }
+    }
+    if constexpr (!LOCAL && NW > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int r = 0; r < TB; r++)
+        if (r % NW == nw) {
+          float y = part[cw * NW][r][lane];
+#pragma unroll
+          for (int w = 1; w < NW; w++) y += part[cw * NW + w][r][lane];
+          y = __builtin_fmaf(skip, x[r], y);
+          if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<T>(z[r]) : y);
+        }
+    }
+  }
+  if (!mine) return;
+  if constexpr (LOCAL) {
+    if (nw == 0) a.sums[(size_t)j0 * a.D_ + d] = sum;
+#pragma unroll
+    for (int k = 0; k < NPL; k++)
+      if (n0 + k < a.N) a.ends[(size_t)j0 * ND + (size_t)(n0 + k) * a.D_ + d] = h[k];
+  } else if (ci == nchunk - 1) {
+#pragma unroll
+    for (int k = 0; k < NPL; k++)
+      if (n0 + k < a.N) a.state_out[((size_t)i * a.D_ + d) * a.N + n0 + k] = h[k];
+  }
+}
+
+// One token each of `rows` sequences.  Bound by memory: the states once in and once out.  LANES lanes share a channel, four states (one
+// after another) each.
+template <class T, int LANES>
+__global__ __launch_bounds__(256) void ssm_one_kernel(SsmArgs<T> a) {
+  const size_t item = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const size_t chan = item / LANES;
+  const int q = (int)(item % LANES), row = (int)(chan / a.D_), d = (int)(chan % a.D_);
+  if (row >= a.rows) return;  // lanes of a channel leave together
+  const int g = d / a.cpg;
+  const float v = (float)a.dt[(size_t)row * a.lddt + d] + (a.dt_bias ? a.dt_bias[d] : 0.f);
+  const float dt = a.softplus ? softplus_f<sizeof(T) == 4>(v) : v;
+  const float x = (float)a.x[(size_t)row * a.ldx + d], u = dt * x;
+  const size_t st = ((size_t)row * a.D_ + d) * a.N;
+  float y = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int n = q * 4 + k;
+    if (n < a.N) {
+      const float decay = __builtin_amdgcn_exp2f(dt * (a.A[(size_t)d * a.N + n] * kLog2e));
+      const float h = __builtin_fmaf(decay, a.state[st + n], u * (float)a.B[(size_t)row * a.ldb + g * a.N + n]);
+      a.state_out[st + n] = h;
+      y = __builtin_fmaf((float)a.C[(size_t)row * a.ldc + g * a.N + n], h, y);
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < LANES; m *= 2) y += __shfl_xor(y, m);
+  if (q == 0) {
+    y = __builtin_fmaf(a.D ? a.D[d] : 0.f, x, y);
+    a.y[(size_t)row * a.ldy + d] = (T)(a.z ? y * silu_f<T>((float)a.z[(size_t)row * a.ldz + d]) : y);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+struct ScanShape {
+  int npl, nw, nblk, wgs;  // states of a wave, waves that share a channel's states, workgroups of a group, workgroups of a chunk
+};
+static ScanShape scan_shape(const frhip_ssm& p) {
+  ScanShape s;
+  s.npl = p.states <= 4 ? 4 : p.states <= 8 ? 8 : 16;
+  s.nw = 1;
+  while (s.nw * s.npl < p.states) s.nw *= 2;
+  const int per = 64 * (scan_waves(s.nw) / s.nw), cpg = p.channels / p.groups;
+  s.nblk = (cpg + per - 1) / per;
+  s.wgs = p.groups * s.nblk;
+  return s;
+}
+
+constexpr int kScanLeast = 16;         // rows of a chunk, at least
+constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
+
+// Rows of a chunk: enough chunks to give every compute unit a workgroup
+static int scan_chunk(const ScanShape& s, int T, int cus) {
+  const int units = cus < kScanMostUnits ? cus : kScanMostUnits;
+  const int q = units / s.wgs > 1 ? units / s.wgs : 1;
+  int len = T / q + (T % q ? 1 : 0);
+  if (len < kScanLeast) len = kScanLeast;
+  return len > INT_MAX - kScanRows ? INT_MAX : (len + kScanRows - 1) / kScanRows * kScanRows;
+}
+
+static size_t scan_most_local(const ScanShape& s, int T) {  // sum of (chunks - 1) <= T / chunk <= both
+  const size_t by_rows = (size_t)T / kScanLeast, by_units = (size_t)(kScanMostUnits / s.wgs > 1 ? kScanMostUnits / s.wgs : 1);
+  return by_rows < by_units ? by_rows : by_units;
+}
+
+static int check_seqs(int nseq, const int32_t* seq_start, const char* what) {
+  if (nseq < 0) return set_error(FRHIP_ESHAPE, what);
+  if (nseq > 0) {
+    if (!seq_start) return set_error(FRHIP_EINVAL, what);
+    if (seq_start[0] < 0) return set_error(FRHIP_ESHAPE, what);
+    for (int i = 0; i < nseq; i++)
+      if (seq_start[i + 1] < seq_start[i]) return set_error(FRHIP_ESHAPE, what);
+  }
+  return 0;
+}
+
+// Whether [rows][cols] of ld elements a row at a and b (ldb) share memory.  Rows of the same pitch may lie side by side.
+static bool rows_overlap(const void* a, size_t lda, const void* b, size_t ldb, size_t rows, size_t cols_a, size_t cols_b, size_t elem) {
+  if (!a || !b || !rows) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  const uintptr_t ea = pa + ((rows - 1) * lda + cols_a) * elem, eb = pb + ((rows - 1) * ldb + cols_b) * elem;
+  if (ea <= pb || eb <= pa) return false;
+  if (lda != ldb) return true;
+  const size_t pitch = lda * elem, off = (pa < pb ? pb - pa : pa - pb) % pitch;
+  // seen from the lower one, the other begins `off` bytes into a row
+  const size_t low = (pa < pb ? cols_a : cols_b) * elem, high = (pa < pb ? cols_b : cols_a) * elem;
+  return off < low || off + high > pitch;
+}
+
+static bool spans_clash(const void* a, const void* b, size_t bytes) {  // neither the same nor apart
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  return pa != pb && pa < pb + bytes && pb < pa + bytes;
+}
+
+static bool off_grid(size_t elem, std::initializer_list<const void*> ptrs) {
+  uintptr_t v = 0;
+  for (const void* p : ptrs) v |= reinterpret_cast<uintptr_t>(p);
+  return v % elem != 0;
+}
+
+template <class T, int W>
+static void conv_one_launch(const ConvArgs<T>& a, hipStream_t st) {
+  const size_t items = (size_t)a.rows * a.ncv;
+  hipLaunchKernelGGL((conv_one_kernel<T, W>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
+}
+
+template <class T>
+static int conv_one_run(ConvArgs<T> a, int W, hipStream_t st) {
+  a.ncv = (a.C + kConvLanes<T> - 1) / kConvLanes<T>;
+  if (((size_t)a.rows * a.ncv + 255) / 256 > INT_MAX) return set_error(FRHIP_ESHAPE, "conv_one: too many rows");
+  if (W == 2) conv_one_launch<T, 2>(a, st);
+  else if (W == 3) conv_one_launch<T, 3>(a, st);
+  else conv_one_launch<T, 4>(a, st);
+  return check_launch("conv_one");
+}
+
+template <class T>
+static int conv_seq_run(ConvArgs<T> a, int W, int nseq, const int32_t* start, hipStream_t st) {
+  constexpr int V = kConvLanes<T>;
+  const int ncv = (a.C + V - 1) / V, blocks = (ncv + 255) / 256, threads = ((ncv + blocks - 1) / blocks + 63) / 64 * 64;
+  a.tile = 16;
+  if (blocks > 65535) return set_error(FRHIP_ESHAPE, "conv_seq: too many channels");
+  const T *state = a.state;
+  T* state_out = a.state_out;
+  for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {
+    SeqTable tab;
+    a.nseq = nseq - s0 < kSeqTable ? nseq - s0 : kSeqTable;
+    int tiles = 0;
+    for (int i = 0; i < a.nseq; i++) {
+      const int len = start[s0 + i + 1] - start[s0 + i];
+      tab.start[i] = start[s0 + i];
+      tab.chunk[i] = tiles;
+      tiles += len ? (len - 1) / a.tile + 1 : 1;
+    }
+    tab.start[a.nseq] = start[s0 + a.nseq];
+    tab.chunk[a.nseq] = tiles;
+    a.state = state + (size_t)s0 * (W - 1) * a.C;
+    a.state_out = state_out + (size_t)s0 * (W - 1) * a.C;
+    const dim3 grid(tiles, blocks);
+    if (W == 2) hipLaunchKernelGGL((conv_seq_kernel<T, 2>), grid, dim3(threads), 0, st, a, tab);
+    else if (W == 3) hipLaunchKernelGGL((conv_seq_kernel<T, 3>), grid, dim3(threads), 0, st, a, tab);
+    else hipLaunchKernelGGL((conv_seq_kernel<T, 4>), grid, dim3(threads), 0, st, a, tab);
+    if (int rc = check_launch("conv_seq")) return rc;
+  }
+  return 0;
+}
+
+// What frhip_conv_one and frhip_conv_seq check alike; row0, rows: the rows of x and y, nstate: sequences
+static int conv_check(int C, int W, const void* x, int ldx, const float* w, const float* bias, int act, const void* state, void* state_out,
+                      void* y, int ldy, int dtype, size_t row0, size_t rows, size_t nstate) {
+  if (dtype != FRHIP_F16 && dtype != FRHIP_F32) return set_error(FRHIP_EINVAL, "conv: dtype must be F16 or F32");
+  if (act != FRHIP_ACT_NONE && act != FRHIP_ACT_SILU) return set_error(FRHIP_EINVAL, "conv: act must be NONE or SILU");
+  if (C <= 0 || W < 2 || W > 4) return set_error(FRHIP_ESHAPE, "conv: W must be 2, 3 or 4 and C positive");
+  if (ldx < C || ldy < C) return set_error(FRHIP_ESHAPE, "conv: rows closer than C elements");
+  if (!w || !state || !state_out || (rows && (!x || !y))) return set_error(FRHIP_EINVAL, "conv: null pointer");
+  const size_t elem = dtype == FRHIP_F16 ? 2 : 4, sbytes = nstate * (W - 1) * C * elem;
+  if (off_grid(elem, {x, y, state, state_out}) || off_grid(4, {w, bias})) return set_error(FRHIP_EINVAL, "conv: pointer not aligned to its element");
+  const char* xr = static_cast<const char*>(x) + row0 * ldx * elem;
+  char* yr = static_cast<char*>(y) + row0 * ldy * elem;
+  const size_t se = sbytes / elem;
+  if (rows && (rows_overlap(xr, ldx, yr, ldy, rows, C, C, elem) || rows_overlap(yr, (rows - 1) * ldy + C, state, se, 1, (rows - 1) * ldy + C, se, elem) ||
+               rows_overlap(yr, (rows - 1) * ldy + C, state_out, se, 1, (rows - 1) * ldy + C, se, elem) ||
+               rows_overlap(xr, (rows - 1) * ldx + C, state_out, se, 1, (rows - 1) * ldx + C, se, elem)))
+    return set_error(FRHIP_EINVAL, "conv: an output overlaps what is read");
+  if (spans_clash(state, state_out, sbytes)) return set_error(FRHIP_EINVAL, "conv: states overlap in part");
+  return 0;
+}
+
+template <class T>
+static ConvArgs<T> conv_args(int C, const void* x, int ldx, const float* w, const float* bias, int act, const void* state, void* state_out,
+                             void* y, int ldy) {
+  ConvArgs<T> a;
+  memset(&a, 0, sizeof(a));
+  a.x = static_cast<const T*>(x);
+  a.state = static_cast<const T*>(state);
+  a.state_out = static_cast<T*>(state_out);
+  a.y = static_cast<T*>(y);
+  a.w = w;
+  a.bias = bias;
+  a.ldx = ldx;
+  a.ldy = ldy;
+  a.C = C;
+  a.silu = act == FRHIP_ACT_SILU;
+  return a;
+}
+
+static int ssm_check_params(const frhip_ssm* p) {
+  if (!p || !p->A) return set_error(FRHIP_EINVAL, "ssm: null pointer");
+  if (p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0) return set_error(FRHIP_ESHAPE, "ssm: channels must be a multiple of groups");
+  if (p->states < 1 || p->states > 256) return set_error(FRHIP_ESHAPE, "ssm: states must be 1 to 256");
+  if ((long long)p->groups * p->states > INT_MAX) return set_error(FRHIP_ESHAPE, "ssm: too many groups");
+  if (off_grid(4, {p->A, p->D, p->dt_bias})) return set_error(FRHIP_EINVAL, "ssm: pointer not aligned to its element");
+  return 0;
+}
+
+struct SsmCall {
+  const void *x, *dt, *B, *C, *z;
+  int ldx, lddt, ldb, ldc, ldz;
+  const float* state;
+  float* state_out;
+  void* y;
+  int ldy, dtype;
+};
+
+static int ssm_check(const frhip_ssm& p, const SsmCall& c, size_t row0, size_t rows, size_t nstate) {
+  if (c.dtype != FRHIP_F16 && c.dtype != FRHIP_F32) return set_error(FRHIP_EINVAL, "ssm: dtype must be F16 or F32");
+  const int bn = p.groups * p.states;
+  if (c.ldx < p.channels || c.lddt < p.channels || c.ldy < p.channels || (c.z && c.ldz < p.channels) || c.ldb < bn || c.ldc < bn)
+    return set_error(FRHIP_ESHAPE, "ssm: rows closer than their elements");
+  if (!c.state || !c.state_out || (rows && (!c.x || !c.dt || !c.B || !c.C || !c.y))) return set_error(FRHIP_EINVAL, "ssm: null pointer");
+  const size_t elem = c.dtype == FRHIP_F16 ? 2 : 4, sn = nstate * p.channels * p.states;
+  if (off_grid(elem, {c.x, c.dt, c.B, c.C, c.z, c.y}) || off_grid(4, {c.state, c.state_out}))
+    return set_error(FRHIP_EINVAL, "ssm: pointer not aligned to its element");
+  if (spans_clash(c.state, c.state_out, sn * 4)) return set_error(FRHIP_EINVAL, "ssm: states overlap in part");
+  if (!rows) return 0;
+  struct In { const void* p; int ld, cols; };
+  const char* y = static_cast<const char*>(c.y) + row0 * c.ldy * elem;
+  const size_t ye = (rows - 1) * c.ldy + p.channels;
+  for (const In& in : {In{c.x, c.ldx, p.channels}, In{c.dt, c.lddt, p.channels}, In{c.B, c.ldb, bn}, In{c.C, c.ldc, bn}, In{c.z, c.ldz, p.channels}}) {
+    if (!in.p) continue;
+    const char* q = static_cast<const char*>(in.p) + row0 * in.ld * elem;
+    const size_t qe = ((rows - 1) * in.ld + in.cols) * elem;
+    if (rows_overlap(q, in.ld, y, c.ldy, rows, in.cols, p.channels, elem) || rows_overlap(q, qe, c.state_out, sn * 4, 1, qe, sn * 4, 1))
+      return set_error(FRHIP_EINVAL, "ssm: an output overlaps what is read");
+  }
+  if (rows_overlap(y, ye * elem, c.state, sn * 4, 1, ye * elem, sn * 4, 1) || rows_overlap(y, ye * elem, c.state_out, sn * 4, 1, ye * elem, sn * 4, 1))
+    return set_error(FRHIP_EINVAL, "ssm: an output overlaps what is read");
+  return 0;
+}
+
+template <class T>
+static SsmArgs<T> ssm_args(const frhip_ssm& p, const SsmCall& c) {
+  SsmArgs<T> a;
+  memset(&a, 0, sizeof(a));
+  a.x = static_cast<const T*>(c.x);
+  a.dt = static_cast<const T*>(c.dt);
+  a.B = static_cast<const T*>(c.B);
+  a.C = static_cast<const T*>(c.C);
+  a.z = static_cast<const T*>(c.z);
+  a.y = static_cast<T*>(c.y);
+  a.A = p.A;
+  a.D = p.D;
+  a.dt_bias = p.dt_bias;
+  a.state = c.state;
+  a.state_out = c.state_out;
+  a.ldx = c.ldx;
+  a.lddt = c.lddt;
+  a.ldb = c.ldb;
+  a.ldc = c.ldc;
+  a.ldz = c.ldz;
+  a.ldy = c.ldy;
+  a.D_ = p.channels;
+  a.N = p.states;
+  a.cpg = p.channels / p.groups;
+  a.softplus = p.dt_softplus != 0;
+  return a;
+}
+
+template <class T, int NPL, int NW>
+static int scan_launch(const SsmArgs<T>& a, const SeqTable& tab, int wgs, int chunks, hipStream_t st) {
+  constexpr int threads = scan_waves(NW) * 64;
+  if (a.nlocal) {
+    hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, true>), dim3(wgs, a.nlocal), dim3(threads), 0, st, a, tab);
+    if (int rc = check_launch("ssm_seq")) return rc;
+  }
+  hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, false>), dim3(wgs, chunks), dim3(threads), 0, st, a, tab);
+  return check_launch("ssm_seq");
+}
+
+// Prompts s0 .. s0 + a.nseq - 1 in one table; returns the chunks
+static int scan_table(SeqTable& tab, const int32_t* start, int s0, int n, int chunk) {
+  int chunks = 0;
+  for (int i = 0; i < n; i++) {
+    const int len = start[s0 + i + 1] - start[s0 + i];
+    tab.start[i] = start[s0 + i];
+    tab.chunk[i] = chunks;
+    chunks += len ? (len - 1) / chunk + 1 : 1;
+  }
+  tab.start[n] = start[s0 + n];
+  tab.chunk[n] = chunks;
+  return chunks;
+}
+
+template <class T>
+static int ssm_seq_run(const frhip_ssm& p, const SsmCall& c, int nseq, const int32_t* start, void* workspace, hipStream_t st) {
+  const ScanShape s = scan_shape(p);
+  SsmArgs<T> a = ssm_args<T>(p, c);
+  a.nblk = s.nblk;
+  const size_t per = (size_t)p.channels * p.states;
+  for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {
+    SeqTable tab;
+    a.nseq = nseq - s0 < kSeqTable ? nseq - s0 : kSeqTable;
+    a.chunk = scan_chunk(s, start[s0 + a.nseq] - start[s0], compute_units());
+    const int chunks = scan_table(tab, start, s0, a.nseq, a.chunk);
+    a.nlocal = chunks - a.nseq;
+    a.state = c.state + (size_t)s0 * per;
+    a.state_out = c.state_out + (size_t)s0 * per;
+    a.ends = static_cast<float*>(workspace);
+    a.sums = a.ends + 2 * (size_t)a.nlocal * per;
+    int rc = FRHIP_ESHAPE;
+    if (s.npl == 4) rc = scan_launch<T, 4, 1>(a, tab, s.wgs, chunks, st);
+    else if (s.npl == 8) rc = scan_launch<T, 8, 1>(a, tab, s.wgs, chunks, st);
+    else if (s.nw == 1) rc = scan_launch<T, 16, 1>(a, tab, s.wgs, chunks, st);
+    else if (s.nw == 2) rc = scan_launch<T, 16, 2>(a, tab, s.wgs, chunks, st);
+    else if (s.nw == 4) rc = scan_launch<T, 16, 4>(a, tab, s.wgs, chunks, st);
+    else if (s.nw == 8) rc = scan_launch<T, 16, 8>(a, tab, s.wgs, chunks, st);
+    else rc = scan_launch<T, 16, 16>(a, tab, s.wgs, chunks, st);
+    if (rc) return rc;
+  }
+  return 0;
+}
+
+template <class T>
+static int ssm_one_run(const frhip_ssm& p, const SsmCall& c, int rows, hipStream_t st) {
+  SsmArgs<T> a = ssm_args<T>(p, c);
+  a.rows = rows;
+  int lanes = 1;
+  while (lanes * 4 < p.states) lanes *= 2;
+  const size_t wgs = ((size_t)rows * p.channels * lanes + 255) / 256;
+  if (wgs > INT_MAX) return set_error(FRHIP_ESHAPE, "ssm_one: too many rows");
+  const dim3 grid((unsigned)wgs);
+  switch (lanes) {
+    case 1: hipLaunchKernelGGL((ssm_one_kernel<T, 1>), grid, dim3(256), 0, st, a); break;
+    case 2: hipLaunchKernelGGL((ssm_one_kernel<T, 2>), grid, dim3(256), 0, st, a); break;
+    case 4: hipLaunchKernelGGL((ssm_one_kernel<T, 4>), grid, dim3(256), 0, st, a); break;
+    case 8: hipLaunchKernelGGL((ssm_one_kernel<T, 8>), grid, dim3(256), 0, st, a); break;
+    case 16: hipLaunchKernelGGL((ssm_one_kernel<T, 16>), grid, dim3(256), 0, st, a); break;
+    case 32: hipLaunchKernelGGL((ssm_one_kernel<T, 32>), grid, dim3(256), 0, st, a); break;
+    default: hipLaunchKernelGGL((ssm_one_kernel<T, 64>), grid, dim3(256), 0, st, a); break;
+  }
+  return check_launch("ssm_one");
+}
+
+}  // namespace frhip
+
+using namespace frhip;
+
+extern "C" int frhip_conv_one(int rows, int C, int W, const void* x, int ldx, const float* w, const float* bias, int act, const void* state,
+                              void* state_out, void* y, int ldy, int dtype, frhip_stream s) {
+  if (rows < 0) return set_error(FRHIP_ESHAPE, "conv_one: negative rows");
+  if (int rc = conv_check(C, W, x, ldx, w, bias, act, state, state_out, y, ldy, dtype, 0, rows, rows)) return rc;
+  if (rows == 0) return 0;
+  hipStream_t st = static_cast<hipStream_t>(s);
+  if (dtype == FRHIP_F16) {
+    auto a = conv_args<h1>(C, x, ldx, w, bias, act, state, state_out, y, ldy);
+    a.rows = rows;
+    return conv_one_run(a, W, st);
+  }
+  auto a = conv_args<float>(C, x, ldx, w, bias, act, state, state_out, y, ldy);
+  a.rows = rows;
+  return conv_one_run(a, W, st);
+}
+
+extern "C" int frhip_conv_seq(int nseq, const int32_t* seq_start, int C, int W, const void* x, int ldx, const float* w, const float* bias,
+                              int act, const void* state, void* state_out, void* y, int ldy, int dtype, frhip_stream s) {
+  if (int rc = check_seqs(nseq, seq_start, "conv_seq: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
+  const size_t row0 = nseq ? seq_start[0] : 0, rows = nseq ? seq_start[nseq] - seq_start[0] : 0;
+  if (int rc = conv_check(C, W, x, ldx, w, bias, act, state, state_out, y, ldy, dtype, row0, rows, nseq)) return rc;
+  if (nseq == 0) return 0;
+  hipStream_t st = static_cast<hipStream_t>(s);
+  if (dtype == FRHIP_F16) return conv_seq_run(conv_args<h1>(C, x, ldx, w, bias, act, state, state_out, y, ldy), W, nseq, seq_start, st);
+  return conv_seq_run(conv_args<float>(C, x, ldx, w, bias, act, state, state_out, y, ldy), W, nseq, seq_start, st);
+}
+
+extern "C" int frhip_ssm_one(const frhip_ssm* p, int rows, const void* x, int ldx, const void* dt, int lddt, const void* B, int ldb,
+                             const void* C, int ldc, const void* z, int ldz, const float* state, float* state_out, void* y, int ldy,
+                             int dtype, frhip_stream s) {
+  if (int rc = ssm_check_params(p)) return rc;
+  if (rows < 0) return set_error(FRHIP_ESHAPE, "ssm_one: negative rows");
+  const SsmCall c = {x, dt, B, C, z, ldx, lddt, ldb, ldc, ldz, state, state_out, y, ldy, dtype};
+  if (int rc = ssm_check(*p, c, 0, rows, rows)) return rc;
+  if (rows == 0) return 0;
+  return dtype == FRHIP_F16 ? ssm_one_run<h1>(*p, c, rows, static_cast<hipStream_t>(s)) : ssm_one_run<float>(*p, c, rows, static_cast<hipStream_t>(s));
+}
+
+extern "C" size_t frhip_ssm_workspace_bytes(const frhip_ssm* p, int nseq, int T) {
+  if (!p || p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0 || p->states < 1 || p->states > 256 || nseq <= 0 || T <= 0) return 0;
+  const ScanShape s = scan_shape(*p);
+  const size_t bytes = scan_most_local(s, T) * (2 * (size_t)p->states + 1) * p->channels * 4;
+  return (bytes + 255) / 256 * 256;
+}
+
+extern "C" int frhip_ssm_seq(const frhip_ssm* p, int nseq, const int32_t* seq_start, const void* x, int ldx, const void* dt, int lddt,
+                             const void* B, int ldb, const void* C, int ldc, const void* z, int ldz, const float* state, float* state_out,
+                             void* y, int ldy, int dtype, void* workspace, frhip_stream s) {
+  if (int rc = ssm_check_params(p)) return rc;
+  if (int rc = check_seqs(nseq, seq_start, "ssm_seq: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
+  const SsmCall c = {x, dt, B, C, z, ldx, lddt, ldb, ldc, ldz, state, state_out, y, ldy, dtype};
+  const size_t row0 = nseq ? seq_start[0] : 0, rows = nseq ? seq_start[nseq] - seq_start[0] : 0;
+  if (int rc = ssm_check(*p, c, row0, rows, nseq)) return rc;
+  if (nseq == 0) return 0;
+  if (scan_shape(*p).wgs > (1 << 24)) return set_error(FRHIP_ESHAPE, "ssm_seq: too many channels");
+  if (frhip_ssm_workspace_bytes(p, nseq, (int)rows) > 0) {
+    if (!workspace) return set_error(FRHIP_EINVAL, "ssm_seq: null workspace");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return set_error(FRHIP_EINVAL, "ssm_seq: workspace must be 16-byte aligned");
+  }
+  hipStream_t st = static_cast<hipStream_t>(s);
+  return dtype == FRHIP_F16 ? ssm_seq_run<h1>(*p, c, nseq, seq_start, workspace, st) : ssm_seq_run<float>(*p, c, nseq, seq_start, workspace, st);
+}
+
+extern "C" int frhip_ssm_cut(const frhip_ssm* p, int nseq, const int32_t* seq_start, int compute_units, int* out) {
+  if (int rc = ssm_check_params(p)) return rc;
+  if (!out) return set_error(FRHIP_EINVAL, "ssm_cut: null pointer");
+  if (compute_units < 1) return set_error(FRHIP_ESHAPE, "ssm_cut: no such scan");
+  if (int rc = check_seqs(nseq, seq_start, "ssm_cut: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
+  if (nseq < 1 || nseq > kSeqTable) return set_error(FRHIP_ESHAPE, "ssm_cut: 1 to 128 prompts");
+  const ScanShape s = scan_shape(*p);
+  SeqTable tab;
+  out[0] = scan_chunk(s, seq_start[nseq] - seq_start[0], compute_units);
+  out[1] = scan_table(tab, seq_start, 0, nseq, out[0]);
+  out[2] = s.wgs;
+  return 0;
+}

@@ -246,6 +246,7 @@ int frhip_gemm(const void *x, const frhip_weight *w, void *y, int T, int out_dty
  * kernels/cuda/ffn_seq.cu:78-79, att.cu:154-159), FRHIP_ACT_RELU2 (InplaceReLUAndSquare,
  * ffn_seq.cu:80-81), FRHIP_ACT_SILU (InplaceSiLU, att_seq.cu:394-395, att.cu:145-152).  This is
  * the epilogue the seq operators below use for r, ffn key and the gate; results are theirs bit for bit. */
+#define FRHIP_ACT_NONE 0 /* frhip_conv_*: no activation */
 #define FRHIP_ACT_SIGMOID 2
 #define FRHIP_ACT_RELU2 3
 #define FRHIP_ACT_SILU 4
@@ -342,6 +343,50 @@ int frhip_seq_codes_way(int T, int K, int nproducts, const int *N, int which, in
 /* How frhip_att_seq_v4's scan of T steps of C channels is cut on a part with that many compute units.  out[0]: channels of a
  * workgroup, out[1]: workgroups, out[2]: blocks of time one after another, out[3]: chunks of a block, out[4]: steps of a chunk. */
 int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
+
+/* ---- operators of a selective state space layer -------------------------------- */
+/* Recurrent layers whose decay depends on the input (no counterpart in the reference; they stand beside att_one / att_seq).
+ * Activations are FRHIP_F16 or FRHIP_F32 (`dtype`: x, dt, B, C, z, y and the convolution's state), rows `ld` elements apart, at any
+ * address that is a multiple of their element's size; parameters and the scan's state are fp32.  Sums, decays and states
+ * are held in fp32; an output is rounded once.  A `_one` call takes one token each of `rows` sequences; a `_seq` call takes
+ * nseq prompts that lie one behind the other: prompt i is rows seq_start[i] .. seq_start[i + 1] - 1 (seq_start: nseq + 1
+ * numbers in HOST memory, read before the call returns, not descending, the first not negative).  A prompt of no rows leaves
+ * its state as it was; rows ahead of the first prompt and behind the last are neither read nor written.  States are [nseq or rows][...],
+ * and the one written may be the one read (the same address, or memory that does not overlap).  y overlaps nothing that is read. */
+
+/* Short causal convolution over time, channel by channel:
+ *   y[t][c] = act(bias[c] + sum_{j < W} w[c][j] * x[t - W + 1 + j][c])
+ * W 2..4; w [C][W]; bias [C] or NULL; act FRHIP_ACT_NONE or FRHIP_ACT_SILU.  state [.][W - 1][C] holds the inputs of the
+ * tokens before, oldest first, in `dtype`; state_out receives those that the next call needs. */
+int frhip_conv_one(int rows, int C, int W, const void *x, int ldx, const float *w, const float *bias, int act,
+                   const void *state, void *state_out, void *y, int ldy, int dtype, frhip_stream s);
+int frhip_conv_seq(int nseq, const int32_t *seq_start, int C, int W, const void *x, int ldx, const float *w, const float *bias, int act,
+                   const void *state, void *state_out, void *y, int ldy, int dtype, frhip_stream s);
+
+/* Selective scan, for every channel d of `channels` with its `states` states n, in group g = d / (channels / groups):
+ *   dt' = softplus(dt[t][d] + dt_bias[d])          (dt_softplus 0: dt[t][d] + dt_bias[d], not negative)
+ *   h[d][n] = exp(dt' A[d][n]) h[d][n] + dt' x[t][d] B[t][g][n]
+ *   y[t][d] = (sum_n C[t][g][n] h[d][n] + D[d] x[t][d]) * silu(z[t][d])
+ * A [channels][states], not positive; D and dt_bias [channels], NULL: zero; z NULL: no gate.  B and C are rows of groups * states.
+ * state [.][channels][states] fp32.  states 1..256.  What is not finite reaches the outputs of its channel from its token on, and
+ * through B or C those of its group. */
+typedef struct frhip_ssm {
+  const float *A, *D, *dt_bias;
+  int32_t channels, states, groups;
+  int32_t dt_softplus;
+} frhip_ssm;
+int frhip_ssm_one(const frhip_ssm *p, int rows, const void *x, int ldx, const void *dt, int lddt, const void *B, int ldb,
+                  const void *C, int ldc, const void *z, int ldz, const float *state, float *state_out, void *y, int ldy,
+                  int dtype, frhip_stream s);
+/* Scratch of frhip_ssm_seq for T rows in nseq prompts: bytes (may be 0), 16-byte aligned, owned by the caller; calls that can
+ * run at the same time need one each. */
+size_t frhip_ssm_workspace_bytes(const frhip_ssm *p, int nseq, int T);
+int frhip_ssm_seq(const frhip_ssm *p, int nseq, const int32_t *seq_start, const void *x, int ldx, const void *dt, int lddt,
+                  const void *B, int ldb, const void *C, int ldc, const void *z, int ldz, const float *state, float *state_out,
+                  void *y, int ldy, int dtype, void *workspace, frhip_stream s);
+/* How that scan is cut on a part with that many compute units, a pure function of the sizes: out[0] rows of a chunk, out[1] chunks of
+ * all prompts, out[2] workgroups a chunk. */
+int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int compute_units, int *out);
 
 /* ---- bandwidth probes: DIAGNOSTICS, not operators (measurement aids of bench.py and of the
  *      hardware-counter calibration; no counterpart in the reference, nothing on the model path calls them) */
