@@ -9,10 +9,10 @@
 // One token is the formula itself.
 #include <climits>
 #include <cstring>
-#include <initializer_list>
 
-#include "device_utils.h"
+#include "activations.h"
 #include "frhip_internal.h"
+#include "spans.h"
 
 #pragma clang fp contract(off)
 
@@ -34,35 +34,6 @@ __device__ __forceinline__ int find_seq(int nseq, int j, F first) {
     else hi = mid - 1;
   }
   return lo;
-}
-
-constexpr float kLog2e = 1.44269504088896340736f;
-
-// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|); log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, with atanh(s) / s as a polynomial
-// in s^2 (Chebyshev fit over [0, 1/9], 8e-9 relative), so that small values keep their relative accuracy.  FINE: the rounding of
-// -|v| log2(e), which exp2 would scale by |v|, is made good.
-template <bool FINE>
-__device__ __forceinline__ float softplus_f(float v) {
-  const float m = __builtin_fabsf(v), t = m * -kLog2e;
-  float e = __builtin_amdgcn_exp2f(t);
-  if constexpr (FINE) {
-    // m log2(e) = -t + r, log2(e) = kLog2e + 1.925963033500752e-8
-    const float r = __builtin_fmaf(m, 1.925963033500752e-8f, __builtin_fmaf(m, kLog2e, t));
-    e = __builtin_fmaf(e, -r * 0.693147180559945f, e);
-    e = m < 80.f ? e : expf(-m);  // beyond, r is no small number of an infinite m, and e is below what exp2 keeps
-  }
-  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
-  float p = __builtin_fmaf(q, 0.1408732831478119f, 0.1398070901632309f);
-  p = __builtin_fmaf(p, q, 0.20012426376342773f);
-  p = __builtin_fmaf(p, q, 0.3333315849304199f);
-  p = __builtin_fmaf(p, q, 1.0f);
-  return __builtin_fmaxf(v, 0.f) + 2.0f * s * p;  // a NaN stays one through s
-}
-
-template <class T>
-__device__ __forceinline__ float silu_f(float v) {
-  if constexpr (sizeof(T) == 4) return v / (1.0f + expf(-v));
-  return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -kLog2e));
 }
 
 // ---------------------------------------------------------------------------
@@ -130,7 +101,7 @@ struct ConvTaps {
       float s = b[i];
 #pragma unroll
       for (int j = 0; j < W; j++) s = __builtin_fmaf(w[j][i], past[j][i], s);
-      y[i] = silu ? silu_f<T>(s) : s;
+      y[i] = silu ? silu_f<sizeof(T) == 4>(s) : s;
     }
   }
 };
@@ -335,7 +306,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64) void ssm_scan_kernel(SsmArgs<T
         sum += dt[r];
       } else if constexpr (NW == 1) {
         const float y = __builtin_fmaf(skip, x[r], y0 + y1);
-        if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<T>(z[r]) : y);
+        if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<sizeof(T) == 4>(z[r]) : y);
       } else {
         part[wave][r][lane] = y0 + y1;
       }
@@ -349,7 +320,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64) void ssm_scan_kernel(SsmArgs<T
 #pragma unroll
           for (int w = 1; w < NW; w++) y += part[cw * NW + w][r][lane];
           y = __builtin_fmaf(skip, x[r], y);
-          if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<T>(z[r]) : y);
+          if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<sizeof(T) == 4>(z[r]) : y);
         }
     }
   }
@@ -394,7 +365,7 @@ __global__ __launch_bounds__(256) void ssm_one_kernel(SsmArgs<T> a) {
   for (int m = 1; m < LANES; m *= 2) y += __shfl_xor(y, m);
   if (q == 0) {
     y = __builtin_fmaf(a.D ? a.D[d] : 0.f, x, y);
-    a.y[(size_t)row * a.ldy + d] = (T)(a.z ? y * silu_f<T>((float)a.z[(size_t)row * a.ldz + d]) : y);
+    a.y[(size_t)row * a.ldy + d] = (T)(a.z ? y * silu_f<sizeof(T) == 4>((float)a.z[(size_t)row * a.ldz + d]) : y);
   }
 }
 
@@ -441,30 +412,6 @@ static int check_seqs(int nseq, const int32_t* seq_start, const char* what) {
       if (seq_start[i + 1] < seq_start[i]) return set_error(FRHIP_ESHAPE, what);
   }
   return 0;
-}
-
-// Whether [rows][cols] of ld elements a row at a and b (ldb) share memory.  Rows of the same pitch may lie side by side.
-static bool rows_overlap(const void* a, size_t lda, const void* b, size_t ldb, size_t rows, size_t cols_a, size_t cols_b, size_t elem) {
-  if (!a || !b || !rows) return false;
-  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-  const uintptr_t ea = pa + ((rows - 1) * lda + cols_a) * elem, eb = pb + ((rows - 1) * ldb + cols_b) * elem;
-  if (ea <= pb || eb <= pa) return false;
-  if (lda != ldb) return true;
-  const size_t pitch = lda * elem, off = (pa < pb ? pb - pa : pa - pb) % pitch;
-  // seen from the lower one, the other begins `off` bytes into a row
-  const size_t low = (pa < pb ? cols_a : cols_b) * elem, high = (pa < pb ? cols_b : cols_a) * elem;
-  return off < low || off + high > pitch;
-}
-
-static bool spans_clash(const void* a, const void* b, size_t bytes) {  // neither the same nor apart
-  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
-  return pa != pb && pa < pb + bytes && pb < pa + bytes;
-}
-
-static bool off_grid(size_t elem, std::initializer_list<const void*> ptrs) {
-  uintptr_t v = 0;
-  for (const void* p : ptrs) v |= reinterpret_cast<uintptr_t>(p);
-  return v % elem != 0;
 }
 
 template <class T, int W>

@@ -246,7 +246,7 @@ int frhip_gemm(const void *x, const frhip_weight *w, void *y, int T, int out_dty
  * kernels/cuda/ffn_seq.cu:78-79, att.cu:154-159), FRHIP_ACT_RELU2 (InplaceReLUAndSquare,
  * ffn_seq.cu:80-81), FRHIP_ACT_SILU (InplaceSiLU, att_seq.cu:394-395, att.cu:145-152).  This is
  * the epilogue the seq operators below use for r, ffn key and the gate; results are theirs bit for bit. */
-#define FRHIP_ACT_NONE 0 /* frhip_conv_*: no activation */
+#define FRHIP_ACT_NONE 0 /* frhip_linear, frhip_conv_*: no activation */
 #define FRHIP_ACT_SIGMOID 2
 #define FRHIP_ACT_RELU2 3
 #define FRHIP_ACT_SILU 4
@@ -353,6 +353,19 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * numbers in HOST memory, read before the call returns, not descending, the first not negative).  A prompt of no rows leaves
  * its state as it was; rows ahead of the first prompt and behind the last are neither read nor written.  States are [nseq or rows][...],
  * and the one written may be the one read (the same address, or memory that does not overlap).  y overlaps nothing that is read. */
+
+/* Product with bias, activation and residual: y = residual + act(x . w + bias), evaluated in fp32 and rounded once (unlike
+ * frhip_gemm_act, which rounds ahead of the activation as the reference does).  x [T] rows of K binary16, ldx elements apart;
+ * bias [N] fp32 or NULL; residual [T] rows of N in out_dtype, ldr apart, or NULL; y [T] rows of N in out_dtype (F16 or F32), ldy
+ * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
+ * K is a multiple of 8, N and T are any; x and w->data are 16-byte aligned and ldx is a multiple of 8, the others lie at
+ * multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
+ * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each. */
+#define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */
+#define FRHIP_ACT_SOFTPLUS 6 /* log(1 + exp(v)) */
+size_t frhip_linear_workspace_bytes(int T, const frhip_weight *w);
+int frhip_linear(const void *x, int ldx, const frhip_weight *w, const float *bias, int act, const void *residual, int ldr,
+                 void *y, int ldy, int T, int out_dtype, void *workspace, frhip_stream s);
 
 /* Short causal convolution over time, channel by channel:
  *   y[t][c] = act(bias[c] + sum_{j < W} w[c][j] * x[t - W + 1 + j][c])

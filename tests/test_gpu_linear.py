@@ -1,0 +1,120 @@
+"""frhip_linear (product, bias, activation, residual, one rounding) against the formula in float64."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+from hipref import DevBuf, L, dev, fr, make_weight
+
+U = 2.0 ** -23
+ACT = {"none": 0, "sigmoid": 2, "relu2": 3, "silu": 4, "gelu": 5, "softplus": 6}
+erfc = np.frompyfunc(math.erfc, 1, 1)
+
+
+def act64(v, act):
+    """The activation, and its tolerance: its slope times the error of v, and the fp32 evaluation's own (an exponential is off by (|v| + 2) U,
+    an erfc by the rounding of its argument, v^2 U, and a few units)"""
+    if act == "none":
+        return v, lambda e: e
+    if act == "relu2":
+        return np.maximum(v, 0) ** 2, lambda e: 2 * np.abs(v) * e + e * e + U * v * v
+    if act == "gelu":
+        f = 0.5 * v * erfc(-v / math.sqrt(2)).astype(np.float64)
+        return f, lambda e: 1.2 * e + (v * v + 12) * U * np.abs(f) + 2.0 ** -126
+    s = 1 / (1 + np.exp(-v))
+    f = {"sigmoid": s, "silu": v * s, "softplus": np.logaddexp(0, v)}[act]
+    return f, lambda e: 1.1 * e + (np.abs(v) + 12) * U * np.abs(f) + 2.0 ** -126
+
+
+def case(T, K, N, act="none", bias=False, res=False, out="f16", quant=False, pad=0, in_place=False, seed=0, stream=None, scale=1.0):
+    g = np.random.default_rng([T, K, N, seed])
+    t, code = (np.float16, fr.F16) if out == "f16" else (np.float32, fr.F32)
+    ldx, ldy, ldr = K + 8 * pad, N + pad, N + (pad if in_place else 2 * pad)
+    x = g.standard_normal((T, ldx)).astype(np.float16)
+    pw, w = make_weight((g.standard_normal((K, N)) * scale / math.sqrt(K)).astype(np.float16), quant)
+    b = g.standard_normal(N).astype(np.float32) if bias else None
+    y0 = g.standard_normal((T, ldy)).astype(t)
+    r = y0 if in_place else g.standard_normal((T, ldr)).astype(t)
+    res = res or in_place
+    dx, dy = dev(x), dev(y0)
+    dr, db = dy if in_place else dev(r), dev(b) if bias else None
+    need = L().frhip_linear_workspace_bytes(T, pw.ref)
+    ws = DevBuf(need) if need else None
+    call = lambda: L().frhip_linear(dx.ptr, ldx, pw.ref, db.ptr if bias else None, ACT[act], dr.ptr if res else None, ldr, dy.ptr, ldy, T,
+                                    code, ws.ptr if ws else None, stream)
+    fr.check(call(), "linear")
+    fr.check(L().frhip_device_sync())
+    got = dy.numpy()
+    xf, wf = x[:, :K].astype(np.float64), w.astype(np.float64)
+    v, mag = xf @ wf, np.abs(xf) @ np.abs(wf)
+    if bias:
+        v, mag = v + b, mag + np.abs(b)
+    # a chain of K / 32 accumulations of sums of 32 exact products (and up to 8 waves' sums), each step within U of the magnitudes
+    f, tol = act64(v, act)
+    err = tol((K / 32 + 40) * U * mag)
+    want = f + (r[:, :N].astype(np.float64) if res else 0)
+    err = err + U * np.abs(want) + (np.abs(want) * 2.0 ** -11 + 2.0 ** -25 if out == "f16" else 0)
+    bad = ~(np.abs(got[:, :N].astype(np.float64) - want) <= err)
+    assert not bad.any(), (bad.sum(), np.argwhere(bad)[:4], got[:, :N][bad][:4], want[bad][:4])
+    assert np.array_equal(got[:, N:], y0[:, N:])
+    return got, call, dy, y0
+
+
+# T on both sides of every form's edge, K with and without a rest of 64 and 32, N with ragged ends
+@pytest.mark.parametrize("quant", [False, True])
+@pytest.mark.parametrize("T,K,N", [(1, 8, 1), (1, 1032, 33), (2, 2048, 130), (3, 40, 7), (4, 64, 64), (5, 256, 515), (16, 104, 48), (17, 2048, 100),
+                                   (33, 160, 37), (64, 520, 96), (65, 72, 130), (97, 584, 200), (129, 64, 32), (300, 168, 77), (513, 320, 264)])
+def test_sizes(T, K, N, quant):
+    case(T, K, N, quant=quant)
+    case(T, K, N, act="silu", bias=True, res=True, out="f32", quant=quant, pad=3, seed=1)
+
+
+@pytest.mark.parametrize("out", ["f16", "f32"])
+@pytest.mark.parametrize("act", sorted(ACT))
+@pytest.mark.parametrize("T", [1, 20, 200])
+def test_activations(T, act, out):
+    case(T, 96, 200, act=act, bias=True, out=out, seed=2, scale=4.0)
+    case(T, 96, 200, act=act, res=True, out=out, seed=3)
+
+
+@pytest.mark.parametrize("out", ["f16", "f32"])
+@pytest.mark.parametrize("T", [1, 40, 150])
+def test_residual_in_place(T, out):
+    case(T, 128, 72, act="gelu", bias=True, out=out, pad=5, in_place=True)
+
+
+def test_a_large_product():
+    case(1030, 1096, 1290, act="softplus", bias=True, out="f32", pad=1)
+
+
+def test_what_is_not_finite_stays_in_its_row():
+    T, K, N = 70, 200, 90
+    g = np.random.default_rng(3)
+    for t in (1, 20, T):
+        x = g.standard_normal((t, K)).astype(np.float16)
+        x[t // 2, 199] = np.nan
+        pw, _ = make_weight((g.standard_normal((K, N)) / 14).astype(np.float16))
+        dx, dy = dev(x), DevBuf.empty((t, N), np.float16)
+        fr.check(L().frhip_linear(dx.ptr, K, pw.ref, None, 3, None, 0, dy.ptr, N, t, fr.F16, None, None))
+        y = dy.numpy()
+        assert np.isnan(y[t // 2]).all() and np.isfinite(np.delete(y, t // 2, 0)).all()
+
+
+@pytest.mark.parametrize("T,quant", [(1, False), (20, True), (200, False), (600, True)])
+def test_a_captured_product_replays(T, quant):
+    st, g = C.c_void_p(), C.c_void_p()
+    fr.check(L().frhip_stream_create(C.byref(st)))
+    first, call, dy, y0 = case(T, 200, 72, act="silu", bias=True, res=True, quant=quant, stream=st)
+    fr.check(L().frhip_graph_begin(st))
+    fr.check(call())
+    fr.check(L().frhip_graph_end(st, C.byref(g)))
+    for _ in range(3):
+        dy.upload(y0)
+        fr.check(L().frhip_graph_launch(g, st))
+        fr.check(L().frhip_stream_sync(st))
+        assert np.array_equal(dy.numpy(), first)
+    fr.check(L().frhip_graph_destroy(g))
+    fr.check(L().frhip_stream_destroy(st))
