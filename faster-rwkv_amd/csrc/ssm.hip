@@ -198,36 +198,42 @@ struct SsmArgs {
   int nseq, rows;            // prompts of the launch; scan of one token: rows
 };
 
-constexpr int kScanRows = 8;  // rows that go through LDS and registers together
-
-// Waves of a workgroup: NW of them share a channel's states, NPL each, and there are four or NW in all.
+// Waves of a workgroup: NW of them share the states of 64 channels, NPL a lane, and there are four or NW in all.
 constexpr int scan_waves(int nw) { return nw < 4 ? 4 : nw; }
+constexpr int scan_rows(int nw) { return nw == 1 ? 8 : 16; }  // of a block of time, the rows that go through LDS together
 
-// LOCAL: step 1 of the scan, otherwise step 2.  A lane has one channel and NPL of its states in registers; B and C of kScanRows rows go
-// through LDS as fp32, where every lane reads the same address.
+// LOCAL: step 1 of the scan, otherwise step 2.  A workgroup walks its chunk in blocks of time.  Of a block, every wave
+//   A. takes some rows to LDS: dt and dt x of a channel a lane (the next block's, while this one is scanned), and B and C as fp32;
+//   B. runs all of its rows with NPL states a lane in registers, and leaves its part of y in LDS;
+//   C. adds the parts of the rows that it took in A, applies skip and gate and stores them.
+// The step width's softplus and the gate are so evaluated once a channel and row, not once a wave.  What bounds it is the issue of
+// vector instructions: 4, and an exponential of twice their length, a state and row.  The waves of a SIMD have to be several for that.
 template <class T, int NPL, int NW, bool LOCAL>
-__global__ __launch_bounds__(scan_waves(NW) * 64) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
-  constexpr int WAVES = scan_waves(NW), CW = WAVES / NW, NT = NPL * NW, TB = kScanRows, STAGE = (TB * 2 * NT + WAVES * 64 - 1) / (WAVES * 64);
+__global__ __launch_bounds__(scan_waves(NW) * 64, 4) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
+  constexpr int WAVES = scan_waves(NW), CW = WAVES / NW, NT = NPL * NW, TB = scan_rows(NW), CH = CW * 64;
+  constexpr int ROWS = TB * CW / WAVES;                                  // rows of a wave in A and C: of its 64 channels
+  constexpr int STAGE = (TB * 2 * NT + WAVES * 64 - 1) / (WAVES * 64);  // elements of B and C of a thread
+  static_assert(ROWS * NW == TB, "every row has its wave");
+  constexpr bool FINE = sizeof(T) == 4;
   __shared__ __attribute__((aligned(16))) float bc[2][TB][2][NT];
-  __shared__ float part[NW > 1 ? WAVES : 1][NW > 1 ? TB : 1][64];
+  __shared__ float2 du[2][TB][CH];
+  __shared__ float part[LOCAL || NW == 1 ? 1 : NW][TB][CH];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cw = wave / NW, nw = wave % NW;
   const int j0 = blockIdx.y;
   const int i = LOCAL ? find_seq(a.nseq, j0, [&](int k) { return tab.chunk[k] - k; })
                       : find_seq(a.nseq, j0, [&](int k) { return tab.chunk[k]; });
   const int nchunk = tab.chunk[i + 1] - tab.chunk[i], ci = j0 - tab.chunk[i] + (LOCAL ? i : 0), local0 = tab.chunk[i] - i;
   const int end = tab.start[i + 1], t0 = tab.start[i] + ci * a.chunk, t1 = end - t0 < a.chunk ? end : t0 + a.chunk;
-  const int g = blockIdx.x / a.nblk, cg = (blockIdx.x - g * a.nblk) * (CW * 64) + cw * 64 + lane;
+  const int g = blockIdx.x / a.nblk, at = cw * 64 + lane, cg = (blockIdx.x - g * a.nblk) * CH + at;
   const bool mine = cg < a.cpg;
   const int d = g * a.cpg + (mine ? cg : a.cpg - 1), n0 = nw * NPL;
 
   float A2[NPL], h[NPL];
 #pragma unroll
   for (int k = 0; k < NPL; k++) {
-    const bool ok = n0 + k < a.N;
-    A2[k] = ok ? a.A[(size_t)d * a.N + n0 + k] * kLog2e : 0.f;
+    A2[k] = n0 + k < a.N ? a.A[(size_t)d * a.N + n0 + k] * kLog2e : 0.f;
     h[k] = 0.f;
   }
-  const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
   const size_t ND = (size_t)a.N * a.D_;
   if constexpr (LOCAL) {
     if (ci == 0 && mine) {  // step 2 reads it here: its last chunk may overwrite the state
@@ -243,6 +249,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64) void ssm_scan_kernel(SsmArgs<T
 #pragma unroll
     for (int k = 0; k < NPL; k++)
       if (n0 + k < a.N) h[k] = a.ends[(size_t)(a.nlocal + local0) * ND + (size_t)(n0 + k) * a.D_ + d];
+#pragma unroll 2
     for (int p = 0; p < ci; p++) {
       const float s = a.sums[(size_t)(local0 + p) * a.D_ + d];
       const float* e = a.ends + (size_t)(local0 + p) * ND + d;
@@ -252,81 +259,101 @@ __global__ __launch_bounds__(scan_waves(NW) * 64) void ssm_scan_kernel(SsmArgs<T
     }
   }
 
-  const T* const Bg = a.B + (size_t)g * a.N;
-  const T* const Cg = a.C + (size_t)g * a.N;
-  const float skip = !LOCAL && a.D ? a.D[d] : 0.f;
-  float sum = 0.f, xr[TB], dr[TB], zr[TB], st[STAGE];
-  auto request = [&](int t) {  // rows past the chunk repeat its last one
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = !LOCAL && a.D ? a.D[d] : 0.f;
+  const T* const zp = a.z ? a.z : a.x;  // without a gate some row that is there, for nothing
+  const int ldz = a.z ? a.ldz : a.ldx;
+  float sum = 0.f;
+  T xr[ROWS], dr[ROWS], zr[ROWS], st[STAGE];
+  auto request = [&](int t) {  // of the block that begins at row t; rows past the chunk repeat its last one
 #pragma unroll
-    for (int r = 0; r < TB; r++) {
-      const int row = t + r < t1 ? t + r : t1 - 1;
-      xr[r] = (float)a.x[(size_t)row * a.ldx + d];
-      dr[r] = (float)a.dt[(size_t)row * a.lddt + d];
-      if constexpr (!LOCAL) zr[r] = a.z ? (float)a.z[(size_t)row * a.ldz + d] : 0.f;
+    for (int r = 0; r < ROWS; r++) {
+      const int row = t + nw * ROWS + r < t1 ? t + nw * ROWS + r : t1 - 1;
+      xr[r] = (a.x + (size_t)row * a.ldx)[(unsigned)d];
+      dr[r] = (a.dt + (size_t)row * a.lddt)[(unsigned)d];
+      if constexpr (!LOCAL) zr[r] = (zp + (size_t)row * ldz)[(unsigned)d];
     }
 #pragma unroll
     for (int q = 0; q < STAGE; q++) {
       const int e = threadIdx.x + q * (WAVES * 64), r = e / (2 * NT), c = (e / NT) & 1, n = e % NT;
-      st[q] = e < TB * 2 * NT && t + r < t1 && n < a.N ? (float)(c ? Cg + (size_t)(t + r) * a.ldc : Bg + (size_t)(t + r) * a.ldb)[n] : 0.f;
+      const bool in = e < TB * 2 * NT && t + r < t1 && n < a.N;
+      st[q] = (T)0.f;
+      if (in) st[q] = ((c ? a.C : a.B) + (size_t)(t + r) * (c ? a.ldc : a.ldb))[g * a.N + n];
     }
   };
-  if (t0 < t1) request(t0);
-  int buf = 0;
-  for (int t = t0; t < t1; t += TB, buf ^= 1) {
-    float x[TB], dt[TB], z[TB];
+  float x[ROWS], z[ROWS];  // of the block that is scanned
+  auto take = [&](int t, int buf, float (&xn)[ROWS], float (&zn)[ROWS]) {
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+      const bool live = t + nw * ROWS + r < t1;
+      const float v = (float)dr[r] + bias, sp = softplus_f<FINE>(v);
+      const float dt = live ? (a.softplus ? sp : v) : 0.f;
+      xn[r] = live ? (float)xr[r] : 0.f;
+      if constexpr (!LOCAL) zn[r] = (float)zr[r];
+      du[buf][nw * ROWS + r][at] = make_float2(dt, dt * xn[r]);
+      if constexpr (LOCAL) sum += dt;
+    }
 #pragma unroll
     for (int q = 0; q < STAGE; q++) {
       const int e = threadIdx.x + q * (WAVES * 64);
-      if (e < TB * 2 * NT) (&bc[buf][0][0][0])[e] = st[q];
+      if (e < TB * 2 * NT) (&bc[buf][0][0][0])[e] = (float)st[q];
     }
-#pragma unroll
-    for (int r = 0; r < TB; r++) {
-      const float v = dr[r] + bias;
-      const bool live = t + r < t1;
-      dt[r] = live ? (a.softplus ? softplus_f<sizeof(T) == 4>(v) : v) : 0.f;
-      x[r] = live ? xr[r] : 0.f;
-      z[r] = zr[r];
-    }
+  };
+  if (t0 < t1) {
+    request(t0);
+    take(t0, 0, x, z);
+    if (t0 + TB < t1) request(t0 + TB);
+  }
+  int buf = 0;
+  for (int t = t0; t < t1; t += TB, buf ^= 1) {
     __syncthreads();
-    if (t + TB < t1) request(t + TB);
-#pragma unroll
+#pragma unroll 8
     for (int r = 0; r < TB; r++) {
-      const float u = dt[r] * x[r];
+      const float2 v = du[buf][r][at];
       float y0 = 0.f, y1 = 0.f;
 #pragma unroll
       for (int k = 0; k < NPL; k++) {
-        const float decay = __builtin_amdgcn_exp2f(dt[r] * A2[k]);
-        h[k] = __builtin_fmaf(decay, h[k], u * bc[buf][r][0][n0 + k]);
+        const float decay = __builtin_amdgcn_exp2f(v.x * A2[k]);
+        h[k] = __builtin_fmaf(decay, h[k], v.y * bc[buf][r][0][n0 + k]);
         if constexpr (!LOCAL) {
           float& y = k & 1 ? y1 : y0;
           y = __builtin_fmaf(bc[buf][r][1][n0 + k], h[k], y);
         }
       }
-      if constexpr (LOCAL) {
-        sum += dt[r];
-      } else if constexpr (NW == 1) {
-        const float y = __builtin_fmaf(skip, x[r], y0 + y1);
-        if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<sizeof(T) == 4>(z[r]) : y);
-      } else {
-        part[wave][r][lane] = y0 + y1;
-      }
+      if constexpr (!LOCAL) part[NW == 1 ? 0 : nw][r][at] = y0 + y1;
     }
-    if constexpr (!LOCAL && NW > 1) {
+    float xn[ROWS], zn[ROWS];
+    if (t + TB < t1) {
+      take(t + TB, buf ^ 1, xn, zn);
+      if (t + 2 * TB < t1) request(t + 2 * TB);
+    }
+    if constexpr (!LOCAL) {
       __syncthreads();
 #pragma unroll
-      for (int r = 0; r < TB; r++)
-        if (r % NW == nw) {
-          float y = part[cw * NW][r][lane];
+      for (int r = 0; r < ROWS; r++) {
+        const int row = nw * ROWS + r;
+        float y = part[0][row][at];
 #pragma unroll
-          for (int w = 1; w < NW; w++) y += part[cw * NW + w][r][lane];
-          y = __builtin_fmaf(skip, x[r], y);
-          if (mine && t + r < t1) a.y[(size_t)(t + r) * a.ldy + d] = (T)(a.z ? y * silu_f<sizeof(T) == 4>(z[r]) : y);
-        }
+        for (int w = 1; w < NW; w++) y += part[w][row][at];
+        y = __builtin_fmaf(skip, x[r], y);
+        if (a.z) y *= silu_f<FINE>(z[r]);
+        if (mine && t + row < t1) (a.y + (size_t)(t + row) * a.ldy)[(unsigned)d] = (T)y;
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) x[r] = xn[r], z[r] = zn[r];
+  }
+  if constexpr (LOCAL) {  // the waves' sums of dt, in wave order
+    __shared__ float total[NW][CH];
+    total[nw][at] = sum;
+    __syncthreads();
+    if (nw == 0 && mine) {
+#pragma unroll
+      for (int w = 1; w < NW; w++) sum += total[w][at];
+      a.sums[(size_t)j0 * a.D_ + d] = sum;
     }
   }
   if (!mine) return;
   if constexpr (LOCAL) {
-    if (nw == 0) a.sums[(size_t)j0 * a.D_ + d] = sum;
 #pragma unroll
     for (int k = 0; k < NPL; k++)
       if (n0 + k < a.N) a.ends[(size_t)j0 * ND + (size_t)(n0 + k) * a.D_ + d] = h[k];
@@ -377,7 +404,7 @@ struct ScanShape {
 };
 static ScanShape scan_shape(const frhip_ssm& p) {
   ScanShape s;
-  s.npl = p.states <= 4 ? 4 : p.states <= 8 ? 8 : 16;
+  s.npl = p.states <= 16 ? 4 : p.states <= 64 ? 8 : 16;
   s.nw = 1;
   while (s.nw * s.npl < p.states) s.nw *= 2;
   const int per = 64 * (scan_waves(s.nw) / s.nw), cpg = p.channels / p.groups;
@@ -389,9 +416,11 @@ static ScanShape scan_shape(const frhip_ssm& p) {
 constexpr int kScanLeast = 16;         // rows of a chunk, at least
 constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
 
-// Rows of a chunk: enough chunks to give every compute unit a workgroup
+constexpr int kScanRows = 16;          // a chunk is a multiple of it
+
+// Rows of a chunk: enough chunks to give every SIMD several waves
 static int scan_chunk(const ScanShape& s, int T, int cus) {
-  const int units = cus < kScanMostUnits ? cus : kScanMostUnits;
+  const int units = cus * 4 < kScanMostUnits ? cus * 4 : kScanMostUnits;
   const int q = units / s.wgs > 1 ? units / s.wgs : 1;
   int len = T / q + (T % q ? 1 : 0);
   if (len < kScanLeast) len = kScanLeast;
@@ -614,11 +643,11 @@ static int ssm_seq_run(const frhip_ssm& p, const SsmCall& c, int nseq, const int
     a.ends = static_cast<float*>(workspace);
     a.sums = a.ends + 2 * (size_t)a.nlocal * per;
     int rc = FRHIP_ESHAPE;
-    if (s.npl == 4) rc = scan_launch<T, 4, 1>(a, tab, s.wgs, chunks, st);
-    else if (s.npl == 8) rc = scan_launch<T, 8, 1>(a, tab, s.wgs, chunks, st);
-    else if (s.nw == 1) rc = scan_launch<T, 16, 1>(a, tab, s.wgs, chunks, st);
-    else if (s.nw == 2) rc = scan_launch<T, 16, 2>(a, tab, s.wgs, chunks, st);
-    else if (s.nw == 4) rc = scan_launch<T, 16, 4>(a, tab, s.wgs, chunks, st);
+    if (s.npl == 4 && s.nw == 1) rc = scan_launch<T, 4, 1>(a, tab, s.wgs, chunks, st);
+    else if (s.npl == 4 && s.nw == 2) rc = scan_launch<T, 4, 2>(a, tab, s.wgs, chunks, st);
+    else if (s.npl == 4) rc = scan_launch<T, 4, 4>(a, tab, s.wgs, chunks, st);
+    else if (s.npl == 8 && s.nw == 4) rc = scan_launch<T, 8, 4>(a, tab, s.wgs, chunks, st);
+    else if (s.npl == 8) rc = scan_launch<T, 8, 8>(a, tab, s.wgs, chunks, st);
     else if (s.nw == 8) rc = scan_launch<T, 16, 8>(a, tab, s.wgs, chunks, st);
     else rc = scan_launch<T, 16, 16>(a, tab, s.wgs, chunks, st);
     if (rc) return rc;
