@@ -16,67 +16,11 @@
 #include <cmath>
 #include <cstring>
 
-#include "gemm_device.h"
+#include "gemm_ring_device.h"
 
 #pragma clang fp contract(off)
 
 namespace frhip {
-
-constexpr int kRingLoaders = 4, kRingThreads = 64 * (4 + kRingLoaders), kRingMostBlocks = 8;
-// K-steps in LDS: as many as 160 KB hold, up to four; tiles of 64 rows and up to 96 columns run two workgroups on a compute unit
-constexpr int ring_stages(int bm, int w) { return bm == 128 && w > 6 ? 3 : 4; }
-static_assert(4 * (128 * 128 + 6 * 4096) <= 160 * 1024 && 3 * (128 * 128 + 8 * 4096) <= 160 * 1024 && 4 * (64 * 128 + 8 * 4096) <= 160 * 1024, "LDS");
-
-template <int BM, int S, int W>
-__device__ __forceinline__ void ring_loader(const GemmSeg& sg, unsigned char* smem, int stage, int p, int m0, int n0, int M, int K, int kbase,
-                                            int nk, int lane) {
-  constexpr int NA = BM / 8 / kRingLoaders, NL = NA + W;
-  static_assert(S == 3 || S == 4, "the waits of the last steps");
-  static_assert((S - 1) * NL <= 63, "the wait counter's range");
-  const int N = sg.N, lr = lane >> 3;
-  unsigned va[NA], vb[W];
-#pragma unroll
-  for (int i = 0; i < NA; i++) {  // groups of 8 rows; rows past the matrix repeat its last one and are never stored
-    const int g = p + kRingLoaders * i;
-    va[i] = (unsigned)(min(m0 + g * 8 + lr, M - 1) - m0) * (unsigned)(K * 2) + (((lane & 7) ^ lr ^ (g & 1)) * 16);
-  }
-#pragma unroll
-  for (int i = 0; i < W; i++) {
-    const int g = p + kRingLoaders * i;
-    vb[i] = (unsigned)(min(n0 + g * 8 + lr, N - 1) - n0) * (unsigned)(K * 2) + (((lane & 7) ^ lr ^ (g & 1)) * 16);
-  }
-  const unsigned char* ak = uniform_ptr(reinterpret_cast<const unsigned char*>(sg.A) + ((size_t)m0 * K + kbase) * 2);
-  const unsigned char* bk = uniform_ptr(sg.B + ((size_t)n0 * K + kbase) * 2);
-  const unsigned lds0 = (unsigned)(size_t)((__attribute__((address_space(3))) unsigned char*)smem) + p * 1024;
-  unsigned at = lds0;
-  const unsigned end = lds0 + S * stage;
-  auto issue = [&] {
-#pragma unroll
-    for (int i = 0; i < W; i++) load_lds_saddr(vb[i], bk, at + BM * 128 + i * (kRingLoaders * 1024));
-#pragma unroll
-    for (int i = 0; i < NA; i++) load_lds_saddr(va[i], ak, at + i * (kRingLoaders * 1024));
-    ak += 128;
-    bk += 128;
-    at += stage;
-    at = at == end ? lds0 : at;
-  };
-#pragma unroll
-  for (int i = 0; i < S - 1; i++)
-    if (i < nk) issue();
-  int k = 0;
-  for (; k + S - 1 < nk; k++) {
-    wait_loads<(S - 2) * NL>();  // step k has landed
-    step_barrier();              // and step k - 1 has been read
-    issue();                     // step k + S - 1, into the slot of step k - 1
-  }
-  for (; k < nk; k++) {
-    const int behind = nk - 1 - k;
-    if (S > 3 && behind >= 2) wait_loads<2 * NL>();
-    else if (behind >= 1) wait_loads<NL>();
-    else wait_loads<0>();
-    step_barrier();
-  }
-}
 
 template <int BM, int S, int NJ>
 __device__ __forceinline__ void ring_mma(const GemmArgs& a, const GemmSeg& sg, unsigned char* smem, int stage, int maxw, bool direct, int m0,
@@ -173,15 +117,16 @@ __global__ __launch_bounds__(kRingThreads) void gemm_ring_kernel(GemmArgs a) {
   const bool direct = sg.epi == G_STORE_F32 && n0 + width * 32 <= sg.N;
   if (wave >= 4) {
     const int p = wave - 4;
+    const RingOperands o = {sg.A, sg.B, a.M, sg.N, a.K, a.K};
     switch (width) {
-      case 1: ring_loader<BM, S, 1>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      case 2: ring_loader<BM, S, 2>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      case 3: ring_loader<BM, S, 3>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      case 4: ring_loader<BM, S, 4>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      case 5: ring_loader<BM, S, 5>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      case 6: ring_loader<BM, S, 6>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      case 7: ring_loader<BM, S, kMost < 7 ? kMost : 7>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
-      default: ring_loader<BM, S, kMost>(sg, ring_smem, stage, p, m0, n0, a.M, a.K, kbase, nk, lane); break;
+      case 1: ring_loader<BM, S, 1>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      case 2: ring_loader<BM, S, 2>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      case 3: ring_loader<BM, S, 3>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      case 4: ring_loader<BM, S, 4>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      case 5: ring_loader<BM, S, 5>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      case 6: ring_loader<BM, S, 6>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      case 7: ring_loader<BM, S, kMost < 7 ? kMost : 7>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
+      default: ring_loader<BM, S, kMost>(o, ring_smem, stage, p, m0, n0, kbase, nk, lane); break;
     }
     if (!direct) step_barrier();
   } else {

@@ -4,7 +4,7 @@
 #include <cstring>
 
 #include "activations.h"
-#include "gemm_device.h"
+#include "gemm_ring_device.h"
 #include "spans.h"
 
 #pragma clang fp contract(off)
@@ -199,6 +199,157 @@ static void few_launch(LinearArgs a, hipStream_t st) {
   hipLaunchKernelGGL((linear_few_kernel<MT, NT, U8, O>), dim3((unsigned)((size_t)tiles * a.strips)), dim3(kLinWaves * 64), kLinWaves * MT * NT * 1024, st, a);
 }
 
+// ---------------------------------------------------------------------------
+// More rows: tiles of 64 or 128 rows, four waves that multiply and four that load (gemm_ring.hip has the form and its reasons), here with
+// rows of any pitch and a K that need not fill its last step.  The sums go through LDS to the epilogue, which all waves share.
+// ---------------------------------------------------------------------------
+struct LinearTiles {
+  LinearArgs l;
+  int base, wide, maxw;  // tiles are `base` blocks of 32 columns wide, the first `wide` of them one more; the widest
+};
+
+// The waves that multiply: the nk steps of a wave's 32 BM / 64 rows and 32 NJ columns (from row `brow0` of the tile's B)
+template <int BM, int S, int NJ, bool TAIL>
+__device__ __forceinline__ void ring_products(f16v (&acc)[BM / 64][NJ], const unsigned char* smem, int stage, int brow0, int nk, int lane, int wm,
+                                              int krest) {
+  constexpr int MI = BM / 64, KG = MI * NJ >= 6 ? 2 : 4;
+#pragma unroll
+  for (int i = 0; i < MI; i++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[i][j][v] = 0.f;
+  const unsigned char* as = smem;
+  for (int k = 0; k < nk; k++) {
+    step_barrier();
+    const unsigned char* bs = as + BM * 128;
+#pragma unroll
+    for (int kh = 0; kh < 4; kh += KG) {
+      h8 fa[KG][MI], fb[KG][NJ];
+#pragma unroll
+      for (int kb = 0; kb < KG; kb++) {
+        const int q = (kh + kb) * 2 + (lane >> 5);
+#pragma unroll
+        for (int i = 0; i < MI; i++) fa[kb][i] = *reinterpret_cast<const h8*>(as + ldw_at(wm * (BM / 2) + i * 32 + (lane & 31), q));
+#pragma unroll
+        for (int j = 0; j < NJ; j++) fb[kb][j] = *reinterpret_cast<const h8*>(bs + ldw_at(brow0 + j * 32 + (lane & 31), q));
+        if constexpr (TAIL) {
+          if (k == nk - 1) {
+            const h8 none = (h8)(h1)0.f;
+#pragma unroll
+            for (int i = 0; i < MI; i++) fa[kb][i] = q * 8 < krest ? fa[kb][i] : none;
+#pragma unroll
+            for (int j = 0; j < NJ; j++) fb[kb][j] = q * 8 < krest ? fb[kb][j] : none;
+          }
+        }
+      }
+#pragma unroll
+      for (int kb = 0; kb < KG; kb++)
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+          for (int j = 0; j < NJ; j++)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[kb][i], fb[kb][j], acc[i][j], 0, 0, 0);
+    }
+    as += stage;
+    as = as == smem + S * stage ? smem : as;
+  }
+}
+
+template <int BM, int S, int NJ, bool TAIL>
+__device__ __forceinline__ void linear_mma(unsigned char* smem, int stage, int maxw, int brow0, int nk, int krest, int lane, int wm) {
+  if constexpr (NJ == 0) {  // a tile of one block: the first wave column has it
+    for (int k = 0; k < nk; k++) step_barrier();
+    step_barrier();
+  } else {
+    f16v acc[BM / 64][NJ];
+    ring_products<BM, S, NJ, TAIL>(acc, smem, stage, brow0, nk, lane, wm, krest);
+    step_barrier();  // all fragments have been read
+    const int pitch = sums_pitch(maxw);
+#pragma unroll
+    for (int i = 0; i < BM / 64; i++) sums_to_lds(acc[i], reinterpret_cast<float*>(smem) + (wm * (BM / 2) + i * 32) * pitch + brow0, pitch, lane);
+  }
+}
+
+template <int BM, int S, bool TAIL, class O>
+__global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearTiles a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char ring_smem[];
+  constexpr int kMost = BM == 128 && S == 4 ? 6 : kRingMostBlocks;
+  int bx, by;
+  xcd_tile(bx, by);
+  const int width = a.base + (bx < a.wide ? 1 : 0), n0 = (bx * a.base + min(bx, a.wide)) * 32, m0 = by * BM;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nk = (a.l.K + kLdwBK - 1) / kLdwBK, krest = a.l.K - (nk - 1) * kLdwBK, stage = BM * 128 + a.maxw * 4096;
+  if (wave >= 4) {
+    const int p = wave - 4;
+    const RingOperands o = {a.l.x, a.l.w, a.l.T, a.l.N, a.l.ldx, a.l.K};
+    switch (width) {
+      case 1: ring_loader<BM, S, 1, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      case 2: ring_loader<BM, S, 2, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      case 3: ring_loader<BM, S, 3, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      case 4: ring_loader<BM, S, 4, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      case 5: ring_loader<BM, S, 5, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      case 6: ring_loader<BM, S, 6, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      case 7: ring_loader<BM, S, kMost < 7 ? kMost : 7, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+      default: ring_loader<BM, S, kMost, TAIL>(o, ring_smem, stage, p, m0, n0, 0, nk, lane, krest); break;
+    }
+    step_barrier();
+  } else {
+    const int wm = wave >> 1, nj0 = (width + 1) >> 1, nj = (wave & 1) ? width - nj0 : nj0, brow0 = (wave & 1) ? nj0 * 32 : 0;
+    switch (nj) {  // every wave passes the same barriers, whatever its width
+      case 0: linear_mma<BM, S, 0, TAIL>(ring_smem, stage, a.maxw, brow0, nk, krest, lane, wm); break;
+      case 1: linear_mma<BM, S, 1, TAIL>(ring_smem, stage, a.maxw, brow0, nk, krest, lane, wm); break;
+      case 2: linear_mma<BM, S, 2, TAIL>(ring_smem, stage, a.maxw, brow0, nk, krest, lane, wm); break;
+      case 3: linear_mma<BM, S, 3, TAIL>(ring_smem, stage, a.maxw, brow0, nk, krest, lane, wm); break;
+      default: linear_mma<BM, S, kMost / 2, TAIL>(ring_smem, stage, a.maxw, brow0, nk, krest, lane, wm); break;
+    }
+  }
+  __syncthreads();
+  const float* const sums = reinterpret_cast<const float*>(ring_smem);
+  const int pitch = sums_pitch(a.maxw), groups = width * 4;  // of 8 outputs
+  for (int i = threadIdx.x; i < BM * groups; i += kRingThreads) {
+    const int row = i / groups, col = (i - row * groups) * 8;
+    if (m0 + row >= a.l.T || n0 + col >= a.l.N) continue;
+    float s[8];
+    read_sums(s, sums + row * pitch + col);
+    finish_outputs<O>(a.l, s, m0 + row, n0 + col, a.l.N - n0 - col);
+  }
+}
+
+template <int BM, int S, bool TAIL, class O>
+static void ring_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st) {
+  static const bool raised = [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_ring_kernel<BM, S, TAIL, O>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    return true;
+  }();
+  (void)raised;
+  const int ring = S * (BM * 128 + t.maxw * 4096), sums = BM * sums_pitch(t.maxw) * 4;
+  hipLaunchKernelGGL((linear_ring_kernel<BM, S, TAIL, O>), p.grid, dim3(kRingThreads), ring > sums ? ring : sums, st, t);
+}
+
+// The cut of such a launch is that of the same product on gemm_ring_kernel; rows = 0: operands whose rows are too long for its offsets
+static TilePlan plan_tiles(const LinearArgs& a) {
+  GemmArgs g;
+  memset(&g, 0, sizeof(g));
+  if (a.K > INT_MAX - kLdwBK || (size_t)a.ldx * 2 * 256 > 0xffffffffull) return TilePlan();
+  g.M = a.T;
+  g.K = (a.K + kLdwBK - 1) / kLdwBK * kLdwBK;
+  g.nseg = 1;
+  g.seg[0].N = a.N;
+  return plan_ring(g, compute_units());
+}
+
+template <bool TAIL, class O>
+static int launch_tiles(const LinearArgs& a, const TilePlan& p, hipStream_t st) {
+  const LinearTiles t = {a, p.a.vw_base[0], p.a.vw_wide[0], p.a.vw_maxw};
+  if (p.rows == 64) ring_launch<64, 4, TAIL, O>(p, t, st);
+  else if (ring_stages(128, t.maxw) == 4) ring_launch<128, 4, TAIL, O>(p, t, st);
+  else ring_launch<128, 3, TAIL, O>(p, t, st);
+  return check_launch("linear");
+}
+
+constexpr int kLinFewRows = 64;  // rows up to which a product goes out as one of few rows
+
 template <bool U8, class O>
 static int linear_run(const LinearArgs& a, hipStream_t st) {
   if (a.T <= 16) few_launch<1, 1, U8, O>(a, st);
@@ -207,14 +358,28 @@ static int linear_run(const LinearArgs& a, hipStream_t st) {
   return check_launch("linear");
 }
 
+template <class O>
+static int linear_any(LinearArgs a, bool u8, void* workspace, hipStream_t st) {
+  if (a.T > kLinFewRows) {
+    const TilePlan p = plan_tiles(a);
+    if (p.rows) {
+      if (u8) {
+        if (int rc = dequant_u8_async(a.w, a.mx, a.rx, a.my, a.ry, static_cast<h1*>(workspace), a.K, a.N, st)) return rc;
+        a.w = static_cast<const unsigned char*>(workspace);
+      }
+      return a.K % kLdwBK ? launch_tiles<true, O>(a, p, st) : launch_tiles<false, O>(a, p, st);
+    }
+  }
+  return u8 ? linear_run<true, O>(a, st) : linear_run<false, O>(a, st);
+}
+
 }  // namespace frhip
 
 using namespace frhip;
 
 extern "C" size_t frhip_linear_workspace_bytes(int T, const frhip_weight* w) {
-  (void)T;
-  (void)w;
-  return 0;
+  if (!w || T <= kLinFewRows || w->dtype != FRHIP_U8 || w->K <= 0 || w->N <= 0) return 0;
+  return ((size_t)w->K * w->N * 2 + 255) / 256 * 256;  // the weight in binary16
 }
 
 extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const float* bias, int act, const void* residual, int ldr, void* y,
@@ -224,7 +389,7 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   if (act != FRHIP_ACT_NONE && (act < FRHIP_ACT_SIGMOID || act > FRHIP_ACT_SOFTPLUS)) return set_error(FRHIP_EINVAL, "linear: unknown act");
   if (w->dtype != FRHIP_F16 && w->dtype != FRHIP_U8) return set_error(FRHIP_EINVAL, "linear: weight dtype must be F16 or U8");
   if (w->dtype == FRHIP_U8 && (!w->mx || !w->rx || !w->my || !w->ry)) return set_error(FRHIP_EINVAL, "linear: uint8 weight without mx/rx/my/ry");
-  if (T < 0 || w->K <= 0 || w->N <= 0 || w->K % 8 != 0) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T not negative");
+  if (T < 0 || T > 1 << 30 || w->K <= 0 || w->N <= 0 || w->K % 8 != 0) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T 0 to 2^30");
   if (ldx < w->K || ldx % 8 != 0 || ldy < w->N || (residual && ldr < w->N)) return set_error(FRHIP_ESHAPE, "linear: rows closer than their elements, or ldx no multiple of 8");
   if (T == 0) return 0;
   if (!x || !y) return set_error(FRHIP_EINVAL, "linear: null pointer");
@@ -259,7 +424,10 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   a.ldy = ldy;
   a.act = act;
   hipStream_t st = static_cast<hipStream_t>(s);
-  (void)workspace;
-  if (w->dtype == FRHIP_U8) return out_dtype == FRHIP_F16 ? linear_run<true, h1>(a, st) : linear_run<true, float>(a, st);
-  return out_dtype == FRHIP_F16 ? linear_run<false, h1>(a, st) : linear_run<false, float>(a, st);
+  const bool u8 = w->dtype == FRHIP_U8;
+  if (frhip_linear_workspace_bytes(T, w) > 0) {
+    if (!workspace) return set_error(FRHIP_EINVAL, "linear: null workspace");
+    if (off_grid(16, {workspace})) return set_error(FRHIP_EINVAL, "linear: workspace must be 16-byte aligned");
+  }
+  return out_dtype == FRHIP_F16 ? linear_any<h1>(a, u8, workspace, st) : linear_any<float>(a, u8, workspace, st);
 }

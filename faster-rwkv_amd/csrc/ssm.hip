@@ -209,7 +209,7 @@ constexpr int scan_rows(int nw) { return nw == 1 ? 8 : 16; }  // of a block of t
 // The step width's softplus and the gate are so evaluated once a channel and row, not once a wave.  What bounds it is the issue of
 // vector instructions: 4, and an exponential of twice their length, a state and row.  The waves of a SIMD have to be several for that.
 template <class T, int NPL, int NW, bool LOCAL>
-__global__ __launch_bounds__(scan_waves(NW) * 64, 4) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
+__global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
   constexpr int WAVES = scan_waves(NW), CW = WAVES / NW, NT = NPL * NW, TB = scan_rows(NW), CH = CW * 64;
   constexpr int ROWS = TB * CW / WAVES;                                  // rows of a wave in A and C: of its 64 channels
   constexpr int STAGE = (TB * 2 * NT + WAVES * 64 - 1) / (WAVES * 64);  // elements of B and C of a thread
