@@ -4,6 +4,7 @@
 #include <cstring>
 
 #include "activations.h"
+#include "gemm_few_device.h"
 #include "gemm_ring_device.h"
 #include "spans.h"
 
@@ -18,7 +19,9 @@ struct LinearArgs {
   const float* bias;
   const void* res;
   void* y;
-  int T, K, N, ldx, ldr, ldy, act, strips;
+  int T, K, N, ldx, ldr, ldy, act;
+  int out32;   // type of y and the residual
+  int strips;  // linear_few_kernel: strips of rows
 };
 
 template <bool FINE>
@@ -35,7 +38,7 @@ __device__ __forceinline__ float activate(float v, int act) {
 
 // W consecutive outputs of a row, the first n of them stored; O: the type of y and the residual
 template <class O, int W>
-__device__ __forceinline__ void finish_outputs(const LinearArgs& a, const float (&acc)[W], int row, int col, int n) {
+__device__ __forceinline__ void finish_as(const LinearArgs& a, const float (&acc)[W], int row, int col, int n) {
   typedef O any __attribute__((ext_vector_type(W), aligned(sizeof(O))));
   constexpr bool FINE = sizeof(O) == 4;
   O* const y = static_cast<O*>(a.y) + (size_t)row * a.ldy + col;
@@ -73,130 +76,229 @@ __device__ __forceinline__ void finish_outputs(const LinearArgs& a, const float 
   }
 }
 
-// ---------------------------------------------------------------------------
-// Few rows: what counts is that all compute units pull at the weights.  A workgroup owns MT x 16 rows and NT x 16 columns; its waves take
-// the K-steps in turn and their sums meet in LDS, in wave order.  Operands go from memory to the registers of the lanes that
-// multiply them: a lane of the 16 x 16 x 32 MFMA takes 8 consecutive k, 16 bytes (8 codes of a uint8 weight), kLinDepth steps ahead.
-// ---------------------------------------------------------------------------
-constexpr int kLinWaves = 8, kLinDepth = 4;
+template <int W>
+__device__ __forceinline__ void finish_outputs(const LinearArgs& a, const float (&acc)[W], int row, int col, int n) {
+  if (a.out32) finish_as<float>(a, acc, row, col, n);
+  else finish_as<h1>(a, acc, row, col, n);
+}
 
-template <int MT, int NT, bool U8, class O>
-__global__ __launch_bounds__(kLinWaves * 64) void linear_few_kernel(LinearArgs a) {
-  extern __shared__ __attribute__((aligned(16))) unsigned char lin_smem[];
-  const int n = gridDim.x, lin = blockIdx.x, xcd = lin & 7;  // the strips that share weights share an L2
-  const int id = xcd * (n >> 3) + min(xcd, n & 7) + (lin >> 3), tile = id / a.strips, strip = id - tile * a.strips;
-  const int m0 = strip * (MT * 16), n0 = tile * (NT * 16), K = a.K;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c16 = lane & 15, grp = lane >> 4;
+// ---------------------------------------------------------------------------
+// A few rows, one launch, K split over the waves of a workgroup (gemm_few.hip has the form, its reasons and its choice of tiles), here with
+// rows of any pitch, any N, and a K that need not fill its last step (a multiple of 8, of uint8 codes 16): the last step's loads of
+// what is not there repeat the step's begin, and what they bring counts as zero.
+// ---------------------------------------------------------------------------
+template <int MT, int NT, bool U8>
+__global__ __launch_bounds__(few_waves(MT, NT) * 64) void linear_few_kernel(LinearArgs a) {
+  constexpr int NW = few_waves(MT, NT), S = few_stages(MT, NT, U8), kStage = few_stage_bytes(MT, NT, U8);
+  constexpr int kBOff = MT * 2048, kScaleOff = kBOff + NT * (U8 ? 1024 : 2048);
+  constexpr int kPer = 2 * MT + (U8 ? NT + 1 : 2 * NT);  // load instructions per step
+  static_assert(S >= 2 && (S - 1) * kPer <= 63, "the wait counter's range");
+  extern __shared__ __attribute__((aligned(16))) unsigned char few_smem[];
 
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-  const h1* xp[MT];
-  const unsigned char* wp[NT];
-  float c[NT], m[NT];
+  // tiles are dealt to the XCDs in contiguous runs, strips of rows fastest: the strips that share weights share an L2
+  const int n = gridDim.x, strips = a.strips, lin = blockIdx.x, xcd = lin & 7;
+  const int id = xcd * (n >> 3) + min(xcd, n & 7) + (lin >> 3);
+  const int tile = id / strips, strip = id - tile * strips;
+  const int M = a.T, K = a.K, N = a.N, n0 = tile * (NT * 16), m0 = strip * (MT * 16);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row16 = lane & 15, grp = lane >> 4;
+
+  unsigned char* const ring = few_smem + wave * few_wave_bytes(MT, NT, U8);
+  const unsigned ring_lds = (unsigned)(size_t)((__attribute__((address_space(3))) unsigned char*)few_smem) + wave * few_wave_bytes(MT, NT, U8);
+
+  // ---- this wave's loads; rows past the matrix repeat its last row and are never stored ----
+  const int lr = lane >> 3;
+  unsigned va[2 * MT], vb[U8 ? NT : 2 * NT];
 #pragma unroll
-  for (int i = 0; i < MT; i++) xp[i] = a.x + (size_t)min(m0 + i * 16 + c16, a.T - 1) * a.ldx + grp * 8;
+  for (int b = 0; b < 2 * MT; b++) {
+    const int row = min(m0 + b * 8 + lr, M - 1) - m0;
+    va[b] = (unsigned)row * (unsigned)(a.ldx * 2) + (((lane & 7) ^ lr ^ (b & 1)) * 16);
+  }
+  if constexpr (U8) {
 #pragma unroll
-  for (int j = 0; j < NT; j++) {
-    const int col = min(n0 + j * 16 + c16, a.N - 1);
-    wp[j] = a.w + ((size_t)col * K + grp * 8) * (U8 ? 1 : 2);
-    if constexpr (U8) {
-      c[j] = dequant_c(a.rx[col]);
-      m[j] = (float)a.mx[col];
+    for (int b = 0; b < NT; b++) {
+      const int col = min(n0 + b * 16 + (lane >> 2), N - 1) - n0;
+      vb[b] = (unsigned)col * (unsigned)K + (((lane & 3) ^ (lane >> 4)) * 16);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < 2 * NT; b++) {
+      const int col = min(n0 + b * 8 + lr, N - 1) - n0;
+      vb[b] = (unsigned)col * (unsigned)(K * 2) + (((lane & 7) ^ lr ^ (b & 1)) * 16);
     }
   }
+  const unsigned char* const abase = uniform_ptr(reinterpret_cast<const unsigned char*>(a.x) + (size_t)m0 * a.ldx * 2);
+  const unsigned char* const bbase = uniform_ptr(a.w + (size_t)n0 * K * (U8 ? 1 : 2));
+  const h1* scale_k = nullptr;  // uint8: lanes 0..31 bring ry, lanes 32..63 my, two values each
+  if constexpr (U8) scale_k = (lane < 32 ? a.ry : a.my) + (lane & 31) * 2;
+  const int nk = (K + 63) >> 6, krest = K - (nk - 1) * 64, mine = wave < nk ? (nk - wave + NW - 1) / NW : 0;
+  auto issue = [&](int i) {
+    const int k0 = (wave + i * NW) * 64;
+    const unsigned st = ring_lds + (i % S) * kStage;
+    const unsigned char* ak = abase + (size_t)k0 * 2;
+    const unsigned char* bk = bbase + (size_t)k0 * (U8 ? 1 : 2);
+    if (k0 + 64 > K) {  // once, and the wave's last: back to the step's begin with the k-segments that are not there
+#pragma unroll
+      for (int b = 0; b < 2 * MT; b++) {
+        const unsigned seg = (lane & 7) ^ lr ^ (b & 1);
+        if ((int)seg * 8 >= krest) va[b] -= seg * 16;
+      }
+#pragma unroll
+      for (int b = 0; b < (U8 ? NT : 2 * NT); b++) {
+        const unsigned seg = U8 ? (lane & 3) ^ (lane >> 4) : (lane & 7) ^ lr ^ (b & 1);
+        if ((int)seg * (U8 ? 16 : 8) >= krest) vb[b] -= seg * 16;
+      }
+      if constexpr (U8)
+        if ((lane & 31) * 2 >= krest) scale_k -= (lane & 31) * 2;
+    }
+#pragma unroll
+    for (int b = 0; b < (U8 ? NT : 2 * NT); b++) load_lds_saddr(vb[b], bk, st + kBOff + b * 1024);
+#pragma unroll
+    for (int b = 0; b < 2 * MT; b++) load_lds_saddr(va[b], ak, st + b * 1024);
+    if constexpr (U8) load_lds_dword(scale_k + k0, st + kScaleOff);
+  };
+  if constexpr (U8) {  // rx, mx of this workgroup's columns, two a lane
+    static_assert(NT * 16 <= 128, "two columns a lane");
+    h1* const sc = reinterpret_cast<h1*>(ring + S * kStage);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int c = min(n0 + lane * 2 + e, N - 1);
+      sc[lane * 2 + e] = a.rx[c];
+      sc[128 + lane * 2 + e] = a.mx[c];
+    }
+    lanes_in_order();
+  }
+#pragma unroll
+  for (int i = 0; i < S; i++)
+    if (i < mine) issue(i);
+
   f4v acc[MT][NT];
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int j = 0; j < NT; j++) acc[i][j] = (f4v){0.f, 0.f, 0.f, 0.f};
-
-  struct Step {
-    h8 x[MT], w[U8 ? 1 : NT], ry, my;
-    u32x2 q[U8 ? NT : 1];
+  // loads complete in order: a step has landed when at most the loads of the steps behind it are outstanding
+  auto landed = [&](int behind) {
+    if (behind >= S - 1) wait_loads<(S - 1) * kPer>();
+    else if (S > 3 && behind == 2) wait_loads<(S > 3 ? 2 : 0) * kPer>();
+    else if (S > 2 && behind == 1) wait_loads<(S > 2 ? 1 : 0) * kPer>();
+    else wait_loads<0>();
   };
-  auto load = [&](Step& s, int k) {  // k: a multiple of 32; this lane's eight begin at k + 8 grp
+  float c[NT], m[NT];  // uint8: rx / 255 and mx of the lane's columns
+  if constexpr (U8) {
+    landed(mine - 1);
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      if constexpr (U8) s.q[j] = *reinterpret_cast<const u32x2*>(wp[j] + k);
-      else s.w[j] = *reinterpret_cast<const h8*>(wp[j] + (size_t)k * 2);
+    for (int t = 0; t < NT; t++) {
+      const h1* sc = reinterpret_cast<const h1*>(ring + S * kStage) + t * 16 + row16;
+      c[t] = dequant_c(sc[0]);
+      m[t] = (float)sc[128];
     }
+  }
+  for (int i = 0; i < mine; i++) {
+    landed(mine - 1 - i);
+    const unsigned char* st = ring + (i % S) * kStage;
+    h8 xa[2][MT], wb[2][NT];
+#pragma unroll
+    for (int t = 0; t < MT; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) xa[h][t] = *reinterpret_cast<const h8*>(st + t * 2048 + few_at(row16, 2 * grp + h));
     if constexpr (U8) {
-      s.ry = *reinterpret_cast<const h8_any*>(a.ry + k + grp * 8);
-      s.my = *reinterpret_cast<const h8_any*>(a.my + k + grp * 8);
-    }
+      u32x4 q[NT];
+      h8 ry[2], my[2];
 #pragma unroll
-    for (int i = 0; i < MT; i++) s.x[i] = *reinterpret_cast<const h8*>(xp[i] + k);
-  };
-  auto weight = [&](const Step& s, int j) {
-    if constexpr (U8) {
-      const h2 p0 = few_dequant<0>(s.q[j][0], c[j], m[j], s.ry.s01, s.my.s01), p1 = few_dequant<1>(s.q[j][0], c[j], m[j], s.ry.s23, s.my.s23);
-      const h2 p2 = few_dequant<0>(s.q[j][1], c[j], m[j], s.ry.s45, s.my.s45), p3 = few_dequant<1>(s.q[j][1], c[j], m[j], s.ry.s67, s.my.s67);
-      return (h8){p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
-    } else {
-      return s.w[j];
-    }
-  };
-  auto multiply = [&](const Step& s) {
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-      const h8 w = weight(s, j);
-#pragma unroll
-      for (int i = 0; i < MT; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, s.x[i], acc[i][j], 0, 0, 0);
-    }
-  };
-  const int full = K / 32, cnt = wave < full ? (full - wave - 1) / kLinWaves + 1 : 0;
-  if (cnt > 0) {
-    Step s[kLinDepth];
-    auto at = [&](int i) { return (wave + min(i, cnt - 1) * kLinWaves) * 32; };  // past the last step: the last one again, not multiplied
-#pragma unroll
-    for (int p = 0; p < kLinDepth; p++) load(s[p], at(p));
-    int i = 0;
-    for (; i + kLinDepth < cnt; i += kLinDepth)
-#pragma unroll
-      for (int p = 0; p < kLinDepth; p++) {
-        multiply(s[p]);
-        load(s[p], at(i + kLinDepth + p));
+      for (int h = 0; h < 2; h++) {
+        ry[h] = *reinterpret_cast<const h8*>(st + kScaleOff + grp * 32 + h * 16);
+        my[h] = *reinterpret_cast<const h8*>(st + kScaleOff + 128 + grp * 32 + h * 16);
       }
 #pragma unroll
-    for (int p = 0; p < kLinDepth; p++)
-      if (i + p < cnt) multiply(s[p]);
-  }
-  if (full * 32 < K && wave == full % kLinWaves) {  // what is left of K
-    Step s;
-    memset(&s, 0, sizeof(s));
-    const bool in = full * 32 + grp * 8 < K;
-    if (in) load(s, full * 32);
+      for (int t = 0; t < NT; t++)
+        q[t] = *reinterpret_cast<const u32x4*>(st + kBOff + t * 1024 + row16 * 64 + ((grp ^ (row16 >> 2)) * 16));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+      if (i + S < mine) issue(i + S);
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-      h8 w = weight(s, j);
-      if (!in) w = (h8)(h1)0.f;
+      for (int t = 0; t < NT; t++)
 #pragma unroll
-      for (int i = 0; i < MT; i++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, s.x[i], acc[i][j], 0, 0, 0);
+        for (int h = 0; h < 2; h++) {
+          const uint32_t w0 = q[t][2 * h], w1 = q[t][2 * h + 1];
+          const h2 p0 = few_dequant<0>(w0, c[t], m[t], ry[h].s01, my[h].s01);
+          const h2 p1 = few_dequant<1>(w0, c[t], m[t], ry[h].s23, my[h].s23);
+          const h2 p2 = few_dequant<0>(w1, c[t], m[t], ry[h].s45, my[h].s45);
+          const h2 p3 = few_dequant<1>(w1, c[t], m[t], ry[h].s67, my[h].s67);
+          wb[h][t] = (h8){p0.x, p0.y, p1.x, p1.y, p2.x, p2.y, p3.x, p3.y};
+        }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NT; t++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) wb[h][t] = *reinterpret_cast<const h8*>(st + kBOff + t * 2048 + few_at(row16, 2 * grp + h));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (i + S < mine) issue(i + S);
     }
+    if ((wave + i * NW) * 64 + 64 > K) {
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const bool in = (2 * grp + h) * 8 < krest;
+#pragma unroll
+        for (int t = 0; t < MT; t++) xa[h][t] = in ? xa[h][t] : (h8)(h1)0.f;
+#pragma unroll
+        for (int j = 0; j < NT; j++) wb[h][j] = in ? wb[h][j] : (h8)(h1)0.f;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int t = 0; t < MT; t++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(wb[h][j], xa[h][t], acc[t][j], 0, 0, 0);
   }
-  // a lane's four sums are four consecutive columns of row c16
-  f4v* const sums = reinterpret_cast<f4v*>(lin_smem);
+
+  // ---- the waves' sums meet: each leaves its tiles in its own ring (a tile is 1 KB; MT NT <= 2 S (MT + NT / 2) of them fit) ----
+  static_assert(MT * NT * 1024 <= S * kStage, "the sums fit the ring");
 #pragma unroll
-  for (int i = 0; i < MT; i++)
+  for (int t = 0; t < MT; t++)
 #pragma unroll
-    for (int j = 0; j < NT; j++) sums[((wave * MT + i) * NT + j) * 64 + lane] = acc[i][j];
+    for (int j = 0; j < NT; j++) *reinterpret_cast<f4v*>(ring + ((t * NT + j) * 64 + lane) * 16) = acc[t][j];
   __syncthreads();
-  for (int t = wave; t < MT * NT; t += kLinWaves) {
-    const int i = t / NT, j = t - i * NT, row = m0 + i * 16 + c16, col = n0 + j * 16 + grp * 4;
-    f4v s = sums[t * 64 + lane];
+  for (int t = wave; t < MT * NT; t += NW) {
+    const int i = t / NT, j = t - i * NT;
+    const int r0 = m0 + i * 16, c0 = n0 + j * 16;
+    if (r0 >= M || c0 >= N) continue;
+    const int row = r0 + row16;
+    f4v s = *reinterpret_cast<const f4v*>(few_smem + (t * 64 + lane) * 16);
 #pragma unroll
-    for (int w = 1; w < kLinWaves; w++) s += sums[(w * MT * NT + t) * 64 + lane];
-    if (row < a.T && col < a.N) {
+    for (int w = 1; w < NW; w++) {
+      const f4v p = *reinterpret_cast<const f4v*>(few_smem + w * few_wave_bytes(MT, NT, U8) + (t * 64 + lane) * 16);
+#pragma unroll
+      for (int v = 0; v < 4; v++) s[v] += p[v];
+    }
+    const int col = c0 + grp * 4;
+    if (row < M && col < N) {
       const float v[4] = {s[0], s[1], s[2], s[3]};
-      finish_outputs<O>(a, v, row, col, a.N - col);
+      finish_outputs(a, v, row, col, N - col);
     }
   }
 }
 
-template <int MT, int NT, bool U8, class O>
-static void few_launch(LinearArgs a, hipStream_t st) {
-  a.strips = (a.T + MT * 16 - 1) / (MT * 16);
-  const int tiles = (a.N + NT * 16 - 1) / (NT * 16);
-  hipLaunchKernelGGL((linear_few_kernel<MT, NT, U8, O>), dim3((unsigned)((size_t)tiles * a.strips)), dim3(kLinWaves * 64), kLinWaves * MT * NT * 1024, st, a);
+template <int MT, int NT, bool U8>
+static void few_launch(const LinearArgs& a, hipStream_t st) {
+  constexpr size_t lds = (size_t)few_waves(MT, NT) * few_wave_bytes(MT, NT, U8);
+  static const bool raised = [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_few_kernel<MT, NT, U8>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    return true;
+  }();
+  (void)raised;
+  const unsigned grid = (unsigned)((a.N + NT * 16 - 1) / (NT * 16)) * a.strips;
+  hipLaunchKernelGGL((linear_few_kernel<MT, NT, U8>), dim3(grid), dim3(few_waves(MT, NT) * 64), lds, st, a);
+}
+
+template <bool U8>
+static int launch_few(LinearArgs a, const FewPlan& p, hipStream_t st) {
+  a.strips = (a.T + 16 * p.mt - 1) / (16 * p.mt);
+#define FR_FEW_GO(MT_, NT_) \
+  if (p.mt == MT_ && p.nt == NT_) few_launch<MT_, NT_, U8>(a, st);
+  FR_FEW_TILES(FR_FEW_GO)
+#undef FR_FEW_GO
+  return check_launch("linear");
 }
 
 // ---------------------------------------------------------------------------
@@ -271,7 +373,7 @@ __device__ __forceinline__ void linear_mma(unsigned char* smem, int stage, int m
   }
 }
 
-template <int BM, int S, bool TAIL, class O>
+template <int BM, int S, bool TAIL>
 __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearTiles a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char ring_smem[];
   constexpr int kMost = BM == 128 && S == 4 ? 6 : kRingMostBlocks;
@@ -312,65 +414,66 @@ __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearTiles a
     if (m0 + row >= a.l.T || n0 + col >= a.l.N) continue;
     float s[8];
     read_sums(s, sums + row * pitch + col);
-    finish_outputs<O>(a.l, s, m0 + row, n0 + col, a.l.N - n0 - col);
+    finish_outputs(a.l, s, m0 + row, n0 + col, a.l.N - n0 - col);
   }
 }
 
-template <int BM, int S, bool TAIL, class O>
+template <int BM, int S, bool TAIL>
 static void ring_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st) {
   static const bool raised = [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_ring_kernel<BM, S, TAIL, O>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_ring_kernel<BM, S, TAIL>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
     return true;
   }();
   (void)raised;
   const int ring = S * (BM * 128 + t.maxw * 4096), sums = BM * sums_pitch(t.maxw) * 4;
-  hipLaunchKernelGGL((linear_ring_kernel<BM, S, TAIL, O>), p.grid, dim3(kRingThreads), ring > sums ? ring : sums, st, t);
+  hipLaunchKernelGGL((linear_ring_kernel<BM, S, TAIL>), p.grid, dim3(kRingThreads), ring > sums ? ring : sums, st, t);
 }
 
-// The cut of such a launch is that of the same product on gemm_ring_kernel; rows = 0: operands whose rows are too long for its offsets
-static TilePlan plan_tiles(const LinearArgs& a) {
-  GemmArgs g;
-  memset(&g, 0, sizeof(g));
-  if (a.K > INT_MAX - kLdwBK || (size_t)a.ldx * 2 * 256 > 0xffffffffull) return TilePlan();
-  g.M = a.T;
-  g.K = (a.K + kLdwBK - 1) / kLdwBK * kLdwBK;
-  g.nseg = 1;
-  g.seg[0].N = a.N;
-  return plan_ring(g, compute_units());
-}
-
-template <bool TAIL, class O>
+template <bool TAIL>
 static int launch_tiles(const LinearArgs& a, const TilePlan& p, hipStream_t st) {
   const LinearTiles t = {a, p.a.vw_base[0], p.a.vw_wide[0], p.a.vw_maxw};
-  if (p.rows == 64) ring_launch<64, 4, TAIL, O>(p, t, st);
-  else if (ring_stages(128, t.maxw) == 4) ring_launch<128, 4, TAIL, O>(p, t, st);
-  else ring_launch<128, 3, TAIL, O>(p, t, st);
+  if (p.rows == 64) ring_launch<64, 4, TAIL>(p, t, st);
+  else if (ring_stages(128, t.maxw) == 4) ring_launch<128, 4, TAIL>(p, t, st);
+  else ring_launch<128, 3, TAIL>(p, t, st);
   return check_launch("linear");
 }
 
-constexpr int kLinFewRows = 64;  // rows up to which a product goes out as one of few rows
+constexpr int kLinearMostK = 8388544;  // whole steps of it keep 256 rows of a tile within 32-bit byte offsets
 
-template <bool U8, class O>
-static int linear_run(const LinearArgs& a, hipStream_t st) {
-  if (a.T <= 16) few_launch<1, 1, U8, O>(a, st);
-  else if (a.T <= 32) few_launch<2, 1, U8, O>(a, st);
-  else few_launch<4, 2, U8, O>(a, st);
-  return check_launch("linear");
+// How a product goes out: the forms and cuts of the same product (K and N rounded up to whole steps and blocks) without a
+// residual on the framework's other kernels, by the same expected times.  A pure function of the sizes.
+struct LinearPlan {
+  FewPlan few;
+  TilePlan tiles;
+};
+static LinearPlan plan_linear(int T, int K, int N, int cus) {
+  GemmArgs g;
+  memset(&g, 0, sizeof(g));
+  g.M = T;
+  g.K = (K + kLdwBK - 1) / kLdwBK * kLdwBK;
+  g.nseg = 1;
+  g.seg[0].N = (N + 15) / 16 * 16;
+  LinearPlan p;
+  p.few = plan_few(g, cus);
+  g.seg[0].N = N;
+  p.tiles = plan_ring(g, cus);
+  if (p.few.mt && p.tiles.rows && p.tiles.us < p.few.us) p.few.mt = 0;
+  return p;
 }
+// uint8 codes are dequantised by the lanes that multiply them, if there are few rows; otherwise, and where their rows are not whole
+// 16 bytes, they are expanded to binary16 first.
+static bool expands(const LinearPlan& p, int K) { return !p.few.mt || K % 16 != 0; }
 
-template <class O>
-static int linear_any(LinearArgs a, bool u8, void* workspace, hipStream_t st) {
-  if (a.T > kLinFewRows) {
-    const TilePlan p = plan_tiles(a);
-    if (p.rows) {
-      if (u8) {
-        if (int rc = dequant_u8_async(a.w, a.mx, a.rx, a.my, a.ry, static_cast<h1*>(workspace), a.K, a.N, st)) return rc;
-        a.w = static_cast<const unsigned char*>(workspace);
-      }
-      return a.K % kLdwBK ? launch_tiles<true, O>(a, p, st) : launch_tiles<false, O>(a, p, st);
-    }
+static int launch_linear(LinearArgs a, bool u8, void* workspace, hipStream_t st) {
+  const LinearPlan p = plan_linear(a.T, a.K, a.N, compute_units());
+  if (!p.few.mt && !p.tiles.rows) return set_error(FRHIP_ESHAPE, "linear: no tiles for this shape");
+  if (u8 && expands(p, a.K)) {
+    if (int rc = dequant_u8_async(a.w, a.mx, a.rx, a.my, a.ry, static_cast<h1*>(workspace), a.K, a.N, st)) return rc;
+    a.w = static_cast<const unsigned char*>(workspace);
+    u8 = false;
   }
-  return u8 ? linear_run<true, O>(a, st) : linear_run<false, O>(a, st);
+  if (p.few.mt) return u8 ? launch_few<true>(a, p.few, st) : launch_few<false>(a, p.few, st);
+  return a.K % kLdwBK ? launch_tiles<true>(a, p.tiles, st) : launch_tiles<false>(a, p.tiles, st);
 }
 
 }  // namespace frhip
@@ -378,7 +481,8 @@ static int linear_any(LinearArgs a, bool u8, void* workspace, hipStream_t st) {
 using namespace frhip;
 
 extern "C" size_t frhip_linear_workspace_bytes(int T, const frhip_weight* w) {
-  if (!w || T <= kLinFewRows || w->dtype != FRHIP_U8 || w->K <= 0 || w->N <= 0) return 0;
+  if (!w || T <= 0 || w->dtype != FRHIP_U8 || w->K <= 0 || w->K > kLinearMostK || w->N <= 0 || !expands(plan_linear(T, w->K, w->N, compute_units()), w->K))
+    return 0;
   return ((size_t)w->K * w->N * 2 + 255) / 256 * 256;  // the weight in binary16
 }
 
@@ -389,12 +493,13 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   if (act != FRHIP_ACT_NONE && (act < FRHIP_ACT_SIGMOID || act > FRHIP_ACT_SOFTPLUS)) return set_error(FRHIP_EINVAL, "linear: unknown act");
   if (w->dtype != FRHIP_F16 && w->dtype != FRHIP_U8) return set_error(FRHIP_EINVAL, "linear: weight dtype must be F16 or U8");
   if (w->dtype == FRHIP_U8 && (!w->mx || !w->rx || !w->my || !w->ry)) return set_error(FRHIP_EINVAL, "linear: uint8 weight without mx/rx/my/ry");
-  if (T < 0 || T > 1 << 30 || w->K <= 0 || w->N <= 0 || w->K % 8 != 0) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T 0 to 2^30");
+  if (T < 0 || T > 1 << 30 || w->K <= 0 || w->K > kLinearMostK || ldx > kLinearMostK || w->N <= 0 || w->N > 1 << 30 || w->K % 8 != 0) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T and N at most 2^30, rows at most 8388544 elements apart");
   if (ldx < w->K || ldx % 8 != 0 || ldy < w->N || (residual && ldr < w->N)) return set_error(FRHIP_ESHAPE, "linear: rows closer than their elements, or ldx no multiple of 8");
   if (T == 0) return 0;
   if (!x || !y) return set_error(FRHIP_EINVAL, "linear: null pointer");
   const size_t elem = out_dtype == FRHIP_F16 ? 2 : 4, rows = T, K = w->K, N = w->N;
-  if (off_grid(16, {x, w->data}) || off_grid(4, {bias}) || off_grid(elem, {residual, y}) || off_grid(2, {w->mx, w->rx, w->my, w->ry}))
+  if (off_grid(16, {x, w->data}) || off_grid(4, {bias}) || off_grid(elem, {residual, y}) || off_grid(2, {w->mx, w->rx}) ||
+      off_grid(4, {w->my, w->ry}))
     return set_error(FRHIP_EINVAL, "linear: pointer not aligned");
   const size_t ye = ((rows - 1) * ldy + N) * elem;
   auto hits = [&](const void* p, size_t bytes) { return rows_overlap(p, bytes, y, ye, 1, bytes, ye, 1); };
@@ -423,11 +528,12 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   a.ldr = ldr;
   a.ldy = ldy;
   a.act = act;
+  a.out32 = out_dtype == FRHIP_F32;
   hipStream_t st = static_cast<hipStream_t>(s);
   const bool u8 = w->dtype == FRHIP_U8;
   if (frhip_linear_workspace_bytes(T, w) > 0) {
     if (!workspace) return set_error(FRHIP_EINVAL, "linear: null workspace");
     if (off_grid(16, {workspace})) return set_error(FRHIP_EINVAL, "linear: workspace must be 16-byte aligned");
   }
-  return out_dtype == FRHIP_F16 ? linear_any<h1>(a, u8, workspace, st) : linear_any<float>(a, u8, workspace, st);
+  return launch_linear(a, u8, workspace, st);
 }

@@ -358,7 +358,7 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * frhip_gemm_act, which rounds ahead of the activation as the reference does).  x [T] rows of K binary16, ldx elements apart;
  * bias [N] fp32 or NULL; residual [T] rows of N in out_dtype, ldr apart, or NULL; y [T] rows of N in out_dtype (F16 or F32), ldy
  * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
- * K is a multiple of 8, N and T are any; x and w->data are 16-byte aligned and ldx is a multiple of 8, the others lie at
+ * K and ldx are multiples of 8, at most 8388544, N and T are any up to 2^30; x and w->data are 16-byte aligned, w->my and w->ry 4-byte, the others lie at
  * multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
  * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each. */
 #define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */

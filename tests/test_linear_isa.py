@@ -22,4 +22,4 @@ def test_no_fragment_read_of_the_linear_tiles_is_outstanding_at_a_barrier(tmp_pa
                 assert any(t == "s_barrier" for _, t, _ in body) and any("mfma" in t for _, t, _ in body), name
                 assert not reads_outstanding_at_barriers(body), name
                 seen += 1
-    assert seen == 12  # tiles of 64 and 128 rows (two depths), K with and without a rest, two types of output
+    assert seen == 6  # tiles of 64 and 128 rows (two depths), K with and without a rest
