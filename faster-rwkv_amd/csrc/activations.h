@@ -14,20 +14,19 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // -|v| log2(e), which exp2 would scale by |v|, is made good.
 template <bool FINE>
 __device__ __forceinline__ float softplus_f(float v) {
-  const float m = __builtin_fabsf(v), t = m * -kLog2e;
+  const float m = FINE ? __builtin_fminf(__builtin_fabsf(v), 120.f) : __builtin_fabsf(v), t = m * -kLog2e;  // exp(-120) is no fp32 number
   float e = __builtin_amdgcn_exp2f(t);
-  if constexpr (FINE) {
-    // m log2(e) = -t + r, log2(e) = kLog2e + 1.925963033500752e-8
+  if constexpr (FINE) {  // m log2(e) = -t + r, log2(e) = kLog2e + 1.925963033500752e-8
     const float r = __builtin_fmaf(m, 1.925963033500752e-8f, __builtin_fmaf(m, kLog2e, t));
     e = __builtin_fmaf(e, -r * 0.693147180559945f, e);
-    e = m < 80.f ? e : expf(-m);  // beyond, r is no small number of an infinite m, and e is below what exp2 keeps
   }
   const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
   float p = __builtin_fmaf(q, 0.1408732831478119f, 0.1398070901632309f);
   p = __builtin_fmaf(p, q, 0.20012426376342773f);
   p = __builtin_fmaf(p, q, 0.3333315849304199f);
   p = __builtin_fmaf(p, q, 1.0f);
-  return __builtin_fmaxf(v, 0.f) + 2.0f * s * p;  // a NaN stays one through s
+  const float y = __builtin_fmaf(2.0f * s, p, __builtin_fmaxf(v, 0.f));
+  return v == v ? y : v;
 }
 
 // FINE: for results that stay fp32; otherwise within a few units of the instructions for exp2 and the reciprocal, far below what the

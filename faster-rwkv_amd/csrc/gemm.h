@@ -95,6 +95,8 @@ struct TilePlan {
 // binary16 weights, four loading waves (gemm_ring.hip)
 TilePlan plan_ring(const GemmArgs& a, int cus);
 int launch_gemm_ring(const TilePlan& p, hipStream_t st, const char* what);
+// binary16 weights, 256 rows, gemm_vw256_kernel's form (gemm.hip)
+TilePlan plan_256(const GemmArgs& a, int cus);
 // uint8 weights whose codes are dequantised on their way into LDS (gemm_q8.hip)
 TilePlan plan_q8(const GemmArgs& a, int cus);
 bool q8_takes(const GemmArgs& a);

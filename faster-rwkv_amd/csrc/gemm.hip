@@ -646,6 +646,18 @@ static GemmRoute plan_vw(const GemmArgs& args, int bm, int cus) {
   return r;
 }
 
+TilePlan plan_256(const GemmArgs& args, int cus) {
+  TilePlan p;
+  const GemmRoute r = plan_vw(args, 256, cus);
+  if (!r.rows) return p;
+  p.rows = 256;
+  p.rounds = r.rounds;
+  p.us = us_256(r.rounds, args.K / 2048.0, r.blocks);
+  p.grid = r.grid;
+  p.a = r.a;
+  return p;
+}
+
 // The cheapest cut.  rows stays 0 where the planned tiles do not fit and fixed 64-row tiles take more than a round.
 static GemmRoute gemm_route(const GemmArgs& a, int cus) {
   GemmRoute r = plan_vw(a, 128, cus);

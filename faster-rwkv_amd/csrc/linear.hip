@@ -57,8 +57,20 @@ __device__ __forceinline__ void finish_as(const LinearArgs& a, const float (&acc
         if (i < n) r[i] = (float)res[i];
     }
   }
+  if (a.bias) {
+    typedef float anyf __attribute__((ext_vector_type(W), aligned(4)));
+    if (n >= W) {
+      const anyf t = *reinterpret_cast<const anyf*>(a.bias + col);
 #pragma unroll
-  for (int i = 0; i < W; i++) v[i] = acc[i] + (a.bias && i < n ? a.bias[col + i] : 0.f);
+      for (int i = 0; i < W; i++) v[i] = acc[i] + t[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; i++) v[i] = i < n ? acc[i] + a.bias[col + i] : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i++) v[i] = acc[i];
+  }
 #pragma unroll
   for (int i = 0; i < W; i++) {
     v[i] = activate<FINE>(v[i], a.act);
@@ -80,6 +92,89 @@ template <int W>
 __device__ __forceinline__ void finish_outputs(const LinearArgs& a, const float (&acc)[W], int row, int col, int n) {
   if (a.out32) finish_as<float>(a, acc, row, col, n);
   else finish_as<h1>(a, acc, row, col, n);
+}
+
+// ---------------------------------------------------------------------------
+// One or two rows: a wave streams COLS consecutive rows of the weight, 16 bytes a lane and load, and multiplies them with its lanes'
+// pieces of x, which stay in registers (lane l has the 8 k of chunks l, l + 64, ... of a slice of K, of x and of every column alike).
+// Reads beyond a row give zeros (buffer descriptors), so K may end anywhere.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ h8 load_chunk(__amdgpu_buffer_rsrc_t r, int byte) {
+  return __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, 0));
+}
+__device__ __forceinline__ h8 load_chunk_once(__amdgpu_buffer_rsrc_t r, int byte) {
+  return __builtin_bit_cast(h8, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, 2));  // non-temporal
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const void* p, unsigned bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(uniform_ptr(p)), 0, bytes, 0x00020000);
+}
+
+template <int TR, int NCH, int COLS>
+__global__ __launch_bounds__(512) void linear_rows_kernel(LinearArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = (blockIdx.x * 8 + wave) * COLS;
+  if (n0 >= a.N) return;
+  const unsigned bytes = (unsigned)a.K * 2;
+  float acc[TR][COLS];
+#pragma unroll
+  for (int t = 0; t < TR; t++)
+#pragma unroll
+    for (int j = 0; j < COLS; j++) acc[t][j] = 0.f;
+  for (int k = 0; k < a.K; k += NCH * 512) {
+    h8 x[TR][NCH], w[COLS][NCH];
+#pragma unroll
+    for (int t = 0; t < TR; t++) {
+      const auto r = row_rsrc(a.x + (size_t)min(t, a.T - 1) * a.ldx, bytes);
+#pragma unroll
+      for (int i = 0; i < NCH; i++) x[t][i] = load_chunk(r, (k + i * 512 + lane * 8) * 2);
+    }
+#pragma unroll
+    for (int j = 0; j < COLS; j++) {
+      const auto r = row_rsrc(a.w + (size_t)min(n0 + j, a.N - 1) * a.K * 2, n0 + j < a.N ? bytes : 0);
+#pragma unroll
+      for (int i = 0; i < NCH; i++) w[j][i] = load_chunk_once(r, (k + i * 512 + lane * 8) * 2);
+    }
+#pragma unroll
+    for (int j = 0; j < COLS; j++)
+#pragma unroll
+      for (int i = 0; i < NCH; i++)
+#pragma unroll
+        for (int t = 0; t < TR; t++) acc[t][j] = dot8acc(w[j][i], x[t][i], acc[t][j]);
+  }
+  // sum t COLS + j goes to lane t COLS + j, which finishes it
+  float mine = 0.f;
+#pragma unroll
+  for (int t = 0; t < TR; t++)
+#pragma unroll
+    for (int j = 0; j < COLS; j++) {
+      const float s = wave_sum(acc[t][j]);
+      mine = lane == t * COLS + j ? s : mine;
+    }
+  const int t = lane / COLS, col = n0 + lane % COLS;
+  if (t < TR && t < a.T && col < a.N) {
+    const float v[1] = {mine};
+    finish_outputs(a, v, t, col, 1);
+  }
+}
+
+template <int TR, int NCH, int COLS>
+static void rows_launch(const LinearArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((linear_rows_kernel<TR, NCH, COLS>), dim3((unsigned)((a.N + 8 * COLS - 1) / (8 * COLS))), dim3(512), 0, st, a);
+}
+template <int TR, int NCH>
+static void rows_cols(const LinearArgs& a, hipStream_t st) {
+  const int waves = compute_units() * 8;  // as many columns a wave as give every compute unit eight waves, while they fit its registers
+  if (NCH <= 4 && a.N >= 4 * waves) rows_launch<TR, NCH, NCH <= 4 ? 4 : 1>(a, st);
+  else if (a.N >= 2 * waves) rows_launch<TR, NCH, 2>(a, st);
+  else rows_launch<TR, NCH, 1>(a, st);
+}
+template <int TR>
+static int launch_rows(const LinearArgs& a, hipStream_t st) {
+  if (a.K <= 512) rows_cols<TR, 1>(a, st);
+  else if (a.K <= 1024) rows_cols<TR, 2>(a, st);
+  else if (a.K <= 2048) rows_cols<TR, 4>(a, st);
+  else rows_cols<TR, 8>(a, st);
+  return check_launch("linear");
 }
 
 // ---------------------------------------------------------------------------
@@ -429,10 +524,139 @@ static void ring_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st)
   hipLaunchKernelGGL((linear_ring_kernel<BM, S, TAIL>), p.grid, dim3(kRingThreads), ring > sums ? ring : sums, st, t);
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: tiles of 256 rows, eight waves of 64 rows by half the width that load for themselves one step ahead (gemm_vw256_kernel has the
+// form and its reasons); the sums go out through a place in LDS of each wave's own.
+// ---------------------------------------------------------------------------
+constexpr int kWideThreads = 512, kWideMostBlocks = 8, kWideABytes = 256 * kLdwBK * 2;
+static_assert(2 * (kWideABytes + kWideMostBlocks * 4096) <= 160 * 1024 && 8 * wave_sums_bytes((kWideMostBlocks + 1) / 2) <= 160 * 1024, "LDS of a compute unit");
+
+template <int NJ, bool TAIL>
+__device__ __forceinline__ void wide_body(const LinearTiles& a, unsigned char* smem, int width, int brow0, int m0, int n0, int lane, int wave) {
+  const int M = a.l.T, K = a.l.K, N = a.l.N, lda = a.l.ldx, nk = TAIL ? (K + kLdwBK - 1) / kLdwBK : K / kLdwBK, krest = TAIL ? K - (nk - 1) * kLdwBK : kLdwBK;
+  const int wm = wave >> 1, nb = 4 * width;
+  const unsigned stage_bytes = kWideABytes + a.maxw * 4096;
+  // this wave's loads: row groups 4 wave .. + 3 of A, row groups wave, wave + 8, ... of B (there are 4 width)
+  unsigned va[4], vb[4];
+  const int lr = lane >> 3, ls = (lane & 7) ^ lr;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const int ga = wave * 4 + i, gb = wave + 8 * i;
+    va[i] = (unsigned)(min(m0 + ga * 8 + lr, M - 1) - m0) * (unsigned)(lda * 2) + (ls ^ (ga & 1)) * 16;
+    vb[i] = (unsigned)(min(n0 + gb * 8 + lr, N - 1) - n0) * (unsigned)(K * 2) + (ls ^ (gb & 1)) * 16;
+  }
+  const unsigned char* abase = uniform_ptr(reinterpret_cast<const unsigned char*>(a.l.x) + (size_t)m0 * lda * 2);
+  const unsigned char* bbase = uniform_ptr(a.l.w + (size_t)n0 * K * 2);
+  const unsigned lds0 = (unsigned)(size_t)((__attribute__((address_space(3))) unsigned char*)smem);
+  auto issue = [&](int step) {
+    const unsigned st = lds0 + (step & 1) * stage_bytes;
+    const unsigned char* ak = abase + (size_t)step * (kLdwBK * 2);
+    const unsigned char* bk = bbase + (size_t)step * (kLdwBK * 2);
+    if constexpr (TAIL) {
+      if (step == nk - 1) {  // the last loads: what is not there repeats the step's begin
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int sa = ls ^ (i & 1), sb = ls ^ (wave & 1);
+          if (sa * 8 >= krest) va[i] -= sa * 16;
+          if (sb * 8 >= krest) vb[i] -= sb * 16;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) load_lds_saddr(va[i], ak, st + (wave * 4 + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (wave + 8 * i < nb) load_lds_saddr(vb[i], bk, st + kWideABytes + (wave + 8 * i) * 1024);
+  };
+  f16v acc[2][NJ];
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++)
+#pragma unroll
+      for (int v = 0; v < 16; v++) acc[i][j][v] = 0.f;
+  issue(0);
+  for (int k = 0; k < nk; k++) {
+    // this wave's loads of step k have landed and its fragments of step k-1 are in registers; behind the
+    // barrier that holds for all eight, so step k may be read and the slot of step k-1 refilled
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    step_barrier();
+    if (k + 1 < nk) issue(k + 1);
+    const unsigned char* st = smem + (k & 1) * stage_bytes;
+#pragma unroll
+    for (int kb = 0; kb < 4; kb++) {
+      h8 fa[2], fb[NJ];
+      const int q = kb * 2 + (lane >> 5);
+#pragma unroll
+      for (int i = 0; i < 2; i++) fa[i] = *reinterpret_cast<const h8*>(st + ldw_at(wm * 64 + i * 32 + (lane & 31), q));
+#pragma unroll
+      for (int j = 0; j < NJ; j++) fb[j] = *reinterpret_cast<const h8*>(st + kWideABytes + ldw_at(brow0 + j * 32 + (lane & 31), q));
+      if constexpr (TAIL) {
+        if (k == nk - 1) {
+#pragma unroll
+          for (int i = 0; i < 2; i++) fa[i] = q * 8 < krest ? fa[i] : (h8)(h1)0.f;
+#pragma unroll
+          for (int j = 0; j < NJ; j++) fb[j] = q * 8 < krest ? fb[j] : (h8)(h1)0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int j = 0; j < NJ; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
+    }
+  }
+  // the last fragments are in registers (the compiler may leave their wait behind the barrier, with the products), then all waves' are
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  step_barrier();  // all fragments have been read
+  float* const sums = reinterpret_cast<float*>(smem + wave * wave_sums_bytes((a.maxw + 1) / 2));
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    if (i > 0) lanes_in_order();  // the rows before have been read
+    sums_to_lds(acc[i], sums, sums_pitch(NJ), lane);
+    lanes_in_order();
+#pragma unroll 1
+    for (int t = lane; t < 32 * NJ * 4; t += 64) {
+      const int row = t / (NJ * 4), c = (t - row * (NJ * 4)) * 8, m = m0 + wm * 64 + i * 32 + row, col = n0 + brow0 + c;
+      if (m >= M || col >= N) continue;
+      float s[8];
+      read_sums(s, sums + row * sums_pitch(NJ) + c);
+      finish_outputs(a.l, s, m, col, N - col);
+    }
+  }
+}
+
+template <bool TAIL>
+__global__ __launch_bounds__(kWideThreads) void linear_wide_kernel(LinearTiles a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char wide_smem[];
+  int bx, by;
+  xcd_tile(bx, by);
+  const int width = a.base + (bx < a.wide ? 1 : 0), n0 = (bx * a.base + min(bx, a.wide)) * 32, m0 = by * 256;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nj0 = (width + 1) >> 1, nj = (wave & 1) ? width - nj0 : nj0, brow0 = (wave & 1) ? nj0 * 32 : 0;
+  switch (nj) {  // every wave passes the same barriers, whatever its width
+    case 1: wide_body<1, TAIL>(a, wide_smem, width, brow0, m0, n0, lane, wave); break;
+    case 2: wide_body<2, TAIL>(a, wide_smem, width, brow0, m0, n0, lane, wave); break;
+    case 3: wide_body<3, TAIL>(a, wide_smem, width, brow0, m0, n0, lane, wave); break;
+    default: wide_body<4, TAIL>(a, wide_smem, width, brow0, m0, n0, lane, wave); break;
+  }
+}
+
+template <bool TAIL>
+static void wide_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st) {
+  static const bool raised = [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_wide_kernel<TAIL>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    return true;
+  }();
+  (void)raised;
+  const int ring = 2 * (kWideABytes + t.maxw * 4096), sums = 8 * wave_sums_bytes((t.maxw + 1) / 2);
+  hipLaunchKernelGGL(linear_wide_kernel<TAIL>, p.grid, dim3(kWideThreads), ring > sums ? ring : sums, st, t);
+}
+
 template <bool TAIL>
 static int launch_tiles(const LinearArgs& a, const TilePlan& p, hipStream_t st) {
   const LinearTiles t = {a, p.a.vw_base[0], p.a.vw_wide[0], p.a.vw_maxw};
-  if (p.rows == 64) ring_launch<64, 4, TAIL>(p, t, st);
+  if (p.rows == 256) wide_launch<TAIL>(p, t, st);
+  else if (p.rows == 64) ring_launch<64, 4, TAIL>(p, t, st);
   else if (ring_stages(128, t.maxw) == 4) ring_launch<128, 4, TAIL>(p, t, st);
   else ring_launch<128, 3, TAIL>(p, t, st);
   return check_launch("linear");
@@ -457,6 +681,8 @@ static LinearPlan plan_linear(int T, int K, int N, int cus) {
   p.few = plan_few(g, cus);
   g.seg[0].N = N;
   p.tiles = plan_ring(g, cus);
+  const TilePlan wide = plan_256(g, cus);
+  if (wide.rows && (!p.tiles.rows || wide.us <= p.tiles.us * 1.05)) p.tiles = wide;
   if (p.few.mt && p.tiles.rows && p.tiles.us < p.few.us) p.few.mt = 0;
   return p;
 }
@@ -464,7 +690,10 @@ static LinearPlan plan_linear(int T, int K, int N, int cus) {
 // 16 bytes, they are expanded to binary16 first.
 static bool expands(const LinearPlan& p, int K) { return !p.few.mt || K % 16 != 0; }
 
+constexpr int kLinearRows = 2;  // binary16 weights, us: 2 x 4096 x 2048 5.2 in rows, 5.5 as a few rows; 3 and 4 x 2048 x 8192 11.2 and 8.6
+
 static int launch_linear(LinearArgs a, bool u8, void* workspace, hipStream_t st) {
+  if (!u8 && a.T <= kLinearRows) return a.T == 1 ? launch_rows<1>(a, st) : launch_rows<2>(a, st);
   const LinearPlan p = plan_linear(a.T, a.K, a.N, compute_units());
   if (!p.few.mt && !p.tiles.rows) return set_error(FRHIP_ESHAPE, "linear: no tiles for this shape");
   if (u8 && expands(p, a.K)) {

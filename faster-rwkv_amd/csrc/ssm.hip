@@ -47,20 +47,26 @@ struct ConvArgs {
   const float *w, *bias;
   int ldx, ldy, C, silu;
   int nseq, tile;  // conv_seq: rows of a tile
-  int rows, ncv;   // conv_one
+  int rows;        // conv_one
 };
 
 template <class T>
 constexpr int kConvLanes = 16 / sizeof(T);  // channels of a thread
+constexpr int kConvBatch = 8;               // rows that are requested together
 
-// Up to V elements at any address of one, the first n of them; the same instruction as for aligned 16 bytes if there are V
+// Up to V elements at any address of one, the first n of them; 16 bytes an instruction if all are there, as for aligned ones
 template <class T, int V>
 __device__ __forceinline__ void load_group(float (&v)[V], const T* p, int n) {
-  typedef T any __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+  constexpr int P = V < kConvLanes<T> ? V : kConvLanes<T>;
+  typedef T any __attribute__((ext_vector_type(P), aligned(sizeof(T))));
+  static_assert(V % P == 0, "whole pieces");
   if (n >= V) {
-    const any t = *reinterpret_cast<const any*>(p);
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = (float)t[i];
+    for (int q = 0; q < V; q += P) {
+      const any t = *reinterpret_cast<const any*>(p + q);
+#pragma unroll
+      for (int i = 0; i < P; i++) v[q + i] = (float)t[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < V; i++) v[i] = i < n ? (float)p[i] : 0.f;
@@ -86,13 +92,15 @@ struct ConvTaps {
   static constexpr int V = kConvLanes<T>;
   float w[W][V], b[V];
   __device__ __forceinline__ void load(const ConvArgs<T>& a, int c, int n) {
+    float t[V * W];
+    load_group<float, V * W>(t, a.w + (size_t)c * W, n * W);
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const int ci = c + (i < n ? i : 0);
-      b[i] = a.bias ? a.bias[ci] : 0.f;
+      b[i] = 0.f;
 #pragma unroll
-      for (int j = 0; j < W; j++) w[j][i] = a.w[(size_t)ci * W + j];
+      for (int j = 0; j < W; j++) w[j][i] = t[i * W + j];
     }
+    if (a.bias) load_group<float, V>(b, a.bias + c, n);
   }
   // past: the last W rows, oldest first
   __device__ __forceinline__ void apply(const float (&past)[W][V], float (&y)[V], int silu) const {
@@ -106,23 +114,25 @@ struct ConvTaps {
   }
 };
 
+// blockIdx.x: a block of channels; blockIdx.y, and so on by gridDim.y: the sequences
 template <class T, int W>
-__global__ __launch_bounds__(256) void conv_one_kernel(ConvArgs<T> a) {
+__global__ __launch_bounds__(64) void conv_one_kernel(ConvArgs<T> a) {
   constexpr int V = kConvLanes<T>;
-  const size_t item = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int row = (int)(item / a.ncv), c = (int)(item % a.ncv) * V, n = a.C - c;
-  if (row >= a.rows) return;
-  float past[W][V], y[V];
-  const size_t st = (size_t)row * (W - 1) * a.C + c;
-#pragma unroll
-  for (int j = 0; j < W - 1; j++) load_group<T, V>(past[j], a.state + st + (size_t)j * a.C, n);
-  load_group<T, V>(past[W - 1], a.x + (size_t)row * a.ldx + c, n);
+  const int c = (blockIdx.x * 64 + threadIdx.x) * V, n = a.C - c;
+  if (n <= 0) return;
   ConvTaps<T, W> taps;
   taps.load(a, c, n);
-  taps.apply(past, y, a.silu);
-  store_group<T, V>(a.y + (size_t)row * a.ldy + c, y, n);
+  for (int row = blockIdx.y; row < a.rows; row += gridDim.y) {
+    float past[W][V], y[V];
+    const size_t st = (size_t)row * (W - 1) * a.C + c;
 #pragma unroll
-  for (int j = 0; j < W - 1; j++) store_group<T, V>(a.state_out + st + (size_t)j * a.C, past[j + 1], n);
+    for (int j = 0; j < W - 1; j++) load_group<T, V>(past[j], a.state + st + (size_t)j * a.C, n);
+    load_group<T, V>(past[W - 1], a.x + (size_t)row * a.ldx + c, n);
+    taps.apply(past, y, a.silu);
+    store_group<T, V>(a.y + (size_t)row * a.ldy + c, y, n);
+#pragma unroll
+    for (int j = 0; j < W - 1; j++) store_group<T, V>(a.state_out + st + (size_t)j * a.C, past[j + 1], n);
+  }
 }
 
 // blockIdx.x: a tile of rows of one prompt, blockIdx.y: a block of channels.  The threads of a prompt's first tile read its state and
@@ -135,19 +145,15 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvArgs<T> a, SeqTable t
   if (n <= 0) return;
   const int first = tab.start[i], end = tab.start[i + 1], t0 = first + (j0 - tab.chunk[i]) * a.tile;
   const int t1 = end - t0 < a.tile ? end : t0 + a.tile;
+  typedef T group __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   ConvTaps<T, W> taps;
   taps.load(a, c, n);
-  float past[W][V];
-  const T* x = a.x + c;
+  float past[W - 1][V];  // the rows ahead of the next one, oldest first
+  const T* const x = a.x + c;
   if (t0 == first) {
     const size_t st = (size_t)i * (W - 1) * a.C + c;
-    float old[W - 1][V];
 #pragma unroll
-    for (int j = 0; j < W - 1; j++) {
-      load_group<T, V>(old[j], a.state + st + (size_t)j * a.C, n);
-#pragma unroll
-      for (int v = 0; v < V; v++) past[j + 1][v] = old[j][v];
-    }
+    for (int j = 0; j < W - 1; j++) load_group<T, V>(past[j], a.state + st + (size_t)j * a.C, n);
     const int len = end - first;
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {  // the input W - 1 - j tokens ahead of the end, or what the old state holds of it
@@ -160,24 +166,46 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvArgs<T> a, SeqTable t
         for (int k = 0; k < W - 1; k++)
           if (k == j + len) {
 #pragma unroll
-            for (int q = 0; q < V; q++) v[q] = old[k][q];
+            for (int q = 0; q < V; q++) v[q] = past[k][q];
           }
       }
       store_group<T, V>(a.state_out + st + (size_t)j * a.C, v, n);
     }
   } else {  // a tile has W - 1 rows at least
 #pragma unroll
-    for (int j = 1; j < W; j++) load_group<T, V>(past[j], x + (size_t)(t0 - W + j) * a.ldx, n);
+    for (int j = 0; j < W - 1; j++) load_group<T, V>(past[j], x + (size_t)(t0 - (W - 1) + j) * a.ldx, n);
   }
-  for (int t = t0; t < t1; t++) {
-    float y[V];
+  auto step = [&](const float (&in)[V], int t) {
+    float rows[W][V], y[V];
 #pragma unroll
-    for (int j = 0; j < W - 1; j++)
+    for (int v = 0; v < V; v++) {
 #pragma unroll
-      for (int v = 0; v < V; v++) past[j][v] = past[j + 1][v];
-    load_group<T, V>(past[W - 1], x + (size_t)t * a.ldx, n);
-    taps.apply(past, y, a.silu);
+      for (int j = 0; j < W - 1; j++) rows[j][v] = past[j][v];
+      rows[W - 1][v] = in[v];
+#pragma unroll
+      for (int j = 0; j < W - 1; j++) past[j][v] = rows[j + 1][v];
+    }
+    taps.apply(rows, y, a.silu);
     store_group<T, V>(a.y + (size_t)t * a.ldy + c, y, n);
+  };
+  int t = t0;
+  if (n >= V)
+    for (; t + kConvBatch <= t1; t += kConvBatch) {
+      group raw[kConvBatch];
+#pragma unroll
+      for (int r = 0; r < kConvBatch; r++) raw[r] = *reinterpret_cast<const group*>(x + (size_t)(t + r) * a.ldx);
+#pragma unroll
+      for (int r = 0; r < kConvBatch; r++) {
+        float in[V];
+#pragma unroll
+        for (int v = 0; v < V; v++) in[v] = (float)raw[r][v];
+        step(in, t + r);
+      }
+    }
+  for (; t < t1; t++) {
+    float in[V];
+    load_group<T, V>(in, x + (size_t)t * a.ldx, n);
+    step(in, t);
   }
 }
 
@@ -364,35 +392,78 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   }
 }
 
-// One token each of `rows` sequences.  Bound by memory: the states once in and once out.  LANES lanes share a channel, four states (one
-// after another) each.
-template <class T, int LANES>
+// One token each of a.rows sequences.  Bound by memory: the states once in and once out.  LANES lanes share a channel, four states each;
+// a thread takes R sequences (blockIdx.y, and so on by gridDim.y), whose loads go out together, and holds A for all.  VEC: the states are
+// a multiple of four.
+template <class T, int LANES, int R, bool VEC>
 __global__ __launch_bounds__(256) void ssm_one_kernel(SsmArgs<T> a) {
-  const size_t item = (size_t)blockIdx.x * 256 + threadIdx.x;
-  const size_t chan = item / LANES;
-  const int q = (int)(item % LANES), row = (int)(chan / a.D_), d = (int)(chan % a.D_);
-  if (row >= a.rows) return;  // lanes of a channel leave together
-  const int g = d / a.cpg;
-  const float v = (float)a.dt[(size_t)row * a.lddt + d] + (a.dt_bias ? a.dt_bias[d] : 0.f);
-  const float dt = a.softplus ? softplus_f<sizeof(T) == 4>(v) : v;
-  const float x = (float)a.x[(size_t)row * a.ldx + d], u = dt * x;
-  const size_t st = ((size_t)row * a.D_ + d) * a.N;
-  float y = 0.f;
+  typedef T t4 __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+  constexpr bool FINE = sizeof(T) == 4;
+  const int q = threadIdx.x % LANES, n0 = q * 4, d = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  if (d >= a.D_) return;  // lanes of a channel leave together
+  const int gn = d / a.cpg * a.N + n0, left = a.N - n0;
+  auto four = [&](const auto* p) {
+    f4 v;
+    if constexpr (VEC) {
+      if (left > 0) {
+        if constexpr (sizeof(*p) == 2) {
+          const t4 t = *reinterpret_cast<const t4*>(p);
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
-    const int n = q * 4 + k;
-    if (n < a.N) {
-      const float decay = __builtin_amdgcn_exp2f(dt * (a.A[(size_t)d * a.N + n] * kLog2e));
-      const float h = __builtin_fmaf(decay, a.state[st + n], u * (float)a.B[(size_t)row * a.ldb + g * a.N + n]);
-      a.state_out[st + n] = h;
-      y = __builtin_fmaf((float)a.C[(size_t)row * a.ldc + g * a.N + n], h, y);
+          for (int k = 0; k < 4; k++) v[k] = (float)t[k];
+        } else {
+          v = *reinterpret_cast<const f4*>(p);
+        }
+      } else {
+        v = (f4){0.f, 0.f, 0.f, 0.f};
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k++) v[k] = k < left ? (float)p[k] : 0.f;
     }
-  }
+    return v;
+  };
+  const f4 A = four(a.A + (size_t)d * a.N + n0);
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
+  for (int r0 = blockIdx.y * R; r0 < a.rows; r0 += gridDim.y * R) {
+    f4 h[R], B[R], C[R];
+    float dt[R], x[R], z[R];
 #pragma unroll
-  for (int m = 1; m < LANES; m *= 2) y += __shfl_xor(y, m);
-  if (q == 0) {
-    y = __builtin_fmaf(a.D ? a.D[d] : 0.f, x, y);
-    a.y[(size_t)row * a.ldy + d] = (T)(a.z ? y * silu_f<sizeof(T) == 4>((float)a.z[(size_t)row * a.ldz + d]) : y);
+    for (int r = 0; r < R; r++) {
+      const int row = min(r0 + r, a.rows - 1);
+      h[r] = four(a.state + ((size_t)row * a.D_ + d) * a.N + n0);
+      dt[r] = (float)a.dt[(size_t)row * a.lddt + d];
+      x[r] = (float)a.x[(size_t)row * a.ldx + d];
+      B[r] = four(a.B + (size_t)row * a.ldb + gn);
+      C[r] = four(a.C + (size_t)row * a.ldc + gn);
+      z[r] = a.z ? (float)a.z[(size_t)row * a.ldz + d] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (R > 1 && r0 + r >= a.rows) break;
+      const float v = dt[r] + bias, step = a.softplus ? softplus_f<FINE>(v) : v, u = step * x[r];
+      float y = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        h[r][k] = __builtin_fmaf(__builtin_amdgcn_exp2f(step * (A[k] * kLog2e)), h[r][k], u * B[r][k]);
+        y = VEC || k < left ? __builtin_fmaf(C[r][k], h[r][k], y) : y;
+      }
+      if (VEC && left <= 0) y = 0.f;  // lanes without a state: not what 0 times a step that is not finite would leave
+      float* const out = a.state_out + ((size_t)(r0 + r) * a.D_ + d) * a.N + n0;
+      if constexpr (VEC) {
+        if (left > 0) *reinterpret_cast<f4*>(out) = h[r];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+          if (k < left) out[k] = h[r][k];
+      }
+#pragma unroll
+      for (int m = 1; m < LANES; m *= 2) y += __shfl_xor(y, m);
+      if (q == 0) {
+        y = __builtin_fmaf(skip, x[r], y);
+        a.y[(size_t)(r0 + r) * a.ldy + d] = (T)(a.z ? y * silu_f<FINE>(z[r]) : y);
+      }
+    }
   }
 }
 
@@ -443,27 +514,21 @@ static int check_seqs(int nseq, const int32_t* seq_start, const char* what) {
   return 0;
 }
 
-template <class T, int W>
-static void conv_one_launch(const ConvArgs<T>& a, hipStream_t st) {
-  const size_t items = (size_t)a.rows * a.ncv;
-  hipLaunchKernelGGL((conv_one_kernel<T, W>), dim3((unsigned)((items + 255) / 256)), dim3(256), 0, st, a);
-}
-
 template <class T>
-static int conv_one_run(ConvArgs<T> a, int W, hipStream_t st) {
-  a.ncv = (a.C + kConvLanes<T> - 1) / kConvLanes<T>;
-  if (((size_t)a.rows * a.ncv + 255) / 256 > INT_MAX) return set_error(FRHIP_ESHAPE, "conv_one: too many rows");
-  if (W == 2) conv_one_launch<T, 2>(a, st);
-  else if (W == 3) conv_one_launch<T, 3>(a, st);
-  else conv_one_launch<T, 4>(a, st);
+static int conv_one_run(const ConvArgs<T>& a, int W, hipStream_t st) {
+  const int lanes = (a.C - 1) / kConvLanes<T> + 1;
+  const dim3 grid((lanes + 63) / 64, a.rows < 65535 ? a.rows : 65535);
+  if (W == 2) hipLaunchKernelGGL((conv_one_kernel<T, 2>), grid, dim3(64), 0, st, a);
+  else if (W == 3) hipLaunchKernelGGL((conv_one_kernel<T, 3>), grid, dim3(64), 0, st, a);
+  else hipLaunchKernelGGL((conv_one_kernel<T, 4>), grid, dim3(64), 0, st, a);
   return check_launch("conv_one");
 }
 
 template <class T>
 static int conv_seq_run(ConvArgs<T> a, int W, int nseq, const int32_t* start, hipStream_t st) {
   constexpr int V = kConvLanes<T>;
-  const int ncv = (a.C + V - 1) / V, blocks = (ncv + 255) / 256, threads = ((ncv + blocks - 1) / blocks + 63) / 64 * 64;
-  a.tile = 16;
+  const int ncv = (a.C - 1) / V + 1, blocks = (ncv + 255) / 256, threads = ((ncv + blocks - 1) / blocks + 63) / 64 * 64;
+  a.tile = (size_t)(start[nseq] - start[0]) / kConvBatch * ((ncv + 63) / 64) > (size_t)compute_units() * 16 ? 2 * kConvBatch : kConvBatch;
   if (blocks > 65535) return set_error(FRHIP_ESHAPE, "conv_seq: too many channels");
   const T *state = a.state;
   T* state_out = a.state_out;
@@ -655,23 +720,35 @@ static int ssm_seq_run(const frhip_ssm& p, const SsmCall& c, int nseq, const int
   return 0;
 }
 
+template <class T, int LANES, int R>
+static void one_launch(const SsmArgs<T>& a, int groups, hipStream_t st) {
+  const dim3 grid((a.D_ - 1) / (256 / LANES) + 1, groups < 65535 ? groups : 65535);
+  if (a.N % 4 == 0) hipLaunchKernelGGL((ssm_one_kernel<T, LANES, R, true>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((ssm_one_kernel<T, LANES, R, false>), grid, dim3(256), 0, st, a);
+}
+
+template <class T, int LANES>
+static void one_rows(const SsmArgs<T>& a, hipStream_t st) {
+  // four sequences a thread from where that still leaves every SIMD several waves
+  const size_t waves = ((size_t)a.D_ * LANES + 63) / 64 * ((a.rows - 1) / 4 + 1);
+  if (waves >= (size_t)compute_units() * 8) one_launch<T, LANES, 4>(a, (a.rows - 1) / 4 + 1, st);
+  else one_launch<T, LANES, 1>(a, a.rows, st);
+}
+
 template <class T>
 static int ssm_one_run(const frhip_ssm& p, const SsmCall& c, int rows, hipStream_t st) {
   SsmArgs<T> a = ssm_args<T>(p, c);
   a.rows = rows;
   int lanes = 1;
   while (lanes * 4 < p.states) lanes *= 2;
-  const size_t wgs = ((size_t)rows * p.channels * lanes + 255) / 256;
-  if (wgs > INT_MAX) return set_error(FRHIP_ESHAPE, "ssm_one: too many rows");
-  const dim3 grid((unsigned)wgs);
   switch (lanes) {
-    case 1: hipLaunchKernelGGL((ssm_one_kernel<T, 1>), grid, dim3(256), 0, st, a); break;
-    case 2: hipLaunchKernelGGL((ssm_one_kernel<T, 2>), grid, dim3(256), 0, st, a); break;
-    case 4: hipLaunchKernelGGL((ssm_one_kernel<T, 4>), grid, dim3(256), 0, st, a); break;
-    case 8: hipLaunchKernelGGL((ssm_one_kernel<T, 8>), grid, dim3(256), 0, st, a); break;
-    case 16: hipLaunchKernelGGL((ssm_one_kernel<T, 16>), grid, dim3(256), 0, st, a); break;
-    case 32: hipLaunchKernelGGL((ssm_one_kernel<T, 32>), grid, dim3(256), 0, st, a); break;
-    default: hipLaunchKernelGGL((ssm_one_kernel<T, 64>), grid, dim3(256), 0, st, a); break;
+    case 1: one_rows<T, 1>(a, st); break;
+    case 2: one_rows<T, 2>(a, st); break;
+    case 4: one_rows<T, 4>(a, st); break;
+    case 8: one_rows<T, 8>(a, st); break;
+    case 16: one_rows<T, 16>(a, st); break;
+    case 32: one_rows<T, 32>(a, st); break;
+    default: one_rows<T, 64>(a, st); break;
   }
   return check_launch("ssm_one");
 }
