@@ -218,7 +218,7 @@ struct SsmArgs {
   T* y;
   const float *A, *D, *dt_bias, *state;
   float* state_out;
-  float *ends, *sums;  // of the chunks that are not a prompt's last: [local chunks, then prompts][N][D], [local chunks][D]
+  float *ends, *sums;  // of the chunks that are not a prompt's last: [local chunks, then prompts][N / 4][D][4], [local chunks][D]
   int ldx, lddt, ldb, ldc, ldz, ldy;
   int D_, N, cpg, softplus;  // channels, states, channels of a group
   int nblk;                  // workgroups of a group's channels
@@ -262,68 +262,114 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
     A2[k] = n0 + k < a.N ? a.A[(size_t)d * a.N + n0 + k] * kLog2e : 0.f;
     h[k] = 0.f;
   }
-  const size_t ND = (size_t)a.N * a.D_;
+  // a chunk's end state in the workspace: [N / 4, rounded up][D][4], 16 bytes a lane and access
+  const int quads = (a.N + 3) / 4;
+  const size_t slot = (size_t)quads * a.D_ * 4;
+  auto quad = [&](size_t chunk, int k) { return reinterpret_cast<f32x4*>(a.ends + chunk * slot + ((size_t)(n0 + k) * a.D_ + (size_t)d * 4)); };
+  const size_t start = (size_t)a.nlocal + local0;  // the prompt's state ahead, of prompts of several chunks
+  const float* const state = a.state + ((size_t)i * a.D_ + d) * a.N + n0;
   if constexpr (LOCAL) {
     if (ci == 0 && mine) {  // step 2 reads it here: its last chunk may overwrite the state
 #pragma unroll
-      for (int k = 0; k < NPL; k++)
-        if (n0 + k < a.N) a.ends[(size_t)(a.nlocal + local0) * ND + (size_t)(n0 + k) * a.D_ + d] = a.state[((size_t)i * a.D_ + d) * a.N + n0 + k];
+      for (int k = 0; k < NPL; k += 4)
+        if (n0 + k < a.N) {
+          f32x4 v;
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = n0 + k + e < a.N ? state[k + e] : 0.f;
+          *quad(start, k) = v;
+        }
     }
   } else if (nchunk == 1) {
 #pragma unroll
     for (int k = 0; k < NPL; k++)
-      if (n0 + k < a.N) h[k] = a.state[((size_t)i * a.D_ + d) * a.N + n0 + k];
+      if (n0 + k < a.N) h[k] = state[k];
   } else {
+    const float* const sums = a.sums + (size_t)local0 * a.D_ + d;
+    constexpr int AHEAD = NPL == 4 ? 8 : NPL == 8 ? 4 : 2;  // chunks that are requested together
 #pragma unroll
-    for (int k = 0; k < NPL; k++)
-      if (n0 + k < a.N) h[k] = a.ends[(size_t)(a.nlocal + local0) * ND + (size_t)(n0 + k) * a.D_ + d];
-#pragma unroll 2
-    for (int p = 0; p < ci; p++) {
-      const float s = a.sums[(size_t)(local0 + p) * a.D_ + d];
-      const float* e = a.ends + (size_t)(local0 + p) * ND + d;
+    for (int k = 0; k < NPL; k += 4)
+      if (n0 + k < a.N) {
+        const f32x4 v = *quad(start, k);
 #pragma unroll
-      for (int k = 0; k < NPL; k++)
-        if (n0 + k < a.N) h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(s * A2[k]), h[k], e[(size_t)(n0 + k) * a.D_]);
+        for (int e = 0; e < 4; e++) h[k + e] = v[e];
+      }
+    for (int p0 = 0; p0 < ci; p0 += AHEAD) {
+      float sum[AHEAD];
+      f32x4 v[AHEAD][NPL / 4];
+#pragma unroll
+      for (int p = 0; p < AHEAD; p++) {
+        const int c = min(p0 + p, ci - 1);
+        sum[p] = sums[(size_t)c * a.D_];
+#pragma unroll
+        for (int k = 0; k < NPL; k += 4) v[p][k / 4] = *quad(local0 + c, n0 + k < a.N ? k : -n0);
+      }
+#pragma unroll
+      for (int p = 0; p < AHEAD; p++)
+        if (p0 + p < ci) {
+#pragma unroll
+          for (int k = 0; k < NPL; k++) h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[p] * A2[k]), h[k], v[p][k / 4][k % 4]);
+        }
     }
+#pragma unroll
+    for (int k = 0; k < NPL; k++) h[k] = n0 + k < a.N ? h[k] : 0.f;
   }
 
   const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = !LOCAL && a.D ? a.D[d] : 0.f;
+  const unsigned at_row = (unsigned)d * sizeof(T);  // of x, dt, z and y: rows are uniform addresses, a lane adds this
+  auto in_row = [&](const T* rows, int ld, int row) {
+    return *reinterpret_cast<const T*>(reinterpret_cast<const char*>(rows + (size_t)row * ld) + at_row);
+  };
   const T* const zp = a.z ? a.z : a.x;  // without a gate some row that is there, for nothing
   const int ldz = a.z ? a.ldz : a.ldx;
   float sum = 0.f;
   T xr[ROWS], dr[ROWS], zr[ROWS], st[STAGE];
+  // B and C of a block: element e = (row, which, state), a thread takes every WAVES x 64th
+  const T* bcp[STAGE];
+  int bcrow[STAGE];
+  unsigned bcld[STAGE];
+#pragma unroll
+  for (int q = 0; q < STAGE; q++) {
+    const int e = threadIdx.x + q * (WAVES * 64), r = e / (2 * NT), c = (e / NT) & 1, n = e % NT;
+    bcrow[q] = e < TB * 2 * NT && n < a.N ? r : INT_MAX;
+    bcld[q] = c ? a.ldc : a.ldb;
+    bcp[q] = (c ? a.C : a.B) + (size_t)g * a.N + (n < a.N ? n : 0);
+  }
   auto request = [&](int t) {  // of the block that begins at row t; rows past the chunk repeat its last one
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
-      const int row = t + nw * ROWS + r < t1 ? t + nw * ROWS + r : t1 - 1;
-      xr[r] = (a.x + (size_t)row * a.ldx)[(unsigned)d];
-      dr[r] = (a.dt + (size_t)row * a.lddt)[(unsigned)d];
-      if constexpr (!LOCAL) zr[r] = (zp + (size_t)row * ldz)[(unsigned)d];
+      const int row = min(t + nw * ROWS + r, t1 - 1);
+      xr[r] = in_row(a.x, a.ldx, row);
+      dr[r] = in_row(a.dt, a.lddt, row);
+      if constexpr (!LOCAL) zr[r] = in_row(zp, ldz, row);
     }
 #pragma unroll
-    for (int q = 0; q < STAGE; q++) {
-      const int e = threadIdx.x + q * (WAVES * 64), r = e / (2 * NT), c = (e / NT) & 1, n = e % NT;
-      const bool in = e < TB * 2 * NT && t + r < t1 && n < a.N;
-      st[q] = (T)0.f;
-      if (in) st[q] = ((c ? a.C : a.B) + (size_t)(t + r) * (c ? a.ldc : a.ldb))[g * a.N + n];
-    }
+    for (int q = 0; q < STAGE; q++) st[q] = bcp[q][(size_t)(unsigned)(t + min(bcrow[q], t1 - 1 - t)) * bcld[q]];
   };
   float x[ROWS], z[ROWS];  // of the block that is scanned
   auto take = [&](int t, int buf, float (&xn)[ROWS], float (&zn)[ROWS]) {
+    float dt[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) dt[r] = (float)dr[r] + bias;
+    if (a.softplus) {
+#pragma unroll
+      for (int r = 0; r < ROWS; r++) dt[r] = softplus_f<FINE>(dt[r]);
+    }
+    if (t + TB > t1) {  // rows past the chunk: no step, no input
+#pragma unroll
+      for (int r = 0; r < ROWS; r++)
+        if (t + nw * ROWS + r >= t1) dt[r] = 0.f, xr[r] = (T)0.f;
+    }
 #pragma unroll
     for (int r = 0; r < ROWS; r++) {
-      const bool live = t + nw * ROWS + r < t1;
-      const float v = (float)dr[r] + bias, sp = softplus_f<FINE>(v);
-      const float dt = live ? (a.softplus ? sp : v) : 0.f;
-      xn[r] = live ? (float)xr[r] : 0.f;
+      xn[r] = (float)xr[r];
       if constexpr (!LOCAL) zn[r] = (float)zr[r];
-      du[buf][nw * ROWS + r][at] = make_float2(dt, dt * xn[r]);
-      if constexpr (LOCAL) sum += dt;
+      du[buf][nw * ROWS + r][at] = make_float2(dt[r], dt[r] * xn[r]);
+      if constexpr (LOCAL) sum += dt[r];
     }
 #pragma unroll
     for (int q = 0; q < STAGE; q++) {
       const int e = threadIdx.x + q * (WAVES * 64);
-      if (e < TB * 2 * NT) (&bc[buf][0][0][0])[e] = (float)st[q];
+      if (TB * 2 * NT % (WAVES * 64) == 0 || e < TB * 2 * NT) (&bc[buf][0][0][0])[e] = bcrow[q] < t1 - t ? (float)st[q] : 0.f;
     }
   };
   if (t0 < t1) {
@@ -364,7 +410,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
         for (int w = 1; w < NW; w++) y += part[w][row][at];
         y = __builtin_fmaf(skip, x[r], y);
         if (a.z) y *= silu_f<FINE>(z[r]);
-        if (mine && t + row < t1) (a.y + (size_t)(t + row) * a.ldy)[(unsigned)d] = (T)y;
+        if (mine && t + row < t1) *reinterpret_cast<T*>(reinterpret_cast<char*>(a.y + (size_t)(t + row) * a.ldy) + at_row) = (T)y;
       }
     }
 #pragma unroll
@@ -383,8 +429,8 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   if (!mine) return;
   if constexpr (LOCAL) {
 #pragma unroll
-    for (int k = 0; k < NPL; k++)
-      if (n0 + k < a.N) a.ends[(size_t)j0 * ND + (size_t)(n0 + k) * a.D_ + d] = h[k];
+    for (int k = 0; k < NPL; k += 4)
+      if (n0 + k < a.N) *quad(j0, k) = (f32x4){h[k], h[k + 1], h[k + 2], h[k + 3]};
   } else if (ci == nchunk - 1) {
 #pragma unroll
     for (int k = 0; k < NPL; k++)
@@ -596,7 +642,8 @@ static ConvArgs<T> conv_args(int C, const void* x, int ldx, const float* w, cons
 
 static int ssm_check_params(const frhip_ssm* p) {
   if (!p || !p->A) return set_error(FRHIP_EINVAL, "ssm: null pointer");
-  if (p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0) return set_error(FRHIP_ESHAPE, "ssm: channels must be a multiple of groups");
+  if (p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0 || p->channels > 1 << 28)
+    return set_error(FRHIP_ESHAPE, "ssm: channels must be a multiple of groups, at most 2^28");
   if (p->states < 1 || p->states > 256) return set_error(FRHIP_ESHAPE, "ssm: states must be 1 to 256");
   if ((long long)p->groups * p->states > INT_MAX) return set_error(FRHIP_ESHAPE, "ssm: too many groups");
   if (off_grid(4, {p->A, p->D, p->dt_bias})) return set_error(FRHIP_EINVAL, "ssm: pointer not aligned to its element");
@@ -706,7 +753,7 @@ static int ssm_seq_run(const frhip_ssm& p, const SsmCall& c, int nseq, const int
     a.state = c.state + (size_t)s0 * per;
     a.state_out = c.state_out + (size_t)s0 * per;
     a.ends = static_cast<float*>(workspace);
-    a.sums = a.ends + 2 * (size_t)a.nlocal * per;
+    a.sums = a.ends + 2 * (size_t)a.nlocal * p.channels * ((p.states + 3) / 4 * 4);
     int rc = FRHIP_ESHAPE;
     if (s.npl == 4 && s.nw == 1) rc = scan_launch<T, 4, 1>(a, tab, s.wgs, chunks, st);
     else if (s.npl == 4 && s.nw == 2) rc = scan_launch<T, 4, 2>(a, tab, s.wgs, chunks, st);
@@ -798,7 +845,7 @@ extern "C" int frhip_ssm_one(const frhip_ssm* p, int rows, const void* x, int ld
 extern "C" size_t frhip_ssm_workspace_bytes(const frhip_ssm* p, int nseq, int T) {
   if (!p || p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0 || p->states < 1 || p->states > 256 || nseq <= 0 || T <= 0) return 0;
   const ScanShape s = scan_shape(*p);
-  const size_t bytes = scan_most_local(s, T) * (2 * (size_t)p->states + 1) * p->channels * 4;
+  const size_t bytes = scan_most_local(s, T) * (2 * (size_t)((p->states + 3) / 4 * 4) + 1) * p->channels * 4;
   return (bytes + 255) / 256 * 256;
 }
 

@@ -87,7 +87,7 @@ def test_time_is_covered_and_the_workspace_holds_the_chunks(channels, states, gr
         rows, chunks, wgs = out
         assert chunks == sum(max(1, -(-n // rows)) for n in lens) <= 65535 and wgs >= 1
         local = chunks - len(lens)
-        need = 4 * (2 * local * channels * states + local * channels)
+        need = 4 * (2 * local * channels * -(-states // 4) * 4 + local * channels)
         assert need <= fr.lib().frhip_ssm_workspace_bytes(C.byref(p), len(lens), total)
 
 
