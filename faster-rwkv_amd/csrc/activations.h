@@ -9,9 +9,9 @@ namespace frhip {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|); log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3, with atanh(s) / s as a polynomial
-// in s^2 (Chebyshev fit over [0, 1/9], 8e-9 relative), so that small values keep their relative accuracy.  FINE: the rounding of
-// -|v| log2(e), which exp2 would scale by |v|, is made good.
+// log(1 + exp(v)) = max(v, 0) + log1p(e), e = exp(-|v|); log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3.  With g = 2 s = e / (1 + e / 2) that is
+// g P(g^2), P a polynomial (Chebyshev fit of atanh(s) / s over s^2 in [0, 1/9], 8e-9 relative), so that small values keep their
+// relative accuracy.  FINE: the rounding of -|v| log2(e), which exp2 would scale by |v|, is made good.
 template <bool FINE>
 __device__ __forceinline__ float softplus_f(float v) {
   const float m = FINE ? __builtin_fminf(__builtin_fabsf(v), 120.f) : __builtin_fabsf(v), t = m * -kLog2e;  // exp(-120) is no fp32 number
@@ -20,13 +20,13 @@ __device__ __forceinline__ float softplus_f(float v) {
     const float r = __builtin_fmaf(m, 1.925963033500752e-8f, __builtin_fmaf(m, kLog2e, t));
     e = __builtin_fmaf(e, -r * 0.693147180559945f, e);
   }
-  const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
-  float p = __builtin_fmaf(q, 0.1408732831478119f, 0.1398070901632309f);
-  p = __builtin_fmaf(p, q, 0.20012426376342773f);
-  p = __builtin_fmaf(p, q, 0.3333315849304199f);
+  const float g = e * __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, e, 1.0f)), q = g * g;
+  float p = __builtin_fmaf(q, 0.1408732831478119f / 256, 0.1398070901632309f / 64);
+  p = __builtin_fmaf(p, q, 0.20012426376342773f / 16);
+  p = __builtin_fmaf(p, q, 0.3333315849304199f / 4);
   p = __builtin_fmaf(p, q, 1.0f);
-  const float y = __builtin_fmaf(2.0f * s, p, __builtin_fmaxf(v, 0.f));
-  return v == v ? y : v;
+  const float y = __builtin_fmaf(g, p, __builtin_amdgcn_fmed3f(v, 0.f, __builtin_inff()));  // a NaN stays one through g
+  return FINE && v != v ? v : y;
 }
 
 // FINE: for results that stay fp32; otherwise within a few units of the instructions for exp2 and the reciprocal, far below what the
