@@ -94,6 +94,71 @@ __device__ __forceinline__ void finish_outputs(const LinearArgs& a, const float 
   else finish_as<h1>(a, acc, row, col, n);
 }
 
+// Groups of eight consecutive outputs whose sums are in LDS: place(t, row, col, sums) says where group t is, false: nowhere; a thread takes t0,
+// t0 + step, ... below `end`, two at a time, whose residuals and biases are requested together.
+template <int ACT, class O, class Place>
+__device__ __forceinline__ void finish_groups_as(const LinearArgs& a, int t0, int step, int end, Place&& place) {
+  typedef O any __attribute__((ext_vector_type(8), aligned(sizeof(O))));
+  typedef float anyf __attribute__((ext_vector_type(8), aligned(4)));
+  constexpr bool FINE = sizeof(O) == 4;
+  constexpr int G = 2;
+  const O* const res = static_cast<const O*>(a.res);
+  O* const out = static_cast<O*>(a.y);
+#pragma unroll 1
+  for (int t = t0; t < end; t += G * step) {
+    int row[G], col[G];
+    const float* sums[G];
+    bool in[G], whole[G];
+    any r[G];
+    anyf b[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      in[g] = t + g * step < end && place(t + g * step, row[g], col[g], sums[g]);
+      whole[g] = in[g] && col[g] + 8 <= a.N;
+      if (whole[g] && res) r[g] = *reinterpret_cast<const any*>(res + (size_t)row[g] * a.ldr + col[g]);
+      if (whole[g] && a.bias) b[g] = *reinterpret_cast<const anyf*>(a.bias + col[g]);
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      if (whole[g]) {
+        float s[8];
+        read_sums(s, sums[g]);
+        any y;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float v = activate<FINE>(a.bias ? s[i] + b[g][i] : s[i], ACT);
+          y[i] = (O)(res ? v + (float)r[g][i] : v);
+        }
+        *reinterpret_cast<any*>(out + (size_t)row[g] * a.ldy + col[g]) = y;
+      } else if (in[g]) {  // the end of a row
+#pragma unroll 1
+        for (int i = 0; col[g] + i < a.N; i++) {
+          const float v = activate<FINE>(a.bias ? sums[g][i] + a.bias[col[g] + i] : sums[g][i], ACT);
+          out[(size_t)row[g] * a.ldy + col[g] + i] = (O)(res ? v + (float)res[(size_t)row[g] * a.ldr + col[g] + i] : v);
+        }
+      }
+    }
+  }
+}
+// One short loop for each activation and type: with the choice inside the loop, unrolled, a tile of 256 rows spent 12 us between its last
+// product and its end, most of it on fetching instructions (4096 x 2560 x 10240, three rounds: 242 us, 220 so).
+template <class O, class Place>
+__device__ __forceinline__ void finish_groups_of(const LinearArgs& a, int t0, int step, int end, Place&& place) {
+  switch (a.act) {
+    case FRHIP_ACT_SIGMOID: finish_groups_as<FRHIP_ACT_SIGMOID, O>(a, t0, step, end, place); break;
+    case FRHIP_ACT_RELU2: finish_groups_as<FRHIP_ACT_RELU2, O>(a, t0, step, end, place); break;
+    case FRHIP_ACT_SILU: finish_groups_as<FRHIP_ACT_SILU, O>(a, t0, step, end, place); break;
+    case FRHIP_ACT_GELU: finish_groups_as<FRHIP_ACT_GELU, O>(a, t0, step, end, place); break;
+    case FRHIP_ACT_SOFTPLUS: finish_groups_as<FRHIP_ACT_SOFTPLUS, O>(a, t0, step, end, place); break;
+    default: finish_groups_as<FRHIP_ACT_NONE, O>(a, t0, step, end, place); break;
+  }
+}
+template <class Place>
+__device__ __forceinline__ void finish_groups(const LinearArgs& a, int t0, int step, int end, Place&& place) {
+  if (a.out32) finish_groups_of<float>(a, t0, step, end, place);
+  else finish_groups_of<h1>(a, t0, step, end, place);
+}
+
 // ---------------------------------------------------------------------------
 // One or two rows: a wave streams COLS consecutive rows of the weight, 16 bytes a lane and load, and multiplies them with its lanes'
 // pieces of x, which stay in registers (lane l has the 8 k of chunks l, l + 64, ... of a slice of K, of x and of every column alike).
@@ -504,13 +569,15 @@ __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearTiles a
   __syncthreads();
   const float* const sums = reinterpret_cast<const float*>(ring_smem);
   const int pitch = sums_pitch(a.maxw), groups = width * 4;  // of 8 outputs
-  for (int i = threadIdx.x; i < BM * groups; i += kRingThreads) {
-    const int row = i / groups, col = (i - row * groups) * 8;
-    if (m0 + row >= a.l.T || n0 + col >= a.l.N) continue;
-    float s[8];
-    read_sums(s, sums + row * pitch + col);
-    finish_outputs(a.l, s, m0 + row, n0 + col, a.l.N - n0 - col);
-  }
+  const unsigned inv = ((1u << 20) + groups - 1) / groups;    // i / groups for i < 4096, groups <= 32
+  static_assert(BM * 4 * kRingMostBlocks <= 4096, "the division");
+  finish_groups(a.l, threadIdx.x, kRingThreads, BM * groups, [&](int i, int& row, int& col, const float*& from) {
+    const int r = (int)((unsigned)i * inv >> 20), c = (i - r * groups) * 8;
+    row = m0 + r;
+    col = n0 + c;
+    from = sums + r * pitch + c;
+    return row < a.l.T && col < a.l.N;
+  });
 }
 
 template <int BM, int S, bool TAIL>
@@ -530,6 +597,33 @@ static void ring_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st)
 // ---------------------------------------------------------------------------
 constexpr int kWideThreads = 512, kWideMostBlocks = 8, kWideABytes = 256 * kLdwBK * 2;
 static_assert(2 * (kWideABytes + kWideMostBlocks * 4096) <= 160 * 1024 && 8 * wave_sums_bytes((kWideMostBlocks + 1) / 2) <= 160 * 1024, "LDS of a compute unit");
+
+// Blocks that lie inside the matrix, without an activation: acc[i][j][v] is C[row0 + 32 i + 8 (v / 4) + v % 4][col0 + 32 j].  4096 x 2560 x 10240 through LDS 220 us,
+// so 208.
+template <class O, int NJ>
+__device__ __forceinline__ void store_blocks(const LinearArgs& a, const f16v (&acc)[2][NJ], int row0, int col0) {
+#pragma unroll
+  for (int j = 0; j < NJ; j++) {
+    const float b = a.bias ? a.bias[col0 + j * 32] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const O* const res = static_cast<const O*>(a.res) + (size_t)(row0 + i * 32) * a.ldr + col0 + j * 32;
+      O* const out = static_cast<O*>(a.y) + (size_t)(row0 + i * 32) * a.ldy + col0 + j * 32;
+      float r[16];
+#pragma unroll
+      for (int v = 0; v < 16; v++) r[v] = 0.f;
+      if (a.res) {
+#pragma unroll
+        for (int v = 0; v < 16; v++) r[v] = (float)res[(size_t)(8 * (v >> 2) + (v & 3)) * a.ldr];
+      }
+#pragma unroll
+      for (int v = 0; v < 16; v++) {
+        const float y = acc[i][j][v] + b;
+        out[(size_t)(8 * (v >> 2) + (v & 3)) * a.ldy] = (O)(a.res ? y + r[v] : y);
+      }
+    }
+  }
+}
 
 template <int NJ, bool TAIL>
 __device__ __forceinline__ void wide_body(const LinearTiles& a, unsigned char* smem, int width, int brow0, int m0, int n0, int lane, int wave) {
@@ -605,23 +699,32 @@ __device__ __forceinline__ void wide_body(const LinearTiles& a, unsigned char* s
         for (int j = 0; j < NJ; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa[i], fb[j], acc[i][j], 0, 0, 0);
     }
   }
+  if (a.l.act == FRHIP_ACT_NONE && m0 + 256 <= M && n0 + width * 32 <= N) {  // whole tiles: straight from the accumulators
+    const int row0 = m0 + wm * 64 + 4 * (lane >> 5), col0 = n0 + brow0 + (lane & 31);
+    if (a.l.out32) store_blocks<float, NJ>(a.l, acc, row0, col0);
+    else store_blocks<h1, NJ>(a.l, acc, row0, col0);
+    return;
+  }
   // the last fragments are in registers (the compiler may leave their wait behind the barrier, with the products), then all waves' are
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   step_barrier();  // all fragments have been read
   float* const sums = reinterpret_cast<float*>(smem + wave * wave_sums_bytes((a.maxw + 1) / 2));
-#pragma unroll
-  for (int i = 0; i < 2; i++) {
-    if (i > 0) lanes_in_order();  // the rows before have been read
-    sums_to_lds(acc[i], sums, sums_pitch(NJ), lane);
-    lanes_in_order();
 #pragma unroll 1
-    for (int t = lane; t < 32 * NJ * 4; t += 64) {
-      const int row = t / (NJ * 4), c = (t - row * (NJ * 4)) * 8, m = m0 + wm * 64 + i * 32 + row, col = n0 + brow0 + c;
-      if (m >= M || col >= N) continue;
-      float s[8];
-      read_sums(s, sums + row * sums_pitch(NJ) + c);
-      finish_outputs(a.l, s, m, col, N - col);
+  for (int i = 0; i < 2; i++) {  // one copy of what follows
+    if (i == 0) {
+      sums_to_lds(acc[0], sums, sums_pitch(NJ), lane);
+    } else {
+      lanes_in_order();  // the rows before have been read
+      sums_to_lds(acc[1], sums, sums_pitch(NJ), lane);
     }
+    lanes_in_order();
+    finish_groups(a.l, lane, 64, 32 * NJ * 4, [&](int t, int& row, int& col, const float*& from) {
+      const int r = t / (NJ * 4), c = (t - r * (NJ * 4)) * 8;
+      row = m0 + wm * 64 + i * 32 + r;
+      col = n0 + brow0 + c;
+      from = sums + r * sums_pitch(NJ) + c;
+      return row < M && col < N;
+    });
   }
 }
 
