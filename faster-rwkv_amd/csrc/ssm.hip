@@ -24,21 +24,21 @@ struct SeqTable {
   int chunk[kSeqTable + 1];  // first chunk (every prompt has one at least)
 };
 
-// The prompt that chunk `j` belongs to: the last i with first(i) <= j.  `first` does not descend.
+// The prompt that chunk `j` belongs to: the last i with first(i) <= j, for all lanes of a wave at once (all of them are here).  `first` does
+// not descend and first(0) is 0.  One load of a lane each: a search by halves waits for one after another.
 template <class F>
 __device__ __forceinline__ int find_seq(int nseq, int j, F first) {
-  int lo = 0, hi = nseq - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first(mid) <= j) lo = mid;
-    else hi = mid - 1;
-  }
-  return lo;
+  static_assert(kSeqTable <= 128, "two prompts a lane");
+  if (nseq == 1) return 0;
+  const int l = threadIdx.x & 63;
+  int n = __builtin_popcountll(__ballot(l < nseq && first(min(l, nseq - 1)) <= j));
+  if (nseq > 64) n += __builtin_popcountll(__ballot(l + 64 < nseq && first(min(l + 64, nseq - 1)) <= j));
+  return __builtin_amdgcn_readfirstlane(n - 1);
 }
 
 // ---------------------------------------------------------------------------
-// Short causal convolution.  Bound by memory: every element once in and once out.  A thread has 16 bytes of channels and walks a tile
-// of rows with the last W rows in registers.
+// Short causal convolution.  Bound by memory: every element once in and once out (4096 x 4096 binary16 out of rows of 8192: 16.8 us, 4.0
+// TB/s).  A thread has 16 bytes of channels and walks a tile of rows with the last W - 1 in registers and the next four requested ahead.
 // ---------------------------------------------------------------------------
 template <class T>
 struct ConvArgs {
@@ -52,7 +52,7 @@ struct ConvArgs {
 
 template <class T>
 constexpr int kConvLanes = 16 / sizeof(T);  // channels of a thread
-constexpr int kConvBatch = 8;               // rows that are requested together
+constexpr int kConvBatch = 4;               // rows that are requested together
 
 // Up to V elements at any address of one, the first n of them; 16 bytes an instruction if all are there, as for aligned ones
 template <class T, int V>
@@ -189,19 +189,24 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvArgs<T> a, SeqTable t
     store_group<T, V>(a.y + (size_t)t * a.ldy + c, y, n);
   };
   int t = t0;
-  if (n >= V)
+  if (n >= V && t + kConvBatch <= t1) {
+    group raw[kConvBatch];
+    auto request = [&](int at) {  // rows past the tile repeat its last one
+#pragma unroll
+      for (int r = 0; r < kConvBatch; r++) raw[r] = *reinterpret_cast<const group*>(x + (size_t)min(at + r, t1 - 1) * a.ldx);
+    };
+    request(t);
     for (; t + kConvBatch <= t1; t += kConvBatch) {
-      group raw[kConvBatch];
+      float in[kConvBatch][V];
 #pragma unroll
-      for (int r = 0; r < kConvBatch; r++) raw[r] = *reinterpret_cast<const group*>(x + (size_t)(t + r) * a.ldx);
+      for (int r = 0; r < kConvBatch; r++)
 #pragma unroll
-      for (int r = 0; r < kConvBatch; r++) {
-        float in[V];
+        for (int v = 0; v < V; v++) in[r][v] = (float)raw[r][v];
+      if (t + 2 * kConvBatch <= t1) request(t + kConvBatch);
 #pragma unroll
-        for (int v = 0; v < V; v++) in[v] = (float)raw[r][v];
-        step(in, t + r);
-      }
+      for (int r = 0; r < kConvBatch; r++) step(in[r], t + r);
     }
+  }
   for (; t < t1; t++) {
     float in[V];
     load_group<T, V>(in, x + (size_t)t * a.ldx, n);
@@ -577,7 +582,9 @@ template <class T>
 static int conv_seq_run(ConvArgs<T> a, int W, int nseq, const int32_t* start, hipStream_t st) {
   constexpr int V = kConvLanes<T>;
   const int ncv = (a.C - 1) / V + 1, blocks = (ncv + 255) / 256, threads = ((ncv + blocks - 1) / blocks + 63) / 64 * 64;
-  a.tile = (size_t)(start[nseq] - start[0]) / kConvBatch * ((ncv + 63) / 64) > (size_t)compute_units() * 16 ? 2 * kConvBatch : kConvBatch;
+  // A tile reads W - 1 rows more than its own, which costs where memory is busy; a short one starts sooner.  us with tiles of 4 and 8 rows:
+  // 300 x 2048 4.9 and 5.5, 2077 x 1536 of fp32 8.0 and 8.7, 1000 x 4096 8.0 and 7.5, 4096 x 4096 19.6 and 16.8
+  a.tile = (size_t)(start[nseq] - start[0]) * a.C < (size_t)4000000 ? kConvBatch : 2 * kConvBatch;
   if (blocks > 65535) return set_error(FRHIP_ESHAPE, "conv_seq: too many channels");
   const T *state = a.state;
   T* state_out = a.state_out;
