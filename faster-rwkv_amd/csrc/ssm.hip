@@ -261,64 +261,6 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   const bool mine = cg < a.cpg;
   const int d = g * a.cpg + (mine ? cg : a.cpg - 1), n0 = nw * NPL;
 
-  float A2[NPL], h[NPL];
-#pragma unroll
-  for (int k = 0; k < NPL; k++) {
-    A2[k] = n0 + k < a.N ? a.A[(size_t)d * a.N + n0 + k] * kLog2e : 0.f;
-    h[k] = 0.f;
-  }
-  // a chunk's end state in the workspace: [N / 4, rounded up][D][4], 16 bytes a lane and access
-  const int quads = (a.N + 3) / 4;
-  const size_t slot = (size_t)quads * a.D_ * 4;
-  auto quad = [&](size_t chunk, int k) { return reinterpret_cast<f32x4*>(a.ends + chunk * slot + ((size_t)(n0 + k) * a.D_ + (size_t)d * 4)); };
-  const size_t start = (size_t)a.nlocal + local0;  // the prompt's state ahead, of prompts of several chunks
-  const float* const state = a.state + ((size_t)i * a.D_ + d) * a.N + n0;
-  if constexpr (LOCAL) {
-    if (ci == 0 && mine) {  // step 2 reads it here: its last chunk may overwrite the state
-#pragma unroll
-      for (int k = 0; k < NPL; k += 4)
-        if (n0 + k < a.N) {
-          f32x4 v;
-#pragma unroll
-          for (int e = 0; e < 4; e++) v[e] = n0 + k + e < a.N ? state[k + e] : 0.f;
-          *quad(start, k) = v;
-        }
-    }
-  } else if (nchunk == 1) {
-#pragma unroll
-    for (int k = 0; k < NPL; k++)
-      if (n0 + k < a.N) h[k] = state[k];
-  } else {
-    const float* const sums = a.sums + (size_t)local0 * a.D_ + d;
-    constexpr int AHEAD = NPL == 4 ? 8 : NPL == 8 ? 4 : 2;  // chunks that are requested together
-#pragma unroll
-    for (int k = 0; k < NPL; k += 4)
-      if (n0 + k < a.N) {
-        const f32x4 v = *quad(start, k);
-#pragma unroll
-        for (int e = 0; e < 4; e++) h[k + e] = v[e];
-      }
-    for (int p0 = 0; p0 < ci; p0 += AHEAD) {
-      float sum[AHEAD];
-      f32x4 v[AHEAD][NPL / 4];
-#pragma unroll
-      for (int p = 0; p < AHEAD; p++) {
-        const int c = min(p0 + p, ci - 1);
-        sum[p] = sums[(size_t)c * a.D_];
-#pragma unroll
-        for (int k = 0; k < NPL; k += 4) v[p][k / 4] = *quad(local0 + c, n0 + k < a.N ? k : -n0);
-      }
-#pragma unroll
-      for (int p = 0; p < AHEAD; p++)
-        if (p0 + p < ci) {
-#pragma unroll
-          for (int k = 0; k < NPL; k++) h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[p] * A2[k]), h[k], v[p][k / 4][k % 4]);
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < NPL; k++) h[k] = n0 + k < a.N ? h[k] : 0.f;
-  }
-
   const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = !LOCAL && a.D ? a.D[d] : 0.f;
   const unsigned at_row = (unsigned)d * sizeof(T);  // of x, dt, z and y: rows are uniform addresses, a lane adds this
   auto in_row = [&](const T* rows, int ld, int row) {
@@ -352,6 +294,74 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
 #pragma unroll
     for (int q = 0; q < STAGE; q++) st[q] = bcp[q][(size_t)(unsigned)(t + min(bcrow[q], t1 - 1 - t)) * bcld[q]];
   };
+  if (t0 < t1) request(t0);  // on its way while the state is found
+
+  float A2[NPL], h[NPL];
+#pragma unroll
+  for (int k = 0; k < NPL; k += 4) {
+    float v[4];
+    load_group<float, 4>(v, a.A + (size_t)d * a.N + n0 + k, a.N - n0 - k);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      A2[k + e] = v[e] * kLog2e;
+      h[k + e] = 0.f;
+    }
+  }
+  // a chunk's end state in the workspace: [N / 4, rounded up][D][4], 16 bytes a lane and access
+  const int quads = (a.N + 3) / 4;
+  const size_t slot = (size_t)quads * a.D_ * 4;
+  auto quad = [&](size_t chunk, int k) { return reinterpret_cast<f32x4*>(a.ends + chunk * slot + ((size_t)(n0 + k) * a.D_ + (size_t)d * 4)); };
+  const size_t start = (size_t)a.nlocal + local0;  // the prompt's state ahead, of prompts of several chunks
+  const float* const state = a.state + ((size_t)i * a.D_ + d) * a.N + n0;
+  if constexpr (LOCAL) {
+    if (ci == 0 && mine) {  // step 2 reads it here: its last chunk may overwrite the state
+#pragma unroll
+      for (int k = 0; k < NPL; k += 4)
+        if (n0 + k < a.N) {
+          float v[4];
+          load_group<float, 4>(v, state + k, a.N - n0 - k);
+          *quad(start, k) = (f32x4){v[0], v[1], v[2], v[3]};
+        }
+    }
+  } else if (nchunk == 1) {
+#pragma unroll
+    for (int k = 0; k < NPL; k += 4) {
+      float v[4];
+      load_group<float, 4>(v, state + k, a.N - n0 - k);
+#pragma unroll
+      for (int e = 0; e < 4; e++) h[k + e] = v[e];
+    }
+  } else {
+    const float* const sums = a.sums + (size_t)local0 * a.D_ + d;
+    constexpr int AHEAD = NPL == 4 ? 8 : NPL == 8 ? 4 : 2;  // chunks that are requested together
+#pragma unroll
+    for (int k = 0; k < NPL; k += 4)
+      if (n0 + k < a.N) {
+        const f32x4 v = *quad(start, k);
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[k + e] = v[e];
+      }
+    for (int p0 = 0; p0 < ci; p0 += AHEAD) {
+      float sum[AHEAD];
+      f32x4 v[AHEAD][NPL / 4];
+#pragma unroll
+      for (int p = 0; p < AHEAD; p++) {
+        const int c = min(p0 + p, ci - 1);
+        sum[p] = sums[(size_t)c * a.D_];
+#pragma unroll
+        for (int k = 0; k < NPL; k += 4) v[p][k / 4] = *quad(local0 + c, n0 + k < a.N ? k : -n0);
+      }
+#pragma unroll
+      for (int p = 0; p < AHEAD; p++)
+        if (p0 + p < ci) {
+#pragma unroll
+          for (int k = 0; k < NPL; k++) h[k] = __builtin_fmaf(__builtin_amdgcn_exp2f(sum[p] * A2[k]), h[k], v[p][k / 4][k % 4]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NPL; k++) h[k] = n0 + k < a.N ? h[k] : 0.f;
+  }
+
   float x[ROWS], z[ROWS];  // of the block that is scanned
   auto take = [&](int t, int buf, float (&xn)[ROWS], float (&zn)[ROWS]) {
     float dt[ROWS];
@@ -380,7 +390,6 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
     }
   };
   if (t0 < t1) {
-    request(t0);
     take(t0, 0, x, z);
     if (t0 + TB < t1) request(t0 + TB);
   }
@@ -440,8 +449,10 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
       if (n0 + k < a.N) *quad(j0, k) = (f32x4){h[k], h[k + 1], h[k + 2], h[k + 3]};
   } else if (ci == nchunk - 1) {
 #pragma unroll
-    for (int k = 0; k < NPL; k++)
-      if (n0 + k < a.N) a.state_out[((size_t)i * a.D_ + d) * a.N + n0 + k] = h[k];
+    for (int k = 0; k < NPL; k += 4) {
+      const float v[4] = {h[k], h[k + 1], h[k + 2], h[k + 3]};
+      store_group<float, 4>(a.state_out + ((size_t)i * a.D_ + d) * a.N + n0 + k, v, a.N - n0 - k);
+    }
   }
 }
 
