@@ -117,6 +117,7 @@ _SIGS = {
     "frhip_seq_gemm_form": (_i, [_i, _i, _i, _vp, _i, _i, _vp]),
     "frhip_seq_codes_way": (_i, [_i, _i, _i, _vp, _i, _i, _vp]),
     "frhip_linear_workspace_bytes": (_sz, [_i, _WP]),
+    "frhip_linear_form": (_i, [_i, _WP, _i, _vp]),
     "frhip_linear": (_i, [_vp, _i, _WP, _vp, _i, _vp, _i, _vp, _i, _i, _i, _vp, _vp]),
     "frhip_conv_one": (_i, [_i, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp]),
     "frhip_conv_seq": (_i, [_i, _vp, _i, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _i, _i, _vp]),

@@ -5,6 +5,7 @@
 
 #include "activations.h"
 #include "gemm_few_device.h"
+#include "gemm_q8_device.h"
 #include "gemm_ring_device.h"
 #include "spans.h"
 
@@ -518,6 +519,21 @@ __device__ __forceinline__ void ring_products(f16v (&acc)[BM / 64][NJ], const un
   }
 }
 
+// A tile of ROWS rows and `width` blocks of 32 columns whose sums are in LDS, shared by all waves of the workgroup
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void finish_tile_of(const LinearTiles& a, const float* sums, int width, int m0, int n0) {
+  const int pitch = sums_pitch(a.maxw), groups = width * 4;  // of 8 outputs
+  const unsigned inv = ((1u << 20) + groups - 1) / groups;   // i / groups for i < 4096, groups <= 32
+  static_assert(ROWS * 4 * 8 <= 4096, "the division");
+  finish_groups(a.l, threadIdx.x, THREADS, ROWS * groups, [&](int i, int& row, int& col, const float*& from) {
+    const int r = (int)((unsigned)i * inv >> 20), c = (i - r * groups) * 8;
+    row = m0 + r;
+    col = n0 + c;
+    from = sums + r * pitch + c;
+    return row < a.l.T && col < a.l.N;
+  });
+}
+
 template <int BM, int S, int NJ, bool TAIL>
 __device__ __forceinline__ void linear_mma(unsigned char* smem, int stage, int maxw, int brow0, int nk, int krest, int lane, int wm) {
   if constexpr (NJ == 0) {  // a tile of one block: the first wave column has it
@@ -567,17 +583,7 @@ __global__ __launch_bounds__(kRingThreads) void linear_ring_kernel(LinearTiles a
     }
   }
   __syncthreads();
-  const float* const sums = reinterpret_cast<const float*>(ring_smem);
-  const int pitch = sums_pitch(a.maxw), groups = width * 4;  // of 8 outputs
-  const unsigned inv = ((1u << 20) + groups - 1) / groups;    // i / groups for i < 4096, groups <= 32
-  static_assert(BM * 4 * kRingMostBlocks <= 4096, "the division");
-  finish_groups(a.l, threadIdx.x, kRingThreads, BM * groups, [&](int i, int& row, int& col, const float*& from) {
-    const int r = (int)((unsigned)i * inv >> 20), c = (i - r * groups) * 8;
-    row = m0 + r;
-    col = n0 + c;
-    from = sums + r * pitch + c;
-    return row < a.l.T && col < a.l.N;
-  });
+  finish_tile_of<BM, kRingThreads>(a, reinterpret_cast<const float*>(ring_smem), width, m0, n0);
 }
 
 template <int BM, int S, bool TAIL>
@@ -755,6 +761,48 @@ static void wide_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st)
   hipLaunchKernelGGL(linear_wide_kernel<TAIL>, p.grid, dim3(kWideThreads), ring > sums ? ring : sums, st, t);
 }
 
+// ---------------------------------------------------------------------------
+// uint8 weights, more rows: the codes are dequantised on their way into LDS by waves of their own (gemm_q8.hip has the form and its
+// reasons), for whole steps of K and whole blocks of 16 columns.
+// ---------------------------------------------------------------------------
+template <int BM>
+__global__ __launch_bounds__(64 * (4 + kQ8Producers)) void linear_q8_kernel(LinearTiles a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char q8_smem[];
+  int bx, by;
+  xcd_tile(bx, by);
+  const int width = a.base + (bx < a.wide ? 1 : 0), n0 = (bx * a.base + min(bx, a.wide)) * 32, m0 = by * BM;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nk = a.l.K / kLdwBK;
+  if (wave >= 4) {
+    const int p = wave - 4;
+    const GemmSeg sg = {a.l.x, a.l.w, a.l.mx, a.l.rx, a.l.my, a.l.ry, nullptr, a.l.N, 0};
+    switch (p < 2 * width ? (2 * width - p + kQ8Producers - 1) / kQ8Producers : 0) {
+      case 0: q8_producer<BM, 0>(sg, q8_smem, a.maxw, p, m0, n0, a.l.T, a.l.K, a.l.ldx, 0, nk, lane); break;
+      case 1: q8_producer<BM, 1>(sg, q8_smem, a.maxw, p, m0, n0, a.l.T, a.l.K, a.l.ldx, 0, nk, lane); break;
+      default: q8_producer<BM, 2>(sg, q8_smem, a.maxw, p, m0, n0, a.l.T, a.l.K, a.l.ldx, 0, nk, lane); break;
+    }
+  } else {
+    const int wm = wave >> 1, nj0 = (width + 1) >> 1, nj = (wave & 1) ? width - nj0 : nj0, brow0 = (wave & 1) ? nj0 * 32 : 0;
+    switch (nj) {  // every wave passes the same barriers, whatever its width
+      case 1: q8_mma<BM, 1>(q8_smem, a.maxw, brow0, nk, lane, wm); break;
+      case 2: q8_mma<BM, 2>(q8_smem, a.maxw, brow0, nk, lane, wm); break;
+      case 3: q8_mma<BM, 3>(q8_smem, a.maxw, brow0, nk, lane, wm); break;
+      default: q8_mma<BM, q8_max_blocks(BM) / 2>(q8_smem, a.maxw, brow0, nk, lane, wm); break;
+    }
+  }
+  __syncthreads();
+  finish_tile_of<BM, 64 * (4 + kQ8Producers)>(a, reinterpret_cast<const float*>(q8_smem), width, m0, n0);
+}
+
+template <int BM>
+static void q8_launch(const TilePlan& p, const LinearTiles& t, hipStream_t st) {
+  static const bool raised = [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&linear_q8_kernel<BM>), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+    return true;
+  }();
+  (void)raised;
+  hipLaunchKernelGGL(linear_q8_kernel<BM>, p.grid, dim3(64 * (4 + kQ8Producers)), q8_lds_bytes(BM, t.maxw), st, t);
+}
+
 template <bool TAIL>
 static int launch_tiles(const LinearArgs& a, const TilePlan& p, hipStream_t st) {
   const LinearTiles t = {a, p.a.vw_base[0], p.a.vw_wide[0], p.a.vw_maxw};
@@ -770,10 +818,12 @@ constexpr int kLinearMostK = 8388544;  // whole steps of it keep 256 rows of a t
 // How a product goes out: the forms and cuts of the same product (K and N rounded up to whole steps and blocks) without a
 // residual on the framework's other kernels, by the same expected times.  A pure function of the sizes.
 struct LinearPlan {
-  FewPlan few;
-  TilePlan tiles;
+  FewPlan few;           // mt: a few rows
+  TilePlan tiles;        // otherwise
+  bool codes = false;    // uint8: the tiles dequantise
+  bool expand = false;   // uint8: the codes are expanded to binary16 first
 };
-static LinearPlan plan_linear(int T, int K, int N, int cus) {
+static LinearPlan plan_linear(int T, int K, int N, bool u8, int cus) {
   GemmArgs g;
   memset(&g, 0, sizeof(g));
   g.M = T;
@@ -786,23 +836,48 @@ static LinearPlan plan_linear(int T, int K, int N, int cus) {
   p.tiles = plan_ring(g, cus);
   const TilePlan wide = plan_256(g, cus);
   if (wide.rows && (!p.tiles.rows || wide.us <= p.tiles.us * 1.05)) p.tiles = wide;
-  if (p.few.mt && p.tiles.rows && p.tiles.us < p.few.us) p.few.mt = 0;
+  if (!u8) {
+    if (p.few.mt && p.tiles.rows && p.tiles.us < p.few.us) p.few.mt = 0;
+    return p;
+  }
+  // codes: dequantised by the lanes that multiply them (rows of whole 16 bytes), on their way into LDS, or expanded ahead of either
+  const double expand = 5.5 + 3.0 * K * N / 6.3e6;
+  if (K % kLdwBK == 0 && N % 16 == 0) {
+    const TilePlan q8 = plan_q8(g, cus);
+    if (q8.rows && (!p.tiles.rows || q8.us <= p.tiles.us + expand)) {
+      p.tiles = q8;
+      p.codes = true;
+    }
+  }
+  const bool direct = K % 16 == 0;
+  const double few = p.few.us + (direct ? 0 : expand), tiles = p.tiles.us + (p.codes ? 0 : expand);
+  if (p.few.mt && p.tiles.rows && tiles < few) p.few.mt = 0;
+  p.expand = p.few.mt ? !direct : !p.codes;
   return p;
 }
-// uint8 codes are dequantised by the lanes that multiply them, if there are few rows; otherwise, and where their rows are not whole
-// 16 bytes, they are expanded to binary16 first.
-static bool expands(const LinearPlan& p, int K) { return !p.few.mt || K % 16 != 0; }
+
+static bool linear_shape(int T, const frhip_weight* w) {
+  return T >= 0 && T <= 1 << 30 && w->K > 0 && w->K <= kLinearMostK && w->K % 8 == 0 && w->N > 0 && w->N <= 1 << 30;
+}
 
 constexpr int kLinearRows = 2;  // binary16 weights, us: 2 x 4096 x 2048 5.2 in rows, 5.5 as a few rows; 3 and 4 x 2048 x 8192 11.2 and 8.6
 
 static int launch_linear(LinearArgs a, bool u8, void* workspace, hipStream_t st) {
   if (!u8 && a.T <= kLinearRows) return a.T == 1 ? launch_rows<1>(a, st) : launch_rows<2>(a, st);
-  const LinearPlan p = plan_linear(a.T, a.K, a.N, compute_units());
+  const LinearPlan p = plan_linear(a.T, a.K, a.N, u8, compute_units());
   if (!p.few.mt && !p.tiles.rows) return set_error(FRHIP_ESHAPE, "linear: no tiles for this shape");
-  if (u8 && expands(p, a.K)) {
+  if (p.expand) {
+    if (!workspace) return set_error(FRHIP_EINVAL, "linear: null workspace");
+    if (off_grid(16, {workspace})) return set_error(FRHIP_EINVAL, "linear: workspace must be 16-byte aligned");
     if (int rc = dequant_u8_async(a.w, a.mx, a.rx, a.my, a.ry, static_cast<h1*>(workspace), a.K, a.N, st)) return rc;
     a.w = static_cast<const unsigned char*>(workspace);
     u8 = false;
+  }
+  if (!p.few.mt && p.codes) {
+    const LinearTiles t = {a, p.tiles.a.vw_base[0], p.tiles.a.vw_wide[0], p.tiles.a.vw_maxw};
+    if (p.tiles.rows == 128) q8_launch<128>(p.tiles, t, st);
+    else q8_launch<64>(p.tiles, t, st);
+    return check_launch("linear");
   }
   if (p.few.mt) return u8 ? launch_few<true>(a, p.few, st) : launch_few<false>(a, p.few, st);
   return a.K % kLdwBK ? launch_tiles<true>(a, p.tiles, st) : launch_tiles<false>(a, p.tiles, st);
@@ -813,9 +888,23 @@ static int launch_linear(LinearArgs a, bool u8, void* workspace, hipStream_t st)
 using namespace frhip;
 
 extern "C" size_t frhip_linear_workspace_bytes(int T, const frhip_weight* w) {
-  if (!w || T <= 0 || w->dtype != FRHIP_U8 || w->K <= 0 || w->K > kLinearMostK || w->N <= 0 || !expands(plan_linear(T, w->K, w->N, compute_units()), w->K))
+  if (!w || T <= 0 || w->dtype != FRHIP_U8 || !linear_shape(T, w) || !plan_linear(T, w->K, w->N, true, compute_units()).expand)
     return 0;
   return ((size_t)w->K * w->N * 2 + 255) / 256 * 256;  // the weight in binary16
+}
+
+extern "C" int frhip_linear_form(int T, const frhip_weight* w, int compute_units, int* out) {
+  if (!w || !out) return set_error(FRHIP_EINVAL, "linear_form: null pointer");
+  if (w->dtype != FRHIP_F16 && w->dtype != FRHIP_U8) return set_error(FRHIP_EINVAL, "linear_form: weight dtype must be F16 or U8");
+  if (T <= 0 || compute_units < 1 || !linear_shape(T, w)) return set_error(FRHIP_ESHAPE, "linear_form: no such product");
+  const bool u8 = w->dtype == FRHIP_U8;
+  out[0] = out[1] = out[2] = 0;
+  if (!u8 && T <= kLinearRows) return FRHIP_LINEAR_ROWS;
+  const LinearPlan p = plan_linear(T, w->K, w->N, u8, compute_units);
+  out[0] = p.few.mt ? p.few.mt * 16 : p.tiles.rows;
+  out[1] = p.few.mt ? p.few.nt * 16 : p.tiles.a.vw_maxw * 32;
+  out[2] = p.expand;
+  return p.few.mt ? FRHIP_LINEAR_FEW : p.codes ? FRHIP_LINEAR_CODES : FRHIP_LINEAR_TILES;
 }
 
 extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const float* bias, int act, const void* residual, int ldr, void* y,
@@ -825,13 +914,12 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   if (act != FRHIP_ACT_NONE && (act < FRHIP_ACT_SIGMOID || act > FRHIP_ACT_SOFTPLUS)) return set_error(FRHIP_EINVAL, "linear: unknown act");
   if (w->dtype != FRHIP_F16 && w->dtype != FRHIP_U8) return set_error(FRHIP_EINVAL, "linear: weight dtype must be F16 or U8");
   if (w->dtype == FRHIP_U8 && (!w->mx || !w->rx || !w->my || !w->ry)) return set_error(FRHIP_EINVAL, "linear: uint8 weight without mx/rx/my/ry");
-  if (T < 0 || T > 1 << 30 || w->K <= 0 || w->K > kLinearMostK || ldx > kLinearMostK || w->N <= 0 || w->N > 1 << 30 || w->K % 8 != 0) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T and N at most 2^30, rows at most 8388544 elements apart");
+  if (!linear_shape(T, w) || ldx > kLinearMostK) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T and N at most 2^30, rows at most 8388544 elements apart");
   if (ldx < w->K || ldx % 8 != 0 || ldy < w->N || (residual && ldr < w->N)) return set_error(FRHIP_ESHAPE, "linear: rows closer than their elements, or ldx no multiple of 8");
   if (T == 0) return 0;
   if (!x || !y) return set_error(FRHIP_EINVAL, "linear: null pointer");
   const size_t elem = out_dtype == FRHIP_F16 ? 2 : 4, rows = T, K = w->K, N = w->N;
-  if (off_grid(16, {x, w->data}) || off_grid(4, {bias}) || off_grid(elem, {residual, y}) || off_grid(2, {w->mx, w->rx}) ||
-      off_grid(4, {w->my, w->ry}))
+  if (off_grid(16, {x, w->data}) || off_grid(4, {bias}) || off_grid(elem, {residual, y}) || off_grid(4, {w->mx, w->rx, w->my, w->ry}))
     return set_error(FRHIP_EINVAL, "linear: pointer not aligned");
   const size_t ye = ((rows - 1) * ldy + N) * elem;
   auto hits = [&](const void* p, size_t bytes) { return rows_overlap(p, bytes, y, ye, 1, bytes, ye, 1); };
@@ -863,9 +951,5 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   a.out32 = out_dtype == FRHIP_F32;
   hipStream_t st = static_cast<hipStream_t>(s);
   const bool u8 = w->dtype == FRHIP_U8;
-  if (frhip_linear_workspace_bytes(T, w) > 0) {
-    if (!workspace) return set_error(FRHIP_EINVAL, "linear: null workspace");
-    if (off_grid(16, {workspace})) return set_error(FRHIP_EINVAL, "linear: workspace must be 16-byte aligned");
-  }
   return launch_linear(a, u8, workspace, st);
 }

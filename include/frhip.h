@@ -358,14 +358,23 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * frhip_gemm_act, which rounds ahead of the activation as the reference does).  x [T] rows of K binary16, ldx elements apart;
  * bias [N] fp32 or NULL; residual [T] rows of N in out_dtype, ldr apart, or NULL; y [T] rows of N in out_dtype (F16 or F32), ldy
  * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
- * K and ldx are multiples of 8, at most 8388544, N and T are any up to 2^30; x and w->data are 16-byte aligned, w->my and w->ry 4-byte, the others lie at
- * multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
+ * K and ldx are multiples of 8, at most 8388544, N and T are any up to 2^30; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte, the others
+ * lie at multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
  * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each. */
 #define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */
 #define FRHIP_ACT_SOFTPLUS 6 /* log(1 + exp(v)) */
 size_t frhip_linear_workspace_bytes(int T, const frhip_weight *w);
 int frhip_linear(const void *x, int ldx, const frhip_weight *w, const float *bias, int act, const void *residual, int ldr,
                  void *y, int ldy, int T, int out_dtype, void *workspace, frhip_stream s);
+
+/* How such a product goes out on a part with that many compute units, a pure function of T and the weight's K, N and dtype, for tests and
+ * measurements.  Returns the form or a negative FRHIP_E*; out[0], out[1]: rows and widest columns of a workgroup's tile (LINEAR_ROWS: 0,
+ * 0), out[2] = 1 if uint8 codes are expanded to binary16 first. */
+#define FRHIP_LINEAR_ROWS 0  /* one or two rows: the weight streamed through the waves */
+#define FRHIP_LINEAR_FEW 1   /* K split over the waves of a workgroup */
+#define FRHIP_LINEAR_TILES 2 /* of 64, 128 or 256 rows */
+#define FRHIP_LINEAR_CODES 3 /* tiles that dequantise uint8 codes on their way into LDS */
+int frhip_linear_form(int T, const frhip_weight *w, int compute_units, int *out);
 
 /* Short causal convolution over time, channel by channel:
  *   y[t][c] = act(bias[c] + sum_{j < W} w[c][j] * x[t - W + 1 + j][c])

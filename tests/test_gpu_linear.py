@@ -66,10 +66,25 @@ def case(T, K, N, act="none", bias=False, res=False, out="f16", quant=False, pad
 # T on both sides of every form's edge, K with and without a rest of 64 and 32, N with ragged ends
 @pytest.mark.parametrize("quant", [False, True])
 @pytest.mark.parametrize("T,K,N", [(1, 8, 1), (1, 1032, 33), (2, 2048, 130), (3, 40, 7), (4, 64, 64), (5, 256, 515), (16, 104, 48), (17, 2048, 100),
-                                   (33, 160, 37), (64, 520, 96), (65, 72, 130), (97, 584, 200), (129, 64, 32), (300, 168, 77), (513, 320, 264)])
+                                   (33, 160, 37), (64, 520, 96), (65, 72, 130), (97, 584, 200), (129, 64, 32), (300, 168, 77), (513, 320, 264),
+                                   (520, 256, 1024), (530, 192, 8192), (700, 200, 4000)])
 def test_sizes(T, K, N, quant):
     case(T, K, N, quant=quant)
     case(T, K, N, act="silu", bias=True, res=True, out="f32", quant=quant, pad=3, seed=1)
+
+
+def form(T, K, N, quant):
+    out = (C.c_int * 3)()
+    return L().frhip_linear_form(T, C.byref(fr.Weight(None, None, None, None, None, K, N, fr.U8 if quant else fr.F16)), 256, out), out[0], out[2]
+
+
+def test_the_sizes_above_reach_every_form():
+    """rows streamed, few rows, tiles of 64, 128 and 256 rows with and without a rest of K, tiles of codes, codes expanded ahead of either"""
+    sizes = next(m for m in test_sizes.pytestmark if m.args[0] == "T,K,N").args[1] + [(1030, 1096, 1290), (2050, 520, 4128), (2050, 512, 4128)]
+    got = {(f, rows if f != 1 else 0, e, K % 64 != 0) for T, K, N in sizes for q in (False, True) for f, rows, e in [form(T, K, N, q)]}
+    for want in [(0, 0, 0, False), (0, 0, 0, True), (1, 0, 0, False), (1, 0, 0, True), (1, 0, 1, True), (2, 64, 0, False), (2, 64, 0, True),
+                 (2, 128, 0, False), (2, 128, 0, True), (2, 128, 1, True), (2, 256, 0, False), (2, 256, 0, True), (3, 128, 0, False), (3, 64, 0, False)]:
+        assert want in got, (want, sorted(got))
 
 
 @pytest.mark.parametrize("out", ["f16", "f32"])
@@ -86,8 +101,11 @@ def test_residual_in_place(T, out):
     case(T, 128, 72, act="gelu", bias=True, out=out, pad=5, in_place=True)
 
 
-def test_a_large_product():
-    case(1030, 1096, 1290, act="softplus", bias=True, out="f32", pad=1)
+@pytest.mark.parametrize("T,K,N", [(1030, 1096, 1290), (2050, 520, 4128), (2050, 512, 4128)])
+def test_large_products(T, K, N):
+    case(T, K, N, act="softplus", bias=True, out="f32", pad=1)
+    case(T, K, N, bias=True, res=True)
+    case(T, K, N, act="silu", quant=True)
 
 
 def test_what_is_not_finite_stays_in_its_row():

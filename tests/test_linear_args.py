@@ -35,3 +35,41 @@ def test_no_weight_and_no_rows():
     assert f(A, 64, None, None, 0, None, 0, 3 * A, 32, 4, fr.F16, None, None) == EINVAL
     assert linear(T=0, x=None, y=None) == 0
     assert fr.lib().frhip_linear_workspace_bytes(4, None) == 0
+
+
+ROWS, FEW, TILES, CODES = range(4)
+
+
+def form(T, K, N, dtype, units=256):
+    out = (C.c_int * 3)()
+    rc = fr.lib().frhip_linear_form(T, C.byref(fr.Weight(A, A, A, A, A, K, N, dtype)), units, out)
+    return rc, tuple(out)
+
+
+def test_forms():
+    """What goes where; uint8 codes whose rows are no whole 16 bytes are expanded, as are those that no tile takes as they are"""
+    assert form(1, 2048, 2048, fr.F16) == (ROWS, (0, 0, 0)) and form(2, 8, 1, fr.F16)[0] == ROWS
+    assert form(3, 2048, 2048, fr.F16)[0] == form(1, 2048, 2048, fr.U8)[0] == FEW
+    assert form(1, 2056, 2048, fr.U8)[1][2] == 1 and form(1, 2064, 2048, fr.U8)[1][2] == 0
+    assert form(4099, 5120, 2560, fr.F16)[:1] + form(4099, 5120, 2560, fr.F16)[1][:1] == (TILES, 256)
+    assert form(512, 2048, 8192, fr.U8)[0] == CODES and form(512, 2056, 8192, fr.U8)[1][2] == form(512, 2048, 8200, fr.U8)[1][2] == 1
+
+
+def test_every_product_has_a_form():
+    for units in (1, 64, 256, 304):
+        for T in (1, 2, 3, 17, 64, 300, 513, 5000, 1 << 20):
+            for K in (8, 56, 64, 1000, 2048, 8388544):
+                for N in (1, 17, 2048, 50277, 1 << 20):
+                    for dtype in (fr.F16, fr.U8):
+                        rc, out = form(T, K, N, dtype, units)
+                        assert rc in (ROWS, FEW, TILES, CODES) and (rc == ROWS or out[0] > 0 and out[1] > 0)
+                        need = fr.lib().frhip_linear_workspace_bytes(T, C.byref(fr.Weight(A, A, A, A, A, K, N, dtype)))
+                        if units == 256:
+                            assert (need >= 2 * K * N) == (out[2] == 1) and (need == 0) == (out[2] == 0)
+
+
+def test_form_arguments():
+    out = (C.c_int * 3)()
+    f, w = fr.lib().frhip_linear_form, C.byref(fr.Weight(A, A, A, A, A, 64, 64, fr.F16))
+    assert f(1, None, 256, out) == f(1, w, 256, None) == EINVAL and f(0, w, 256, out) == f(1, w, 0, out) == ESHAPE
+    assert form(1, 60, 64, fr.F16)[0] == form(1, 8388552, 64, fr.F16)[0] == form(1, 64, (1 << 30) + 1, fr.F16)[0] == ESHAPE

@@ -18,8 +18,8 @@ def test_no_fragment_read_of_the_linear_tiles_is_outstanding_at_a_barrier(tmp_pa
         path.write_bytes(obj)
         listing = subprocess.run([OBJDUMP, "-d", "--mcpu=gfx950", str(path)], capture_output=True, text=True, check=True).stdout
         for name, body in functions(listing).items():
-            if re.search("linear_(ring|wide)_kernel", name):
+            if re.search("linear_(ring|wide|q8)_kernel", name):
                 assert any(t == "s_barrier" for _, t, _ in body) and any("mfma" in t for _, t, _ in body), name
                 assert not reads_outstanding_at_barriers(body), name
                 seen += 1
-    assert seen == 8  # tiles of 64, 128 (two depths) and 256 rows, K with and without a rest
+    assert seen == 10  # tiles of 64, 128 (two depths) and 256 rows, K with and without a rest; uint8: 64 and 128 rows
