@@ -2,6 +2,7 @@
 // any pitch.  Sums are fp32 on the MFMA units, the epilogue is fp32, and a result is rounded once.
 #include <climits>
 #include <cstring>
+#include <type_traits>
 
 #include "activations.h"
 #include "gemm_few_device.h"
@@ -37,127 +38,85 @@ __device__ __forceinline__ float activate(float v, int act) {
   }
 }
 
-// W consecutive outputs of a row, the first n of them stored; O: the type of y and the residual
-template <class O, int W>
-__device__ __forceinline__ void finish_as(const LinearArgs& a, const float (&acc)[W], int row, int col, int n) {
-  typedef O any __attribute__((ext_vector_type(W), aligned(sizeof(O))));
-  constexpr bool FINE = sizeof(O) == 4;
-  O* const y = static_cast<O*>(a.y) + (size_t)row * a.ldy + col;
-  const O* const res = a.res ? static_cast<const O*>(a.res) + (size_t)row * a.ldr + col : nullptr;
-  float r[W], v[W];
-#pragma unroll
-  for (int i = 0; i < W; i++) r[i] = 0.f;
-  if (res) {
-    if (n >= W) {
-      const any t = *reinterpret_cast<const any*>(res);
-#pragma unroll
-      for (int i = 0; i < W; i++) r[i] = (float)t[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < W; i++)
-        if (i < n) r[i] = (float)res[i];
+// f(activation, type of y and the residual), as types.  What ends a tile is a short loop for each of them: with the choice inside the loop,
+// unrolled, a tile of 256 rows spent 12 us between its last product and its end, most of it on fetching instructions (4096 x 2560 x
+// 10240, three rounds: 242 us, 220 so).
+template <class F>
+__device__ __forceinline__ void by_choice(const LinearArgs& a, F&& f) {
+  auto typed = [&](auto type) {
+    switch (a.act) {
+      case FRHIP_ACT_SIGMOID: f(std::integral_constant<int, FRHIP_ACT_SIGMOID>(), type); break;
+      case FRHIP_ACT_RELU2: f(std::integral_constant<int, FRHIP_ACT_RELU2>(), type); break;
+      case FRHIP_ACT_SILU: f(std::integral_constant<int, FRHIP_ACT_SILU>(), type); break;
+      case FRHIP_ACT_GELU: f(std::integral_constant<int, FRHIP_ACT_GELU>(), type); break;
+      case FRHIP_ACT_SOFTPLUS: f(std::integral_constant<int, FRHIP_ACT_SOFTPLUS>(), type); break;
+      default: f(std::integral_constant<int, FRHIP_ACT_NONE>(), type); break;
     }
-  }
-  if (a.bias) {
-    typedef float anyf __attribute__((ext_vector_type(W), aligned(4)));
-    if (n >= W) {
-      const anyf t = *reinterpret_cast<const anyf*>(a.bias + col);
-#pragma unroll
-      for (int i = 0; i < W; i++) v[i] = acc[i] + t[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < W; i++) v[i] = i < n ? acc[i] + a.bias[col + i] : 0.f;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; i++) v[i] = acc[i];
-  }
-#pragma unroll
-  for (int i = 0; i < W; i++) {
-    v[i] = activate<FINE>(v[i], a.act);
-    if (res) v[i] += r[i];
-  }
-  if (n >= W) {
-    any t;
-#pragma unroll
-    for (int i = 0; i < W; i++) t[i] = (O)v[i];
-    *reinterpret_cast<any*>(y) = t;
-  } else {
-#pragma unroll
-    for (int i = 0; i < W; i++)
-      if (i < n) y[i] = (O)v[i];
-  }
+  };
+  if (a.out32) typed(float());
+  else typed(h1());
 }
 
-template <int W>
-__device__ __forceinline__ void finish_outputs(const LinearArgs& a, const float (&acc)[W], int row, int col, int n) {
-  if (a.out32) finish_as<float>(a, acc, row, col, n);
-  else finish_as<h1>(a, acc, row, col, n);
+// One output from its sum
+template <int ACT, class O>
+__device__ __forceinline__ void finish_one(const LinearArgs& a, float sum, int row, int col) {
+  const float v = activate<sizeof(O) == 4>(a.bias ? sum + a.bias[col] : sum, ACT);
+  static_cast<O*>(a.y)[(size_t)row * a.ldy + col] = (O)(a.res ? v + (float)static_cast<const O*>(a.res)[(size_t)row * a.ldr + col] : v);
 }
+
+// Residual and bias of W consecutive outputs, requested ahead of their sums, and the outputs from these
+template <int ACT, class O, int W>
+struct Outputs {
+  typedef O any __attribute__((ext_vector_type(W), aligned(sizeof(O))));
+  typedef float anyf __attribute__((ext_vector_type(W), aligned(4)));
+  any r;
+  anyf b;
+  __device__ __forceinline__ void request(const LinearArgs& a, int row, int col) {
+    if (a.res) r = *reinterpret_cast<const any*>(static_cast<const O*>(a.res) + (size_t)row * a.ldr + col);
+    if (a.bias) b = *reinterpret_cast<const anyf*>(a.bias + col);
+  }
+  __device__ __forceinline__ void finish(const LinearArgs& a, const float (&s)[W], int row, int col) const {
+    any y;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+      const float v = activate<sizeof(O) == 4>(a.bias ? s[i] + b[i] : s[i], ACT);
+      y[i] = (O)(a.res ? v + (float)r[i] : v);
+    }
+    *reinterpret_cast<any*>(static_cast<O*>(a.y) + (size_t)row * a.ldy + col) = y;
+  }
+};
 
 // Groups of eight consecutive outputs whose sums are in LDS: place(t, row, col, sums) says where group t is, false: nowhere; a thread takes t0,
 // t0 + step, ... below `end`, two at a time, whose residuals and biases are requested together.
-template <int ACT, class O, class Place>
-__device__ __forceinline__ void finish_groups_as(const LinearArgs& a, int t0, int step, int end, Place&& place) {
-  typedef O any __attribute__((ext_vector_type(8), aligned(sizeof(O))));
-  typedef float anyf __attribute__((ext_vector_type(8), aligned(4)));
-  constexpr bool FINE = sizeof(O) == 4;
-  constexpr int G = 2;
-  const O* const res = static_cast<const O*>(a.res);
-  O* const out = static_cast<O*>(a.y);
+template <class Place>
+__device__ __forceinline__ void finish_groups(const LinearArgs& a, int t0, int step, int end, Place&& place) {
+  by_choice(a, [&](auto act, auto type) {
+    constexpr int G = 2;
 #pragma unroll 1
-  for (int t = t0; t < end; t += G * step) {
-    int row[G], col[G];
-    const float* sums[G];
-    bool in[G], whole[G];
-    any r[G];
-    anyf b[G];
+    for (int t = t0; t < end; t += G * step) {
+      int row[G], col[G];
+      const float* sums[G];
+      bool in[G], whole[G];
+      Outputs<decltype(act)::value, decltype(type), 8> o[G];
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-      in[g] = t + g * step < end && place(t + g * step, row[g], col[g], sums[g]);
-      whole[g] = in[g] && col[g] + 8 <= a.N;
-      if (whole[g] && res) r[g] = *reinterpret_cast<const any*>(res + (size_t)row[g] * a.ldr + col[g]);
-      if (whole[g] && a.bias) b[g] = *reinterpret_cast<const anyf*>(a.bias + col[g]);
-    }
+      for (int g = 0; g < G; g++) {
+        in[g] = t + g * step < end && place(t + g * step, row[g], col[g], sums[g]);
+        whole[g] = in[g] && col[g] + 8 <= a.N;
+        if (whole[g]) o[g].request(a, row[g], col[g]);
+      }
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-      if (whole[g]) {
-        float s[8];
-        read_sums(s, sums[g]);
-        any y;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float v = activate<FINE>(a.bias ? s[i] + b[g][i] : s[i], ACT);
-          y[i] = (O)(res ? v + (float)r[g][i] : v);
-        }
-        *reinterpret_cast<any*>(out + (size_t)row[g] * a.ldy + col[g]) = y;
-      } else if (in[g]) {  // the end of a row
+      for (int g = 0; g < G; g++) {
+        if (whole[g]) {
+          float s[8];
+          read_sums(s, sums[g]);
+          o[g].finish(a, s, row[g], col[g]);
+        } else if (in[g]) {  // the end of a row
 #pragma unroll 1
-        for (int i = 0; col[g] + i < a.N; i++) {
-          const float v = activate<FINE>(a.bias ? sums[g][i] + a.bias[col[g] + i] : sums[g][i], ACT);
-          out[(size_t)row[g] * a.ldy + col[g] + i] = (O)(res ? v + (float)res[(size_t)row[g] * a.ldr + col[g] + i] : v);
+          for (int i = 0; col[g] + i < a.N; i++) finish_one<decltype(act)::value, decltype(type)>(a, sums[g][i], row[g], col[g] + i);
         }
       }
     }
-  }
-}
-// One short loop for each activation and type: with the choice inside the loop, unrolled, a tile of 256 rows spent 12 us between its last
-// product and its end, most of it on fetching instructions (4096 x 2560 x 10240, three rounds: 242 us, 220 so).
-template <class O, class Place>
-__device__ __forceinline__ void finish_groups_of(const LinearArgs& a, int t0, int step, int end, Place&& place) {
-  switch (a.act) {
-    case FRHIP_ACT_SIGMOID: finish_groups_as<FRHIP_ACT_SIGMOID, O>(a, t0, step, end, place); break;
-    case FRHIP_ACT_RELU2: finish_groups_as<FRHIP_ACT_RELU2, O>(a, t0, step, end, place); break;
-    case FRHIP_ACT_SILU: finish_groups_as<FRHIP_ACT_SILU, O>(a, t0, step, end, place); break;
-    case FRHIP_ACT_GELU: finish_groups_as<FRHIP_ACT_GELU, O>(a, t0, step, end, place); break;
-    case FRHIP_ACT_SOFTPLUS: finish_groups_as<FRHIP_ACT_SOFTPLUS, O>(a, t0, step, end, place); break;
-    default: finish_groups_as<FRHIP_ACT_NONE, O>(a, t0, step, end, place); break;
-  }
-}
-template <class Place>
-__device__ __forceinline__ void finish_groups(const LinearArgs& a, int t0, int step, int end, Place&& place) {
-  if (a.out32) finish_groups_of<float>(a, t0, step, end, place);
-  else finish_groups_of<h1>(a, t0, step, end, place);
+  });
 }
 
 // ---------------------------------------------------------------------------
@@ -218,8 +177,7 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(LinearArgs a) {
     }
   const int t = lane / COLS, col = n0 + lane % COLS;
   if (t < TR && t < a.T && col < a.N) {
-    const float v[1] = {mine};
-    finish_outputs(a, v, t, col, 1);
+    by_choice(a, [&](auto act, auto type) { finish_one<decltype(act)::value, decltype(type)>(a, mine, t, col); });
   }
 }
 
@@ -420,24 +378,29 @@ __global__ __launch_bounds__(few_waves(MT, NT) * 64) void linear_few_kernel(Line
 #pragma unroll
     for (int j = 0; j < NT; j++) *reinterpret_cast<f4v*>(ring + ((t * NT + j) * 64 + lane) * 16) = acc[t][j];
   __syncthreads();
-  for (int t = wave; t < MT * NT; t += NW) {
-    const int i = t / NT, j = t - i * NT;
-    const int r0 = m0 + i * 16, c0 = n0 + j * 16;
-    if (r0 >= M || c0 >= N) continue;
-    const int row = r0 + row16;
-    f4v s = *reinterpret_cast<const f4v*>(few_smem + (t * 64 + lane) * 16);
+  by_choice(a, [&](auto act, auto type) {
+#pragma unroll 1
+    for (int t = wave; t < MT * NT; t += NW) {
+      const int i = t / NT, j = t - i * NT, row = m0 + i * 16 + row16, col = n0 + j * 16 + grp * 4;
+      const bool in = row < M && col < N, whole = in && col + 4 <= N;
+      Outputs<decltype(act)::value, decltype(type), 4> o;
+      if (whole) o.request(a, row, col);
+      float s[4];
 #pragma unroll
-    for (int w = 1; w < NW; w++) {
-      const f4v p = *reinterpret_cast<const f4v*>(few_smem + w * few_wave_bytes(MT, NT, U8) + (t * 64 + lane) * 16);
+      for (int w = 0; w < NW; w++) {  // in wave order
+        const f4v p = *reinterpret_cast<const f4v*>(few_smem + w * few_wave_bytes(MT, NT, U8) + (t * 64 + lane) * 16);
 #pragma unroll
-      for (int v = 0; v < 4; v++) s[v] += p[v];
+        for (int v = 0; v < 4; v++) s[v] = w == 0 ? p[v] : s[v] + p[v];
+      }
+      if (whole) {
+        o.finish(a, s, row, col);
+      } else if (in) {
+#pragma unroll
+        for (int v = 0; v < 4; v++)
+          if (col + v < N) finish_one<decltype(act)::value, decltype(type)>(a, s[v], row, col + v);
+      }
     }
-    const int col = c0 + grp * 4;
-    if (row < M && col < N) {
-      const float v[4] = {s[0], s[1], s[2], s[3]};
-      finish_outputs(a, v, row, col, N - col);
-    }
-  }
+  });
 }
 
 template <int MT, int NT, bool U8>
