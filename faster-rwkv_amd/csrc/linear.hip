@@ -797,7 +797,7 @@ static LinearPlan plan_linear(int T, int K, int N, bool u8, int cus) {
   p.few = plan_few(g, cus);
   g.seg[0].N = N;
   p.tiles = plan_ring(g, cus);
-  const TilePlan wide = plan_256(g, cus);
+  const TilePlan wide = T > 128 ? plan_256(g, cus) : TilePlan();
   if (wide.rows && (!p.tiles.rows || wide.us <= p.tiles.us * 1.05)) p.tiles = wide;
   if (!u8) {
     if (p.few.mt && p.tiles.rows && p.tiles.us < p.few.us) p.few.mt = 0;
