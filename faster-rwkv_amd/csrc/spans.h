@@ -25,6 +25,11 @@ inline bool spans_clash(const void* a, const void* b, size_t bytes) {  // neithe
   return pa != pb && pa < pb + bytes && pb < pa + bytes;
 }
 
+inline bool spans_meet(const void* a, size_t bytes_a, const void* b, size_t bytes_b) {
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  return a && b && pa < pb + bytes_b && pb < pa + bytes_a;
+}
+
 inline bool off_grid(size_t elem, std::initializer_list<const void*> ptrs) {
   uintptr_t v = 0;
   for (const void* p : ptrs) v |= reinterpret_cast<uintptr_t>(p);

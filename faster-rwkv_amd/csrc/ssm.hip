@@ -396,7 +396,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   int buf = 0;
   for (int t = t0; t < t1; t += TB, buf ^= 1) {
     __syncthreads();
-#pragma unroll 8
+#pragma unroll 4
     for (int r = 0; r < TB; r++) {
       const float2 v = du[buf][r][at];
       float y0 = 0.f, y1 = 0.f;
@@ -548,6 +548,7 @@ static ScanShape scan_shape(const frhip_ssm& p) {
   return s;
 }
 
+constexpr int kMostRows = 1 << 30;     // of a call of single tokens: a loop over them counts in steps of up to 2^18
 constexpr int kScanLeast = 16;         // rows of a chunk, at least
 constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
 
@@ -639,6 +640,12 @@ static int conv_check(int C, int W, const void* x, int ldx, const float* w, cons
                rows_overlap(yr, (rows - 1) * ldy + C, state_out, se, 1, (rows - 1) * ldy + C, se, elem) ||
                rows_overlap(xr, (rows - 1) * ldx + C, state_out, se, 1, (rows - 1) * ldx + C, se, elem)))
     return set_error(FRHIP_EINVAL, "conv: an output overlaps what is read");
+  const size_t ye = rows ? ((rows - 1) * ldy + C) * elem : 0;
+  for (const void* out : {static_cast<const void*>(yr), static_cast<const void*>(state_out)}) {
+    const size_t bytes = out == yr ? ye : sbytes;
+    if (spans_meet(out, bytes, w, (size_t)C * W * 4) || spans_meet(out, bytes, bias, (size_t)C * 4))
+      return set_error(FRHIP_EINVAL, "conv: an output overlaps a parameter");
+  }
   if (spans_clash(state, state_out, sbytes)) return set_error(FRHIP_EINVAL, "conv: states overlap in part");
   return 0;
 }
@@ -690,10 +697,16 @@ static int ssm_check(const frhip_ssm& p, const SsmCall& c, size_t row0, size_t r
   if (off_grid(elem, {c.x, c.dt, c.B, c.C, c.z, c.y}) || off_grid(4, {c.state, c.state_out}))
     return set_error(FRHIP_EINVAL, "ssm: pointer not aligned to its element");
   if (spans_clash(c.state, c.state_out, sn * 4)) return set_error(FRHIP_EINVAL, "ssm: states overlap in part");
+  const size_t dn = (size_t)p.channels * 4;
+  auto meets_parameter = [&](const void* out, size_t bytes) {
+    return spans_meet(out, bytes, p.A, dn * p.states) || spans_meet(out, bytes, p.D, dn) || spans_meet(out, bytes, p.dt_bias, dn);
+  };
+  if (meets_parameter(c.state_out, sn * 4)) return set_error(FRHIP_EINVAL, "ssm: an output overlaps a parameter");
   if (!rows) return 0;
   struct In { const void* p; int ld, cols; };
   const char* y = static_cast<const char*>(c.y) + row0 * c.ldy * elem;
   const size_t ye = (rows - 1) * c.ldy + p.channels;
+  if (meets_parameter(y, ye * elem)) return set_error(FRHIP_EINVAL, "ssm: an output overlaps a parameter");
   for (const In& in : {In{c.x, c.ldx, p.channels}, In{c.dt, c.lddt, p.channels}, In{c.B, c.ldb, bn}, In{c.C, c.ldc, bn}, In{c.z, c.ldz, p.channels}}) {
     if (!in.p) continue;
     const char* q = static_cast<const char*>(in.p) + row0 * in.ld * elem;
@@ -829,7 +842,7 @@ using namespace frhip;
 
 extern "C" int frhip_conv_one(int rows, int C, int W, const void* x, int ldx, const float* w, const float* bias, int act, const void* state,
                               void* state_out, void* y, int ldy, int dtype, frhip_stream s) {
-  if (rows < 0) return set_error(FRHIP_ESHAPE, "conv_one: negative rows");
+  if (rows < 0 || rows > kMostRows) return set_error(FRHIP_ESHAPE, "conv_one: rows must be 0 to 2^30");
   if (int rc = conv_check(C, W, x, ldx, w, bias, act, state, state_out, y, ldy, dtype, 0, rows, rows)) return rc;
   if (rows == 0) return 0;
   hipStream_t st = static_cast<hipStream_t>(s);
@@ -858,7 +871,7 @@ extern "C" int frhip_ssm_one(const frhip_ssm* p, int rows, const void* x, int ld
                              const void* C, int ldc, const void* z, int ldz, const float* state, float* state_out, void* y, int ldy,
                              int dtype, frhip_stream s) {
   if (int rc = ssm_check_params(p)) return rc;
-  if (rows < 0) return set_error(FRHIP_ESHAPE, "ssm_one: negative rows");
+  if (rows < 0 || rows > kMostRows) return set_error(FRHIP_ESHAPE, "ssm_one: rows must be 0 to 2^30");
   const SsmCall c = {x, dt, B, C, z, ldx, lddt, ldb, ldc, ldz, state, state_out, y, ldy, dtype};
   if (int rc = ssm_check(*p, c, 0, rows, rows)) return rc;
   if (rows == 0) return 0;

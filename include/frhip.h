@@ -348,7 +348,7 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
 /* Recurrent layers whose decay depends on the input (no counterpart in the reference; they stand beside att_one / att_seq).
  * Activations are FRHIP_F16 or FRHIP_F32 (`dtype`: x, dt, B, C, z, y and the convolution's state), rows `ld` elements apart, at any
  * address that is a multiple of their element's size; parameters and the scan's state are fp32.  Sums, decays and states
- * are held in fp32; an output is rounded once.  A `_one` call takes one token each of `rows` sequences; a `_seq` call takes
+ * are held in fp32; an output is rounded once.  A `_one` call takes one token each of `rows` sequences (up to 2^30); a `_seq` call takes
  * nseq prompts that lie one behind the other: prompt i is rows seq_start[i] .. seq_start[i + 1] - 1 (seq_start: nseq + 1
  * numbers in HOST memory, read before the call returns, not descending, the first not negative).  A prompt of no rows leaves
  * its state as it was; rows ahead of the first prompt and behind the last are neither read nor written.  States are [nseq or rows][...],

@@ -199,6 +199,7 @@ class Scan:
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("d,n,groups,lens", [(1, 1, 1, [1]), (65, 3, 1, [9]), (64, 16, 1, [0]), (130, 5, 2, [8, 0, 17, 1]),
                                              (96, 16, 1, [700]), (48, 24, 3, [33, 40]), (70, 64, 1, [260, 3]), (10, 130, 2, [50]), (33, 256, 1, [70]),
+                                             (20, 100, 2, [40, 3]), (65, 40, 1, [21]),
                                              (300, 8, 1, [16, 15, 250])])
 def test_scan_seq(d, n, groups, lens, dtype):
     s = Scan(d * n, d, n, lens, dtype, groups)

@@ -25,7 +25,8 @@ def conv(seq=True, **kw):
     (dict(n=-1), ESHAPE), (dict(C=0), ESHAPE), (dict(W=1), ESHAPE), (dict(W=5), ESHAPE), (dict(ldx=7), ESHAPE), (dict(ldy=7), ESHAPE),
     (dict(x=None), EINVAL), (dict(w=None), EINVAL), (dict(state=None), EINVAL), (dict(out=None), EINVAL), (dict(y=None), EINVAL),
     (dict(act=2), EINVAL), (dict(dtype=fr.U8), EINVAL), (dict(x=A + 1), EINVAL), (dict(w=2 * A + 2), EINVAL), (dict(dtype=fr.F32, y=5 * A + 2), EINVAL),
-    (dict(y=A), EINVAL), (dict(y=A + 14), EINVAL), (dict(out=3 * A + 2), EINVAL), (dict(y=3 * A), EINVAL), (dict(y=4 * A + 40), EINVAL), (dict(out=A), EINVAL)])
+    (dict(y=A), EINVAL), (dict(y=A + 14), EINVAL), (dict(out=3 * A + 2), EINVAL), (dict(y=3 * A), EINVAL), (dict(y=4 * A + 40), EINVAL), (dict(out=A), EINVAL),
+    (dict(w=5 * A + 4), EINVAL), (dict(bias=5 * A), EINVAL), (dict(w=4 * A), EINVAL)])
 def test_conv_refusals(kw, code, seq):
     assert conv(seq, **kw) == code and fr.lib().frhip_error_string()
 
@@ -33,6 +34,10 @@ def test_conv_refusals(kw, code, seq):
 def test_conv_seq_refuses_starts_that_descend():
     assert conv(at=None) == EINVAL
     assert conv(at=starts(-1, 4)) == ESHAPE and conv(n=2, at=starts(0, 4, 3)) == ESHAPE
+
+
+def test_single_tokens_of_too_many_sequences():
+    assert conv(False, n=(1 << 30) + 1) == scan(False, n=(1 << 30) + 1) == ESHAPE
 
 
 def test_conv_of_nothing():
@@ -58,7 +63,7 @@ def scan(seq=True, params=None, **kw):
     (dict(ldy=7), ESHAPE), (dict(x=None), EINVAL), (dict(dt=None), EINVAL), (dict(B=None), EINVAL), (dict(C=None), EINVAL), (dict(state=None), EINVAL),
     (dict(out=None), EINVAL), (dict(y=None), EINVAL), (dict(dtype=fr.U8), EINVAL), (dict(x=2 * A + 1), EINVAL), (dict(state=7 * A + 2), EINVAL),
     (dict(y=2 * A), EINVAL), (dict(y=6 * A), EINVAL), (dict(y=4 * A + 2), EINVAL), (dict(out=7 * A + 4), EINVAL), (dict(out=2 * A), EINVAL), (dict(y=7 * A), EINVAL),
-    (dict(params=dict(A=None)), EINVAL), (dict(params=dict(A=A + 2)), EINVAL), (dict(params=dict(D=A + 1)), EINVAL), (dict(params=dict(channels=9)), ESHAPE),
+    (dict(params=dict(A=9 * A)), EINVAL), (dict(params=dict(D=8 * A)), EINVAL), (dict(params=dict(bias=9 * A + 4)), EINVAL), (dict(params=dict(A=None)), EINVAL), (dict(params=dict(A=A + 2)), EINVAL), (dict(params=dict(D=A + 1)), EINVAL), (dict(params=dict(channels=9)), ESHAPE),
     (dict(params=dict(channels=0)), ESHAPE), (dict(params=dict(states=0)), ESHAPE), (dict(params=dict(states=257)), ESHAPE), (dict(params=dict(groups=0)), ESHAPE)])
 def test_scan_refusals(kw, code, seq):
     assert scan(seq, **kw) == code and fr.lib().frhip_error_string()
