@@ -248,8 +248,9 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   constexpr int STAGE = (TB * 2 * NT + WAVES * 64 - 1) / (WAVES * 64);  // elements of B and C of a thread
   static_assert(ROWS * NW == TB, "every row has its wave");
   constexpr bool FINE = sizeof(T) == 4;
-  __shared__ __attribute__((aligned(16))) float bc[2][TB][2][NT];
-  __shared__ float2 du[2][TB][CH];
+  constexpr int BUFS = LOCAL ? 2 : 1;  // LOCAL takes the next block's rows while waves still scan this one
+  __shared__ __attribute__((aligned(16))) float bc[BUFS][TB][2][NT];
+  __shared__ float2 du[BUFS][TB][CH];
   __shared__ float part[LOCAL || NW == 1 ? 1 : NW][TB][CH];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), cw = wave / NW, nw = wave % NW;
   const int j0 = blockIdx.y;
@@ -394,27 +395,19 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
     if (t0 + TB < t1) request(t0 + TB);
   }
   int buf = 0;
-  for (int t = t0; t < t1; t += TB, buf ^= 1) {
+  for (int t = t0; t < t1; t += TB, buf ^= BUFS - 1) {
     __syncthreads();
 #pragma unroll 4
     for (int r = 0; r < TB; r++) {
       const float2 v = du[buf][r][at];
-      float y0 = 0.f, y1 = 0.f;
+      float y = 0.f;
 #pragma unroll
       for (int k = 0; k < NPL; k++) {
         const float decay = __builtin_amdgcn_exp2f(v.x * A2[k]);
         h[k] = __builtin_fmaf(decay, h[k], v.y * bc[buf][r][0][n0 + k]);
-        if constexpr (!LOCAL) {
-          float& y = k & 1 ? y1 : y0;
-          y = __builtin_fmaf(bc[buf][r][1][n0 + k], h[k], y);
-        }
+        if constexpr (!LOCAL) y = k ? __builtin_fmaf(bc[buf][r][1][n0 + k], h[k], y) : bc[buf][r][1][n0] * h[0];
       }
-      if constexpr (!LOCAL) part[NW == 1 ? 0 : nw][r][at] = y0 + y1;
-    }
-    float xn[ROWS], zn[ROWS];
-    if (t + TB < t1) {
-      take(t + TB, buf ^ 1, xn, zn);
-      if (t + 2 * TB < t1) request(t + 2 * TB);
+      if constexpr (!LOCAL) part[NW == 1 ? 0 : nw][r][at] = y;
     }
     if constexpr (!LOCAL) {
       __syncthreads();
@@ -429,8 +422,10 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
         if (mine && t + row < t1) *reinterpret_cast<T*>(reinterpret_cast<char*>(a.y + (size_t)(t + row) * a.ldy) + at_row) = (T)y;
       }
     }
-#pragma unroll
-    for (int r = 0; r < ROWS; r++) x[r] = xn[r], z[r] = zn[r];
+    if (t + TB < t1) {
+      take(t + TB, buf ^ (BUFS - 1), x, z);
+      if (t + 2 * TB < t1) request(t + 2 * TB);
+    }
   }
   if constexpr (LOCAL) {  // the waves' sums of dt, in wave order
     __shared__ float total[NW][CH];
