@@ -247,6 +247,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   constexpr int ROWS = TB * CW / WAVES;                                  // rows of a wave in A and C: of its 64 channels
   constexpr int STAGE = (TB * 2 * NT + WAVES * 64 - 1) / (WAVES * 64);  // elements of B and C of a thread
   static_assert(ROWS * NW == TB, "every row has its wave");
+  constexpr int UNROLL = NPL == 4 ? 4 : 2;  // rows in B; 8 and 16 of four states took 1 and 8 % longer, 4 of eight spilled
   constexpr bool FINE = sizeof(T) == 4;
   constexpr int BUFS = LOCAL ? 2 : 1;  // LOCAL takes the next block's rows while waves still scan this one
   __shared__ __attribute__((aligned(16))) float bc[BUFS][TB][2][NT];
@@ -397,7 +398,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   int buf = 0;
   for (int t = t0; t < t1; t += TB, buf ^= BUFS - 1) {
     __syncthreads();
-#pragma unroll 4
+#pragma unroll UNROLL
     for (int r = 0; r < TB; r++) {
       const float2 v = du[buf][r][at];
       float y = 0.f;
@@ -546,13 +547,12 @@ static ScanShape scan_shape(const frhip_ssm& p) {
 constexpr int kMostRows = 1 << 30;     // of a call of single tokens: a loop over them counts in steps of up to 2^18
 constexpr int kScanLeast = 16;         // rows of a chunk, at least
 constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
-
 constexpr int kScanRows = 16;          // a chunk is a multiple of it
 
-// Rows of a chunk: enough chunks for four workgroups a compute unit, four waves a SIMD (4096 rows of 4096 channels x 16 states, with two,
-// three, four: 165, 142, 130 us)
+// Rows of a chunk: enough chunks for four workgroups a compute unit (4096 rows of 4096 channels x 16 states, with two, three, four: 165, 142,
+// 130 us, six and eight in shorter blocks 136 and 127; 830 rows of 1280 x 64, workgroups of eight waves, with two, four: 46, 41)
 static int scan_chunk(const ScanShape& s, int T, int cus) {
-  const int units = cus * 4 < kScanMostUnits ? cus * 4 : kScanMostUnits;
+  const int units = cus < kScanMostUnits / 4 ? cus * 4 : kScanMostUnits;
   const int q = units / s.wgs > 1 ? units / s.wgs : 1;
   int len = T / q + (T % q ? 1 : 0);
   if (len < kScanLeast) len = kScanLeast;
