@@ -236,11 +236,16 @@ constexpr int scan_waves(int nw) { return nw < 4 ? 4 : nw; }
 constexpr int scan_rows(int nw) { return nw == 1 ? 8 : 16; }  // of a block of time, the rows that go through LDS together
 
 // LOCAL: step 1 of the scan, otherwise step 2.  A workgroup walks its chunk in blocks of time.  Of a block, every wave
-//   A. takes some rows to LDS: dt and dt x of a channel a lane (the next block's, while this one is scanned), and B and C as fp32;
+//   A. takes some rows to LDS: dt and dt x of a channel a lane, and B and C as fp32;
 //   B. runs all of its rows with NPL states a lane in registers, and leaves its part of y in LDS;
 //   C. adds the parts of the rows that it took in A, applies skip and gate and stores them.
-// The step width's softplus and the gate are so evaluated once a channel and row, not once a wave.  What bounds it is the issue of
-// vector instructions: 4, and an exponential of twice their length, a state and row.  The waves of a SIMD have to be several for that.
+// The step width's softplus and the gate are so evaluated once a channel and row, not once a wave, and a chunk's states are over several
+// waves, which a SIMD needs to keep issuing.  What bounds it are vector instructions: a state and row takes two products, two
+// multiply-adds and an exponential (3.6 and 8.4 cycles a wave), in step 1 one less, and the softplus, gate, conversions and sums of A and C come
+// to a third as much again; they are issued in three quarters of the cycles.  4096 rows of 4096 channels x 16 states, binary16: 126 us
+// (55 + 71 in the two steps), memory alone would be 26; a lane with all 16 states of a channel and one wave a SIMD took 368.
+// Not kept: dt x times B as an outer product on the matrix units, 152; shorter blocks of time or five to eight workgroups a compute unit, 127 to
+// 136; rows through buffer descriptors, 131.
 template <class T, int NPL, int NW, bool LOCAL>
 __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
   constexpr int WAVES = scan_waves(NW), CW = WAVES / NW, NT = NPL * NW, TB = scan_rows(NW), CH = CW * 64;
