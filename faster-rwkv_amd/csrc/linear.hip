@@ -208,8 +208,8 @@ static int launch_rows(const LinearArgs& a, hipStream_t st) {
 
 // ---------------------------------------------------------------------------
 // A few rows, one launch, K split over the waves of a workgroup (gemm_few.hip has the form, its reasons and its choice of tiles), here with
-// rows of any pitch, any N, and a K that need not fill its last step (a multiple of 8, of uint8 codes 16): the last step's loads of
-// what is not there repeat the step's begin, and what they bring counts as zero.
+// rows of any pitch, any N, and a K that need not fill its last step (a multiple of 8): the last step's loads of
+// what is not there repeat the step's begin, and what they bring counts as zero.  Codes are loaded 16 a lane, from any multiple of 8 bytes.
 // ---------------------------------------------------------------------------
 template <int MT, int NT, bool U8>
 __global__ __launch_bounds__(few_waves(MT, NT) * 64) void linear_few_kernel(LinearArgs a) {
@@ -270,10 +270,16 @@ __global__ __launch_bounds__(few_waves(MT, NT) * 64) void linear_few_kernel(Line
 #pragma unroll
       for (int b = 0; b < (U8 ? NT : 2 * NT); b++) {
         const unsigned seg = U8 ? (lane & 3) ^ (lane >> 4) : (lane & 7) ^ lr ^ (b & 1);
-        if ((int)seg * (U8 ? 16 : 8) >= krest) vb[b] -= seg * 16;
+        if (U8 && (krest & 8)) {  // the last 16 codes, of which the half that ends K is wanted; they may begin ahead of the step
+          vb[b] += (int)seg * 16 + 16 > krest ? krest - seg * 16 : 16;
+        } else if ((int)seg * (U8 ? 16 : 8) >= krest) {
+          vb[b] -= seg * 16;
+        }
       }
-      if constexpr (U8)
+      if constexpr (U8) {
+        if (krest & 8) bk -= 16;
         if ((lane & 31) * 2 >= krest) scale_k -= (lane & 31) * 2;
+      }
     }
 #pragma unroll
     for (int b = 0; b < (U8 ? NT : 2 * NT); b++) load_lds_saddr(vb[b], bk, st + kBOff + b * 1024);
@@ -339,6 +345,11 @@ __global__ __launch_bounds__(few_waves(MT, NT) * 64) void linear_few_kernel(Line
         q[t] = *reinterpret_cast<const u32x4*>(st + kBOff + t * 1024 + row16 * 64 + ((grp ^ (row16 >> 2)) * 16));
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
       if (i + S < mine) issue(i + S);
+      if ((krest & 8) && (wave + i * NW) * 64 + 64 > K) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+          if (grp == krest >> 4) q[t][0] = q[t][2], q[t][1] = q[t][3];
+      }
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -808,7 +819,7 @@ static LinearPlan plan_linear(int T, int K, int N, bool u8, int cus) {
     if (p.few.mt && p.tiles.rows && p.tiles.us < p.few.us) p.few.mt = 0;
     return p;
   }
-  // codes: dequantised by the lanes that multiply them (rows of whole 16 bytes), on their way into LDS, or expanded ahead of either
+  // codes: dequantised by the lanes that multiply them (K of 24 and more, or 16), on their way into LDS, or expanded ahead of either
   const double expand = 5.5 + 3.0 * K * N / 6.3e6;
   if (K % kLdwBK == 0 && N % 16 == 0) {
     const TilePlan q8 = plan_q8(g, cus);
@@ -817,7 +828,7 @@ static LinearPlan plan_linear(int T, int K, int N, bool u8, int cus) {
       p.codes = true;
     }
   }
-  const bool direct = K % 16 == 0;
+  const bool direct = K >= 16;
   const double few = p.few.us + (direct ? 0 : expand), tiles = p.tiles.us + (p.codes ? 0 : expand);
   if (p.few.mt && p.tiles.rows && tiles < few) p.few.mt = 0;
   p.expand = p.few.mt ? !direct : !p.codes;

@@ -230,7 +230,7 @@ __global__ void dequant_u8_kernel(const uint32_t* __restrict__ q, const h1* __re
   out[i] = (h4){lo.x, lo.y, hi.x, hi.y};
 }
 
-// The same, eight consecutive codes of four rows per thread (K a multiple of 16): ry and my are read once for four
+// The same, eight consecutive codes of four rows per thread (K a multiple of 8): ry and my are read once for four
 // rows, a wave reads 512 and writes 1024 consecutive bytes of a row per instruction.  Where a seq-mode
 // launch does not dequantise its uint8 weights by itself (from about 512 rows on), it expands them with this before the
 // binary16 GEMM, so it runs at copy rate or the expansion eats what it saves.
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(1024) void argmax_f32_kernel(const float* __restric
 int dequant_u8_async(const unsigned char* q, const h1* mx, const h1* rx, const h1* my, const h1* ry, h1* dst, int K, int N,
                      hipStream_t st) {
   const size_t words = (size_t)N * (K / 4);
-  if (K % 16 != 0 || (size_t)N * (K / 16) >= (1u << 31) || reinterpret_cast<uintptr_t>(q) % 16 != 0 ||
+  if (K % 8 != 0 || (size_t)N * (K / 16) >= (1u << 31) || reinterpret_cast<uintptr_t>(q) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(dst) % 16 != 0 || reinterpret_cast<uintptr_t>(ry) % 16 != 0 || reinterpret_cast<uintptr_t>(my) % 16 != 0) {
     hipLaunchKernelGGL(dequant_u8_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, st, (const uint32_t*)q, mx, rx, my, ry,
                        (h4*)dst, K, N);
@@ -402,7 +402,7 @@ int dequant_u8_async(const unsigned char* q, const h1* mx, const h1* rx, const h
 
 int dequant_u8_group_async(int nseg, const unsigned char* const* q, const h1* const* mx, const h1* const* rx, const h1* const* my,
                            const h1* const* ry, h1* const* dst, int K, const int* N, hipStream_t st) {
-  bool fast = K % 16 == 0 && nseg >= 1 && nseg <= 4;
+  bool fast = K % 8 == 0 && nseg >= 1 && nseg <= 4;
   int most = 0;
   DequantGroup g = {};
   for (int s = 0; fast && s < nseg; s++) {

@@ -310,7 +310,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
     load_group<float, 4>(v, a.A + (size_t)d * a.N + n0 + k, a.N - n0 - k);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      A2[k + e] = v[e] * kLog2e;
+      A2[k + e] = v[e] < -1e38f ? -1e38f : v[e] * kLog2e;  // rows past the chunk have a step of zero, which an infinite rate would make a NaN
       h[k + e] = 0.f;
     }
   }

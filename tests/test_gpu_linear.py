@@ -101,6 +101,14 @@ def test_residual_in_place(T, out):
     case(T, 128, 72, act="gelu", bias=True, out=out, pad=5, in_place=True)
 
 
+@pytest.mark.parametrize("K", [16, 24, 32, 40, 56, 72, 88, 120, 520, 1032, 1048])
+def test_codes_of_rows_of_any_multiple_of_eight(K):
+    """The last 16 codes of a row may begin ahead of the last step, and the next row's begin inside them"""
+    for T, N in ((1, 33), (20, 130), (70, 17)):
+        assert form(T, K, N, True)[0] == 1 and form(T, K, N, True)[2] == 0
+        case(T, K, N, quant=True, seed=K)
+
+
 @pytest.mark.parametrize("T,K,N", [(1030, 1096, 1290), (2050, 520, 4128), (2050, 512, 4128)])
 def test_large_products(T, K, N):
     case(T, K, N, act="softplus", bias=True, out="f32", pad=1)

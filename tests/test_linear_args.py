@@ -47,10 +47,10 @@ def form(T, K, N, dtype, units=256):
 
 
 def test_forms():
-    """What goes where; uint8 codes whose rows are no whole 16 bytes are expanded, as are those that no tile takes as they are"""
+    """What goes where; uint8 codes that no tile takes as they are, and rows of eight, are expanded"""
     assert form(1, 2048, 2048, fr.F16) == (ROWS, (0, 0, 0)) and form(2, 8, 1, fr.F16)[0] == ROWS
     assert form(3, 2048, 2048, fr.F16)[0] == form(1, 2048, 2048, fr.U8)[0] == FEW
-    assert form(1, 2056, 2048, fr.U8)[1][2] == 1 and form(1, 2064, 2048, fr.U8)[1][2] == 0
+    assert form(1, 8, 2048, fr.U8)[1][2] == 1 and form(1, 16, 2048, fr.U8)[1][2] == form(1, 24, 2048, fr.U8)[1][2] == form(1, 2056, 2048, fr.U8)[1][2] == 0
     assert form(4099, 5120, 2560, fr.F16)[:1] + form(4099, 5120, 2560, fr.F16)[1][:1] == (TILES, 256)
     assert form(512, 2048, 8192, fr.U8)[0] == CODES and form(512, 2056, 8192, fr.U8)[1][2] == form(512, 2048, 8200, fr.U8)[1][2] == 1
 
