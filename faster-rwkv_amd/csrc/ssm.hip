@@ -553,14 +553,22 @@ constexpr int kMostRows = 1 << 30;     // of a call of single tokens: a loop ove
 constexpr int kScanLeast = 16;         // rows of a chunk, at least
 constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
 constexpr int kScanRows = 16;          // a chunk is a multiple of it
+constexpr int kScanWhole = 32;         // prompts of up to so many rows are not cut
 
 // Rows of a chunk: enough chunks for four workgroups a compute unit (4096 rows of 4096 channels x 16 states, with two, three, four: 165, 142,
-// 130 us, six and eight in shorter blocks 136 and 127; 830 rows of 1280 x 64, workgroups of eight waves, with two, four: 46, 41)
-static int scan_chunk(const ScanShape& s, int T, int cus) {
+// 130 us, six and eight in shorter blocks 136 and 127; 830 rows of 1280 x 64, workgroups of eight waves, with two, four: 46, 41).
+// Where no prompt has more than kScanWhole rows the first launch costs more than it shares out (1536 channels x 16 states, in chunks of 16 and
+// whole: 17 rows 8.8 and 7.0 us, 32 rows 8.9 and 7.0, 48 rows 8.9 and 9.1; x 64 states: 13.6 and 10.6, 13.6 and 10.7, 13.9 and 14.7).
+static int scan_chunk(const ScanShape& s, int nseq, const int32_t* start, int cus) {
+  const int T = start[nseq] - start[0];
+  int longest = 0;
+  for (int i = 0; i < nseq; i++)
+    if (start[i + 1] - start[i] > longest) longest = start[i + 1] - start[i];
   const int units = cus < kScanMostUnits / 4 ? cus * 4 : kScanMostUnits;
   const int q = units / s.wgs > 1 ? units / s.wgs : 1;
   int len = T / q + (T % q ? 1 : 0);
   if (len < kScanLeast) len = kScanLeast;
+  if (longest <= kScanWhole && len < longest) len = longest;
   return len > INT_MAX - kScanRows ? INT_MAX : (len + kScanRows - 1) / kScanRows * kScanRows;
 }
 
@@ -782,7 +790,7 @@ static int ssm_seq_run(const frhip_ssm& p, const SsmCall& c, int nseq, const int
   for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {
     SeqTable tab;
     a.nseq = nseq - s0 < kSeqTable ? nseq - s0 : kSeqTable;
-    a.chunk = scan_chunk(s, start[s0 + a.nseq] - start[s0], compute_units());
+    a.chunk = scan_chunk(s, a.nseq, start + s0, compute_units());
     const int chunks = scan_table(tab, start, s0, a.nseq, a.chunk);
     a.nlocal = chunks - a.nseq;
     if ((size_t)a.nlocal > scan_most_local(s, rows)) return set_error(FRHIP_ESTATE, "ssm_seq: more chunks than the workspace holds");
@@ -911,7 +919,7 @@ extern "C" int frhip_ssm_cut(const frhip_ssm* p, int nseq, const int32_t* seq_st
   if (nseq < 1 || nseq > kSeqTable) return set_error(FRHIP_ESHAPE, "ssm_cut: 1 to 128 prompts");
   const ScanShape s = scan_shape(*p);
   SeqTable tab;
-  out[0] = scan_chunk(s, seq_start[nseq] - seq_start[0], compute_units);
+  out[0] = scan_chunk(s, nseq, seq_start, compute_units);
   out[1] = scan_table(tab, seq_start, 0, nseq, out[0]);
   out[2] = s.wgs;
   return 0;

@@ -200,7 +200,8 @@ class Scan:
 @pytest.mark.parametrize("d,n,groups,lens", [(1, 1, 1, [1]), (65, 3, 1, [9]), (64, 16, 1, [0]), (130, 5, 2, [8, 0, 17, 1]),
                                              (96, 16, 1, [700]), (48, 24, 3, [33, 40]), (70, 64, 1, [260, 3]), (10, 130, 2, [50]), (33, 256, 1, [70]),
                                              (20, 100, 2, [40, 3]), (65, 40, 1, [21]),
-                                             (300, 8, 1, [16, 15, 250])])
+                                             (300, 8, 1, [16, 15, 250]),
+                                             (70, 16, 1, [32, 17, 0, 31]), (130, 64, 1, [32]), (66, 16, 1, [33])])
 def test_scan_seq(d, n, groups, lens, dtype):
     s = Scan(d * n, d, n, lens, dtype, groups)
     fr.check(s.call(), "ssm_seq")
@@ -294,3 +295,13 @@ def test_what_is_not_finite_stays_in_its_channel():
     assert np.isfinite(y[ok].astype(np.float32)).all() and not np.isfinite(y[~ok].astype(np.float32)).any()
     fine = np.isfinite(left).all(1)
     assert fine.sum() == 94 and not fine[5] and not fine[70]  # a step of width zero (softplus(-inf)) is fine
+
+
+@pytest.mark.parametrize("one", [False, True])
+def test_a_rate_of_minus_infinity_forgets(one):
+    s = Scan(13, 70, 16, [1] * 5 if one else [90, 0, 7], "f32", one=one)
+    s.A[:, 3] = -np.inf
+    s.buf["A"].upload(s.A)
+    s.A[:, 3] = -1e30  # for every step width here the decay is zero as well
+    fr.check(s.call())
+    s.check()

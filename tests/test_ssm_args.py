@@ -96,6 +96,13 @@ def test_time_is_covered_and_the_workspace_holds_the_chunks(channels, states, gr
         assert need <= fr.lib().frhip_ssm_workspace_bytes(C.byref(p), len(lens), total)
 
 
+@pytest.mark.parametrize("lens", [[17], [32], [1, 32, 0, 20], [32] * 128])
+def test_short_prompts_are_not_cut(lens):
+    p, out = fr.Ssm(A, None, None, 64, 16, 1, 1), (C.c_int * 3)()
+    at = [sum(lens[:i]) for i in range(len(lens) + 1)]
+    assert fr.lib().frhip_ssm_cut(C.byref(p), len(lens), starts(*at), 256, out) == 0 and out[1] == len(lens)
+
+
 def test_cut_arguments():
     p, out, f = fr.Ssm(A, None, None, 64, 16, 1, 1), (C.c_int * 3)(), fr.lib().frhip_ssm_cut
     assert f(None, 1, starts(0, 4), 256, out) == f(C.byref(p), 1, starts(0, 4), 256, None) == EINVAL
