@@ -793,6 +793,8 @@ static int launch_tiles(const LinearArgs& a, const TilePlan& p, hipStream_t st) 
 }
 
 constexpr int kLinearMostK = 8388544;  // whole steps of it keep 256 rows of a tile within 32-bit byte offsets
+constexpr int kLinearMostN = 1 << 24;                    // a launch's threads stay in 32 bits
+constexpr size_t kLinearMostWeight = (size_t)1 << 34;    // and those of the launch that expands codes
 
 // How a product goes out: the forms and cuts of the same product (K and N rounded up to whole steps and blocks) without a
 // residual on the framework's other kernels, by the same expected times.  A pure function of the sizes.
@@ -836,7 +838,8 @@ static LinearPlan plan_linear(int T, int K, int N, bool u8, int cus) {
 }
 
 static bool linear_shape(int T, const frhip_weight* w) {
-  return T >= 0 && T <= 1 << 30 && w->K > 0 && w->K <= kLinearMostK && w->K % 8 == 0 && w->N > 0 && w->N <= 1 << 30;
+  return T >= 0 && T <= 1 << 30 && w->K > 0 && w->K <= kLinearMostK && w->K % 8 == 0 && w->N > 0 && w->N <= kLinearMostN &&
+         (size_t)w->K * w->N <= kLinearMostWeight;
 }
 
 constexpr int kLinearRows = 2;  // binary16 weights, us: 2 x 4096 x 2048 5.2 in rows, 5.5 as a few rows; 3 and 4 x 2048 x 8192 11.2 and 8.6
@@ -893,7 +896,7 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
   if (act != FRHIP_ACT_NONE && (act < FRHIP_ACT_SIGMOID || act > FRHIP_ACT_SOFTPLUS)) return set_error(FRHIP_EINVAL, "linear: unknown act");
   if (w->dtype != FRHIP_F16 && w->dtype != FRHIP_U8) return set_error(FRHIP_EINVAL, "linear: weight dtype must be F16 or U8");
   if (w->dtype == FRHIP_U8 && (!w->mx || !w->rx || !w->my || !w->ry)) return set_error(FRHIP_EINVAL, "linear: uint8 weight without mx/rx/my/ry");
-  if (!linear_shape(T, w) || ldx > kLinearMostK) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T and N at most 2^30, rows at most 8388544 elements apart");
+  if (!linear_shape(T, w) || ldx > kLinearMostK) return set_error(FRHIP_ESHAPE, "linear: K must be a multiple of 8, T at most 2^30, N 2^24, K N 2^34, rows at most 8388544 elements apart");
   if (ldx < w->K || ldx % 8 != 0 || ldy < w->N || (residual && ldr < w->N)) return set_error(FRHIP_ESHAPE, "linear: rows closer than their elements, or ldx no multiple of 8");
   if (T == 0) return 0;
   if (!x || !y) return set_error(FRHIP_EINVAL, "linear: null pointer");

@@ -550,6 +550,8 @@ static ScanShape scan_shape(const frhip_ssm& p) {
 }
 
 constexpr int kMostRows = 1 << 30;     // of a call of single tokens: a loop over them counts in steps of up to 2^18
+constexpr int kMostTime = 1 << 28;     // row numbers of prompts: sums of a few of them stay in 32 bits, and so do a launch's threads
+constexpr int kMostChannels = 1 << 24;
 constexpr int kScanLeast = 16;         // rows of a chunk, at least
 constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
 constexpr int kScanRows = 16;          // a chunk is a multiple of it
@@ -577,13 +579,14 @@ static size_t scan_most_local(const ScanShape& s, int T) {  // sum of (chunks - 
   return by_rows < by_units ? by_rows : by_units;
 }
 
-static int check_seqs(int nseq, const int32_t* seq_start, const char* what) {
+static int check_seqs(int nseq, const int32_t* seq_start, int most, const char* what) {
   if (nseq < 0) return set_error(FRHIP_ESHAPE, what);
   if (nseq > 0) {
     if (!seq_start) return set_error(FRHIP_EINVAL, what);
     if (seq_start[0] < 0) return set_error(FRHIP_ESHAPE, what);
     for (int i = 0; i < nseq; i++)
       if (seq_start[i + 1] < seq_start[i]) return set_error(FRHIP_ESHAPE, what);
+    if (seq_start[nseq] > most) return set_error(FRHIP_ESHAPE, what);
   }
   return 0;
 }
@@ -605,7 +608,6 @@ static int conv_seq_run(ConvArgs<T> a, int W, int nseq, const int32_t* start, hi
   // A tile reads W - 1 rows more than its own, which costs where memory is busy; a short one starts sooner.  us with tiles of 4 and 8 rows:
   // 300 x 2048 4.9 and 5.5, 2077 x 1536 of fp32 8.0 and 8.7, 1000 x 4096 8.0 and 7.5, 4096 x 4096 19.6 and 16.8
   a.tile = (size_t)(start[nseq] - start[0]) * a.C < (size_t)4000000 ? kConvBatch : 2 * kConvBatch;
-  if (blocks > 65535) return set_error(FRHIP_ESHAPE, "conv_seq: too many channels");
   const T *state = a.state;
   T* state_out = a.state_out;
   for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {
@@ -636,7 +638,7 @@ static int conv_check(int C, int W, const void* x, int ldx, const float* w, cons
                       void* y, int ldy, int dtype, size_t row0, size_t rows, size_t nstate) {
   if (dtype != FRHIP_F16 && dtype != FRHIP_F32) return set_error(FRHIP_EINVAL, "conv: dtype must be F16 or F32");
   if (act != FRHIP_ACT_NONE && act != FRHIP_ACT_SILU) return set_error(FRHIP_EINVAL, "conv: act must be NONE or SILU");
-  if (C <= 0 || W < 2 || W > 4) return set_error(FRHIP_ESHAPE, "conv: W must be 2, 3 or 4 and C positive");
+  if (C <= 0 || C > kMostChannels || W < 2 || W > 4) return set_error(FRHIP_ESHAPE, "conv: W must be 2, 3 or 4 and C 1 to 2^24");
   if (ldx < C || ldy < C) return set_error(FRHIP_ESHAPE, "conv: rows closer than C elements");
   if (!w || !state || !state_out || (rows && (!x || !y))) return set_error(FRHIP_EINVAL, "conv: null pointer");
   const size_t elem = dtype == FRHIP_F16 ? 2 : 4, sbytes = nstate * (W - 1) * C * elem;
@@ -678,8 +680,8 @@ static ConvArgs<T> conv_args(int C, const void* x, int ldx, const float* w, cons
 
 static int ssm_check_params(const frhip_ssm* p) {
   if (!p || !p->A) return set_error(FRHIP_EINVAL, "ssm: null pointer");
-  if (p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0 || p->channels > 1 << 28)
-    return set_error(FRHIP_ESHAPE, "ssm: channels must be a multiple of groups, at most 2^28");
+  if (p->channels <= 0 || p->groups <= 0 || p->channels % p->groups != 0 || p->channels > kMostChannels)
+    return set_error(FRHIP_ESHAPE, "ssm: channels must be a multiple of groups, at most 2^24");
   if (p->states < 1 || p->states > 256) return set_error(FRHIP_ESHAPE, "ssm: states must be 1 to 256");
   if ((long long)p->groups * p->states > INT_MAX) return set_error(FRHIP_ESHAPE, "ssm: too many groups");
   if (off_grid(4, {p->A, p->D, p->dt_bias})) return set_error(FRHIP_EINVAL, "ssm: pointer not aligned to its element");
@@ -866,7 +868,7 @@ extern "C" int frhip_conv_one(int rows, int C, int W, const void* x, int ldx, co
 
 extern "C" int frhip_conv_seq(int nseq, const int32_t* seq_start, int C, int W, const void* x, int ldx, const float* w, const float* bias,
                               int act, const void* state, void* state_out, void* y, int ldy, int dtype, frhip_stream s) {
-  if (int rc = check_seqs(nseq, seq_start, "conv_seq: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
+  if (int rc = check_seqs(nseq, seq_start, kMostTime, "conv_seq: seq_start must be nseq + 1 row numbers up to 2^28 that do not descend")) return rc;
   const size_t row0 = nseq ? seq_start[0] : 0, rows = nseq ? seq_start[nseq] - seq_start[0] : 0;
   if (int rc = conv_check(C, W, x, ldx, w, bias, act, state, state_out, y, ldy, dtype, row0, rows, nseq)) return rc;
   if (nseq == 0) return 0;
@@ -897,12 +899,12 @@ extern "C" int frhip_ssm_seq(const frhip_ssm* p, int nseq, const int32_t* seq_st
                              const void* B, int ldb, const void* C, int ldc, const void* z, int ldz, const float* state, float* state_out,
                              void* y, int ldy, int dtype, void* workspace, frhip_stream s) {
   if (int rc = ssm_check_params(p)) return rc;
-  if (int rc = check_seqs(nseq, seq_start, "ssm_seq: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
+  if (int rc = check_seqs(nseq, seq_start, kMostTime, "ssm_seq: seq_start must be nseq + 1 row numbers up to 2^28 that do not descend")) return rc;
   const SsmCall c = {x, dt, B, C, z, ldx, lddt, ldb, ldc, ldz, state, state_out, y, ldy, dtype};
   const size_t row0 = nseq ? seq_start[0] : 0, rows = nseq ? seq_start[nseq] - seq_start[0] : 0;
   if (int rc = ssm_check(*p, c, row0, rows, nseq)) return rc;
   if (nseq == 0) return 0;
-  if (scan_shape(*p).wgs > (1 << 24)) return set_error(FRHIP_ESHAPE, "ssm_seq: too many channels");
+  if (scan_shape(*p).wgs > (1 << 21)) return set_error(FRHIP_ESHAPE, "ssm_seq: too many groups");
   if (frhip_ssm_workspace_bytes(p, nseq, (int)rows) > 0) {
     if (!workspace) return set_error(FRHIP_EINVAL, "ssm_seq: null workspace");
     if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return set_error(FRHIP_EINVAL, "ssm_seq: workspace must be 16-byte aligned");
@@ -915,7 +917,7 @@ extern "C" int frhip_ssm_cut(const frhip_ssm* p, int nseq, const int32_t* seq_st
   if (int rc = ssm_check_params(p)) return rc;
   if (!out) return set_error(FRHIP_EINVAL, "ssm_cut: null pointer");
   if (compute_units < 1) return set_error(FRHIP_ESHAPE, "ssm_cut: no such scan");
-  if (int rc = check_seqs(nseq, seq_start, "ssm_cut: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
+  if (int rc = check_seqs(nseq, seq_start, INT_MAX, "ssm_cut: seq_start must be nseq + 1 row numbers that do not descend")) return rc;
   if (nseq < 1 || nseq > kSeqTable) return set_error(FRHIP_ESHAPE, "ssm_cut: 1 to 128 prompts");
   const ScanShape s = scan_shape(*p);
   SeqTable tab;

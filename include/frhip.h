@@ -349,7 +349,7 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * Activations are FRHIP_F16 or FRHIP_F32 (`dtype`: x, dt, B, C, z, y and the convolution's state), rows `ld` elements apart, at any
  * address that is a multiple of their element's size; parameters and the scan's state are fp32.  Sums, decays and states
  * are held in fp32; an output is rounded once.  A `_one` call takes one token each of `rows` sequences (up to 2^30); a `_seq` call takes
- * nseq prompts that lie one behind the other: prompt i is rows seq_start[i] .. seq_start[i + 1] - 1 (seq_start: nseq + 1
+ * nseq prompts that lie one behind the other (rows 0 to 2^28): prompt i is rows seq_start[i] .. seq_start[i + 1] - 1 (seq_start: nseq + 1
  * numbers in HOST memory, read before the call returns, not descending, the first not negative).  A prompt of no rows leaves
  * its state as it was; rows ahead of the first prompt and behind the last are neither read nor written.  States are [nseq or rows][...],
  * and the one written may be the one read (the same address, or memory that does not overlap).  y overlaps nothing that is read. */
@@ -358,7 +358,7 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * frhip_gemm_act, which rounds ahead of the activation as the reference does).  x [T] rows of K binary16, ldx elements apart;
  * bias [N] fp32 or NULL; residual [T] rows of N in out_dtype, ldr apart, or NULL; y [T] rows of N in out_dtype (F16 or F32), ldy
  * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
- * K and ldx are multiples of 8, at most 8388544, N and T are any up to 2^30; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte, the others
+ * K and ldx are multiples of 8, at most 8388544, T is any up to 2^30, N up to 2^24, K N up to 2^34; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte, the others
  * lie at multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
  * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each. */
 #define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */
@@ -378,7 +378,7 @@ int frhip_linear_form(int T, const frhip_weight *w, int compute_units, int *out)
 
 /* Short causal convolution over time, channel by channel:
  *   y[t][c] = act(bias[c] + sum_{j < W} w[c][j] * x[t - W + 1 + j][c])
- * W 2..4; w [C][W]; bias [C] or NULL; act FRHIP_ACT_NONE or FRHIP_ACT_SILU.  state [.][W - 1][C] holds the inputs of the
+ * W 2..4, C up to 2^24; w [C][W]; bias [C] or NULL; act FRHIP_ACT_NONE or FRHIP_ACT_SILU.  state [.][W - 1][C] holds the inputs of the
  * tokens before, oldest first, in `dtype`; state_out receives those that the next call needs. */
 int frhip_conv_one(int rows, int C, int W, const void *x, int ldx, const float *w, const float *bias, int act,
                    const void *state, void *state_out, void *y, int ldy, int dtype, frhip_stream s);
@@ -390,7 +390,7 @@ int frhip_conv_seq(int nseq, const int32_t *seq_start, int C, int W, const void 
  *   h[d][n] = exp(dt' A[d][n]) h[d][n] + dt' x[t][d] B[t][g][n]
  *   y[t][d] = (sum_n C[t][g][n] h[d][n] + D[d] x[t][d]) * silu(z[t][d])
  * A [channels][states], not positive; D and dt_bias [channels], NULL: zero; z NULL: no gate.  B and C are rows of groups * states.
- * state [.][channels][states] fp32.  states 1..256.  What is not finite reaches the outputs of its channel from its token on, and
+ * state [.][channels][states] fp32.  states 1..256, channels up to 2^24.  What is not finite reaches the outputs of its channel from its token on, and
  * through B or C those of its group. */
 typedef struct frhip_ssm {
   const float *A, *D, *dt_bias;

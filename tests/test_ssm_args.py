@@ -40,6 +40,15 @@ def test_single_tokens_of_too_many_sequences():
     assert conv(False, n=(1 << 30) + 1) == scan(False, n=(1 << 30) + 1) == ESHAPE
 
 
+def test_row_numbers_and_channels_beyond_the_limits():
+    far = starts(0, (1 << 28) + 1)
+    assert conv(at=far) == scan(at=far) == ESHAPE
+    c = (1 << 24) + 1
+    assert conv(C=c, ldx=c, ldy=c) == conv(False, C=c, ldx=c, ldy=c) == ESHAPE
+    for seq in (True, False):
+        assert scan(seq, params=dict(channels=c, groups=1), ldx=c, lddt=c, ldz=c, ldy=c) == ESHAPE
+
+
 def test_conv_of_nothing():
     assert conv(n=0, at=None) == 0 and conv(False, n=0) == 0
 
