@@ -369,7 +369,7 @@ int frhip_linear(const void *x, int ldx, const frhip_weight *w, const float *bia
 
 /* How such a product goes out on a part with that many compute units, a pure function of T and the weight's K, N and dtype, for tests and
  * measurements.  Returns the form or a negative FRHIP_E*; out[0], out[1]: rows and widest columns of a workgroup's tile (LINEAR_ROWS: 0,
- * 0), out[2] = 1 if uint8 codes are expanded to binary16 first. */
+ * 0), out[2] = 1 if uint8 codes are expanded to binary16 first, + 2 if the rows behind the last whole tile go out in a launch of their own. */
 #define FRHIP_LINEAR_ROWS 0  /* one or two rows: the weight streamed through the waves */
 #define FRHIP_LINEAR_FEW 1   /* K split over the waves of a workgroup */
 #define FRHIP_LINEAR_TILES 2 /* of 64, 128 or 256 rows */

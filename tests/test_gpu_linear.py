@@ -116,6 +116,14 @@ def test_large_products(T, K, N):
     case(T, K, N, act="silu", quant=True)
 
 
+@pytest.mark.parametrize("T,K,N,quant", [(2051, 72, 8192, False), (2050, 64, 8190, False), (2050, 72, 8190, True), (1027, 1000, 8192, False)])
+def test_rows_behind_whole_tiles(T, K, N, quant):
+    f, rows, how = form(T, K, N, quant)
+    assert f == 2 and how == 2 + quant and T % rows
+    case(T, K, N, act="silu", bias=True, res=True, quant=quant, pad=3)
+    case(T, K, N, out="f32", quant=quant, in_place=True)
+
+
 def test_what_is_not_finite_stays_in_its_row():
     T, K, N = 70, 200, 90
     g = np.random.default_rng(3)
