@@ -873,6 +873,17 @@ static LinearPlan plan_linear(int T, int K, int N, bool u8, int cus) {
   return p;
 }
 
+// Whether a product of uint8 weights of T rows, or of fewer, expands its codes: a workspace for T rows serves fewer as well, though `expand` comes and
+// goes with the expected times (2048 x 8192 codes: 641 to 1024 rows, 1153 to 1280, from 1409 on).  Every expected time is one number for all rows
+// of a strip: of 16 while a few rows are among the forms, of 64 beyond.  Above kExpandRows the answer is yes unasked.
+constexpr int kExpandRows = 8192;
+static bool expands_up_to(int T, int K, int N, int cus) {
+  if (T > kExpandRows || plan_linear(T, K, N, true, cus).expand) return true;
+  for (int rows = 16; rows < T; rows += rows < kFewKernelRows ? 16 : 64)
+    if (plan_linear(rows, K, N, true, cus).expand) return true;
+  return false;
+}
+
 static bool linear_shape(int T, const frhip_weight* w) {
   return T >= 0 && T <= 1 << 30 && w->K > 0 && w->K <= kLinearMostK && w->K % 8 == 0 && w->N > 0 && w->N <= kLinearMostN &&
          (size_t)w->K * w->N <= kLinearMostWeight;
@@ -915,7 +926,7 @@ static int launch_linear(LinearArgs a, bool u8, void* workspace, hipStream_t st)
 using namespace frhip;
 
 extern "C" size_t frhip_linear_workspace_bytes(int T, const frhip_weight* w) {
-  if (!w || T <= 0 || w->dtype != FRHIP_U8 || !linear_shape(T, w) || !plan_linear(T, w->K, w->N, true, compute_units()).expand)
+  if (!w || T <= 0 || w->dtype != FRHIP_U8 || !linear_shape(T, w) || !expands_up_to(T, w->K, w->N, compute_units()))
     return 0;
   return ((size_t)w->K * w->N * 2 + 255) / 256 * 256;  // the weight in binary16
 }

@@ -360,7 +360,8 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
  * K and ldx are multiples of 8, at most 8388544, T is any up to 2^30, N up to 2^24, K N up to 2^34; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte, the others
  * lie at multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
- * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each. */
+ * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each.  The
+ * bytes do not fall as T grows: a workspace for the most rows that a program has serves every call of fewer. */
 #define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */
 #define FRHIP_ACT_SOFTPLUS 6 /* log(1 + exp(v)) */
 size_t frhip_linear_workspace_bytes(int T, const frhip_weight *w);

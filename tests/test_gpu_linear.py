@@ -152,3 +152,23 @@ def test_a_captured_product_replays(T, quant):
         assert np.array_equal(dy.numpy(), first)
     fr.check(L().frhip_graph_destroy(g))
     fr.check(L().frhip_stream_destroy(st))
+
+
+def test_a_workspace_for_the_most_rows_serves_fewer():
+    """2048 x 8192 codes: 1100 rows dequantise on their way, 700 expand; nothing is written behind the workspace that 1100 rows ask for"""
+    K, N, guard = 2048, 8192, 1 << 16
+    assert form(1100, K, N, True)[2] == 0 and form(700, K, N, True)[2] & 1 == 1
+    g = np.random.default_rng(11)
+    pw, _ = make_weight((g.standard_normal((K, N)) / math.sqrt(K)).astype(np.float16), True)
+    x = g.standard_normal((1100, K)).astype(np.float16)
+    need = L().frhip_linear_workspace_bytes(1100, pw.ref)
+    assert need >= L().frhip_linear_workspace_bytes(700, pw.ref) >= 2 * K * N
+    dx, shared, own = dev(x), dev(np.full(need + guard, 0x5a, np.uint8)), DevBuf(2 * K * N)
+    for T in (1100, 700, 3, 1100):
+        got = []
+        for ws in (shared, own):
+            dy = dev(np.full((T, N), 7, np.float16))
+            fr.check(L().frhip_linear(dx.ptr, K, pw.ref, None, 0, None, 0, dy.ptr, N, T, fr.F16, ws.ptr, None), "linear")
+            got.append(dy.numpy())
+        assert np.isfinite(got[0].astype(np.float32)).all() and np.array_equal(*got)
+    assert (shared.numpy()[need:] == 0x5a).all()

@@ -81,3 +81,17 @@ def test_form_arguments():
     f, w = fr.lib().frhip_linear_form, C.byref(fr.Weight(A, A, A, A, A, 64, 64, fr.F16))
     assert f(1, None, 256, out) == f(1, w, 256, None) == EINVAL and f(0, w, 256, out) == f(1, w, 0, out) == ESHAPE
     assert form(1, 60, 64, fr.F16)[0] == form(1, 8388552, 64, fr.F16)[0] == form(1, 64, (1 << 24) + 1, fr.F16)[0] == form((1 << 30) + 1, 64, 64, fr.F16)[0] == ESHAPE
+
+
+@pytest.mark.parametrize("K,N", [(2048, 8192), (4096, 2048), (5120, 2048), (64, 8192), (128, 2048), (512, 10240), (4096, 50288), (2048, 512), (64, 1 << 20),
+                                 (8, 40), (24, 8192), (2056, 8192), (2048, 8200), (64, 160)])
+def test_a_workspace_for_some_rows_serves_fewer(K, N):
+    """Codes are expanded at some numbers of rows and not at others above them: what one call writes, a workspace for more rows holds"""
+    w, most = fr.Weight(A, A, A, A, A, K, N, fr.U8), 0
+    for T in range(1, 2400):
+        if form(T, K, N, fr.U8)[1][2] & 1:
+            most = 2 * K * N
+        if T % 64 in (0, 1, 33) or T < 140:
+            assert fr.lib().frhip_linear_workspace_bytes(T, C.byref(w)) >= most, T
+    sizes = [fr.lib().frhip_linear_workspace_bytes(T, C.byref(w)) for T in (1, 16, 100, 512, 513, 1024, 1153, 1409, 3000, 4100, 8192, 8193, 100000, 1 << 30)]
+    assert sizes == sorted(sizes)
