@@ -7,6 +7,7 @@
 //   1. every chunk but a prompt's last is scanned from an empty state -> its end state and its sum of dt;
 //   2. every chunk folds the chunks before it into its true start state and is scanned again, with outputs.
 // One token is the formula itself.
+#include <cfloat>
 #include <climits>
 #include <cstring>
 
@@ -217,6 +218,13 @@ __global__ __launch_bounds__(256) void conv_seq_kernel(ConvArgs<T> a, SeqTable t
 // ---------------------------------------------------------------------------
 // Selective scan
 // ---------------------------------------------------------------------------
+// A rate as exp2 takes it.  One of minus infinity stays a number: it forgets at any step but that of width zero, which keeps the state (0 times
+// infinity would be a NaN).
+__device__ __forceinline__ float exp2_rate(float A) {
+  const float r = A * kLog2e;
+  return r < -FLT_MAX ? -FLT_MAX : r;
+}
+
 template <class T>
 struct SsmArgs {
   const T *x, *dt, *B, *C, *z;
@@ -310,7 +318,7 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
     load_group<float, 4>(v, a.A + (size_t)d * a.N + n0 + k, a.N - n0 - k);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      A2[k + e] = v[e] < -1e38f ? -1e38f : v[e] * kLog2e;  // rows past the chunk have a step of zero, which an infinite rate would make a NaN
+      A2[k + e] = exp2_rate(v[e]);  // rows past the chunk have a step of zero
       h[k + e] = 0.f;
     }
   }
@@ -488,7 +496,9 @@ __global__ __launch_bounds__(256) void ssm_one_kernel(SsmArgs<T> a) {
     }
     return v;
   };
-  const f4 A = four(a.A + (size_t)d * a.N + n0);
+  f4 A2 = four(a.A + (size_t)d * a.N + n0);
+#pragma unroll
+  for (int k = 0; k < 4; k++) A2[k] = exp2_rate(A2[k]);
   const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, skip = a.D ? a.D[d] : 0.f;
   for (int r0 = blockIdx.y * R; r0 < a.rows; r0 += gridDim.y * R) {
     f4 h[R], B[R], C[R];
@@ -510,7 +520,7 @@ __global__ __launch_bounds__(256) void ssm_one_kernel(SsmArgs<T> a) {
       float y = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        h[r][k] = __builtin_fmaf(__builtin_amdgcn_exp2f(step * (A[k] * kLog2e)), h[r][k], u * B[r][k]);
+        h[r][k] = __builtin_fmaf(__builtin_amdgcn_exp2f(step * A2[k]), h[r][k], u * B[r][k]);
         y = VEC || k < left ? __builtin_fmaf(C[r][k], h[r][k], y) : y;
       }
       if (VEC && left <= 0) y = 0.f;  // lanes without a state: not what 0 times a step that is not finite would leave

@@ -390,7 +390,7 @@ int frhip_conv_seq(int nseq, const int32_t *seq_start, int C, int W, const void 
  *   dt' = softplus(dt[t][d] + dt_bias[d])          (dt_softplus 0: dt[t][d] + dt_bias[d], not negative)
  *   h[d][n] = exp(dt' A[d][n]) h[d][n] + dt' x[t][d] B[t][g][n]
  *   y[t][d] = (sum_n C[t][g][n] h[d][n] + D[d] x[t][d]) * silu(z[t][d])
- * A [channels][states], not positive; D and dt_bias [channels], NULL: zero; z NULL: no gate.  B and C are rows of groups * states.
+ * A [channels][states], not positive (minus infinity: forgets, but in a step of width zero, which keeps the state); D and dt_bias [channels], NULL: zero; z NULL: no gate.  B and C are rows of groups * states.
  * state [.][channels][states] fp32.  states 1..256, channels up to 2^24.  What is not finite reaches the outputs of its channel from its token on, and
  * through B or C those of its group. */
 typedef struct frhip_ssm {

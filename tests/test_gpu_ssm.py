@@ -305,3 +305,22 @@ def test_a_rate_of_minus_infinity_forgets(one):
     s.A[:, 3] = -1e30  # for every step width here the decay is zero as well
     fr.check(s.call())
     s.check()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("softplus", [False, True])
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("n", [16, 6])
+def test_a_step_of_width_zero_keeps_the_state_at_any_rate(n, one, softplus, dtype):
+    """Padding tokens: rates of minus infinity, and finite ones whose product with log2(e) is none, times zero"""
+    s = Scan(14, 70, n, [1] * 5 if one else [90, 0, 7], dtype, one=one, softplus=softplus)
+    s.A[:, 2], s.A[:, 5] = -np.inf, -3e38
+    s.buf["A"].upload(s.A)
+    s.A[:, 2] = -1e30  # for every step width here the decay is 0 or 1 as well
+    none = [0, 3] if one else [GUARD, GUARD + 3, GUARD + 15, GUARD + 16, *range(GUARD + 30, GUARD + 50), GUARD + 89, GUARD + 90, GUARD + 96]
+    s.dt[none] = -60000 if softplus else 0
+    s.dt[:, 7] = -60000 if softplus else 0  # a channel of nothing else
+    s.buf["dt"].upload(s.dt)
+    fr.check(s.call())
+    y, left = s.check()
+    assert np.isfinite(y.astype(np.float32)).all() and all(np.array_equal(a[7], b[7]) for a, b in zip(left, s.state))
