@@ -10,6 +10,7 @@
 #include <cfloat>
 #include <climits>
 #include <cstring>
+#include <type_traits>
 
 #include "activations.h"
 #include "frhip_internal.h"
@@ -243,7 +244,8 @@ struct SsmArgs {
 constexpr int scan_waves(int nw) { return nw < 4 ? 4 : nw; }
 constexpr int scan_rows(int nw) { return nw == 1 ? 8 : 16; }  // of a block of time, the rows that go through LDS together
 
-// LOCAL: step 1 of the scan, otherwise step 2.  A workgroup walks its chunk in blocks of time.  Of a block, every wave
+// LOCAL: step 1 of the scan, otherwise step 2.  PAD: the waves have room for more states than there are; step 2 leaves those out, since zero times
+// a step or an input that is not finite is no zero (step 1's are never read).  A workgroup walks its chunk in blocks of time.  Of a block, every wave
 //   A. takes some rows to LDS: dt and dt x of a channel a lane, and B and C as fp32;
 //   B. runs all of its rows with NPL states a lane in registers, and leaves its part of y in LDS;
 //   C. adds the parts of the rows that it took in A, applies skip and gate and stores them.
@@ -254,7 +256,7 @@ constexpr int scan_rows(int nw) { return nw == 1 ? 8 : 16; }  // of a block of t
 // (55 + 71 in the two steps), memory alone would be 26; a lane with all 16 states of a channel and one wave a SIMD took 368.
 // Not kept: dt x times B as an outer product on the matrix units, 152; shorter blocks of time or five to eight workgroups a compute unit, 127 to
 // 136; rows through buffer descriptors, 131.
-template <class T, int NPL, int NW, bool LOCAL>
+template <class T, int NPL, int NW, bool LOCAL, bool PAD>
 __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_kernel(SsmArgs<T> a, SeqTable tab) {
   constexpr int WAVES = scan_waves(NW), CW = WAVES / NW, NT = NPL * NW, TB = scan_rows(NW), CH = CW * 64;
   constexpr int ROWS = TB * CW / WAVES;                                  // rows of a wave in A and C: of its 64 channels
@@ -411,18 +413,23 @@ __global__ __launch_bounds__(scan_waves(NW) * 64, NW < 4 ? 3 : 4) void ssm_scan_
   int buf = 0;
   for (int t = t0; t < t1; t += TB, buf ^= BUFS - 1) {
     __syncthreads();
+    auto scan = [&](auto whole) {  // whole: all of the wave's states are there
 #pragma unroll UNROLL
-    for (int r = 0; r < TB; r++) {
-      const float2 v = du[buf][r][at];
-      float y = 0.f;
+      for (int r = 0; r < TB; r++) {
+        const float2 v = du[buf][r][at];
+        float y = 0.f;
 #pragma unroll
-      for (int k = 0; k < NPL; k++) {
-        const float decay = __builtin_amdgcn_exp2f(v.x * A2[k]);
-        h[k] = __builtin_fmaf(decay, h[k], v.y * bc[buf][r][0][n0 + k]);
-        if constexpr (!LOCAL) y = k ? __builtin_fmaf(bc[buf][r][1][n0 + k], h[k], y) : bc[buf][r][1][n0] * h[0];
+        for (int k = 0; k < NPL; k++) {
+          if (!decltype(whole)::value && n0 + k >= a.N) break;
+          const float decay = __builtin_amdgcn_exp2f(v.x * A2[k]);
+          h[k] = __builtin_fmaf(decay, h[k], v.y * bc[buf][r][0][n0 + k]);
+          if constexpr (!LOCAL) y = k ? __builtin_fmaf(bc[buf][r][1][n0 + k], h[k], y) : bc[buf][r][1][n0] * h[0];
+        }
+        if constexpr (!LOCAL) part[NW == 1 ? 0 : nw][r][at] = y;
       }
-      if constexpr (!LOCAL) part[NW == 1 ? 0 : nw][r][at] = y;
-    }
+    };
+    if (PAD && n0 + NPL > a.N) scan(std::false_type());
+    else scan(std::true_type());
     if constexpr (!LOCAL) {
       __syncthreads();
 #pragma unroll
@@ -771,10 +778,11 @@ template <class T, int NPL, int NW>
 static int scan_launch(const SsmArgs<T>& a, const SeqTable& tab, int wgs, int chunks, hipStream_t st) {
   constexpr int threads = scan_waves(NW) * 64;
   if (a.nlocal) {
-    hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, true>), dim3(wgs, a.nlocal), dim3(threads), 0, st, a, tab);
+    hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, true, false>), dim3(wgs, a.nlocal), dim3(threads), 0, st, a, tab);
     if (int rc = check_launch("ssm_seq")) return rc;
   }
-  hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, false>), dim3(wgs, chunks), dim3(threads), 0, st, a, tab);
+  if (a.N == NPL * NW) hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, false, false>), dim3(wgs, chunks), dim3(threads), 0, st, a, tab);
+  else hipLaunchKernelGGL((ssm_scan_kernel<T, NPL, NW, false, true>), dim3(wgs, chunks), dim3(threads), 0, st, a, tab);
   return check_launch("ssm_seq");
 }
 

@@ -324,3 +324,35 @@ def test_a_step_of_width_zero_keeps_the_state_at_any_rate(n, one, softplus, dtyp
     fr.check(s.call())
     y, left = s.check()
     assert np.isfinite(y.astype(np.float32)).all() and all(np.array_equal(a[7], b[7]) for a, b in zip(left, s.state))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("what", ["x", "dt"])
+@pytest.mark.parametrize("one", [False, True])
+@pytest.mark.parametrize("n", [1, 3, 6, 16, 24, 40, 100, 130, 256])
+def test_an_infinite_input_is_infinity_whatever_the_states(n, one, what, dtype):
+    """Everything positive: h is infinite from that token on and so is y; a form's states beyond `states` have no part in it"""
+    s = Scan(15, 70, n, [1] * 5 if one else [60, 0, 7], dtype, one=one)
+    for v in (s.x, s.bc, s.z, s.D, s.state):
+        np.abs(v, out=v)
+    s.A = (s.A / (16 * n)).astype(np.float32)  # decays of 60 rows are far from zero
+    for k in ("x", "bc", "z", "D", "state", "A"):
+        s.buf[k].upload(getattr(s, k))
+    start = s.state.copy()
+    fr.check(s.call())
+    clean = [v.copy() for v in s.check()]
+    rows = [1, 2] if one else [GUARD + 19, GUARD + 62]  # in the second chunk of the first prompt; in the last prompt
+    v = getattr(s, what)
+    for r, c in zip(rows, (5, 69)):
+        v[r, c] = np.inf
+    s.buf[what].upload(v)
+    s.buf["state"].upload(start)
+    s.buf["y"].upload(s.mark)
+    fr.check(s.call())
+    fr.check(L().frhip_device_sync())
+    y, left = s.buf["y"].numpy(), s.out.numpy()
+    for r, c in zip(rows, (5, 69)):
+        i = int(np.searchsorted(s.at, r, side="right")) - 1
+        clean[0][r:s.at[i + 1], c] = np.inf
+        clean[1][i, c] = np.inf
+    assert np.array_equal(y, clean[0]) and np.array_equal(left, clean[1])
