@@ -794,7 +794,7 @@ static int launch_tiles(const LinearArgs& a, const TilePlan& p, hipStream_t st) 
 
 constexpr int kLinearMostK = 8388544;  // whole steps of it keep 256 rows of a tile within 32-bit byte offsets
 constexpr int kLinearMostN = 1 << 24;                    // a launch's threads stay in 32 bits
-constexpr size_t kLinearMostWeight = (size_t)1 << 34;    // and those of the launch that expands codes
+constexpr size_t kLinearMostWeight = (size_t)1 << 34;    // 32 GiB of binary16
 
 // How a product goes out: the forms and cuts of the same product (K and N rounded up to whole steps and blocks) without a
 // residual on the framework's other kernels, by the same expected times.  A pure function of the sizes.

@@ -211,23 +211,25 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ sr
   }
 }
 
-// Packed uint8 [N][K] -> packed binary16 [N][K]; thread handles 4 codes of one row.
-__global__ void dequant_u8_kernel(const uint32_t* __restrict__ q, const h1* __restrict__ mx, const h1* __restrict__ rx,
-                                  const h1* __restrict__ my, const h1* __restrict__ ry, h4* __restrict__ out, int K,
-                                  int N) {
-  const size_t i = (size_t)blockIdx.x * blockDim.x + threadIdx.x;  // index of a 4-code word
-  const size_t words = (size_t)N * (K >> 2);
-  if (i >= words) return;
-  const int n = (int)(i / (K >> 2));
-  const int k = (int)(i % (K >> 2)) * 4;
-  const float c2 = dequant_c(rx[n]);
-  const float m2 = (float)mx[n];
-  const uint32_t w = q[i];
-  h2 ry01 = {ry[k], ry[k + 1]}, ry23 = {ry[k + 2], ry[k + 3]};
-  h2 my01 = {my[k], my[k + 1]}, my23 = {my[k + 2], my[k + 3]};
-  h2 lo = dequant_pair<0>(w, c2, m2, ry01, my01);
-  h2 hi = dequant_pair<1>(w, c2, m2, ry23, my23);
-  out[i] = (h4){lo.x, lo.y, hi.x, hi.y};
+// Packed uint8 [N][K] -> packed binary16 [N][K]; thread handles 4 codes of one row at a time.  For codes, scales or outputs at any address of
+// four or two bytes; the launch is at most kDequantBlocks wide, so that its threads stay in 32 bits whatever N K is.
+constexpr unsigned kDequantBlocks = 1u << 22;
+__global__ __launch_bounds__(256) void dequant_u8_kernel(const uint32_t* __restrict__ q, const h1* __restrict__ mx, const h1* __restrict__ rx,
+                                                         const h1* __restrict__ my, const h1* __restrict__ ry, h4* __restrict__ out, int K,
+                                                         int N) {
+  const size_t words = (size_t)N * (K >> 2), step = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < words; i += step) {  // index of a 4-code word
+    const int n = (int)(i / (K >> 2));
+    const int k = (int)(i % (K >> 2)) * 4;
+    const float c2 = dequant_c(rx[n]);
+    const float m2 = (float)mx[n];
+    const uint32_t w = q[i];
+    h2 ry01 = {ry[k], ry[k + 1]}, ry23 = {ry[k + 2], ry[k + 3]};
+    h2 my01 = {my[k], my[k + 1]}, my23 = {my[k + 2], my[k + 3]};
+    h2 lo = dequant_pair<0>(w, c2, m2, ry01, my01);
+    h2 hi = dequant_pair<1>(w, c2, m2, ry23, my23);
+    out[i] = (h4){lo.x, lo.y, hi.x, hi.y};
+  }
 }
 
 // The same, eight consecutive codes of four rows per thread (K a multiple of 8): ry and my are read once for four
@@ -393,8 +395,9 @@ int dequant_u8_async(const unsigned char* q, const h1* mx, const h1* rx, const h
   const size_t words = (size_t)N * (K / 4);
   if (K % 8 != 0 || (size_t)N * (K / 16) >= (1u << 31) || reinterpret_cast<uintptr_t>(q) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(dst) % 16 != 0 || reinterpret_cast<uintptr_t>(ry) % 16 != 0 || reinterpret_cast<uintptr_t>(my) % 16 != 0) {
-    hipLaunchKernelGGL(dequant_u8_kernel, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, st, (const uint32_t*)q, mx, rx, my, ry,
-                       (h4*)dst, K, N);
+    const size_t blocks = (words + 255) / 256;
+    hipLaunchKernelGGL(dequant_u8_kernel, dim3(blocks < kDequantBlocks ? (unsigned)blocks : kDequantBlocks), dim3(256), 0, st,
+                       (const uint32_t*)q, mx, rx, my, ry, (h4*)dst, K, N);
     return check_launch("dequant_u8");
   }
   return dequant_u8_group_async(1, &q, &mx, &rx, &my, &ry, &dst, K, &N, st);

@@ -358,8 +358,8 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * frhip_gemm_act, which rounds ahead of the activation as the reference does).  x [T] rows of K binary16, ldx elements apart;
  * bias [N] fp32 or NULL; residual [T] rows of N in out_dtype, ldr apart, or NULL; y [T] rows of N in out_dtype (F16 or F32), ldy
  * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
- * K and ldx are multiples of 8, at most 8388544, T is any up to 2^30, N up to 2^24, K N up to 2^34; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte, the others
- * lie at multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
+ * K and ldx are multiples of 8, at most 8388544, T is any up to 2^30, N up to 2^24, K N up to 2^34; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte (my and ry
+ * 16-byte for the quick expansion of codes, where a product expands them), the others lie at multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
  * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each.  The
  * bytes do not fall as T grows: a workspace for the most rows that a program has serves every call of fewer. */
 #define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */

@@ -135,3 +135,51 @@ def test_more_strips_of_rows_than_sixteen_bits_count():
     dx, dy = dev(x), DevBuf.empty((T, N), np.float16)
     fr.check(L().frhip_linear(dx.ptr, K, w.ref, None, 0, None, 0, dy.ptr, N, T, fr.F16, None, None))
     assert np.array_equal(dy.numpy(), (x.astype(np.float32) @ wt.astype(np.float32)).astype(np.float16))
+
+
+def test_the_largest_weight_of_codes_with_scales_at_any_address():
+    """2^34 codes, ry and my four bytes behind a multiple of 16: expanded a word at a time, in a launch of fewer threads than words.  Rows at the
+    begin, the end and on both sides of where the threads begin again are those of a small weight, to the bit; the others hold anything."""
+    K, N = 1 << 14, 1 << 20
+    rows = np.array([0, 1, 2, (1 << 18) - 1, 1 << 18, (1 << 19) - 1, 1 << 19, 3 << 18, N - 2, N - 1])
+    g = np.random.default_rng(6)
+    q = g.integers(0, 256, (len(rows), K)).astype(np.uint8)
+    mx, rx = (g.uniform(-1, 1, N) / 64).astype(np.float16), (g.uniform(0.5, 1, N) / 64).astype(np.float16)
+    my, ry = (g.uniform(-1, 1, K) / 64).astype(np.float16), g.uniform(0.5, 1, K).astype(np.float16)
+    off = [dev(np.concatenate([np.zeros(2, np.float16), v])) for v in (my, ry)]
+    codes, image = DevBuf(K * N), DevBuf(2 * K * N)
+    for r, v in zip(rows, q):
+        copy(codes.ptr + int(r) * K, v.ctypes.data, K, H2D)
+    dmx, drx = dev(mx), dev(rx)
+    w = fr.Weight(codes.ptr, dmx.ptr, drx.ptr, off[0].ptr + 4, off[1].ptr + 4, K, N, fr.U8)
+    few = [dev(v) for v in (q, mx[rows], rx[rows], my, ry)]
+    small = fr.Weight(*(b.ptr for b in few), K, len(rows), fr.U8)
+    want = DevBuf.empty((len(rows), K), np.float16)
+    fr.check(L().frhip_dequant_u8(C.byref(small), want.ptr, None))
+    want = want.numpy()
+
+    def check():
+        fr.check(L().frhip_device_sync())
+        for r, v in zip(rows, want):
+            got = np.empty(K, np.float16)
+            copy(got.ctypes.data, image.ptr + int(r) * K * 2, K * 2, D2H)
+            assert np.array_equal(got.view(np.uint16), v.view(np.uint16)), r
+    fr.check(L().frhip_dequant_u8(C.byref(w), image.ptr, None))
+    check()
+    # and as the workspace of a product
+    T, form = 1000, (C.c_int * 3)()
+    assert L().frhip_linear_form(T, C.byref(w), 256, form) >= 0 and form[2] & 1
+    assert L().frhip_linear_workspace_bytes(T, C.byref(w)) == image.nbytes
+    clear = np.zeros(K, np.float16)
+    for r in rows:
+        copy(image.ptr + int(r) * K * 2, clear.ctypes.data, K * 2, H2D)
+    x = g.standard_normal((T, K)).astype(np.float16)
+    dx, y = dev(x), DevBuf(T * N * 2)
+    fr.check(L().frhip_linear(dx.ptr, K, C.byref(w), None, 0, None, 0, y.ptr, N, T, fr.F16, image.ptr, None))
+    check()
+    for t in (0, T - 1):
+        got = np.empty(N, np.float16)
+        copy(got.ctypes.data, y.ptr + t * N * 2, N * 2, D2H)
+        a, b = x[t].astype(np.float64), want.astype(np.float64)
+        tol = (K / 32 + 40) * 2.0 ** -23 * (np.abs(b) @ np.abs(a)) + np.abs(b @ a) * 2.0 ** -11 + 2.0 ** -25
+        assert (np.abs(got[rows].astype(np.float64) - b @ a) <= tol).all()
