@@ -172,3 +172,59 @@ def test_a_workspace_for_the_most_rows_serves_fewer():
             got.append(dy.numpy())
         assert np.isfinite(got[0].astype(np.float32)).all() and np.array_equal(*got)
     assert (shared.numpy()[need:] == 0x5a).all()
+
+
+FAR = np.array([v for m in (0.0, 1e-30, 1e-3, 30, 60, 80, 87, 87.5, 88, 89, 95, 103, 110, 125, 1e3, 1e10, 1e30, 3e38) for v in (m, -m)], np.float32)
+
+
+@pytest.mark.parametrize("out", ["f16", "f32"])
+@pytest.mark.parametrize("act", sorted(ACT))
+@pytest.mark.parametrize("T", [1, 20, 200])
+def test_activations_far_from_zero(T, act, out):
+    """v = bias exactly.  A sigmoid below the normal numbers may be 0 (its reciprocal is subnormal), which silu multiplies by |v| <= 104."""
+    N, t = len(FAR), np.float16 if out == "f16" else np.float32
+    pw, _ = make_weight(np.zeros((8, N), np.float16))
+    dx, db, dy = dev(np.zeros((T, 8), np.float16)), dev(FAR), DevBuf.empty((T, N), t)
+    fr.check(L().frhip_linear(dx.ptr, 8, pw.ref, db.ptr, ACT[act], None, 0, dy.ptr, N, T, fr.F16 if out == "f16" else fr.F32, None, None))
+    with np.errstate(over="ignore"):
+        v = FAR.astype(np.float64)
+        f, tol = act64(v, act)
+        tol = tol(0.0) + np.where((v < -87) & (v > -104), -v, 1) * 2.0 ** -126 + (np.abs(f) * 2.0 ** -11 + 2.0 ** -25 if out == "f16" else np.abs(f) * 2.0 ** -24)
+        rounded = f.astype(t)
+    got = dy.numpy()
+    for row in got:
+        bad = ~(np.abs(row.astype(np.float64) - f) <= tol) & (row != rounded)  # what overflows is infinite in both
+        assert not bad.any(), (v[bad], row[bad], f[bad])
+
+
+@pytest.mark.parametrize("T,K,N,quant", [(1, 200, 90, False), (2, 1032, 33, False), (1, 200, 90, True), (20, 200, 90, False), (48, 72, 130, True), (300, 168, 80, False),
+                                         (200, 2048, 8192, True), (1030, 200, 4000, False), (700, 200, 4000, True)])
+@pytest.mark.parametrize("act", sorted(ACT))
+def test_infinities_are_those_of_the_formula(act, T, K, N, quant):
+    """An infinite x gives infinite sums of its weights' signs; what multiplies minus infinity by the zero that its sigmoid or erfc is may be 0 or a NaN"""
+    g = np.random.default_rng(12)
+    w = g.uniform(0.25, 1, (K, N)) * np.where(g.random(N) < 0.5, -1, 1)  # the codes' signs are the weights'
+    pw, wf = make_weight(w.astype(np.float16), quant)
+    assert (np.sign(wf) == np.sign(w)).all()
+    x = (g.standard_normal((T, K)) / K).astype(np.float16)
+    where = [(0, K - 1, np.inf), (T // 2, 0, -np.inf), (T - 1, K - 9, np.inf)]
+    for r, k, v in where:
+        x[r] = 0
+        x[r, k] = v
+    dx, out = dev(x), []
+    need = L().frhip_linear_workspace_bytes(T, pw.ref)
+    ws = DevBuf(need) if need else None
+    for code, t in ((fr.F16, np.float16), (fr.F32, np.float32)):
+        dy = DevBuf.empty((T, N), t)
+        fr.check(L().frhip_linear(dx.ptr, K, pw.ref, None, ACT[act], None, 0, dy.ptr, N, T, code, ws.ptr if ws else None, None))
+        y = dy.numpy()
+        last = {r: v for r, _, v in where}
+        for r, v in last.items():
+            up = np.sign(w[0]) * np.sign(v) > 0
+            assert (y[r, up] == (1 if act == "sigmoid" else np.inf)).all(), (code, r)
+            down = y[r, ~up].astype(np.float64)
+            if act == "none":
+                assert (down == -np.inf).all()
+            else:
+                assert ((np.abs(down) <= 2.0 ** -126) | (np.isnan(down) if act in ("silu", "gelu") else False)).all(), (code, r, down)
+        assert np.isfinite(np.delete(y, list(last), 0).astype(np.float32)).all()

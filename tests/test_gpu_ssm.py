@@ -356,3 +356,64 @@ def test_an_infinite_input_is_infinity_whatever_the_states(n, one, what, dtype):
         clean[0][r:s.at[i + 1], c] = np.inf
         clean[1][i, c] = np.inf
     assert np.array_equal(y, clean[0]) and np.array_equal(left, clean[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("d,n,groups,lens", [(130, 129, 1, [1000]), (70, 256, 1, [700, 130]), (200, 200, 2, [300, 0, 40, 600]), (640, 256, 1, [200]), (65, 128, 1, [400, 33])])
+def test_many_states_over_many_chunks(d, n, groups, lens, dtype):
+    s = Scan(d + n, d, n, lens, dtype, groups)
+    cut, at = (C.c_int * 3)(), np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    assert L().frhip_ssm_cut(C.byref(s.p), len(lens), at.ctypes.data_as(C.c_void_p), 256, cut) == 0 and cut[1] > len(lens) + 4
+    fr.check(s.call(), "ssm_seq")
+    y, left = s.check()
+    assert np.isfinite(y.astype(np.float32)).all() and np.isfinite(left).all()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("one", [False, True])
+def test_gates_far_from_zero(one, dtype):
+    """silu(z) of a convolution's sums and of a scan's gates where its exponential leaves fp32: what is below the normal numbers may be 0"""
+    t = TYPE[dtype][0]
+    far = np.array([v for m in (30, 60, 80, 87, 87.5, 88, 89, 95, 103, 110, 125, 1e3, 6e4, 1e30, 3e38) for v in (m, -m) if dtype == "f32" or m < 65504], t)
+    c = len(far)
+    with np.errstate(over="ignore"):
+        want, tol = silu64(far.astype(np.float64)), silu_error(far.astype(np.float64), 0)
+    tol = np.where(np.isfinite(tol), tol, 0) + half_step(t, want) + np.where((far < -87) & (far > -104), -far.astype(np.float64), 1) * 2.0 ** -126
+
+    def close(rows):
+        bad = ~(np.abs(rows.astype(np.float64) - want) <= tol)
+        assert not bad.any(), (np.argwhere(bad)[:4], rows[bad][:4])
+    # a convolution that takes x as it is
+    x = np.tile(far, (9, 1))
+    w = np.zeros((c, 4), np.float32)
+    w[:, 3] = 1
+    dx, dw, st, dy = dev(x), dev(w), dev(np.zeros((9, 3, c), t)), DevBuf.empty((9, c), t)
+    args = (c, 4, dx.ptr, c, dw.ptr, None, 4, st.ptr, st.ptr, dy.ptr, c, TYPE[dtype][1], None)
+    fr.check(L().frhip_conv_one(9, *args) if one else L().frhip_conv_seq(1, (C.c_int32 * 2)(0, 9), *args))
+    close(dy.numpy())
+    # a scan whose y is 1 ahead of the gate: D x, an empty state and no input
+    zero, ones = dev(np.zeros((9, c), t)), dev(np.ones((9, c), t))
+    A, D, h, dy = dev(-np.ones((c, 4), np.float32)), dev(np.ones(c, np.float32)), dev(np.zeros((9, c, 4), np.float32)), DevBuf.empty((9, c), t)
+    p = fr.Ssm(A.ptr, D.ptr, None, c, 4, 1, 0)
+    mid = (ones.ptr, c, zero.ptr, c, zero.ptr, c, zero.ptr, c, dx.ptr, c, h.ptr, h.ptr, dy.ptr, c, TYPE[dtype][1])
+    ws = DevBuf(max(L().frhip_ssm_workspace_bytes(C.byref(p), 1, 9), 16))
+    fr.check(L().frhip_ssm_one(C.byref(p), 9, *mid, None) if one else L().frhip_ssm_seq(C.byref(p), 1, (C.c_int32 * 2)(0, 9), *mid, ws.ptr, None))
+    close(dy.numpy())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_outputs_of_finite_inputs_are_numbers(dtype):
+    """Every size of the tests above: the comparisons that they make let a NaN pass"""
+    sizes = lambda test, names: next(m for m in test.pytestmark if m.args[0] == names).args[1]
+    for d, n, groups, lens in sizes(test_scan_seq, "d,n,groups,lens"):
+        s = Scan(d * n, d, n, lens, dtype, groups)
+        fr.check(s.call())
+        assert all(np.isfinite(v.numpy().astype(np.float32)).all() for v in (s.buf["y"], s.out)), (d, n, lens)
+    for d, n, groups, rows in sizes(test_scan_one, "d,n,groups,rows"):
+        s = Scan(d * n + rows, d, n, [1] * rows, dtype, groups, one=True)
+        fr.check(s.call())
+        assert all(np.isfinite(v.numpy().astype(np.float32)).all() for v in (s.buf["y"], s.out)), (d, n, rows)
+    for c, W, lens in sizes(test_conv_seq, "c,W,lens"):
+        assert np.isfinite(conv_case(c, c, W, lens, dtype, ldx=c + c % 3).astype(np.float32)).all(), (c, W, lens)
+    for c, W, rows in sizes(test_conv_one, "c,W,rows"):
+        assert np.isfinite(conv_case(c + rows, c, W, [1] * rows, dtype, ldx=2 * c, one=True).astype(np.float32)).all(), (c, W, rows)
