@@ -961,8 +961,7 @@ extern "C" int frhip_linear(const void* x, int ldx, const frhip_weight* w, const
     return set_error(FRHIP_EINVAL, "linear: pointer not aligned");
   const size_t ye = ((rows - 1) * ldy + N) * elem;
   auto hits = [&](const void* p, size_t bytes) { return rows_overlap(p, bytes, y, ye, 1, bytes, ye, 1); };
-  const size_t xe = ((rows - 1) * ldx + K) * 2;
-  if (out_dtype == FRHIP_F16 ? rows_overlap(x, ldx, y, ldy, rows, K, N, 2) : hits(x, xe)) return set_error(FRHIP_EINVAL, "linear: y overlaps x");
+  if (rows_overlap(x, (size_t)ldx * 2, y, ldy * elem, rows, K * 2, N * elem, 1)) return set_error(FRHIP_EINVAL, "linear: y overlaps x");
   if (residual && !(residual == y && ldr == ldy) && rows_overlap(residual, ldr, y, ldy, rows, N, N, elem))
     return set_error(FRHIP_EINVAL, "linear: y overlaps the residual in part");
   if (hits(w->data, N * K * (w->dtype == FRHIP_U8 ? 1 : 2)) || hits(bias, N * 4) || hits(w->mx, N * 2) || hits(w->rx, N * 2) || hits(w->my, K * 2) ||

@@ -228,3 +228,16 @@ def test_infinities_are_those_of_the_formula(act, T, K, N, quant):
             else:
                 assert ((np.abs(down) <= 2.0 ** -126) | (np.isnan(down) if act in ("silu", "gelu") else False)).all(), (code, r, down)
         assert np.isfinite(np.delete(y, list(last), 0).astype(np.float32)).all()
+
+
+@pytest.mark.parametrize("T", [1, 20, 200])
+def test_rows_of_fp32_beside_those_of_x(T):
+    """One buffer of 256 bytes a row: 64 binary16, then 32 fp32 that receive their product"""
+    g = np.random.default_rng(T)
+    buf = g.standard_normal((T, 128)).astype(np.float16)
+    pw, _ = make_weight((g.standard_normal((64, 32)) / 8).astype(np.float16))
+    near, d, dy = dev(np.ascontiguousarray(buf[:, :64])), dev(buf), DevBuf.empty((T, 32), np.float32)
+    fr.check(L().frhip_linear(near.ptr, 64, pw.ref, None, 0, None, 0, dy.ptr, 32, T, fr.F32, None, None))
+    fr.check(L().frhip_linear(d.ptr, 128, pw.ref, None, 0, None, 0, d.ptr + 128, 64, T, fr.F32, None, None))
+    got = d.numpy()
+    assert np.array_equal(got[:, :64], buf[:, :64]) and np.array_equal(np.ascontiguousarray(got[:, 64:]).view(np.float32), dy.numpy())

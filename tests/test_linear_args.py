@@ -95,3 +95,9 @@ def test_a_workspace_for_some_rows_serves_fewer(K, N):
             assert fr.lib().frhip_linear_workspace_bytes(T, C.byref(w)) >= most, T
     sizes = [fr.lib().frhip_linear_workspace_bytes(T, C.byref(w)) for T in (1, 16, 100, 512, 513, 1024, 1153, 1409, 3000, 4100, 8192, 8193, 100000, 1 << 30)]
     assert sizes == sorted(sizes)
+
+
+@pytest.mark.parametrize("kw", [dict(y=A + 124, ldy=64), dict(y=A + 132, ldy=64), dict(y=A + 252, ldy=64), dict(y=A + 128, ldy=66)])
+def test_rows_of_fp32_beside_those_of_x_that_overlap_them(kw):
+    """x: 64 of 128 binary16 a row of 256 bytes; y: 32 fp32 at a byte of such a row"""
+    assert linear(ldx=128, out=fr.F32, **kw) == EINVAL
