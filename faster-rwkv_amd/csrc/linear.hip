@@ -1,7 +1,9 @@
 // Products with bias, activation and residual: y = residual + act(x . w + bias), for any number of rows, K a multiple of 8, any N, rows of
 // any pitch.  Sums are fp32 on the MFMA units (rows streamed: v_dot2_f32_f16), the epilogue is fp32, and a result is rounded once.
 // The forms are those of the framework's other products, each with its reasons there, and so are the cuts and the expected times that
-// choose among them (plan_linear); what differs is the pitch of x, a K that need not fill its last step, and the end.
+// choose among them (plan_linear), which know nothing of what an end reads and evaluates; what differs is the pitch of x, a K that need not fill its last step,
+// and the end.  Not among them: the loading waves that frhip_gemm has for whole tiles of 256 rows and up to 160 columns, and rows of uint8 weights streamed (one and
+// two go out as a few rows).
 // us here and of frhip_gemm (no epilogue) on the same operands: 48 x 2048 x 8192 9.9 and 10.3, 512 x 2048 x 8192 25.5 and 25.3, 1024 x 2048 x
 // 8192 40.3 and 40.8, 4099 x 5120 x 2560 114 and 114, 4096 x 2560 x 10240 208 and 205; the vendor library's binary16 product 18.5 (its
 // call), 26.2, 38.2, 96.7, 251.

@@ -250,10 +250,11 @@ constexpr int scan_rows(int nw) { return nw == 1 ? 8 : 16; }  // of a block of t
 //   B. runs all of its rows with NPL states a lane in registers, and leaves its part of y in LDS;
 //   C. adds the parts of the rows that it took in A, applies skip and gate and stores them.
 // The step width's softplus and the gate are so evaluated once a channel and row, not once a wave, and a chunk's states are over several
-// waves, which a SIMD needs to keep issuing.  What bounds it are vector instructions: a state and row takes two products, two
-// multiply-adds and an exponential (3.6 and 8.4 cycles a wave), in step 1 one less, and the softplus, gate, conversions and sums of A and C come
-// to a third as much again; they are issued in three quarters of the cycles.  4096 rows of 4096 channels x 16 states, binary16: 126 us
-// (55 + 71 in the two steps), memory alone would be 26; a lane with all 16 states of a channel and one wave a SIMD took 368.
+// waves, which a SIMD needs to keep issuing.  4096 rows of 4096 channels x 16 states, binary16: 125 us (launched by themselves the steps take 50
+// and 75), memory alone would be 26; a lane with all 16 states of a channel and one wave a SIMD took 368.  What bounds it are vector instructions: a
+// state and row takes two products, two multiply-adds and an exponential (3.6 and 8.4 cycles a wave), in step 1 a multiply-add less, which is
+// 70 us; softplus, gate, conversions, addresses and the sums of A and C are about half as many instructions again, and a quarter of the cycles issue none.
+// Shorter chunks issue in less: 2077 rows of nine prompts of 1536 x 16 (36 us) in 0.4 of the cycles, between the fold, the first block's way to LDS and its end.
 // Not kept: dt x times B as an outer product on the matrix units, 152; shorter blocks of time or five to eight workgroups a compute unit, 127 to
 // 136; rows through buffer descriptors, 131.
 template <class T, int NPL, int NW, bool LOCAL, bool PAD>
@@ -575,7 +576,9 @@ constexpr int kScanRows = 16;          // a chunk is a multiple of it
 constexpr int kScanWhole = 32;         // prompts of up to so many rows are not cut
 
 // Rows of a chunk: enough chunks for four workgroups a compute unit (4096 rows of 4096 channels x 16 states, with two, three, four: 165, 142,
-// 130 us, six and eight in shorter blocks 136 and 127; 830 rows of 1280 x 64, workgroups of eight waves, with two, four: 46, 41).
+// 130 us, six and eight in shorter blocks 136 and 127; 830 rows of 1280 x 64, workgroups of eight waves, with two, four: 46, 41).  A compute unit holds four of the forms with
+// four waves, but of step 2 of those with eight and sixteen (33 states and more) two and one: what is over runs in further rounds (1280 x 64: 540 workgroups of
+// step 2 over 512 places; 1024 rows of 2560 x 128, 880 over 512: 146 us; 4096 of 1280 x 256, 860 over 256: 638).
 // Where no prompt has more than kScanWhole rows the first launch costs more than it shares out (1536 channels x 16 states, in chunks of 16 and
 // whole: 17 rows 8.8 and 7.0 us, 32 rows 8.9 and 7.0, 48 rows 8.9 and 9.1; x 64 states: 13.6 and 10.6, 13.6 and 10.7, 13.9 and 14.7).
 static int scan_chunk(const ScanShape& s, int nseq, const int32_t* start, int cus) {

@@ -358,9 +358,9 @@ int frhip_wkv4_cut(int T, int C, int compute_units, int *out);
  * frhip_gemm_act, which rounds ahead of the activation as the reference does).  x [T] rows of K binary16, ldx elements apart;
  * bias [N] fp32 or NULL; residual [T] rows of N in out_dtype, ldr apart, or NULL; y [T] rows of N in out_dtype (F16 or F32), ldy
  * apart; the residual may be y itself (the same address and pitch), otherwise y overlaps nothing that is read.  act: one of FRHIP_ACT_*.
- * K and ldx are multiples of 8, at most 8388544, T is any up to 2^30, N up to 2^24, K N up to 2^34; x and w->data are 16-byte aligned, w->mx, rx, my and ry 4-byte (my and ry
- * 16-byte for the quick expansion of codes, where a product expands them), the others lie at multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace:
- * frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each.  The
+ * K and ldx are multiples of 8, at most 8388544, T is any up to 2^30, N up to 2^24, K N up to 2^34; x and w->data are 16-byte aligned,
+ * w->mx, rx, my and ry 4-byte (my and ry 16-byte for the quick expansion of codes, where a product expands them), the others lie at
+ * multiples of their elements.  uint8 weights stand for the w^ of frhip_dequant_u8, at any T.  workspace: frhip_linear_workspace_bytes(T, w) bytes (0: may be NULL), 16-byte aligned; calls that can run at the same time need one each.  The
  * bytes do not fall as T grows: a workspace for the most rows that a program has serves every call of fewer. */
 #define FRHIP_ACT_GELU 5     /* v/2 (1 + erf(v / sqrt 2)) */
 #define FRHIP_ACT_SOFTPLUS 6 /* log(1 + exp(v)) */
@@ -390,7 +390,8 @@ int frhip_conv_seq(int nseq, const int32_t *seq_start, int C, int W, const void 
  *   dt' = softplus(dt[t][d] + dt_bias[d])          (dt_softplus 0: dt[t][d] + dt_bias[d], not negative)
  *   h[d][n] = exp(dt' A[d][n]) h[d][n] + dt' x[t][d] B[t][g][n]
  *   y[t][d] = (sum_n C[t][g][n] h[d][n] + D[d] x[t][d]) * silu(z[t][d])
- * A [channels][states], not positive (minus infinity: forgets, but in a step of width zero, which keeps the state); D and dt_bias [channels], NULL: zero; z NULL: no gate.  B and C are rows of groups * states.
+ * A [channels][states], not positive (minus infinity: forgets, but in a step of width zero, which keeps the state); D and dt_bias
+ * [channels], NULL: zero; z NULL: no gate.  B and C are rows of groups * states.
  * state [.][channels][states] fp32.  states 1..256, channels up to 2^24.  What is not finite reaches the outputs of its channel from its token on, and
  * through B or C those of its group. */
 typedef struct frhip_ssm {
@@ -402,7 +403,7 @@ int frhip_ssm_one(const frhip_ssm *p, int rows, const void *x, int ldx, const vo
                   const void *C, int ldc, const void *z, int ldz, const float *state, float *state_out, void *y, int ldy,
                   int dtype, frhip_stream s);
 /* Scratch of frhip_ssm_seq for T rows in nseq prompts: bytes (may be 0), 16-byte aligned, owned by the caller; calls that can
- * run at the same time need one each. */
+ * run at the same time need one each.  One for more rows serves fewer, in however many prompts. */
 size_t frhip_ssm_workspace_bytes(const frhip_ssm *p, int nseq, int T);
 int frhip_ssm_seq(const frhip_ssm *p, int nseq, const int32_t *seq_start, const void *x, int ldx, const void *dt, int lddt,
                   const void *B, int ldb, const void *C, int ldc, const void *z, int ldz, const float *state, float *state_out,

@@ -116,3 +116,10 @@ def test_cut_arguments():
     p, out, f = fr.Ssm(A, None, None, 64, 16, 1, 1), (C.c_int * 3)(), fr.lib().frhip_ssm_cut
     assert f(None, 1, starts(0, 4), 256, out) == f(C.byref(p), 1, starts(0, 4), 256, None) == EINVAL
     assert f(C.byref(p), 1, starts(0, 4), 0, out) == f(C.byref(p), 0, None, 256, out) == f(C.byref(p), 129, starts(*range(130)), 256, out) == ESHAPE
+
+
+@pytest.mark.parametrize("channels,states,groups", [(1, 1, 1), (96, 16, 1), (300, 24, 3), (5120, 256, 1), (100000, 16, 1)])
+def test_a_workspace_for_more_rows_serves_fewer(channels, states, groups):
+    p = C.byref(fr.Ssm(A, None, None, channels, states, groups, 1))
+    sizes = [fr.lib().frhip_ssm_workspace_bytes(p, n, T) for T in [*range(600), 4096, 100000, 1 << 28] for n in (1, 200)]
+    assert sizes == sorted(sizes) and sizes[0::2] == sizes[1::2]
