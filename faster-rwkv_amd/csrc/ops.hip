@@ -211,8 +211,8 @@ __global__ __launch_bounds__(256) void transpose_kernel(const T* __restrict__ sr
   }
 }
 
-// Packed uint8 [N][K] -> packed binary16 [N][K]; thread handles 4 codes of one row at a time.  For codes, scales or outputs at any address of
-// four or two bytes; the launch is at most kDequantBlocks wide, so that its threads stay in 32 bits whatever N K is.
+// Packed uint8 [N][K] -> packed binary16 [N][K]; thread handles 4 codes of one row at a time.  For codes at any multiple of four bytes,
+// scales of two, outputs of eight; the launch is at most kDequantBlocks wide, so that its threads stay in 32 bits whatever N K is.
 constexpr unsigned kDequantBlocks = 1u << 22;
 __global__ __launch_bounds__(256) void dequant_u8_kernel(const uint32_t* __restrict__ q, const h1* __restrict__ mx, const h1* __restrict__ rx,
                                                          const h1* __restrict__ my, const h1* __restrict__ ry, h4* __restrict__ out, int K,
