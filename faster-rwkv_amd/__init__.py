@@ -50,8 +50,20 @@ class Ssm(C.Structure):
                 ("groups", C.c_int32), ("dt_softplus", C.c_int32)]
 
 
+class Delta(C.Structure):
+    """struct frhip_delta"""
+    _fields_ = [("A", C.c_void_p), ("dt_bias", C.c_void_p), ("heads", C.c_int32), ("key_heads", C.c_int32), ("key_dim", C.c_int32),
+                ("value_dim", C.c_int32), ("scale", C.c_float), ("norm_eps", C.c_float), ("dt_softplus", C.c_int32), ("beta_sigmoid", C.c_int32)]
+
+
+class BlockNorm(C.Structure):
+    """struct frhip_block_norm"""
+    _fields_ = [("after_w", C.c_void_p), ("after_b", C.c_void_p), ("before_w", C.c_void_p), ("before_b", C.c_void_p), ("channels", C.c_void_p),
+                ("cols", C.c_int32), ("after", C.c_int32), ("before", C.c_int32), ("gate_act", C.c_int32), ("scale", C.c_float), ("eps", C.c_float)]
+
+
 _vp, _i, _sz = C.c_void_p, C.c_int, C.c_size_t
-_WP, _SP = C.POINTER(Weight), C.POINTER(Ssm)
+_WP, _SP, _DP, _BP = C.POINTER(Weight), C.POINTER(Ssm), C.POINTER(Delta), C.POINTER(BlockNorm)
 
 _SIGS = {
     "frhip_abi_version": (_i, []),
@@ -124,6 +136,11 @@ _SIGS = {
     "frhip_ssm_one": (_i, [_SP, _i] + [_vp, _i] * 5 + [_vp, _vp, _vp, _i, _i, _vp]),
     "frhip_ssm_workspace_bytes": (_sz, [_SP, _i, _i]),
     "frhip_ssm_seq": (_i, [_SP, _i, _vp] + [_vp, _i] * 5 + [_vp, _vp, _vp, _i, _i, _vp, _vp]),
+    "frhip_delta_one": (_i, [_DP, _i] + [_vp, _i] * 5 + [_vp, _vp, _vp, _i, _i, _vp]),
+    "frhip_delta_workspace_bytes": (_sz, [_DP, _i, _i]),
+    "frhip_delta_seq": (_i, [_DP, _i, _vp] + [_vp, _i] * 5 + [_vp, _vp, _vp, _i, _i, _vp, _vp]),
+    "frhip_norm_gate": (_i, [_i, _i, _i, _i, _vp, _vp, C.c_float, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp]),
+    "frhip_norm_residual": (_i, [_BP, _i, _vp, _i, _vp, _i, _vp, _i, _vp, _i, _i, _vp, _i, _i, _vp]),
     "frhip_ssm_cut": (_i, [_SP, _i, _vp, _i, _vp]),
     "frhip_copy_probe": (_i, [_vp, _vp, _sz, _vp]),
     "frhip_read_probe": (_i, [_vp, _sz, _vp, _vp]),

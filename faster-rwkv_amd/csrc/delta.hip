@@ -1,0 +1,261 @@
+// The gated delta rule: a matrix per head as the state of a recurrence.
+//
+//   S = a S + b k (v - a S^T k)^T,   y = scale S^T q,   a = exp(A dt'), dt' = softplus(dt + dt_bias), b = sigmoid(beta)
+//
+// with q and k divided by their length.  S is [key][value] and its columns do not mix: a column of S, v and y is a recurrence of its own.
+#include <climits>
+#include <cstring>
+
+#include "activations.h"
+#include "frhip_internal.h"
+#include "groups.h"
+#include "lanes.h"
+#include "prompts.h"
+#include "spans.h"
+
+#pragma clang fp contract(off)
+
+namespace frhip {
+
+constexpr int kMostDim = 256;  // of a key, of a value
+
+template <class T>
+struct DeltaArgs {
+  const T *q, *k, *v, *dt, *beta;
+  T* y;
+  const float *A, *dt_bias, *state;
+  float* state_out;
+  int ldq, ldk, ldv, lddt, ldbeta, ldy;
+  int heads, share, dk, dv;  // share: heads of values to a head of keys
+  float scale, eps;          // eps < 0: q and k as they are
+  int softplus, sigmoid;
+  int nseq, rows;  // prompts of the launch; of single tokens: rows
+};
+
+// exp(g) for the logarithm of a decay: below -120 it is zero in fp32, above 88 it stays there
+__device__ __forceinline__ float decay_f(float g) {
+  const float a = exp_neg_fine(__builtin_fmaxf(__builtin_fminf(-g, 120.f), -88.f));
+  return g == g ? a : g;
+}
+
+// The logarithm of a row's decay.  A rate of minus infinity stays a number (times a step of width zero it keeps the state).
+template <class T>
+__device__ __forceinline__ float log_decay(const DeltaArgs<T>& a, float dt, float rate, float bias) {
+  const float v = dt + bias;
+  return rate * (a.softplus ? softplus_f<true>(v) : v);
+}
+__device__ __forceinline__ float finite_rate(float r) { return r < -__FLT_MAX__ ? -__FLT_MAX__ : r; }
+
+// ---------------------------------------------------------------------------
+// Token by token.  A wave has CL x 4 columns of a head, and CL lanes of a row of S: lane l has its columns 4 (l % CL) and the R keys from R (l / CL) on.
+// Bound by memory where there are many sequences of one token: the states once in and once out.
+// ---------------------------------------------------------------------------
+template <class T, int CL, int R, bool ONE>
+__global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, SeqTable tab) {
+  constexpr int W = 4 * CL;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int slices = (a.dv + W - 1) / W, unit = blockIdx.x * 4 + wave;
+  if (unit >= a.heads * slices) return;  // whole waves; nothing here waits for another one
+  const int head = unit / slices, kh = head / a.share, c = (unit - head * slices) * W + (lane % CL) * 4, d0 = lane / CL * R;
+  const int nc = a.dv - c, nd = a.dk - d0;
+  const float rate = a.A ? finite_rate(a.A[head]) : 1.f, bias = a.dt_bias ? a.dt_bias[head] : 0.f;
+  const size_t kat = (size_t)kh * a.dk + (nd > 0 ? d0 : 0), vat = (size_t)head * a.dv + (nc > 0 ? c : 0);
+  const int nseq = ONE ? a.rows : a.nseq;
+  for (int i = blockIdx.y; i < nseq; i += gridDim.y) {
+    const size_t st = ((size_t)i * a.heads + head) * a.dk * a.dv + c;
+    float S[R][4];
+#pragma unroll
+    for (int r = 0; r < R; r++) load_group<float, 4>(S[r], a.state + st + (size_t)(r < nd ? d0 + r : 0) * a.dv, r < nd ? nc : 0);
+    const int begin = ONE ? i : tab.start[i], end = ONE ? i + 1 : tab.start[i + 1];
+    for (int t = begin; t < end; t++) {
+      float q[R], k[R], v[4];
+      load_group<T, R>(q, a.q + (size_t)t * a.ldq + kat, nd);
+      load_group<T, R>(k, a.k + (size_t)t * a.ldk + kat, nd);
+      load_group<T, 4>(v, a.v + (size_t)t * a.ldv + vat, nc);
+      const float g = log_decay(a, (float)a.dt[(size_t)t * a.lddt + head], rate, bias), br = (float)a.beta[(size_t)t * a.ldbeta + head];
+      const float keep = decay_f(g), b = a.sigmoid ? sigmoid_f<true>(br) : br;
+      float kk = 0.f, qq = 0.f, qk = 0.f, kS[4] = {}, qS[4] = {};
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        kk = __builtin_fmaf(k[r], k[r], kk);
+        qq = __builtin_fmaf(q[r], q[r], qq);
+        qk = __builtin_fmaf(q[r], k[r], qk);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          kS[j] = __builtin_fmaf(k[r], S[r][j], kS[j]);
+          qS[j] = __builtin_fmaf(q[r], S[r][j], qS[j]);
+        }
+      }
+      qk = stride_sum<CL>(qk);
+      float kn = 1.f, qn = a.scale;
+      if (a.eps >= 0.f) {
+        kn = __builtin_amdgcn_rsqf(stride_sum<CL>(kk) + a.eps);
+        qn = __builtin_amdgcn_rsqf(stride_sum<CL>(qq) + a.eps) * a.scale;
+      }
+      float u[4], o[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        u[j] = b * (v[j] - keep * kn * stride_sum<CL>(kS[j]));
+        o[j] = qn * __builtin_fmaf(keep, stride_sum<CL>(qS[j]), qk * kn * u[j]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) S[r][j] = __builtin_fmaf(k[r] * kn, u[j], keep * S[r][j]);
+      if (lane < CL && nc > 0) store_group<T, 4>(a.y + (size_t)t * a.ldy + vat, o, nc);
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+      if (r < nd && nc > 0) store_group<float, 4>(a.state_out + st + (size_t)(d0 + r) * a.dv, S[r], nc);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+template <class T, int CL, bool ONE>
+static int step_launch(const DeltaArgs<T>& a, const SeqTable& tab, int nseq, hipStream_t st) {
+  const int slices = (a.dv + 4 * CL - 1) / (4 * CL), units = a.heads * slices;
+  const dim3 grid((units + 3) / 4, nseq < 65535 ? nseq : 65535);
+  const int rows = (a.dk + 64 / CL - 1) / (64 / CL);  // keys of a lane
+  if (rows <= 4) hipLaunchKernelGGL((delta_step_kernel<T, CL, 4, ONE>), grid, dim3(256), 0, st, a, tab);
+  else if (rows <= 8) hipLaunchKernelGGL((delta_step_kernel<T, CL, 8, ONE>), grid, dim3(256), 0, st, a, tab);
+  else if (rows <= 16) hipLaunchKernelGGL((delta_step_kernel<T, CL, 16, ONE>), grid, dim3(256), 0, st, a, tab);
+  else hipLaunchKernelGGL((delta_step_kernel<T, CL, 32, ONE>), grid, dim3(256), 0, st, a, tab);
+  return check_launch("delta");
+}
+
+static int delta_check_params(const frhip_delta* p) {
+  if (!p) return set_error(FRHIP_EINVAL, "delta: null pointer");
+  if (p->heads <= 0 || p->key_heads <= 0 || p->heads % p->key_heads != 0) return set_error(FRHIP_ESHAPE, "delta: heads must be a multiple of key_heads");
+  if (p->key_dim < 1 || p->key_dim > kMostDim || p->value_dim < 1 || p->value_dim > kMostDim) return set_error(FRHIP_ESHAPE, "delta: dimensions must be 1 to 256");
+  if ((long long)p->heads * p->value_dim > kMostChannels || (long long)p->key_heads * p->key_dim > kMostChannels)
+    return set_error(FRHIP_ESHAPE, "delta: a row may have up to 2^24 elements");
+  if (off_grid(4, {p->A, p->dt_bias})) return set_error(FRHIP_EINVAL, "delta: pointer not aligned to its element");
+  return 0;
+}
+
+struct DeltaCall {
+  const void *q, *k, *v, *dt, *beta;
+  int ldq, ldk, ldv, lddt, ldbeta;
+  const float* state;
+  float* state_out;
+  void* y;
+  int ldy, dtype;
+};
+
+static int delta_check(const frhip_delta& p, const DeltaCall& c, size_t row0, size_t rows, size_t nstate) {
+  if (c.dtype != FRHIP_F16 && c.dtype != FRHIP_F32) return set_error(FRHIP_EINVAL, "delta: dtype must be F16 or F32");
+  const int kn = p.key_heads * p.key_dim, vn = p.heads * p.value_dim;
+  if (c.ldq < kn || c.ldk < kn || c.ldv < vn || c.lddt < p.heads || c.ldbeta < p.heads || c.ldy < vn)
+    return set_error(FRHIP_ESHAPE, "delta: rows closer than their elements");
+  if (!c.state || !c.state_out || (rows && (!c.q || !c.k || !c.v || !c.dt || !c.beta || !c.y))) return set_error(FRHIP_EINVAL, "delta: null pointer");
+  const size_t elem = c.dtype == FRHIP_F16 ? 2 : 4, sbytes = nstate * p.heads * p.key_dim * p.value_dim * 4, pbytes = (size_t)p.heads * 4;
+  if (off_grid(elem, {c.q, c.k, c.v, c.dt, c.beta, c.y}) || off_grid(4, {c.state, c.state_out}))
+    return set_error(FRHIP_EINVAL, "delta: pointer not aligned to its element");
+  if (spans_clash(c.state, c.state_out, sbytes)) return set_error(FRHIP_EINVAL, "delta: states overlap in part");
+  if (spans_meet(c.state_out, sbytes, p.A, pbytes) || spans_meet(c.state_out, sbytes, p.dt_bias, pbytes))
+    return set_error(FRHIP_EINVAL, "delta: an output overlaps a parameter");
+  if (!rows) return 0;
+  struct In { const void* p; int ld, cols; };
+  const char* y = static_cast<const char*>(c.y) + row0 * c.ldy * elem;
+  const size_t ybytes = ((rows - 1) * c.ldy + vn) * elem;
+  if (spans_meet(y, ybytes, p.A, pbytes) || spans_meet(y, ybytes, p.dt_bias, pbytes)) return set_error(FRHIP_EINVAL, "delta: an output overlaps a parameter");
+  for (const In& in : {In{c.q, c.ldq, kn}, In{c.k, c.ldk, kn}, In{c.v, c.ldv, vn}, In{c.dt, c.lddt, p.heads}, In{c.beta, c.ldbeta, p.heads}}) {
+    const char* r = static_cast<const char*>(in.p) + row0 * in.ld * elem;
+    if (rows_overlap(r, in.ld, y, c.ldy, rows, in.cols, vn, elem) || spans_meet(r, ((rows - 1) * in.ld + in.cols) * elem, c.state_out, sbytes))
+      return set_error(FRHIP_EINVAL, "delta: an output overlaps what is read");
+  }
+  if (spans_meet(y, ybytes, c.state, sbytes) || spans_meet(y, ybytes, c.state_out, sbytes)) return set_error(FRHIP_EINVAL, "delta: an output overlaps what is read");
+  return 0;
+}
+
+template <class T>
+static DeltaArgs<T> delta_args(const frhip_delta& p, const DeltaCall& c) {
+  DeltaArgs<T> a;
+  memset(&a, 0, sizeof(a));
+  a.q = static_cast<const T*>(c.q);
+  a.k = static_cast<const T*>(c.k);
+  a.v = static_cast<const T*>(c.v);
+  a.dt = static_cast<const T*>(c.dt);
+  a.beta = static_cast<const T*>(c.beta);
+  a.y = static_cast<T*>(c.y);
+  a.A = p.A;
+  a.dt_bias = p.dt_bias;
+  a.state = c.state;
+  a.state_out = c.state_out;
+  a.ldq = c.ldq;
+  a.ldk = c.ldk;
+  a.ldv = c.ldv;
+  a.lddt = c.lddt;
+  a.ldbeta = c.ldbeta;
+  a.ldy = c.ldy;
+  a.heads = p.heads;
+  a.share = p.heads / p.key_heads;
+  a.dk = p.key_dim;
+  a.dv = p.value_dim;
+  a.scale = p.scale;
+  a.eps = p.norm_eps;
+  a.softplus = p.dt_softplus != 0;
+  a.sigmoid = p.beta_sigmoid != 0;
+  return a;
+}
+
+template <class T>
+static int delta_one_run(const frhip_delta& p, const DeltaCall& c, int rows, hipStream_t st) {
+  DeltaArgs<T> a = delta_args<T>(p, c);
+  a.rows = rows;
+  SeqTable none;
+  memset(&none, 0, sizeof(none));
+  return step_launch<T, 8, true>(a, none, rows, st);
+}
+
+template <class T>
+static int delta_seq_run(const frhip_delta& p, const DeltaCall& c, int nseq, const int32_t* start, void* workspace, hipStream_t st) {
+  DeltaArgs<T> a = delta_args<T>(p, c);
+  const size_t per = (size_t)p.heads * p.key_dim * p.value_dim;
+  for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {
+    SeqTable tab;
+    memset(&tab, 0, sizeof(tab));
+    a.nseq = nseq - s0 < kSeqTable ? nseq - s0 : kSeqTable;
+    for (int i = 0; i <= a.nseq; i++) tab.start[i] = start[s0 + i];
+    a.state = c.state + (size_t)s0 * per;
+    a.state_out = c.state_out + (size_t)s0 * per;
+    if (int rc = step_launch<T, 8, false>(a, tab, a.nseq, st)) return rc;
+  }
+  return 0;
+}
+
+}  // namespace frhip
+
+using namespace frhip;
+
+extern "C" int frhip_delta_one(const frhip_delta* p, int rows, const void* q, int ldq, const void* k, int ldk, const void* v, int ldv, const void* dt,
+                               int lddt, const void* beta, int ldbeta, const float* state, float* state_out, void* y, int ldy, int dtype,
+                               frhip_stream s) {
+  if (int rc = delta_check_params(p)) return rc;
+  if (rows < 0 || rows > kMostRows) return set_error(FRHIP_ESHAPE, "delta_one: rows must be 0 to 2^30");
+  const DeltaCall c = {q, k, v, dt, beta, ldq, ldk, ldv, lddt, ldbeta, state, state_out, y, ldy, dtype};
+  if (int rc = delta_check(*p, c, 0, rows, rows)) return rc;
+  if (rows == 0) return 0;
+  hipStream_t st = static_cast<hipStream_t>(s);
+  return dtype == FRHIP_F16 ? delta_one_run<h1>(*p, c, rows, st) : delta_one_run<float>(*p, c, rows, st);
+}
+
+extern "C" size_t frhip_delta_workspace_bytes(const frhip_delta* p, int nseq, int T) {
+  if (!p || nseq <= 0 || T <= 0) return 0;
+  return 0;
+}
+
+extern "C" int frhip_delta_seq(const frhip_delta* p, int nseq, const int32_t* seq_start, const void* q, int ldq, const void* k, int ldk, const void* v,
+                               int ldv, const void* dt, int lddt, const void* beta, int ldbeta, const float* state, float* state_out, void* y, int ldy,
+                               int dtype, void* workspace, frhip_stream s) {
+  if (int rc = delta_check_params(p)) return rc;
+  if (int rc = check_seqs(nseq, seq_start, kMostTime, "delta_seq: seq_start must be nseq + 1 row numbers up to 2^28 that do not descend")) return rc;
+  const DeltaCall c = {q, k, v, dt, beta, ldq, ldk, ldv, lddt, ldbeta, state, state_out, y, ldy, dtype};
+  const size_t row0 = nseq ? seq_start[0] : 0, rows = nseq ? seq_start[nseq] - seq_start[0] : 0;
+  if (int rc = delta_check(*p, c, row0, rows, nseq)) return rc;
+  if (nseq == 0) return 0;
+  hipStream_t st = static_cast<hipStream_t>(s);
+  return dtype == FRHIP_F16 ? delta_seq_run<h1>(*p, c, nseq, seq_start, workspace, st) : delta_seq_run<float>(*p, c, nseq, seq_start, workspace, st);
+}

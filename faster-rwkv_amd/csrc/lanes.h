@@ -1,0 +1,60 @@
+// Sums over groups of neighbouring lanes, of a wave and of a workgroup, in fp32: every lane of the group gets the sum, whose order is fixed.
+#pragma once
+
+#include "device_utils.h"
+
+#pragma clang fp contract(off)
+
+namespace frhip {
+
+// v of the lane and of the one 16 or 32 lanes away: the instruction swaps the odd rows (of 16 or 32 lanes) of its first operand with the even
+// ones of its second, so of a value and itself the results are the even rows twice and the odd rows twice
+__device__ __forceinline__ float add_across_16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_across_32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Over the LANES lanes that share lane / LANES
+template <int LANES>
+__device__ __forceinline__ float lane_sum(float v) {
+  if constexpr (LANES >= 2) v += dpp_mov<0xB1>(v);   // quad_perm [1,0,3,2]
+  if constexpr (LANES >= 4) v += dpp_mov<0x4E>(v);   // quad_perm [2,3,0,1]
+  if constexpr (LANES >= 8) v += dpp_mov<0x141>(v);  // row_half_mirror
+  if constexpr (LANES >= 16) v += dpp_mov<0x140>(v);  // row_mirror
+  if constexpr (LANES >= 32) v = add_across_16(v);
+  if constexpr (LANES >= 64) v = add_across_32(v);
+  return v;
+}
+
+// Over the lanes of a wave that share lane % STEP, STEP 4 to 64: the lanes of a row of 16 by rotations, then the rows
+template <int STEP>
+__device__ __forceinline__ float stride_sum(float v) {
+  if constexpr (STEP <= 4) v += dpp_mov<0x124>(v);  // row_ror:4
+  if constexpr (STEP <= 8) v += dpp_mov<0x128>(v);  // row_ror:8
+  if constexpr (STEP <= 16) v = add_across_16(v);
+  if constexpr (STEP <= 32) v = add_across_32(v);
+  return v;
+}
+
+// Over LANES lanes, up to a workgroup of LANES threads where they are more than a wave: then all threads call it, and `red` is LANES / 64 floats of LDS
+// that were last read ahead of a barrier (callers take turns between two)
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v, float* red) {
+  if constexpr (LANES <= 64) {
+    return lane_sum<LANES>(v);
+  } else {
+    v = lane_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float t = red[0];
+#pragma unroll
+    for (int i = 1; i < LANES / 64; i++) t += red[i];
+    return t;
+  }
+}
+
+}  // namespace frhip

@@ -14,29 +14,13 @@
 
 #include "activations.h"
 #include "frhip_internal.h"
+#include "groups.h"
+#include "prompts.h"
 #include "spans.h"
 
 #pragma clang fp contract(off)
 
 namespace frhip {
-
-constexpr int kSeqTable = 128;  // prompts of a launch; more go out in several
-struct SeqTable {
-  int start[kSeqTable + 1];  // first row
-  int chunk[kSeqTable + 1];  // first chunk (every prompt has one at least)
-};
-
-// The prompt that chunk `j` belongs to: the last i with first(i) <= j, for all lanes of a wave at once (all of them are here).  `first` does
-// not descend and first(0) is 0.  One load of a lane each: a search by halves waits for one after another.
-template <class F>
-__device__ __forceinline__ int find_seq(int nseq, int j, F first) {
-  static_assert(kSeqTable <= 128, "two prompts a lane");
-  if (nseq == 1) return 0;
-  const int l = threadIdx.x & 63;
-  int n = __builtin_popcountll(__ballot(l < nseq && first(min(l, nseq - 1)) <= j));
-  if (nseq > 64) n += __builtin_popcountll(__ballot(l + 64 < nseq && first(min(l + 64, nseq - 1)) <= j));
-  return __builtin_amdgcn_readfirstlane(n - 1);
-}
 
 // ---------------------------------------------------------------------------
 // Short causal convolution.  Bound by memory: every element once in and once out (4096 x 4096 binary16 out of rows of 8192: 16.8 us, 4.0
@@ -53,41 +37,8 @@ struct ConvArgs {
 };
 
 template <class T>
-constexpr int kConvLanes = 16 / sizeof(T);  // channels of a thread
+constexpr int kConvLanes = kGroup<T>;  // channels of a thread
 constexpr int kConvBatch = 4;               // rows that are requested together
-
-// Up to V elements at any address of one, the first n of them; 16 bytes an instruction if all are there, as for aligned ones
-template <class T, int V>
-__device__ __forceinline__ void load_group(float (&v)[V], const T* p, int n) {
-  constexpr int P = V < kConvLanes<T> ? V : kConvLanes<T>;
-  typedef T any __attribute__((ext_vector_type(P), aligned(sizeof(T))));
-  static_assert(V % P == 0, "whole pieces");
-  if (n >= V) {
-#pragma unroll
-    for (int q = 0; q < V; q += P) {
-      const any t = *reinterpret_cast<const any*>(p + q);
-#pragma unroll
-      for (int i = 0; i < P; i++) v[q + i] = (float)t[i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++) v[i] = i < n ? (float)p[i] : 0.f;
-  }
-}
-template <class T, int V>
-__device__ __forceinline__ void store_group(T* p, const float (&v)[V], int n) {
-  typedef T any __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-  if (n >= V) {
-    any t;
-#pragma unroll
-    for (int i = 0; i < V; i++) t[i] = (T)v[i];
-    *reinterpret_cast<any*>(p) = t;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; i++)
-      if (i < n) p[i] = (T)v[i];
-  }
-}
 
 template <class T, int W>
 struct ConvTaps {
@@ -567,9 +518,6 @@ static ScanShape scan_shape(const frhip_ssm& p) {
   return s;
 }
 
-constexpr int kMostRows = 1 << 30;     // of a call of single tokens: a loop over them counts in steps of up to 2^18
-constexpr int kMostTime = 1 << 28;     // row numbers of prompts: sums of a few of them stay in 32 bits, and so do a launch's threads
-constexpr int kMostChannels = 1 << 24;
 constexpr int kScanLeast = 16;         // rows of a chunk, at least
 constexpr int kScanMostUnits = 1024;   // workgroups of all chunks, at most about: what the workspace is sized for
 constexpr int kScanRows = 16;          // a chunk is a multiple of it
@@ -597,18 +545,6 @@ static int scan_chunk(const ScanShape& s, int nseq, const int32_t* start, int cu
 static size_t scan_most_local(const ScanShape& s, int T) {  // sum of (chunks - 1) <= T / chunk <= both
   const size_t by_rows = (size_t)T / kScanLeast, by_units = (size_t)(kScanMostUnits / s.wgs > 1 ? kScanMostUnits / s.wgs : 1);
   return by_rows < by_units ? by_rows : by_units;
-}
-
-static int check_seqs(int nseq, const int32_t* seq_start, int most, const char* what) {
-  if (nseq < 0) return set_error(FRHIP_ESHAPE, what);
-  if (nseq > 0) {
-    if (!seq_start) return set_error(FRHIP_EINVAL, what);
-    if (seq_start[0] < 0) return set_error(FRHIP_ESHAPE, what);
-    for (int i = 0; i < nseq; i++)
-      if (seq_start[i + 1] < seq_start[i]) return set_error(FRHIP_ESHAPE, what);
-    if (seq_start[nseq] > most) return set_error(FRHIP_ESHAPE, what);
-  }
-  return 0;
 }
 
 template <class T>

@@ -412,6 +412,58 @@ int frhip_ssm_seq(const frhip_ssm *p, int nseq, const int32_t *seq_start, const 
  * all prompts, out[2] workgroups a chunk. */
 int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int compute_units, int *out);
 
+/* ---- operators of a gated delta-rule layer -------------------------------------- */
+/* Recurrent layers whose state is a matrix per head, and the norms around their blocks (no counterpart in the reference; they stand beside
+ * att_one / att_seq, whose state is one too, and frhip_layernorm and frhip_groupnorm_f32).  Types, rows, prompts, states and overlaps are those of the
+ * state space operators above. */
+
+/* Gated delta rule, for every head h of `heads` with a state S [key_dim][value_dim], in groups of heads / key_heads that share q and k:
+ *   dt' = softplus(dt[t][h] + dt_bias[h])          (dt_softplus 0: dt[t][h] + dt_bias[h])
+ *   a = exp(A[h] dt'),  b = sigmoid(beta[t][h])    (beta_sigmoid 0: beta[t][h])
+ *   q, k = q[t], k[t] / sqrt(sum of their squares + norm_eps)      (norm_eps negative: as they are)
+ *   S = a S + b k (v[t][h] - a S^T k)^T
+ *   y[t][h] = scale S^T q
+ * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (up to 88 is computed; minus infinity
+ * forgets).  q and k are rows of key_heads * key_dim, v and y of heads * value_dim, dt and beta of heads.  state
+ * [.][heads][key_dim][value_dim] fp32.  Dimensions 1 to 256; heads * value_dim and key_heads * key_dim up to 2^24. */
+typedef struct frhip_delta {
+  const float *A, *dt_bias;
+  int32_t heads, key_heads, key_dim, value_dim;
+  float scale, norm_eps;
+  int32_t dt_softplus, beta_sigmoid;
+} frhip_delta;
+int frhip_delta_one(const frhip_delta *p, int rows, const void *q, int ldq, const void *k, int ldk, const void *v, int ldv, const void *dt, int lddt,
+                    const void *beta, int ldbeta, const float *state, float *state_out, void *y, int ldy, int dtype, frhip_stream s);
+/* Scratch of frhip_delta_seq for T rows in nseq prompts: bytes (may be 0), 16-byte aligned, owned by the caller; calls that can
+ * run at the same time need one each.  One for more rows serves fewer, in however many prompts. */
+size_t frhip_delta_workspace_bytes(const frhip_delta *p, int nseq, int T);
+int frhip_delta_seq(const frhip_delta *p, int nseq, const int32_t *seq_start, const void *q, int ldq, const void *k, int ldk, const void *v, int ldv,
+                    const void *dt, int lddt, const void *beta, int ldbeta, const float *state, float *state_out, void *y, int ldy, int dtype,
+                    void *workspace, frhip_stream s);
+
+/* Norms: v / sqrt(mean of v^2 + eps), FRHIP_NORM_MEAN of v less its mean.  Evaluated in fp32 (so are the squares), rounded once. */
+#define FRHIP_NORM_NONE 0
+#define FRHIP_NORM_RMS 1
+#define FRHIP_NORM_MEAN 2
+/* Behind a recurrence: y = (norm(x) w + b) act(z), each of the `heads` heads of a row normalised by itself.  w, b [heads * dim], NULL: one, zero; z
+ * NULL: no gate.  act FRHIP_ACT_NONE, _SIGMOID or _SILU.  dim up to 2^15, heads * dim up to 2^24, rows up to 2^30; y may be x itself (the
+ * same address and pitch), otherwise it overlaps nothing that is read. */
+int frhip_norm_gate(int rows, int heads, int dim, int kind, const float *w, const float *b, float eps, const void *x, int ldx, const void *z, int ldz,
+                    int act, void *y, int ldy, int dtype, frhip_stream s);
+/* From one block's output to the next one's input:
+ *   h = x + scale * channels * act(gate) * after(block),   y = before(h)
+ * x and h, the stream, in stream_dtype; block, gate and y in dtype.  The norm of h is that of its fp32 value, ahead of its rounding.  after, before: FRHIP_NORM_*, their
+ * weights and biases [cols], NULL: one, zero; channels [cols], NULL: one; gate_act as frhip_norm_gate's.  block NULL: h = x; gate
+ * NULL: one; ldg 0: one row of gates for all; h or y NULL: not wanted.  cols up to 2^15, rows up to 2^30.  h may be x itself (the same address and pitch),
+ * otherwise the outputs overlap nothing that is read, nor each other. */
+typedef struct frhip_block_norm {
+  const float *after_w, *after_b, *before_w, *before_b, *channels;
+  int32_t cols, after, before, gate_act;
+  float scale, eps;
+} frhip_block_norm;
+int frhip_norm_residual(const frhip_block_norm *p, int rows, const void *x, int ldx, const void *block, int ldb, const void *gate, int ldg, void *h, int ldh,
+                        int stream_dtype, void *y, int ldy, int dtype, frhip_stream s);
+
 /* ---- bandwidth probes: DIAGNOSTICS, not operators (measurement aids of bench.py and of the
  *      hardware-counter calibration; no counterpart in the reference, nothing on the model path calls them) */
 /* Plain device copy, 16 bytes per lane: the kernel of known traffic (bytes read + bytes
