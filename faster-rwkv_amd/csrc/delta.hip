@@ -6,52 +6,19 @@
 #include <climits>
 #include <cstring>
 
-#include "activations.h"
-#include "frhip_internal.h"
-#include "groups.h"
-#include "lanes.h"
-#include "prompts.h"
+#include "delta.h"
 #include "spans.h"
 
 #pragma clang fp contract(off)
 
 namespace frhip {
 
-constexpr int kMostDim = 256;  // of a key, of a value
-
-template <class T>
-struct DeltaArgs {
-  const T *q, *k, *v, *dt, *beta;
-  T* y;
-  const float *A, *dt_bias, *state;
-  float* state_out;
-  int ldq, ldk, ldv, lddt, ldbeta, ldy;
-  int heads, share, dk, dv;  // share: heads of values to a head of keys
-  float scale, eps;          // eps < 0: q and k as they are
-  int softplus, sigmoid;
-  int nseq, rows;  // prompts of the launch; of single tokens: rows
-};
-
-// exp(g) for the logarithm of a decay: below -120 it is zero in fp32, above 88 it stays there
-__device__ __forceinline__ float decay_f(float g) {
-  const float a = exp_neg_fine(__builtin_fmaxf(__builtin_fminf(-g, 120.f), -88.f));
-  return g == g ? a : g;
-}
-
-// The logarithm of a row's decay.  A rate of minus infinity stays a number (times a step of width zero it keeps the state).
-template <class T>
-__device__ __forceinline__ float log_decay(const DeltaArgs<T>& a, float dt, float rate, float bias) {
-  const float v = dt + bias;
-  return rate * (a.softplus ? softplus_f<true>(v) : v);
-}
-__device__ __forceinline__ float finite_rate(float r) { return r < -__FLT_MAX__ ? -__FLT_MAX__ : r; }
-
 // ---------------------------------------------------------------------------
 // Token by token.  A wave has CL x 4 columns of a head, and CL lanes of a row of S: lane l has its columns 4 (l % CL) and the R keys from R (l / CL) on.
 // Bound by memory where there are many sequences of one token: the states once in and once out.
 // ---------------------------------------------------------------------------
 template <class T, int CL, int R, bool ONE>
-__global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, SeqTable tab) {
+__global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, DeltaTable tab) {
   constexpr int W = 4 * CL;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slices = (a.dv + W - 1) / W, unit = blockIdx.x * 4 + wave;
@@ -62,11 +29,11 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, SeqTabl
   const size_t kat = (size_t)kh * a.dk + (nd > 0 ? d0 : 0), vat = (size_t)head * a.dv + (nc > 0 ? c : 0);
   const int nseq = ONE ? a.rows : a.nseq;
   for (int i = blockIdx.y; i < nseq; i += gridDim.y) {
-    const size_t st = ((size_t)i * a.heads + head) * a.dk * a.dv + c;
+    const size_t st = ((size_t)(ONE ? i : tab.seq[i]) * a.heads + head) * a.dk * a.dv + c;
     float S[R][4];
 #pragma unroll
     for (int r = 0; r < R; r++) load_group<float, 4>(S[r], a.state + st + (size_t)(r < nd ? d0 + r : 0) * a.dv, r < nd ? nc : 0);
-    const int begin = ONE ? i : tab.start[i], end = ONE ? i + 1 : tab.start[i + 1];
+    const int begin = ONE ? i : tab.start[i], end = ONE ? i + 1 : tab.end[i];
     for (int t = begin; t < end; t++) {
       float q[R], k[R], v[4];
       load_group<T, R>(q, a.q + (size_t)t * a.ldq + kat, nd);
@@ -114,7 +81,7 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, SeqTabl
 // Host side
 // ---------------------------------------------------------------------------
 template <class T, int CL, bool ONE>
-static int step_launch(const DeltaArgs<T>& a, const SeqTable& tab, int nseq, hipStream_t st) {
+static int step_launch(const DeltaArgs<T>& a, const DeltaTable& tab, int nseq, hipStream_t st) {
   const int slices = (a.dv + 4 * CL - 1) / (4 * CL), units = a.heads * slices;
   const dim3 grid((units + 3) / 4, nseq < 65535 ? nseq : 65535);
   const int rows = (a.dk + 64 / CL - 1) / (64 / CL);  // keys of a lane
@@ -128,6 +95,7 @@ static int step_launch(const DeltaArgs<T>& a, const SeqTable& tab, int nseq, hip
 static int delta_check_params(const frhip_delta* p) {
   if (!p) return set_error(FRHIP_EINVAL, "delta: null pointer");
   if (p->heads <= 0 || p->key_heads <= 0 || p->heads % p->key_heads != 0) return set_error(FRHIP_ESHAPE, "delta: heads must be a multiple of key_heads");
+  if (p->heads > kMostHeads) return set_error(FRHIP_ESHAPE, "delta: up to 65535 heads");
   if (p->key_dim < 1 || p->key_dim > kMostDim || p->value_dim < 1 || p->value_dim > kMostDim) return set_error(FRHIP_ESHAPE, "delta: dimensions must be 1 to 256");
   if ((long long)p->heads * p->value_dim > kMostChannels || (long long)p->key_heads * p->key_dim > kMostChannels)
     return set_error(FRHIP_ESHAPE, "delta: a row may have up to 2^24 elements");
@@ -205,7 +173,7 @@ template <class T>
 static int delta_one_run(const frhip_delta& p, const DeltaCall& c, int rows, hipStream_t st) {
   DeltaArgs<T> a = delta_args<T>(p, c);
   a.rows = rows;
-  SeqTable none;
+  DeltaTable none;
   memset(&none, 0, sizeof(none));
   return step_launch<T, 8, true>(a, none, rows, st);
 }
@@ -214,14 +182,28 @@ template <class T>
 static int delta_seq_run(const frhip_delta& p, const DeltaCall& c, int nseq, const int32_t* start, void* workspace, hipStream_t st) {
   DeltaArgs<T> a = delta_args<T>(p, c);
   const size_t per = (size_t)p.heads * p.key_dim * p.value_dim;
-  for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {
-    SeqTable tab;
-    memset(&tab, 0, sizeof(tab));
-    a.nseq = nseq - s0 < kSeqTable ? nseq - s0 : kSeqTable;
-    for (int i = 0; i <= a.nseq; i++) tab.start[i] = start[s0 + i];
+  for (int s0 = 0; s0 < nseq; s0 += kSeqTable) {  // short prompts token by token, the others chunk by chunk
+    const int n = nseq - s0 < kSeqTable ? nseq - s0 : kSeqTable;
     a.state = c.state + (size_t)s0 * per;
     a.state_out = c.state_out + (size_t)s0 * per;
-    if (int rc = step_launch<T, 8, false>(a, tab, a.nseq, st)) return rc;
+    DeltaTable tab;
+    memset(&tab, 0, sizeof(tab));
+    int many[kSeqTable], nmany = 0;
+    a.nseq = 0;
+    for (int i = 0; i < n; i++) {
+      const int from = start[s0 + i], to = start[s0 + i + 1];
+      if (to - from >= kDeltaChunkLeast) {
+        many[nmany++] = i;
+        continue;
+      }
+      tab.start[a.nseq] = from;
+      tab.end[a.nseq] = to;
+      tab.seq[a.nseq++] = i;
+    }
+    if (a.nseq)
+      if (int rc = step_launch<T, 8, false>(a, tab, a.nseq, st)) return rc;
+    if (nmany)
+      if (int rc = delta_chunk_run<T>(a, many, nmany, start + s0, start[nseq] - start[0], workspace, st)) return rc;
   }
   return 0;
 }
@@ -243,8 +225,9 @@ extern "C" int frhip_delta_one(const frhip_delta* p, int rows, const void* q, in
 }
 
 extern "C" size_t frhip_delta_workspace_bytes(const frhip_delta* p, int nseq, int T) {
-  if (!p || nseq <= 0 || T <= 0) return 0;
-  return 0;
+  if (nseq <= 0 || T <= 0 || delta_check_params(p)) return 0;
+  const size_t bytes = delta_chunk_bytes(*p, 4, T) > delta_chunk_bytes(*p, 2, T) ? delta_chunk_bytes(*p, 4, T) : delta_chunk_bytes(*p, 2, T);
+  return (bytes + 255) / 256 * 256;
 }
 
 extern "C" int frhip_delta_seq(const frhip_delta* p, int nseq, const int32_t* seq_start, const void* q, int ldq, const void* k, int ldk, const void* v,
@@ -256,6 +239,10 @@ extern "C" int frhip_delta_seq(const frhip_delta* p, int nseq, const int32_t* se
   const size_t row0 = nseq ? seq_start[0] : 0, rows = nseq ? seq_start[nseq] - seq_start[0] : 0;
   if (int rc = delta_check(*p, c, row0, rows, nseq)) return rc;
   if (nseq == 0) return 0;
+  if (frhip_delta_workspace_bytes(p, nseq, (int)rows) > 0) {
+    if (!workspace) return set_error(FRHIP_EINVAL, "delta_seq: null workspace");
+    if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return set_error(FRHIP_EINVAL, "delta_seq: workspace must be 16-byte aligned");
+  }
   hipStream_t st = static_cast<hipStream_t>(s);
   return dtype == FRHIP_F16 ? delta_seq_run<h1>(*p, c, nseq, seq_start, workspace, st) : delta_seq_run<float>(*p, c, nseq, seq_start, workspace, st);
 }

@@ -37,7 +37,7 @@ def delta(seq=True, p=None, **kw):
     (dict(y=3 * A), EINVAL), (dict(y=4 * A + 2), EINVAL), (dict(y=5 * A), EINVAL), (dict(y=6 * A), EINVAL), (dict(y=7 * A + 2), EINVAL), (dict(y=8 * A), EINVAL),
     (dict(y=9 * A + 64), EINVAL), (dict(out=8 * A + 4), EINVAL), (dict(out=5 * A), EINVAL), (dict(p=dict(A=10 * A)), EINVAL), (dict(p=dict(bias=9 * A)), EINVAL),
     (dict(p=dict(A=A + 2)), EINVAL), (dict(p=dict(heads=3)), ESHAPE), (dict(p=dict(heads=0)), ESHAPE), (dict(p=dict(key_heads=0)), ESHAPE), (dict(p=dict(dk=0)), ESHAPE),
-    (dict(p=dict(dk=257)), ESHAPE), (dict(p=dict(dv=0)), ESHAPE), (dict(p=dict(dv=257)), ESHAPE), (dict(p=dict(heads=1 << 22, key_heads=1), ldv=1 << 27, ldy=1 << 27), ESHAPE)])
+    (dict(p=dict(heads=65536, key_heads=1, dv=1), lddt=65536, ldbeta=65536, ldv=65536, ldy=65536), ESHAPE), (dict(p=dict(dk=257)), ESHAPE), (dict(p=dict(dv=0)), ESHAPE), (dict(p=dict(dv=257)), ESHAPE), (dict(p=dict(heads=1 << 22, key_heads=1), ldv=1 << 27, ldy=1 << 27), ESHAPE)])
 def test_refusals(kw, code, seq):
     assert delta(seq, **kw) == code and fr.lib().frhip_error_string()
 
