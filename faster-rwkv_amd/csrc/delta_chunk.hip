@@ -74,6 +74,7 @@ constexpr uint32_t kNotFinite = 0x7f800000u;  // magnitudes from here on
 
 // v as hi + lo
 __device__ __forceinline__ void split(float v, h1& hi, h1& lo) {
+  asm("" : "+v"(v));  // rounded to fp32 ahead of both conversions: a product that v_fma_mixlo_f16 rounds once gives another hi, now and then
   hi = (h1)v;
   lo = (h1)(v - (float)hi);
 }
