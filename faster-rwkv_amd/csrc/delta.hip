@@ -3,6 +3,7 @@
 //   S = a S + b k (v - a S^T k)^T,   y = scale S^T q,   a = exp(A dt'), dt' = softplus(dt + dt_bias), b = sigmoid(beta)
 //
 // with q and k divided by their length.  S is [key][value] and its columns do not mix: a column of S, v and y is a recurrence of its own.
+#include <algorithm>
 #include <climits>
 #include <cstring>
 
@@ -97,8 +98,8 @@ static int delta_check_params(const frhip_delta* p) {
   if (p->heads <= 0 || p->key_heads <= 0 || p->heads % p->key_heads != 0) return set_error(FRHIP_ESHAPE, "delta: heads must be a multiple of key_heads");
   if (p->heads > kMostHeads) return set_error(FRHIP_ESHAPE, "delta: up to 65535 heads");
   if (p->key_dim < 1 || p->key_dim > kMostDim || p->value_dim < 1 || p->value_dim > kMostDim) return set_error(FRHIP_ESHAPE, "delta: dimensions must be 1 to 256");
-  if ((long long)p->heads * p->value_dim > kMostChannels || (long long)p->key_heads * p->key_dim > kMostChannels)
-    return set_error(FRHIP_ESHAPE, "delta: a row may have up to 2^24 elements");
+  if ((long long)p->heads * p->value_dim > kMostPitch || (long long)p->key_heads * p->key_dim > kMostPitch)
+    return set_error(FRHIP_ESHAPE, "delta: a row may have up to 2^23 elements");
   if (off_grid(4, {p->A, p->dt_bias})) return set_error(FRHIP_EINVAL, "delta: pointer not aligned to its element");
   return 0;
 }
@@ -117,6 +118,8 @@ static int delta_check(const frhip_delta& p, const DeltaCall& c, size_t row0, si
   const int kn = p.key_heads * p.key_dim, vn = p.heads * p.value_dim;
   if (c.ldq < kn || c.ldk < kn || c.ldv < vn || c.lddt < p.heads || c.ldbeta < p.heads || c.ldy < vn)
     return set_error(FRHIP_ESHAPE, "delta: rows closer than their elements");
+  for (int ld : {c.ldq, c.ldk, c.ldv, c.lddt, c.ldbeta, c.ldy})
+    if (ld > kMostPitch) return set_error(FRHIP_ESHAPE, "delta: rows more than 2^23 elements apart");
   if (!c.state || !c.state_out || (rows && (!c.q || !c.k || !c.v || !c.dt || !c.beta || !c.y))) return set_error(FRHIP_EINVAL, "delta: null pointer");
   const size_t elem = c.dtype == FRHIP_F16 ? 2 : 4, sbytes = nstate * p.heads * p.key_dim * p.value_dim * 4, pbytes = (size_t)p.heads * 4;
   if (off_grid(elem, {c.q, c.k, c.v, c.dt, c.beta, c.y}) || off_grid(4, {c.state, c.state_out}))
@@ -202,6 +205,10 @@ static int delta_seq_run(const frhip_delta& p, const DeltaCall& c, int nseq, con
     }
     if (a.nseq)
       if (int rc = step_launch<T, 8, false>(a, tab, a.nseq, st)) return rc;
+    std::sort(many, many + nmany, [&](int x, int y) {  // long ones first
+      const int lx = start[s0 + x + 1] - start[s0 + x], ly = start[s0 + y + 1] - start[s0 + y];
+      return lx != ly ? lx > ly : x < y;
+    });
     if (nmany)
       if (int rc = delta_chunk_run<T>(a, many, nmany, start + s0, start[nseq] - start[0], workspace, st)) return rc;
   }

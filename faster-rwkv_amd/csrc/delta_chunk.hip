@@ -1,14 +1,16 @@
 // The gated delta rule chunk by chunk, on the matrix units.
 //
-// In a chunk of 64 rows that begins at the state S, with a_ij the decay from row j to row i, a_i0 that from the chunk's start and k, q of unit length,
+// In a chunk of 64 rows that begins at the state S, with a_ij the decay from row j to row i, a_i0 that from the chunk's start, a_Ci that to its end and k, q of
+// unit length, the rows write the values U:
 //   R_i = b_i (v_i - a_i0 S^T k_i),   U = T R,   T = (1 + L)^-1,   L_ij = b_i a_ij k_i . k_j  (j < i)
 //   y_i = scale a_i0 S^T q_i + (P R)_i,   P = A T,   A_ij = scale a_ij q_i . k_j  (j <= i)
-//   S' = a_C0 S + sum_i k_i (a_Ci U_i)^T
-// T and P do not depend on S: a first launch finds them for all chunks at once; a second one walks the chunks of a prompt, a head and 16 columns of S
-// a workgroup, with three products a chunk that wait for each other: [K; Q] S, [T; P] R, K^T U.
+//   S' = a_C0 S + W R,   W = sum_i k_i (a_Ci T_i)^T
+// P and W do not depend on S: a first launch finds them for all chunks at once; a second one walks the chunks of a prompt, a head and 16 columns of S
+// a workgroup, with two products a chunk that wait for each other: [K; Q] S and [W; P] R.
 //
-// The products multiply binary16 with fp32 sums.  What is fp32 goes in as a pair hi + lo, 22 bits and more, scaled by a power of two: rows of T and P, of q
-// and k where they are fp32, columns of S, R and U.  Rows of q and k go in as they are but for a power of two, binary16 exactly, and their lengths are made good behind the products.
+// The products multiply binary16 with fp32 sums.  What is fp32 goes in as a pair hi + lo, 22 bits and more, scaled by a power of two: rows of W and P, of q
+// and k where they are fp32, columns of S and R.  Rows of k go in as they are but for a power of two, binary16 exactly, those of q as they are, and their
+// lengths are made good behind the products.
 #include <algorithm>
 #include <climits>
 #include <cstring>
@@ -20,26 +22,33 @@
 namespace frhip {
 
 constexpr int kChunk = 64;
+constexpr int kXcds = 8;
 constexpr float kLeastLog = -1e4f;  // of a row's decay, which is zero there; sums of a chunk's stay exact enough in float64
 
-// Per chunk and head: [T: 6 blocks][P: 6 blocks], a block 32 columns of 16 rows as {hi, lo}[64 lanes] operands; [5][64] row factors; bounds
+// Per chunk and head: P, W, the rows' factors, W's rows' factors, bounds.  A block is 64 columns' half of 16 rows as {hi, lo}[64 lanes] operands: lane l has
+// row l % 16, and of block ks the columns 32 ks + 4 (l / 16) and on and those 16 further, four each: as the results lie that it is made of.
 constexpr int kBlockBytes = 2 * 64 * 16;
+__device__ __forceinline__ constexpr int block_of(int tile, int ks) { return (tile == 3 ? 4 : tile) + ks; }  // of P; its tiles 0 and 1 have one
 constexpr int kTriBytes = 6 * kBlockBytes;
-__device__ __forceinline__ constexpr int block_of(int tile, int ks) { return (tile == 3 ? 4 : tile) + ks; }  // tiles 0 and 1 have one block
-enum { kRowBeta, kRowK, kRowQ, kRowP, kRowT, kRowKinds };
+enum { kRowBeta, kRowK, kRowQ, kRowP, kRowKinds };
 struct ChunkBounds {
-  float key[4], tri[4], back[4];  // of each wave's rows, see the scan
-  float keep;                     // the decay of the whole chunk
-  int bad;                        // the first row of which something is not finite, or kChunk
-  float pad[2];
+  float key, back;  // see the scan
+  float keep;       // the decay of the whole chunk
+  int bad;          // the first row of which something is not finite, or kChunk
 };
-constexpr int kRowsAt = 2 * kTriBytes, kBoundsAt = kRowsAt + kRowKinds * kChunk * 4, kHeadBytes = (kBoundsAt + (int)sizeof(ChunkBounds) + 255) / 256 * 256;
+template <int KS>
+struct HeadLayout {
+  static constexpr int W = kTriBytes, rows = W + KS * 2 * 2 * kBlockBytes, back = rows + kRowKinds * kChunk * 4, bounds = back + KS * 32 * 4,
+                       bytes = (bounds + (int)sizeof(ChunkBounds) + 255) / 256 * 256;
+};
 
 // Per chunk and head of keys: [K][Q], each [4 tiles of 16 rows][steps of 32 dimensions][parts][64 lanes] operands
 constexpr size_t key_bytes(int dkp, int parts) { return (size_t)kChunk * dkp * 2 * parts * 2; }
 
 template <class T>
 constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ f32x4 mfma_h(h8 a, h8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma_f(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
@@ -56,13 +65,6 @@ __device__ __forceinline__ uint32_t max_across_rows(uint32_t v) {
   const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return max((uint32_t)s[0], (uint32_t)s[1]);
 }
-template <class F>
-__device__ __forceinline__ float wave_fold(float v, F f) {
-#pragma unroll
-  for (int m = 1; m < 64; m *= 2) v = f(v, __shfl_xor(v, m));
-  return v;
-}
-
 // A power of two that takes what is not above `bound` (its bits, sign off) below 2^15, and its reciprocal.  For no bound that is finite: any
 __device__ __forceinline__ float scale_for(uint32_t bound) {
   const int field = 268 - (int)(bound >> 23);
@@ -72,61 +74,95 @@ __device__ __forceinline__ float inverse_of(float power) { return __uint_as_floa
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 constexpr uint32_t kNotFinite = 0x7f800000u;  // magnitudes from here on
 
-// v as hi + lo
-__device__ __forceinline__ void split(float v, h1& hi, h1& lo) {
-  asm("" : "+v"(v));  // rounded to fp32 ahead of both conversions: a product that v_fma_mixlo_f16 rounds once gives another hi, now and then
-  hi = (h1)v;
-  lo = (h1)(v - (float)hi);
+// x, y as hi + lo
+__device__ __forceinline__ void split(float x, float y, h2& hi, h2& lo) {
+  asm("" : "+v"(x), "+v"(y));  // rounded to fp32 first: a product that a conversion rounds once gives another hi, now and then
+  hi = __builtin_convertvector((f32x2){x, y}, h2);
+  lo = __builtin_convertvector((f32x2){__builtin_fmaf((float)hi[0], -1.f, x), __builtin_fmaf((float)hi[1], -1.f, y)}, h2);
+}
+__device__ __forceinline__ void split(const f32x4& v, h4& hi, h4& lo) {
+  h2 h[2], l[2];
+  split(v[0], v[1], h[0], l[0]);
+  split(v[2], v[3], h[1], l[1]);
+  hi = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3);
+  lo = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3);
 }
 
 // ---------------------------------------------------------------------------
-// First launch: T, P and the row factors of every chunk and head, and q and k as operands of every chunk and head of keys
+// First launch: P, W and the factors of every chunk and head, and q and k as operands of every chunk and head of keys
 // ---------------------------------------------------------------------------
-// A tile of 16 rows as operands: lane l has row l % 16, of step ks the dimensions 32 ks + 8 (l / 16) and on, times a power of two that takes the
-// row's largest value to [2^8, 2^9), fp32 as hi + lo.  Of the lane's row: the sum of squares, the sum of magnitudes and the largest one of what the operands
-// hold, and the power of two; a row with something that is not finite is zero.
+// A tile of 16 rows as operands: lane l has row l % 16, of step ks the dimensions 32 ks + 8 (l / 16) and on.  fp32 goes in times a power of two that takes the
+// row's largest value to [2^8, 2^9), as hi + lo; binary16 as it is or (SCALED) times one that takes the row's length to [2^7, 2^8], in the range of
+// binary16.  Of the lane's row: the sum of squares of what the operands hold, and the power; a row with something that is not finite is zero.
 template <class T, int KS>
 struct KeyTile {
   h8 f[KS][kParts<T>];
-  float squares, sum, most, power;
+  float squares, power;
   bool finite;
 
+  template <bool SCALED>
   __device__ __forceinline__ void load(const T* rows, size_t ld, int row0, int nrows, int dk) {
     const int lane = threadIdx.x & 63, row = row0 + (lane & 15), d0 = (lane >> 4) * 8;
     const bool there = row < nrows;
     const T* const p = rows + (size_t)(there ? row : 0) * ld;
-    float v[KS][8];
-    uint32_t top = 0;
+    squares = 0.f;
+    if constexpr (kParts<T> == 2) {
+      float v[KS][8];
+      uint32_t top = 0;
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      const int d = ks * 32 + d0;
-      load_group<T, 8>(v[ks], p + (d < dk ? d : 0), there ? dk - d : 0);
-#pragma unroll
-      for (int i = 0; i < 8; i++) top = max(top, magnitude(v[ks][i]));
-    }
-    top = max_across_rows(top);
-    finite = top < kNotFinite;
-    power = __uint_as_float((uint32_t)max(1, min(262 - (int)(top >> 23), 127 + 60)) << 23);  // 2^60 at most: its square times norm_eps stays in fp32
-    squares = sum = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float x = finite ? v[ks][i] * power : 0.f;
-        squares = __builtin_fmaf(x, x, squares);
-        sum += __builtin_fabsf(x);
-        if constexpr (kParts<T> == 2) {
-          h1 hi, lo;
-          split(x, hi, lo);
-          f[ks][0][i] = hi;
-          f[ks][1][i] = lo;
-        } else {
-          f[ks][0][i] = (h1)x;
-        }
+      for (int ks = 0; ks < KS; ks++) {
+        const int d = ks * 32 + d0;
+        load_group<T, 8>(v[ks], p + (d < dk ? d : 0), there ? dk - d : 0);
       }
-    squares = add_across_32(add_across_16(squares));
-    sum = add_across_32(add_across_16(sum));
-    most = finite ? __uint_as_float(top) * power : 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = max(top, magnitude(v[ks][i]));
+      top = max_across_rows(top);
+      finite = top < kNotFinite;
+      power = __uint_as_float((uint32_t)max(1, min(262 - (int)(top >> 23), 127 + 60)) << 23);  // 2^60 at most: its square times norm_eps stays in fp32
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+          const float x = finite ? v[ks][i] * power : 0.f, y = finite ? v[ks][i + 1] * power : 0.f;
+          squares = __builtin_fmaf(x, x, squares);
+          squares = __builtin_fmaf(y, y, squares);
+          h2 hi, lo;
+          split(x, y, hi, lo);
+          f[ks][0][i] = hi[0], f[ks][0][i + 1] = hi[1];
+          f[ks][1][i] = lo[0], f[ks][1][i + 1] = lo[1];
+        }
+      squares = add_across_32(add_across_16(squares));
+    } else {
+      typedef h1 any8 __attribute__((ext_vector_type(8), aligned(2)));
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const int d = ks * 32 + d0, n = there ? dk - d : 0;
+        h8 x = {};
+        if (n >= 8) {
+          x = *reinterpret_cast<const any8*>(p + d);
+        } else if (n > 0) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[i] = i < n ? p[d + i] : (h1)0.f;
+        }
+        f[ks][0] = x;
+      }
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) squares = dot8acc(f[ks][0], f[ks][0], squares);
+      squares = add_across_32(add_across_16(squares));
+      finite = magnitude(squares) < kNotFinite;
+      power = 1.f;
+      if constexpr (SCALED) power = __uint_as_float((uint32_t)(127 + min(8 - (((int)(__float_as_uint(squares) >> 23) - 125) >> 1), 15)) << 23);
+      if (!finite) power = 0.f;
+      if (SCALED || !finite) {
+        const h1 by = (h1)power;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) f[ks][0] = finite ? f[ks][0] * by : (h8){};
+        squares = finite ? squares * power * power : 0.f;
+      }
+      if (!finite) power = 1.f;
+    }
   }
   // what the operands' row is to be multiplied by
   __device__ __forceinline__ float factor(float eps) const {
@@ -141,236 +177,313 @@ struct KeyTile {
   }
 };
 
-template <class T, int KS>
-__device__ __forceinline__ f32x4 gram(const KeyTile<T, KS>& a, const KeyTile<T, KS>& b) {
-  f32x4 s = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (kParts<T> == 2) {
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      s = mfma_h(a.f[ks][1], b.f[ks][0], s);
-      s = mfma_h(a.f[ks][0], b.f[ks][1], s);
-    }
-  }
-#pragma unroll
-  for (int ks = 0; ks < KS; ks++) s = mfma_h(a.f[ks][0], b.f[ks][0], s);
-  return s;
+constexpr int kLd = kChunk + 4;  // of an fp32 matrix in LDS: 16 rows, 16 bytes each, are on all banks
+constexpr int kLdT = kChunk + 8;
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+// Four rows of 16 columns of a matrix in LDS by the 16 lanes of a row of lanes: lane p gives row p / 4, columns 4 (p % 4) and on, and gets column p
+__device__ __forceinline__ h4 read_columns(const h1* p) {
+  return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(void*)p));
 }
 
-constexpr int kLd = kChunk + 4;  // of a matrix in LDS: 16 rows apart, 16 bytes each, on all banks
-
-// The operands of 16 rows of a lower triangular matrix m, by rows' powers of two; returns the sum of magnitudes of the lane's row
-__device__ __forceinline__ float store_tri(const float (*m)[kLd], int tile, char* to, float* inv) {
-  const int lane = threadIdx.x & 63, row = tile * 16 + (lane & 15), g = lane >> 4;
-  float v[2][8], sum = 0.f;
-  uint32_t top = 0;
-#pragma unroll
-  for (int ks = 0; ks < 2; ks++) {
-    const bool there = 2 * ks + (g >> 1) <= tile;  // the others were never written
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-      f32x4 t = {0.f, 0.f, 0.f, 0.f};
-      if (there) t = *reinterpret_cast<const f32x4*>(&m[row][ks * 32 + g * 8 + i]);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        v[ks][i + e] = t[e];
-        top = max(top, magnitude(t[e]));
-        sum += __builtin_fabsf(t[e]);
-      }
-    }
-  }
-  const float power = scale_for(max_across_rows(top));
-  *inv = inverse_of(power);
-#pragma unroll
-  for (int ks = 0; ks < 2; ks++) {
-    if (ks * 2 > tile) break;
-    h8 hi, lo;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      h1 a, b;
-      split(v[ks][i] * power, a, b);
-      hi[i] = a;
-      lo[i] = b;
-    }
-    h8* const block = reinterpret_cast<h8*>(to + block_of(tile, ks) * kBlockBytes);
-    block[lane] = hi;
-    block[64 + lane] = lo;
-  }
-  return add_across_32(add_across_16(sum));
+// Operands of a block and its row's power, of two tiles of results whose rows are its columns
+__device__ __forceinline__ void store_block(char* to, const f32x4& a, const f32x4& b, float power) {
+  const int lane = threadIdx.x & 63;
+  h4 h[2], l[2];
+  split(a * power, h[0], l[0]);
+  split(b * power, h[1], l[1]);
+  reinterpret_cast<h8*>(to)[lane] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
+  reinterpret_cast<h8*>(to)[64 + lane] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_fmaxf(x, y); }
+__device__ __forceinline__ float most_of(const f32x4& v) {
+  return larger(larger(__builtin_fabsf(v[0]), __builtin_fabsf(v[1])), larger(__builtin_fabsf(v[2]), __builtin_fabsf(v[3])));
+}
+__device__ __forceinline__ float most_of_16(float v) {  // over the lanes that share lane / 16
+  v = larger(v, dpp_mov<0xB1>(v));
+  v = larger(v, dpp_mov<0x4E>(v));
+  v = larger(v, dpp_mov<0x141>(v));
+  return larger(v, dpp_mov<0x140>(v));
 }
 
-// blockIdx.x: a chunk, blockIdx.y: a head.  Wave w has the rows 16 w to 16 w + 15 of every matrix, but of T behind its diagonal the columns.
 template <class T, int KS>
-__global__ __launch_bounds__(256) void delta_prep_kernel(DeltaArgs<T> a, DeltaTable tab, char* keys, char* heads) {
-  __shared__ __attribute__((aligned(16))) float Lm[kChunk][kLd], Am[kChunk][kLd], Tm[kChunk][kLd];
-  __shared__ double Gs[kChunk];
-  __shared__ float fk[kChunk], fq[kChunk], beta[kChunk], l1[kChunk];
-  __shared__ int spoilt[kChunk];
+struct PrepLds {
+  h1 K[kParts<T>][kChunk][KS * 32 + 8];
+  union {
+    float LT[kChunk][kLd];  // blocks of 16: behind the diagonal L's, as they are; on it T's, as they are; ahead of it T's from behind it, transposed
+    h1 C[2][kChunk][kLdT];  // [column][row] of T with its rows' a_Ci, hi and lo
+  };
+  double G[kChunk];  // sums of the logarithms of the rows' decays
+  float fk[kChunk], fq[kChunk], length[kChunk], write[kChunk], back[kChunk], inv[kChunk], ref[4][kChunk];
+  float most[4];
+  int bad;
+};
+
+// blockIdx.x: a chunk, blockIdx.y: a head.  Wave w has the rows 16 w to 16 w + 15 of K, Q, L and P, those columns of T, and a quarter of W; wave 0 the gates.
+template <class T, int KS>
+__global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 ? 2 : 1) void delta_prep_kernel(DeltaArgs<T> a, DeltaTable tab, char* keys, char* heads) {
+  constexpr int NK = kParts<T>, ST = KS / 2;
+  typedef PrepLds<T, KS> Lds;
+  typedef HeadLayout<KS> Out;
+  __shared__ __attribute__((aligned(16))) Lds lds;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cj = blockIdx.x, head = blockIdx.y, kh = head / a.share;
   const int i0 = find_seq(a.nseq, cj, [&](int k) { return tab.chunk[k]; });
   const int t0 = tab.start[i0] + (cj - tab.chunk[i0]) * kChunk, len = min(tab.end[i0] - t0, kChunk);
-  const T* const kr = a.k + (size_t)t0 * a.ldk + (size_t)kh * a.dk;
-  const T* const qr = a.q + (size_t)t0 * a.ldq + (size_t)kh * a.dk;
+  char* const out = heads + ((size_t)cj * a.heads + head) * Out::bytes;
+  const int row = w * 16 + c, r0 = w * 16 + g * 4;  // the lane's row of an operand, the first one of results
   KeyTile<T, KS> K, Q;
-  K.load(kr, a.ldk, w * 16, len, a.dk);
-  Q.load(qr, a.ldq, w * 16, len, a.dk);
+  K.template load<true>(a.k + (size_t)t0 * a.ldk + (size_t)kh * a.dk, a.ldk, w * 16, len, a.dk);
+  Q.template load<false>(a.q + (size_t)t0 * a.ldq + (size_t)kh * a.dk, a.ldq, w * 16, len, a.dk);
+  const bool there = lane < len;  // wave 0: a lane a row
+  float rate = 1.f, bias = 0.f, dt = 0.f, raw = 0.f;
+  if (w == 0) {
+    if (a.A) rate = finite_rate(a.A[head]);
+    if (a.dt_bias) bias = a.dt_bias[head];
+    if (there) {
+      dt = (float)a.dt[(size_t)(t0 + lane) * a.lddt + head];
+      raw = (float)a.beta[(size_t)(t0 + lane) * a.ldbeta + head];
+    }
+  }
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+    for (int n = 0; n < NK; n++) *reinterpret_cast<h8*>(&lds.K[n][row][ks * 32 + g * 8]) = K.f[ks][n];
+  if (g == 0) {
+    const float nan = __builtin_nanf("");
+    lds.fk[row] = K.finite ? K.factor(a.eps) : nan;
+    lds.fq[row] = (Q.finite ? Q.factor(a.eps) : nan) * a.scale;
+    lds.length[row] = __builtin_sqrtf(K.squares * (KS * 32));  // not below the sum of the row's magnitudes
+  }
   if (head % a.share == 0) {
-    constexpr int tile = KS * kParts<T> * 64;
-    h8* const to = reinterpret_cast<h8*>(keys + ((size_t)cj * (a.heads / a.share) + kh) * key_bytes(KS * 32, kParts<T>));
+    constexpr int tile = KS * NK * 64;
+    h8* const to = reinterpret_cast<h8*>(keys + ((size_t)cj * (a.heads / a.share) + kh) * key_bytes(KS * 32, NK));
     K.store(to + w * tile);
     Q.store(to + (4 + w) * tile);
   }
-  if (g == 0) {
-    const float f = K.factor(a.eps);
-    fk[w * 16 + c] = f;
-    fq[w * 16 + c] = (Q.finite ? Q.factor(a.eps) : __builtin_nanf("")) * a.scale;
-    l1[w * 16 + c] = K.sum;
-    spoilt[w * 16 + c] = !K.finite || magnitude(f) >= kNotFinite;  // (nothing divided by its length)
-  }
   __syncthreads();
-  // a lane a row, in every wave alike
-  int bad;
-  double G;
-  {
-    const bool there = lane < len;
-    const size_t t = t0 + (there ? lane : 0);
-    const float rate = a.A ? finite_rate(a.A[head]) : 1.f, bias = a.dt_bias ? a.dt_bias[head] : 0.f;
-    const float lg = there ? log_decay(a, (float)a.dt[t * a.lddt + head], rate, bias) : 0.f, raw = there ? (float)a.beta[t * a.ldbeta + head] : 0.f;
+  f32x4 kk[4], kq[4];  // K K^T, rows 4 g and on of the wave's, column c of tile j; K Q^T, rows 4 g and on of tile j, column c of the wave's
+#pragma unroll
+  for (int j = 0; j < 4; j++) {
+    kk[j] = kq[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (j > w) continue;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      const h8 b = *reinterpret_cast<const h8*>(&lds.K[0][j * 16 + c][ks * 32 + g * 8]);
+      if constexpr (NK == 2) {
+        const h8 lo = *reinterpret_cast<const h8*>(&lds.K[1][j * 16 + c][ks * 32 + g * 8]);
+        kk[j] = mfma_h(K.f[ks][0], lo, kk[j]);
+        kq[j] = mfma_h(lo, Q.f[ks][0], kq[j]);
+        kk[j] = mfma_h(K.f[ks][1], b, kk[j]);
+        kq[j] = mfma_h(b, Q.f[ks][1], kq[j]);
+      }
+      kk[j] = mfma_h(K.f[ks][0], b, kk[j]);
+      kq[j] = mfma_h(b, Q.f[ks][0], kq[j]);
+    }
+  }
+  if (w == 0) {
+    const float lg = log_decay(a, dt, rate, bias), fk = lds.fk[lane];
     float b = there ? (a.sigmoid ? sigmoid_f<true>(raw) : raw) : 0.f;
-    const unsigned long long off = __ballot(there && (spoilt[lane] || magnitude(b) >= kNotFinite || !(lg < __builtin_inff())));
-    bad = off ? __builtin_ctzll(off) : kChunk;
-    G = lane < bad ? (double)__builtin_fmaxf(lg, kLeastLog) : 0.0;
+    const unsigned long long off = __ballot(there && (magnitude(fk) >= kNotFinite || magnitude(b) >= kNotFinite || !(lg < __builtin_inff())));
+    const int bad = off ? __builtin_ctzll(off) : kChunk;
+    double G = there && lane < bad ? (double)__builtin_fmaxf(lg, kLeastLog) : 0.0;
     if (lane >= bad) b = 0.f;
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
       const double up = __shfl_up(G, m);
       if (lane >= m) G += up;
     }
-    if (w == 0) {
-      Gs[lane] = G;
-      beta[lane] = b;
+    const float f = lane < bad ? fk : 0.f, from = decay_f((float)G), key = b * from * f;
+    lds.G[lane] = G;
+    lds.write[lane] = b * f;
+    lds.back[lane] = f * decay_f((float)(__shfl(G, 63) - G));
+    float* const rows = reinterpret_cast<float*>(out + Out::rows) + lane;
+    rows[kRowBeta * kChunk] = b;
+    rows[kRowK * kChunk] = key;
+    rows[kRowQ * kChunk] = lds.fq[lane] * from;
+    const float bkey = max_across_rows(most_of_16(__builtin_fabsf(key) * lds.length[lane]));
+    if (lane == 63) {
+      lds.bad = bad;
+      ChunkBounds* const to = reinterpret_cast<ChunkBounds*>(out + Out::bounds);
+      to->key = bkey;
+      to->keep = from;
+      to->bad = bad;
     }
   }
   __syncthreads();
-  const int r0 = w * 16 + g * 4;  // the lane's rows of a tile of results, whose column is c
-  double Gi[4];
-  float bi[4], fi[4], qi[4];
+  const int bad = lds.bad;
+  f32x4 X[4];  // T's tiles (w + n, w), as results
+  {
+    // Decays between a row of the wave's and one ahead of them go by way of the row in between: each half is at most one where decays are
+    const double Gref = lds.G[w ? w * 16 - 1 : 0], Gl = lds.G[lane];
+    const bool ahead = lane < w * 16;
+    lds.ref[w][lane] = decay_f((float)(ahead ? Gref - Gl : Gl - Gref)) * (ahead ? (lane < bad ? lds.fk[lane] : 0.f) : 1.f);
+    __builtin_amdgcn_wave_barrier();
+    const f32x4 lw = *reinterpret_cast<const f32x4*>(&lds.write[r0]), lref = *reinterpret_cast<const f32x4*>(&lds.ref[w][r0]);
+    const float qi = row < bad ? lds.fq[row] : 0.f, qref = lds.ref[w][row];
+    f32x4 ld;  // L on the diagonal
 #pragma unroll
-  for (int r = 0; r < 4; r++) {
-    Gi[r] = Gs[r0 + r];
-    bi[r] = beta[r0 + r];
-    fi[r] = fk[r0 + r];
-    qi[r] = fq[r0 + r];
-  }
-  for (int j = 0; j <= w; j++) {
-    KeyTile<T, KS> B;
-    if (j < w) B.load(kr, a.ldk, j * 16, len, a.dk);
-    else B = K;
-    const f32x4 kk = gram<T, KS>(K, B), qk = gram<T, KS>(Q, B);
-    const int col = j * 16 + c;
-    const double Gj = Gs[col];
-    const float fj = fk[col];
+    for (int j = 0; j < 4; j++) {
+      if (j > w) continue;
+      const int col = j * 16 + c, col4 = j * 16 + g * 4;
+      if (j < w) {
+        const float at = lds.ref[w][col];
+        const f32x4 at4 = *reinterpret_cast<const f32x4*>(&lds.ref[w][col4]);
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int row = r0 + r;
-      const float d = decay_f((float)(Gi[r] - Gj)) * fj;
-      Lm[row][col] = col < row && row < bad ? bi[r] * fi[r] * (d * kk[r]) : 0.f;
-      Am[row][col] = col <= row && row < bad ? qi[r] * (d * qk[r]) : 0.f;
+        for (int r = 0; r < 4; r++) {
+          lds.LT[r0 + r][col] = lw[r] * (lref[r] * at * kk[j][r]);
+          kq[j][r] = qi * (qref * at4[r] * kq[j][r]);
+        }
+      } else {
+        const double Gc = lds.G[col];  // of the lane's column of L, and of its row of A
+        const float fc = col < bad ? lds.fk[col] : 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const double Gr = lds.G[r0 + r];
+          const float f4 = r0 + r < bad ? lds.fk[r0 + r] : 0.f;
+          ld[r] = col < r0 + r ? lw[r] * (decay_f((float)(Gr - Gc)) * fc * kk[j][r]) : 0.f;
+          kq[j][r] = r0 + r <= col ? qi * (decay_f((float)(Gc - Gr)) * f4 * kq[j][r]) : 0.f;
+        }
+      }
     }
-  }
-  // (a wave's own rows of Lm and Am: written and read by the same wave, in order)
-  __builtin_amdgcn_wave_barrier();
-  {  // T on its diagonal, column c of 16, row by row
+    // T on the diagonal: column c, row by row, L's values from their lanes
     float t[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      float s = i == c ? 1.f : 0.f;
+    for (int i = 0; i < 16; i++) t[i] = i == c ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < i; j++) s = __builtin_fmaf(-Lm[w * 16 + i][w * 16 + j], t[j], s);
-      t[i] = s;
-    }
-    if (g == 0) {
+    for (int j = 0; j < 15; j++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) Tm[w * 16 + i][w * 16 + c] = t[i];
+      for (int i = 1; i < 16; i++) {
+        if (i <= j) continue;
+        const float l = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ld[i % 4]), i / 4 * 16 + j));
+        t[i] = __builtin_fmaf(-l, t[j], t[i]);
+      }
+#pragma unroll
+    for (int s = 0; s < 4; s++) {
+      const float ta = t[s], tb = t[4 + s], tc = t[8 + s], td = t[12 + s];
+      const float x = g & 1 ? tb : ta, y = g & 1 ? td : tc;
+      X[0][s] = g & 2 ? y : x;
+      lds.LT[r0 + s][w * 16 + c] = X[0][s];
     }
   }
   __syncthreads();
-  // T behind its diagonal, wave j the columns of tile j: T_ij = -T_ii sum_m L_im T_mj (m = j to i - 1).  An operand of results as they lie (row 4 g + s of
-  // step s) goes with the columns 4 g + s of the other matrix.
-  f32x4 X[4];
-#pragma unroll
-  for (int s = 0; s < 4; s++) X[0][s] = Tm[w * 16 + g * 4 + s][w * 16 + c];  // X[n]: tile w + n
+  // T behind it: T_ij = -T_ii sum_m L_im T_mj (m = j to i - 1).  An operand of results as they lie (row 4 g + s of step s) goes with the columns 4 g + s of
+  // the other matrix.
 #pragma unroll
   for (int n = 1; n < 4; n++) {
-    if (w + n > 3) break;
+    X[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    if (w + n > 3) continue;
     const int i = w + n;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    f32x4 acc[2] = {X[n], X[n]};
 #pragma unroll
-    for (int m = 0; m < n; m++) {
-      const f32x4 l = *reinterpret_cast<const f32x4*>(&Lm[i * 16 + c][(w + m) * 16 + g * 4]);
+    for (int m = 0; m < 3; m++) {
+      if (m >= n) continue;
+      const f32x4 l = *reinterpret_cast<const f32x4*>(&lds.LT[i * 16 + c][(w + m) * 16 + g * 4]);
 #pragma unroll
-      for (int s = 0; s < 4; s++) acc = mfma_f(l[s], X[m][s], acc);
+      for (int s = 0; s < 4; s++) acc[s & 1] = mfma_f(l[s], X[m][s], acc[s & 1]);
     }
-    const f32x4 ti = *reinterpret_cast<const f32x4*>(&Tm[i * 16 + c][i * 16 + g * 4]);
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    const f32x4 ti = *reinterpret_cast<const f32x4*>(&lds.LT[i * 16 + c][i * 16 + g * 4]), sum = acc[0] + acc[1];
 #pragma unroll
-    for (int s = 0; s < 4; s++) x = mfma_f(ti[s], -acc[s], x);
-    X[n] = x;
-#pragma unroll
-    for (int s = 0; s < 4; s++) Tm[i * 16 + g * 4 + s][w * 16 + c] = x[s];
+    for (int s = 0; s < 4; s++) X[n] = mfma_f(ti[s], -sum[s], X[n]);
+    *reinterpret_cast<f32x4*>(&lds.LT[w * 16 + c][i * 16 + g * 4]) = X[n];
   }
   __syncthreads();
-  // P = A T, the wave's rows
-  f32x4 Pt[4];
+  {  // P = A T, as its transpose T^T A^T: a lane has columns 4 g and on of every tile, of its row
+    f32x4 P[4];
+    float top = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    if (j > w) break;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int m = j; m <= w; m++) {
-      const f32x4 am = *reinterpret_cast<const f32x4*>(&Am[w * 16 + c][m * 16 + g * 4]);
+    for (int j = 0; j < 4; j++) {
+      P[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      if (j > w) continue;
 #pragma unroll
-      for (int s = 0; s < 4; s++) acc = mfma_f(am[s], Tm[m * 16 + g * 4 + s][j * 16 + c], acc);
+      for (int m = 0; m < 4; m++) {
+        if (m < j || m > w) continue;
+        f32x4 t;
+        if (m == j) {
+#pragma unroll
+          for (int s = 0; s < 4; s++) t[s] = lds.LT[j * 16 + g * 4 + s][j * 16 + c];
+        } else {
+          t = *reinterpret_cast<const f32x4*>(&lds.LT[j * 16 + c][m * 16 + g * 4]);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; s++) P[j] = mfma_f(t[s], kq[m][s], P[j]);
+      }
     }
-    Pt[j] = acc;
-  }
-  __builtin_amdgcn_wave_barrier();
 #pragma unroll
-  for (int j = 0; j < 4; j++) {
-    if (j > w) break;
+    for (int j = 0; j < 4; j++) top = larger(top, most_of(P[j]));
+    const float power = scale_for(magnitude(max_across_rows(top)));
+    store_block(out + block_of(w, 0) * kBlockBytes, P[0], P[1], power);
+    if (w >= 2) store_block(out + block_of(w, 1) * kBlockBytes, P[2], P[3], power);
+    if (g == 0) reinterpret_cast<float*>(out + Out::rows)[kRowP * kChunk + row] = inverse_of(power);
+  }
+  float top = 0.f;  // T with a_Ci
 #pragma unroll
-    for (int r = 0; r < 4; r++) Am[r0 + r][j * 16 + c] = Pt[j][r];
+  for (int n = 0; n < 4; n++) {
+    if (w + n > 3) continue;
+    X[n] *= *reinterpret_cast<const f32x4*>(&lds.back[(w + n) * 16 + g * 4]);
+    top = larger(top, most_of(X[n]));
   }
-  __builtin_amdgcn_wave_barrier();
-  char* const out = heads + ((size_t)cj * a.heads + head) * kHeadBytes;
-  float invt, invp;
-  const float rowsum = store_tri(Tm, w, out, &invt);
-  store_tri(Am, w, out + kTriBytes, &invp);
-  // of row 16 w + c
-  const int row = w * 16 + c;
-  const double Grow = Gs[row], Gend = Gs[kChunk - 1];
-  const float from = decay_f((float)Grow), back = row < bad ? decay_f((float)(Gend - Grow)) * fk[row] : 0.f;
-  const float key = row < bad ? beta[row] * from * fk[row] : 0.f;
-  float* const rows = reinterpret_cast<float*>(out + kRowsAt);
-  if (g == 0) {
-    rows[kRowBeta * kChunk + row] = beta[row];
-    rows[kRowK * kChunk + row] = key;
-    rows[kRowQ * kChunk + row] = fq[row] * from;
-    rows[kRowP * kChunk + row] = invp;
-    rows[kRowT * kChunk + row] = back * invt;
+  const float power = scale_for(magnitude(max_across_rows(top)));
+  if (g == 0) lds.inv[row] = inverse_of(power);
+  __syncthreads();
+  if (w & 1) {  // the block of 32 rows begins ahead of the diagonal
+    *reinterpret_cast<h4*>(&lds.C[0][row][(w - 1) * 16 + g * 4]) = (h4){};
+    *reinterpret_cast<h4*>(&lds.C[1][row][(w - 1) * 16 + g * 4]) = (h4){};
   }
-  const auto larger = [](float x, float y) { return __builtin_fmaxf(x, y); };
-  const float bkey = wave_fold(__builtin_fabsf(key) * l1[row], larger), btri = wave_fold(__builtin_fabsf(back) * rowsum, larger);
-  const float bback = wave_fold(g == 0 ? K.most * __builtin_fabsf(back) * rowsum : 0.f, [](float x, float y) { return x + y; });
-  if (lane == 0) {
-    ChunkBounds* const b = reinterpret_cast<ChunkBounds*>(out + kBoundsAt);
-    b->key[w] = bkey;
-    b->tri[w] = btri;
-    b->back[w] = bback;
-    if (w == 0) {
-      b->keep = decay_f((float)Gend);
-      b->bad = bad;
+#pragma unroll
+  for (int n = 0; n < 4; n++) {
+    if (w + n > 3) continue;
+    h4 hi, lo;
+    split(X[n] * power, hi, lo);
+    *reinterpret_cast<h4*>(&lds.C[0][row][(w + n) * 16 + g * 4]) = hi;
+    *reinterpret_cast<h4*>(&lds.C[1][row][(w + n) * 16 + g * 4]) = lo;
+  }
+  __syncthreads();
+  // W = K^T T, as its transpose: a lane has columns 4 g and on of every tile, of row c of a tile
+  float wide = 0.f;
+#pragma unroll
+  for (int t = 0; t < ST; t++) {
+    const int d0 = (w * ST + t) * 16;
+    f32x4 W[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) W[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      h8 k[NK];
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        const h1* const at = &lds.K[n][ks * 32 + g * 8 + c / 4][d0 + (c & 3) * 4];
+        k[n] = __builtin_shufflevector(read_columns(at), read_columns(at + 4 * (KS * 32 + 8)), 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (j >= 2 + 2 * ks) continue;
+        const h8 hi = *reinterpret_cast<const h8*>(&lds.C[0][j * 16 + c][ks * 32 + g * 8]), lo = *reinterpret_cast<const h8*>(&lds.C[1][j * 16 + c][ks * 32 + g * 8]);
+        W[j] = mfma_h(lo, k[0], W[j]);
+        if constexpr (NK == 2) W[j] = mfma_h(hi, k[1], W[j]);
+        W[j] = mfma_h(hi, k[0], W[j]);
+      }
     }
+    float most = 0.f, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      W[j] *= *reinterpret_cast<const f32x4*>(&lds.inv[j * 16 + g * 4]);
+      most = larger(most, most_of(W[j]));
+      sum += (__builtin_fabsf(W[j][0]) + __builtin_fabsf(W[j][1])) + (__builtin_fabsf(W[j][2]) + __builtin_fabsf(W[j][3]));
+    }
+    const float by = scale_for(magnitude(max_across_rows(most)));
+    wide = larger(wide, add_across_32(add_across_16(sum)));
+    char* const to = out + Out::W + (w * ST + t) * 2 * kBlockBytes;
+    store_block(to, W[0], W[1], by);
+    store_block(to + kBlockBytes, W[2], W[3], by);
+    if (g == 0) reinterpret_cast<float*>(out + Out::back)[d0 + c] = inverse_of(by);
   }
+  wide = most_of_16(wide);
+  if (lane == 0) lds.most[w] = wide;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    reinterpret_cast<ChunkBounds*>(out + Out::bounds)->back = larger(larger(lds.most[0], lds.most[1]), larger(lds.most[2], lds.most[3]));
 }
 
 // ---------------------------------------------------------------------------
@@ -384,321 +497,303 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-typedef short s4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s4 lds_s4;
-// Four rows of 16 columns of a matrix in LDS by the 16 lanes of a row of lanes: lane p gives row p / 4, columns 4 (p % 4) and on, and gets column p
-__device__ __forceinline__ h4 read_columns(const h1* p) {
-  return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(void*)p));
-}
-
-template <class T, int KS, int NT>
+template <class T, int KS>
 struct ScanLds {
-  static constexpr int DK = KS * 32, SL = DK + 8, RL = kChunk + 8, KL = DK + 16;
-  h1 S[2][NT * 16][SL], R[2][NT * 16][RL], U[2][NT * 16][RL];  // [column][row], hi and lo
-  h1 K[kParts<T>][kChunk][KL];
-  uint32_t smost[NT * 16][4], vmost[NT * 16][4];  // of each wave's rows
+  h1 S[2][16][KS * 32 + 8], R[2][16][kChunk + 8];  // [column][row], hi and lo; R's rows as the blocks of P and W have their columns
+  float smost[16][4];                              // of each wave's rows
+  uint32_t vmost[16][4];                           // (as bits, which tell what is not finite)
+  float rows[2][4][kRowKinds][16], back[2][4][KS * 8];  // factors, of this chunk and the next one, of each wave's rows
 };
 
-// blockIdx.x: a prompt, a head and 16 NT columns of its state.  A wave has 16 rows of a chunk, of K, Q, T and P, and a quarter of the rows of S.  A lane has
-// column c of every tile of 16 columns, rows 4 g and on of one of 16 rows.
+// An element `off` bytes behind a uniform address (or the compiler adds the two ahead of the loop, and keeps 64 bits a lane)
+template <class T>
+__device__ __forceinline__ T* behind(T* uniform, uint32_t off) {
+  asm("" : "+v"(off));
+  return reinterpret_cast<T*>(const_cast<char*>(reinterpret_cast<const char*>(uniform)) + off);
+}
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// blockIdx.x: a prompt, a head and 16 columns of its state.  A wave has 16 rows each of a chunk's K, Q and P, and a quarter of the rows of W and so of S.  A
+// lane has column c of a tile, rows 4 g and on of one of 16 rows.
 //
 // The powers of two by which columns are scaled come from bounds, a step ahead of the values and without waiting for the other waves' values:
-//   |R| <= max |b v| + max_i |b_i a_i0| |k_i|_1 max |S|,   |a U| <= max_i |a_Ci| |T_i|_1 max |R|,   |S'| <= a max |S| + sum_i max_d |k_id| |a_Ci| |T_i|_1 max |R|
+//   |R| <= max |b v| + max_i |b_i a_i0| |k_i|_1 max |S|,   |S'| <= a_C0 max |S| + max_d |W_d|_1 max |R|
 // They may be 2^16 too high before a pair holds a column's largest value to less than fp32 does.
-template <class T, int KS, int NT>
-__global__ __launch_bounds__(256) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
+//
+// Requests of operands are spread over the chunk: 64 bytes a cycle reach a compute unit, and its four waves wait for each other where all request at once.
+template <class T, int KS>
+__global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 2 : 1) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;  // ST: tiles of 16 rows of S of a wave
-  typedef ScanLds<T, KS, NT> Lds;
+  typedef ScanLds<T, KS> Lds;
+  typedef HeadLayout<KS> In;
   __shared__ __attribute__((aligned(16))) Lds lds;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int slices = (a.dv + NT * 16 - 1) / (NT * 16), per = a.heads * slices;
-  const int i0 = blockIdx.x / per, head = (blockIdx.x - i0 * per) / slices, col0 = (blockIdx.x - i0 * per - head * slices) * (NT * 16), kh = head / a.share;
-  const int begin = tab.start[i0], end = tab.end[i0], nchunk = tab.chunk[i0 + 1] - tab.chunk[i0];
+  // Workgroups go round the eight XCDs: those of a prompt and head of keys, which read the same operands, come to be on one
+  const int slices = (a.dv + 15) / 16, nkh = a.heads / a.share, alike = a.share * slices, sets = a.nseq * nkh;
+  const int whole_sets = sets / kXcds * kXcds, at = blockIdx.x < whole_sets * alike ? blockIdx.x : blockIdx.x - whole_sets * alike;
+  const int round = blockIdx.x < whole_sets * alike ? kXcds : sets - whole_sets;
+  const int turn = at / round, set = (blockIdx.x < whole_sets * alike ? turn / alike * kXcds : whole_sets) + at % round, member = turn % alike;
+  const int i0 = set / nkh, kh = set % nkh, head = kh * a.share + member / slices, col0 = member % slices * 16;
+  const int begin = tab.start[i0], end = tab.end[i0], nchunk = tab.chunk[i0 + 1] - tab.chunk[i0], first = tab.chunk[i0];
   const size_t st = ((size_t)tab.seq[i0] * a.heads + head) * a.dk * a.dv;
   const float* const from = i0 == 0 && tab.ahead ? a.state_out : a.state;
-  int col[NT];
-  bool mine[NT];
-  f32x4 S[ST][NT];
-  const int d0 = w * (ST * 16) + g * 4;  // row of S[.][.][0], 16 rows a tile
+  const bool mine = col0 + c < a.dv;
+  const int col = mine ? col0 + c : a.dv - 1;
+  const int row0 = w * 16 + g * 4, at_row = (w >> 1) * 32 + g * 8 + (w & 1) * 4, d0 = w * (ST * 16) + g * 4;  // the lane's rows of a chunk, in R, of S[0]
+  uint32_t vat[4], yat[4];  // of the lane's values in a chunk, bytes
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    mine[n] = col0 + n * 16 + c < a.dv;
-    col[n] = mine[n] ? col0 + n * 16 + c : a.dv - 1;
-#pragma unroll
-    for (int t = 0; t < ST; t++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int d = d0 + t * 16 + r;
-        S[t][n][r] = d < a.dk ? from[st + (size_t)d * a.dv + col[n]] : 0.f;
-      }
+  for (int r = 0; r < 4; r++) {
+    vat[r] = ((uint32_t)(row0 + r) * a.ldv + col) * sizeof(T);
+    yat[r] = ((uint32_t)(row0 + r) * a.ldy + col) * sizeof(T);
   }
-  h8 Kf[KS][NK], Qf[KS][NK], Tf[2][2], Pf[2][2];
-  T v[NT][4];
-  f32x4 rb, rk, rq, rp, rt;
-  const int nkh = a.heads / a.share;
-  auto load_keys = [&](int j) {
-    const h8* const p = reinterpret_cast<const h8*>(keys + ((size_t)j * nkh + kh) * key_bytes(KS * 32, NK)) + lane;
+  h8 Kf[KS][NK], Qf[KS][NK], Pf[2][2], Wf[ST][2][2];
+  T v[4];
+  float row_factor, back_factor;
+  auto head_of = [&](int j) { return heads + ((size_t)j * a.heads + head) * In::bytes; };
+  auto keys_of = [&](int j) { return reinterpret_cast<const h8*>(keys + ((size_t)j * nkh + kh) * key_bytes(KS * 32, NK)) + lane; };
+  auto load_key = [&](const h8* p, int ks) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-      for (int n = 0; n < NK; n++) {
-        Kf[ks][n] = p[((w * KS + ks) * NK + n) * 64];
-        Qf[ks][n] = p[(((4 + w) * KS + ks) * NK + n) * 64];
-      }
-  };
-  auto load_values = [&](int t0) {
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int t = t0 + w * 16 + g * 4 + r;
-#pragma unroll
-      for (int n = 0; n < NT; n++) v[n][r] = t < end ? a.v[(size_t)t * a.ldv + (size_t)head * a.dv + col[n]] : (T)0.f;
+    for (int n = 0; n < NK; n++) {
+      Kf[ks][n] = p[((w * KS + ks) * NK + n) * 64];
+      Qf[ks][n] = p[(((4 + w) * KS + ks) * NK + n) * 64];
     }
   };
-  auto head_of = [&](int j) { return heads + ((size_t)j * a.heads + head) * kHeadBytes; };
-  auto load_tri = [&](int j) {
-    const char* const p = head_of(j);
+  auto load_back = [&](const char* p, int t) {
 #pragma unroll
     for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        if (2 * ks > w) break;
-        Tf[ks][n] = reinterpret_cast<const h8*>(p + block_of(w, ks) * kBlockBytes)[n * 64 + lane];
-        Pf[ks][n] = reinterpret_cast<const h8*>(p + kTriBytes + block_of(w, ks) * kBlockBytes)[n * 64 + lane];
-      }
+      for (int n = 0; n < 2; n++) Wf[t][ks][n] = reinterpret_cast<const h8*>(p + In::W + ((w * ST + t) * 2 + ks) * kBlockBytes)[n * 64 + lane];
   };
-  auto row_factors = [&](int j, int kind) { return *reinterpret_cast<const f32x4*>(head_of(j) + kRowsAt + (kind * kChunk + w * 16 + g * 4) * 4); };
-  const int first = tab.chunk[i0];
-  if (nchunk > 0) {
-    load_keys(first);
-    load_values(begin);
-    load_tri(first);
-    rb = row_factors(first, kRowBeta), rk = row_factors(first, kRowK), rq = row_factors(first, kRowQ);
-    rp = row_factors(first, kRowP), rt = row_factors(first, kRowT);
-  }
-  uint32_t sbound[NT];  // of the columns of S; the first chunk's is its own largest value
+  auto load_tri = [&](const char* p) {
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int n = 0; n < 2; n++)
+        if (2 * ks <= w) Pf[ks][n] = reinterpret_cast<const h8*>(p + block_of(w, ks) * kBlockBytes)[n * 64 + lane];
+  };
+  // A lane requests a factor of each kind for the wave, and they go by LDS: four rows a lane, 16 lanes alike
+  auto load_factors = [&](const char* p) {
+    row_factor = reinterpret_cast<const float*>(p + In::rows)[g * kChunk + w * 16 + c];
+    back_factor = reinterpret_cast<const float*>(p + In::back)[w * (ST * 16) + (lane < ST * 16 ? lane : 0)];
+  };
+  auto keep_factors = [&](int buf) {
+    lds.rows[buf][w][g][c] = row_factor;
+    if (lane < ST * 16) lds.back[buf][w][lane] = back_factor;
+  };
+  auto row_factors = [&](int buf, int kind) { return *reinterpret_cast<const f32x4*>(&lds.rows[buf][w][kind][g * 4]); };
+  auto load_values = [&](int t0) {
+    const T* const p = a.v + (size_t)t0 * a.ldv + (size_t)head * a.dv;
+    const bool whole = t0 + kChunk <= end;
+#pragma unroll
+    for (int r = 0; r < 4; r++) v[r] = whole || t0 + row0 + r < end ? *behind(p, vat[r]) : (T)0.f;
+  };
+  auto bounds_of = [&](int j) {
+    typedef const __attribute__((address_space(4))) u32x4 constant;  // to scalar registers
+    return __builtin_bit_cast(ChunkBounds, *(constant*)(reinterpret_cast<uintptr_t>(head_of(j) + In::bounds)));
+  };
+  f32x4 S[ST], bv;
+  // b v of a chunk, and its largest value, to LDS
+  auto take_values = [&](int buf) {
+    const f32x4 rb = row_factors(buf, kRowBeta);
     uint32_t m = 0;
 #pragma unroll
-    for (int t = 0; t < ST; t++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) m = max(m, magnitude(S[t][n][r]));
+    for (int r = 0; r < 4; r++) {
+      bv[r] = rb[r] * (float)v[r];
+      m = max(m, magnitude(bv[r]));
+    }
     m = max_across_rows(m);
-    if (g == 0) lds.smost[n * 16 + c][w] = m;
-  }
-  lds_barrier();
+    if (g == 0) lds.vmost[c][w] = m;
+  };
+  {
+    const h8* const p = keys_of(first);
 #pragma unroll
-  for (int n = 0; n < NT; n++) {
-    const u32x4 m = *reinterpret_cast<const u32x4*>(lds.smost[n * 16 + c]);
-    sbound[n] = max(max(m[0], m[1]), max(m[2], m[3]));
+    for (int ks = 0; ks < KS; ks++) load_key(p, ks);
   }
+  load_values(begin);
+  load_factors(head_of(first));
+  ChunkBounds bound = bounds_of(first);
+#pragma unroll
+  for (int t = 0; t < ST; t++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int d = d0 + t * 16 + r;
+      S[t][r] = d < a.dk ? from[st + (size_t)d * a.dv + col] : 0.f;
+    }
+  auto most_of_S = [&] {
+    float m = 0.f;
+#pragma unroll
+    for (int t = 0; t < ST; t++) m = larger(m, most_of(S[t]));
+    m = max_across_rows(m);
+    if (g == 0) lds.smost[c][w] = m;
+  };
+  most_of_S();
+  keep_factors(0);
+  load_factors(head_of(first + (nchunk > 1)));
+  take_values(0);
+  if (nchunk > 1) load_values(begin + kChunk);
   lds_barrier();
+  float sbound = most_of(*reinterpret_cast<const f32x4*>(lds.smost[c]));  // of the column of S; the first chunk's is its own largest value
+  lds_barrier();
+  f32x4 y = {0.f, 0.f, 0.f, 0.f}, before = y;  // of the chunk before: its P R and what is to be added; stored while the next one's products run
+  f32x4 yp = y;
+  int spoilt = kChunk;
+  float rinv = 0.f;
+  auto finish = [&](int t0, int buf) {
+    const f32x4 rp = row_factors(buf, kRowP);
+#pragma unroll
+    for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(rp[r], rinv * yp[r], before[r]);
+    if (__ballot(spoilt < kChunk)) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (row0 + r >= spoilt) y[r] = __builtin_nanf("");
+    }
+    T* const p = a.y + (size_t)t0 * a.ldy + (size_t)head * a.dv;
+    const bool whole = t0 + kChunk <= end;
+    if (mine) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (whole || t0 + row0 + r < end) *behind(p, yat[r]) = (T)y[r];
+    }
+  };
   for (int j = 0; j < nchunk; j++) {
-    const int t0 = begin + j * kChunk, next = first + (j + 1 < nchunk ? j + 1 : j);
-    const ChunkBounds& bounds = *reinterpret_cast<const ChunkBounds*>(head_of(first + j) + kBoundsAt);
-    const float keep = bounds.keep, bkey = __builtin_fmaxf(__builtin_fmaxf(bounds.key[0], bounds.key[1]), __builtin_fmaxf(bounds.key[2], bounds.key[3]));
-    const float btri = __builtin_fmaxf(__builtin_fmaxf(bounds.tri[0], bounds.tri[1]), __builtin_fmaxf(bounds.tri[2], bounds.tri[3]));
-    const float bback = bounds.back[0] + bounds.back[1] + bounds.back[2] + bounds.back[3];
-    const int bad = bounds.bad;
-    float sinv[NT], bv[NT][4];
-    // S to LDS, and the largest values of S and b v
+    const int t0 = begin + j * kChunk, next = first + min(j + 1, nchunk - 1), buf = j & 1;
+    const char* const here = head_of(first + j);
+    // S to LDS, and its largest values; this chunk's W and P on their way
+    const float power = scale_for(magnitude(sbound)), sinv = inverse_of(power);
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-      const float power = scale_for(sbound[n]);
-      sinv[n] = inverse_of(power);
-      uint32_t m = 0, mv = 0;
-#pragma unroll
-      for (int t = 0; t < ST; t++) {
-        h4 hi, lo;
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          h1 x, y;
-          m = max(m, magnitude(S[t][n][r]));
-          split(S[t][n][r] * power, x, y);
-          hi[r] = x;
-          lo[r] = y;
-        }
-        *reinterpret_cast<h4*>(&lds.S[0][n * 16 + c][d0 + t * 16]) = hi;
-        *reinterpret_cast<h4*>(&lds.S[1][n * 16 + c][d0 + t * 16]) = lo;
-      }
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        bv[n][r] = rb[r] * (float)v[n][r];
-        mv = max(mv, magnitude(bv[n][r]));
-      }
-      m = max_across_rows(m);
-      mv = max_across_rows(mv);
-      if (g == 0) {
-        lds.smost[n * 16 + c][w] = m;
-        lds.vmost[n * 16 + c][w] = mv;
-      }
-    }
-    lds_barrier();
-    // [K; Q] S
-    f32x4 ks_[NT], qs[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      ks_[n] = qs[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const h8 hi = *reinterpret_cast<const h8*>(&lds.S[0][n * 16 + c][ks * 32 + g * 8]), lo = *reinterpret_cast<const h8*>(&lds.S[1][n * 16 + c][ks * 32 + g * 8]);
-        ks_[n] = mfma_h(Kf[ks][0], lo, ks_[n]);
-        qs[n] = mfma_h(Qf[ks][0], lo, qs[n]);
-        if constexpr (NK == 2) {
-          ks_[n] = mfma_h(Kf[ks][1], hi, ks_[n]);
-          qs[n] = mfma_h(Qf[ks][1], hi, qs[n]);
-        }
-        ks_[n] = mfma_h(Kf[ks][0], hi, ks_[n]);
-        qs[n] = mfma_h(Qf[ks][0], hi, qs[n]);
-      }
-    }
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-      for (int n = 0; n < NK; n++) *reinterpret_cast<h8*>(&lds.K[n][w * 16 + c][ks * 32 + g * 8]) = Kf[ks][n];
-    load_keys(next);
-    int spoilt[NT];  // the column's first row of which something is not finite
-    bool any = bad < kChunk;
-    float rinv[NT], upower[NT], uinv[NT];
-#pragma unroll
-    for (int n = 0; n < NT; n++) {
-      const u32x4 ms = *reinterpret_cast<const u32x4*>(lds.smost[n * 16 + c]), mv = *reinterpret_cast<const u32x4*>(lds.vmost[n * 16 + c]);
-      const uint32_t sm = max(max(ms[0], ms[1]), max(ms[2], ms[3]));
-      uint32_t vm = max(max(mv[0], mv[1]), max(mv[2], mv[3]));
-      spoilt[n] = bad;
-      if (__ballot(vm >= kNotFinite)) {  // seldom: every wave looks for the first such value itself
-        if (vm >= kNotFinite) {
-          const float* const b = reinterpret_cast<const float*>(head_of(first + j) + kRowsAt) + kRowBeta * kChunk;
-          vm = 0;
-          for (int r = min(end - t0, kChunk) - 1; r >= 0; r--) {
-            const uint32_t m = magnitude(b[r] * (float)a.v[(size_t)(t0 + r) * a.ldv + (size_t)head * a.dv + col[n]]);
-            if (m >= kNotFinite) spoilt[n] = min(spoilt[n], r);
-            else vm = max(vm, m);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; r++)
-            if (magnitude(bv[n][r]) >= kNotFinite) bv[n][r] = 0.f;
-        }
-        any = true;
-      }
-      const float rbound = __builtin_fmaf(bkey, __uint_as_float(sm), __uint_as_float(vm)), ubound = btri * rbound;
-      const float rpower = scale_for(magnitude(rbound));
-      rinv[n] = inverse_of(rpower);
-      upower[n] = scale_for(magnitude(ubound));
-      uinv[n] = inverse_of(upower[n]);
-      sbound[n] = magnitude(__builtin_fmaf(keep, __uint_as_float(sm), bback * rbound));
+    for (int t = 0; t < ST; t++) {
       h4 hi, lo;
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        h1 x, y;
-        split((bv[n][r] - rk[r] * (sinv[n] * ks_[n][r])) * rpower, x, y);
-        hi[r] = x;
-        lo[r] = y;
-      }
-      *reinterpret_cast<h4*>(&lds.R[0][n * 16 + c][w * 16 + g * 4]) = hi;
-      *reinterpret_cast<h4*>(&lds.R[1][n * 16 + c][w * 16 + g * 4]) = lo;
+      split(S[t] * power, hi, lo);
+      *reinterpret_cast<h4*>(&lds.S[0][c][d0 + t * 16]) = hi;
+      *reinterpret_cast<h4*>(&lds.S[1][c][d0 + t * 16]) = lo;
+      load_back(here, t);
+      in_order();
     }
-    if (j + 1 < nchunk) load_values(t0 + kChunk);
-    rb = row_factors(next, kRowBeta), rk = row_factors(next, kRowK);
+    most_of_S();
+    load_tri(here);
     lds_barrier();
-    // [T; P] R
-    f32x4 tr[NT], pr[NT];
+    // [K; Q] S, in sums of their own: a product waits for the one ahead of it
+    const h8* const kp = keys_of(next);
+    f32x4 s[4];
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-      tr[n] = pr[n] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < 4; k++) s[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    h8 hi[KS], lo[KS];
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        if (2 * ks > w) break;
-        const h8 hi = *reinterpret_cast<const h8*>(&lds.R[0][n * 16 + c][ks * 32 + g * 8]), lo = *reinterpret_cast<const h8*>(&lds.R[1][n * 16 + c][ks * 32 + g * 8]);
-        tr[n] = mfma_h(Tf[ks][0], lo, tr[n]);
-        pr[n] = mfma_h(Pf[ks][0], lo, pr[n]);
-        tr[n] = mfma_h(Tf[ks][1], hi, tr[n]);
-        pr[n] = mfma_h(Pf[ks][1], hi, pr[n]);
-        tr[n] = mfma_h(Tf[ks][0], hi, tr[n]);
-        pr[n] = mfma_h(Pf[ks][0], hi, pr[n]);
-      }
-      h4 hi, lo;
-      const float to = rinv[n] * upower[n];
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        h1 x, y;
-        split(rt[r] * (to * tr[n][r]), x, y);
-        hi[r] = x;
-        lo[r] = y;
-      }
-      *reinterpret_cast<h4*>(&lds.U[0][n * 16 + c][w * 16 + g * 4]) = hi;
-      *reinterpret_cast<h4*>(&lds.U[1][n * 16 + c][w * 16 + g * 4]) = lo;
+    for (int ks = 0; ks < KS; ks++) {
+      hi[ks] = *reinterpret_cast<const h8*>(&lds.S[0][c][ks * 32 + g * 8]);
+      lo[ks] = *reinterpret_cast<const h8*>(&lds.S[1][c][ks * 32 + g * 8]);
     }
-    load_tri(next);
-    rt = row_factors(next, kRowT);
-    lds_barrier();
-    // S' = keep S + K^T U
-    f32x4 ku[ST][NT];
+    const u32x4 mv = *reinterpret_cast<const u32x4*>(lds.vmost[c]);
+    const float sm = most_of(*reinterpret_cast<const f32x4*>(lds.smost[c]));
+    const f32x4 rk = row_factors(buf, kRowK), rq = row_factors(buf, kRowQ);
+    in_order();
 #pragma unroll
-    for (int t = 0; t < ST; t++)
-#pragma unroll
-      for (int n = 0; n < NT; n++) ku[t][n] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-      h8 hi[NT], lo[NT];
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        hi[n] = *reinterpret_cast<const h8*>(&lds.U[0][n * 16 + c][ks * 32 + g * 8]);
-        lo[n] = *reinterpret_cast<const h8*>(&lds.U[1][n * 16 + c][ks * 32 + g * 8]);
-      }
-#pragma unroll
-      for (int t = 0; t < ST; t++) {
-        h8 kt[NK];
-#pragma unroll
-        for (int p = 0; p < NK; p++) {
-          const h1* const at = &lds.K[p][ks * 32 + g * 8 + c / 4][w * (ST * 16) + t * 16 + (c & 3) * 4];
-          const h4 x = read_columns(at), y = read_columns(at + 4 * Lds::KL);
-          kt[p] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; n++) {
-          ku[t][n] = mfma_h(kt[0], lo[n], ku[t][n]);
-          if constexpr (NK == 2) ku[t][n] = mfma_h(kt[1], hi[n], ku[t][n]);
-          ku[t][n] = mfma_h(kt[0], hi[n], ku[t][n]);
-        }
-      }
+    for (int ks = 0; ks < KS; ks++) {
+      s[0] = mfma_h(Kf[ks][0], lo[ks], s[0]);
+      s[1] = mfma_h(Kf[ks][0], hi[ks], s[1]);
+      if constexpr (NK == 2) s[0] = mfma_h(Kf[ks][1], hi[ks], s[0]);
     }
+    if (j > 0) finish(t0 - kChunk, buf ^ 1);
+    in_order();
 #pragma unroll
-    for (int n = 0; n < NT; n++) {
-#pragma unroll
-      for (int t = 0; t < ST; t++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) S[t][n][r] = __builtin_fmaf(uinv[n], ku[t][n][r], keep * S[t][n][r]);
-      float y[4];
-#pragma unroll
-      for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(rq[r], sinv[n] * qs[n][r], rp[r] * (rinv[n] * pr[n][r]));
-      if (any) {
-        const float nan = __builtin_nanf("");
+    for (int ks = 0; ks < KS; ks++) {
+      s[2] = mfma_h(Qf[ks][0], lo[ks], s[2]);
+      s[3] = mfma_h(Qf[ks][0], hi[ks], s[3]);
+      if constexpr (NK == 2) s[2] = mfma_h(Qf[ks][1], hi[ks], s[2]);
+    }
+    // R, to LDS
+    const int bad = bound.bad;  // the first row of which something is not finite; of a column:
+    spoilt = bad;
+    uint32_t vm = max(max(mv[0], mv[1]), max(mv[2], mv[3]));
+    if (__ballot(vm >= kNotFinite)) {  // seldom: every wave looks for the first such value itself
+      if (vm >= kNotFinite) {
+        const float* const b = reinterpret_cast<const float*>(here + In::rows) + kRowBeta * kChunk;
+        vm = 0;
+        for (int r = min(end - t0, kChunk) - 1; r >= 0; r--) {
+          const uint32_t m = magnitude(b[r] * (float)a.v[(size_t)(t0 + r) * a.ldv + (size_t)head * a.dv + col]);
+          if (m >= kNotFinite) spoilt = min(spoilt, r);
+          else vm = max(vm, m);
+        }
 #pragma unroll
         for (int r = 0; r < 4; r++)
-          if (w * 16 + g * 4 + r >= spoilt[n]) y[r] = nan;
-        if (spoilt[n] < kChunk) {
-#pragma unroll
-          for (int t = 0; t < ST; t++) S[t][n] = (f32x4){nan, nan, nan, nan};
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int t = t0 + w * 16 + g * 4 + r;
-        if (mine[n] && t < end) a.y[(size_t)t * a.ldy + (size_t)head * a.dv + col[n]] = (T)y[r];
+          if (magnitude(bv[r]) >= kNotFinite) bv[r] = 0.f;
       }
     }
-    rq = row_factors(next, kRowQ), rp = row_factors(next, kRowP);
-  }
+    const float rbound = __builtin_fmaf(bound.key, sm, __uint_as_float(vm)), rpower = scale_for(magnitude(rbound)), keep = bound.keep;
+    rinv = inverse_of(rpower);
+    sbound = __builtin_fmaf(keep, sm, bound.back * rbound);
+    {
+      const f32x4 ks_ = s[1] + s[0];
+      f32x4 R;
 #pragma unroll
-  for (int n = 0; n < NT; n++)
+      for (int r = 0; r < 4; r++) R[r] = (bv[r] - rk[r] * (sinv * ks_[r])) * rpower;
+      h4 rhi, rlo;
+      split(R, rhi, rlo);
+      *reinterpret_cast<h4*>(&lds.R[0][c][at_row]) = rhi;
+      *reinterpret_cast<h4*>(&lds.R[1][c][at_row]) = rlo;
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) load_key(kp, ks);
+    lds_barrier();
+    // [W; P] R
+    h8 rh[2], rl[2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][ks * 32 + g * 8]);
+      rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][ks * 32 + g * 8]);
+    }
+    f32x4 rw[ST], ws[ST][2], p[2];
+#pragma unroll
+    for (int t = 0; t < ST; t++) {
+      rw[t] = *reinterpret_cast<const f32x4*>(&lds.back[buf][w][t * 16 + g * 4]);
+      ws[t][0] = ws[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    p[0] = p[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const f32x4 qs = s[3] + s[2];
+#pragma unroll
+    for (int r = 0; r < 4; r++) before[r] = rq[r] * (sinv * qs[r]);
+    keep_factors(buf ^ 1);
+    in_order();
 #pragma unroll
     for (int t = 0; t < ST; t++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int d = d0 + t * 16 + r;
-        if (mine[n] && d < a.dk) a.state_out[st + (size_t)d * a.dv + col[n]] = S[t][n][r];
+      for (int ks = 0; ks < 2; ks++) {
+        ws[t][0] = mfma_h(Wf[t][ks][0], rl[ks], ws[t][0]);
+        ws[t][1] = mfma_h(Wf[t][ks][0], rh[ks], ws[t][1]);
+        ws[t][0] = mfma_h(Wf[t][ks][1], rh[ks], ws[t][0]);
       }
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++) {
+      if (2 * ks > w) break;
+      p[0] = mfma_h(Pf[ks][0], rl[ks], p[0]);
+      p[1] = mfma_h(Pf[ks][0], rh[ks], p[1]);
+      p[0] = mfma_h(Pf[ks][1], rh[ks], p[0]);
+    }
+    bound = bounds_of(next);
+    take_values(buf ^ 1);
+    if (j + 2 < nchunk) load_values(t0 + 2 * kChunk);
+    load_factors(head_of(first + min(j + 2, nchunk - 1)));
+#pragma unroll
+    for (int t = 0; t < ST; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) S[t][r] = __builtin_fmaf(rw[t][r], rinv * (ws[t][1][r] + ws[t][0][r]), keep * S[t][r]);
+    if (__ballot(spoilt < kChunk)) {
+      const float nan = __builtin_nanf("");
+      if (spoilt < kChunk) {
+#pragma unroll
+        for (int t = 0; t < ST; t++) S[t] = (f32x4){nan, nan, nan, nan};
+      }
+    }
+    yp = p[1] + p[0];
+  }
+  finish(begin + (nchunk - 1) * kChunk, (nchunk - 1) & 1);
+#pragma unroll
+  for (int t = 0; t < ST; t++)
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int d = d0 + t * 16 + r;
+      if (mine && d < a.dk) a.state_out[st + (size_t)d * a.dv + col] = S[t][r];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -707,7 +802,8 @@ __global__ __launch_bounds__(256) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
 constexpr size_t kPassBytes = (size_t)256 << 20;  // scratch of a pair of launches, about: longer calls go out in several
 static int key_steps(int dk) { return dk <= 64 ? 2 : dk <= 128 ? 4 : 8; }
 static size_t chunk_bytes(int heads, int key_heads, int dk, int parts) {
-  return (size_t)heads * kHeadBytes + (size_t)key_heads * key_bytes(key_steps(dk) * 32, parts);
+  const int ks = key_steps(dk), head = ks == 2 ? HeadLayout<2>::bytes : ks == 4 ? HeadLayout<4>::bytes : HeadLayout<8>::bytes;
+  return (size_t)heads * head + (size_t)key_heads * key_bytes(ks * 32, parts);
 }
 // Chunks of a pair of launches: prompts have kDeltaChunkLeast rows at least, so there are no more chunks than rows / kDeltaChunkLeast + 1
 static size_t most_chunks(size_t per, int T) {
@@ -728,7 +824,7 @@ static int chunk_launch(const DeltaArgs<T>& a, const DeltaTable& tab, char* keys
     hipLaunchKernelGGL((delta_prep_kernel<T, KS>), dim3(chunks, a.heads), dim3(256), 0, st, a, tab, keys, heads);
     if (int rc = check_launch("delta_seq")) return rc;
   }
-  hipLaunchKernelGGL((delta_scan_kernel<T, KS, 1>), dim3(a.nseq * a.heads * slices), dim3(256), 0, st, a, tab, keys, heads);
+  hipLaunchKernelGGL((delta_scan_kernel<T, KS>), dim3(a.nseq * a.heads * slices), dim3(256), 0, st, a, tab, keys, heads);
   return check_launch("delta_seq");
 }
 
@@ -737,7 +833,7 @@ int delta_chunk_run(const DeltaArgs<T>& args, const int* seqs, int nseq, const i
   DeltaArgs<T> a = args;
   const int nkh = a.heads / a.share, steps = key_steps(a.dk);
   const size_t per = chunk_bytes(a.heads, nkh, a.dk, kParts<T>), most = most_chunks(per, rows);
-  const int together = std::min(kSeqTable, (1 << 23) / (a.heads * ((a.dv + 15) / 16)));  // prompts of a launch, which has less than 2^32 threads
+  const int together = std::min(kSeqTable, (1 << 22) / (a.heads * ((a.dv + 15) / 16)));  // prompts of a launch, which has less than 2^32 threads
   char* const keys = static_cast<char*>(workspace);
   char* const heads = keys + most * nkh * key_bytes(steps * 32, kParts<T>);
   DeltaTable tab;
