@@ -32,9 +32,10 @@ __device__ __forceinline__ constexpr int block_of(int tile, int ks) { return (ti
 constexpr int kTriBytes = 6 * kBlockBytes;
 enum { kRowBeta, kRowK, kRowQ, kRowP, kRowKinds };
 struct ChunkBounds {
-  float key, back;  // see the scan
-  float keep;       // the decay of the whole chunk
-  int bad;          // the first row of which something is not finite, or kChunk
+  float key, back, both;  // see the scan
+  float keep;             // the decay of the whole chunk
+  int bad;                // the first row of which something is not finite, or kChunk
+  int none[3];
 };
 template <int KS>
 struct HeadLayout {
@@ -216,7 +217,7 @@ struct PrepLds {
   };
   double G[kChunk];  // sums of the logarithms of the rows' decays
   float fk[kChunk], fq[kChunk], length[kChunk], write[kChunk], back[kChunk], inv[kChunk], ref[4][kChunk];
-  float most[4];
+  __attribute__((aligned(16))) float most[2][4];
   int bad;
 };
 
@@ -231,7 +232,7 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
   const int cj = blockIdx.x, head = blockIdx.y, kh = head / a.share;
   const int i0 = find_seq(a.nseq, cj, [&](int k) { return tab.chunk[k]; });
   const int t0 = tab.start[i0] + (cj - tab.chunk[i0]) * kChunk, len = min(tab.end[i0] - t0, kChunk);
-  char* const out = heads + ((size_t)cj * a.heads + head) * Out::bytes;
+  char* const out = heads + ((size_t)head * gridDim.x + cj) * Out::bytes;  // a head's chunks one behind the other: pages stay
   const int row = w * 16 + c, r0 = w * 16 + g * 4;  // the lane's row of an operand, the first one of results
   KeyTile<T, KS> K, Q;
   K.template load<true>(a.k + (size_t)t0 * a.ldk + (size_t)kh * a.dk, a.ldk, w * 16, len, a.dk);
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
   }
   if (head % a.share == 0) {
     constexpr int tile = KS * NK * 64;
-    h8* const to = reinterpret_cast<h8*>(keys + ((size_t)cj * (a.heads / a.share) + kh) * key_bytes(KS * 32, NK));
+    h8* const to = reinterpret_cast<h8*>(keys + ((size_t)kh * gridDim.x + cj) * key_bytes(KS * 32, NK));
     K.store(to + w * tile);
     Q.store(to + (4 + w) * tile);
   }
@@ -302,7 +303,8 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
     rows[kRowBeta * kChunk] = b;
     rows[kRowK * kChunk] = key;
     rows[kRowQ * kChunk] = lds.fq[lane] * from;
-    const float bkey = max_across_rows(most_of_16(__builtin_fabsf(key) * lds.length[lane]));
+    const float reach = __builtin_fabsf(key) * lds.length[lane], bkey = max_across_rows(most_of_16(reach));
+    lds.length[lane] = reach;
     if (lane == 63) {
       lds.bad = bad;
       ChunkBounds* const to = reinterpret_cast<ChunkBounds*>(out + Out::bounds);
@@ -441,7 +443,7 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
   }
   __syncthreads();
   // W = K^T T, as its transpose: a lane has columns 4 g and on of every tile, of row c of a tile
-  float wide = 0.f;
+  float wide = 0.f, both = 0.f;
 #pragma unroll
   for (int t = 0; t < ST; t++) {
     const int d0 = (w * ST + t) * 16;
@@ -465,25 +467,37 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
         W[j] = mfma_h(hi, k[0], W[j]);
       }
     }
-    float most = 0.f, sum = 0.f;
+    float most = 0.f, sum = 0.f, reach = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
+      const f32x4 far = *reinterpret_cast<const f32x4*>(&lds.length[j * 16 + g * 4]);
       W[j] *= *reinterpret_cast<const f32x4*>(&lds.inv[j * 16 + g * 4]);
       most = larger(most, most_of(W[j]));
-      sum += (__builtin_fabsf(W[j][0]) + __builtin_fabsf(W[j][1])) + (__builtin_fabsf(W[j][2]) + __builtin_fabsf(W[j][3]));
+#pragma unroll
+      for (int s = 0; s < 4; s++) {
+        sum += __builtin_fabsf(W[j][s]);
+        reach = __builtin_fmaf(__builtin_fabsf(W[j][s]), far[s], reach);
+      }
     }
     const float by = scale_for(magnitude(max_across_rows(most)));
     wide = larger(wide, add_across_32(add_across_16(sum)));
+    both = larger(both, add_across_32(add_across_16(reach)));
     char* const to = out + Out::W + (w * ST + t) * 2 * kBlockBytes;
     store_block(to, W[0], W[1], by);
     store_block(to + kBlockBytes, W[2], W[3], by);
     if (g == 0) reinterpret_cast<float*>(out + Out::back)[d0 + c] = inverse_of(by);
   }
   wide = most_of_16(wide);
-  if (lane == 0) lds.most[w] = wide;
+  both = most_of_16(both);
+  if (lane == 0) {
+    lds.most[0][w] = wide;
+    lds.most[1][w] = both;
+  }
   __syncthreads();
-  if (threadIdx.x == 0)
-    reinterpret_cast<ChunkBounds*>(out + Out::bounds)->back = larger(larger(lds.most[0], lds.most[1]), larger(lds.most[2], lds.most[3]));
+  if (threadIdx.x < 2) {
+    const f32x4 m = *reinterpret_cast<const f32x4*>(lds.most[threadIdx.x]);
+    (&reinterpret_cast<ChunkBounds*>(out + Out::bounds)->back)[threadIdx.x] = most_of(m);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -500,9 +514,11 @@ __device__ __forceinline__ void lds_barrier() {
 template <class T, int KS>
 struct ScanLds {
   h1 S[2][16][KS * 32 + 8], R[2][16][kChunk + 8];  // [column][row], hi and lo; R's rows as the blocks of P and W have their columns
-  float smost[16][4];                              // of each wave's rows
-  uint32_t vmost[16][4];                           // (as bits, which tell what is not finite)
-  float rows[2][4][kRowKinds][16], back[2][4][KS * 8];  // factors, of this chunk and the next one, of each wave's rows
+  float bv[2][4][64][4];                           // b v of this chunk and the next one, of the lanes of waves 0 to 3
+  float qs[4][64][4];                              // Q S, of their lanes
+  float most[16][16];                              // of S, of each lane's rows
+  uint32_t vmost[16][4];                           // of b v of the next chunk (as bits, which tell what is not finite)
+  float cols[16][2], rinv[16];                     // of each column: the largest b v, the decay of the chunk (or NaN: see spoilt); R's inverse power
 };
 
 // An element `off` bytes behind a uniform address (or the compiler adds the two ahead of the loop, and keeps 64 bits a lane)
@@ -511,23 +527,50 @@ __device__ __forceinline__ T* behind(T* uniform, uint32_t off) {
   asm("" : "+v"(off));
   return reinterpret_cast<T*>(const_cast<char*>(reinterpret_cast<const char*>(uniform)) + off);
 }
+
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// blockIdx.x: a prompt, a head and 16 columns of its state.  A wave has 16 rows each of a chunk's K, Q and P, and a quarter of the rows of W and so of S.  A
-// lane has column c of a tile, rows 4 g and on of one of 16 rows.
+// Rows of v or y of a chunk as a buffer of the rows that are there: what lies behind its end is read as zero and not written.  So the code
+// has no branches around requests, where the compiler would have to wait for all that may be on their way.
+template <class T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_of(T* rows, int nrows, int ld) {
+  const int there = __builtin_amdgcn_readfirstlane(nrows < 0 ? 0 : nrows < kChunk ? nrows : kChunk);  // (or the compiler takes it for the lanes' own)
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(static_cast<const void*>(rows)), 0, (int)((uint32_t)there * (uint32_t)ld * (uint32_t)sizeof(T)), 0x00027000);
+}
+template <class T>
+__device__ __forceinline__ T load_row(__amdgpu_buffer_rsrc_t rows, uint32_t at) {
+  if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(rows, at, 0, 0));
+  else return __builtin_bit_cast(T, (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(rows, at, 0, 0));
+}
+template <class T>
+__device__ __forceinline__ void store_row(__amdgpu_buffer_rsrc_t rows, uint32_t at, T v) {
+  if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), rows, at, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rows, at, 0, 0);
+}
+
+// Four rows' factors of the one that each lane of a quad requested
+__device__ __forceinline__ f32x4 of_quad(float f) { return (f32x4){dpp_mov<0x00>(f), dpp_mov<0x55>(f), dpp_mov<0xAA>(f), dpp_mov<0xFF>(f)}; }
+template <int LANE>
+__device__ __forceinline__ float of_lane(float f) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), LANE)); }
+
+// blockIdx.x: a prompt, a head and 16 columns of its state.  A lane has column c of a tile, rows 4 g and on of one of 16 rows.
 //
-// The powers of two by which columns are scaled come from bounds, a step ahead of the values and without waiting for the other waves' values:
-//   |R| <= max |b v| + max_i |b_i a_i0| |k_i|_1 max |S|,   |S'| <= a_C0 max |S| + max_d |W_d|_1 max |R|
+// What the next chunk waits for is a row of dependent steps, S to LDS, K S, R to LDS, W R, and it is their latency that counts: waves 0 to 3 do them, with
+// 16 rows each of K and a quarter of those of W and S, and Q S, whose operands of S they have, besides.  Waves 4 to 7 do the rest, with 16 rows each of
+// P and v: they hand over b v and what belongs to it, and make y.  LDS passes 128 bytes a cycle, 16 bytes a lane in eight whether the lanes read
+// the same or not: rows' factors go from memory to registers, one a lane, and round the quads of lanes.
+//
+// The powers of two by which columns are scaled come from bounds, of S ahead of its values (without waiting for the other waves' ones):
+//   |R| <= max |b v| + key max |S|,   key = max_i |b_i a_i0| |k_i|_1
+//   |S'| <= a_C0 max |S| + back max |b v| + both max |S|,   back = max_d sum_i |W_di|,   both = max_d sum_i |W_di| |b_i a_i0| |k_i|_1
 // They may be 2^16 too high before a pair holds a column's largest value to less than fp32 does.
-//
-// Requests of operands are spread over the chunk: 64 bytes a cycle reach a compute unit, and its four waves wait for each other where all request at once.
 template <class T, int KS>
-__global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 2 : 1) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
+__global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;  // ST: tiles of 16 rows of S of a wave
   typedef ScanLds<T, KS> Lds;
   typedef HeadLayout<KS> In;
   __shared__ __attribute__((aligned(16))) Lds lds;
-  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   // Workgroups go round the eight XCDs: those of a prompt and head of keys, which read the same operands, come to be on one
   const int slices = (a.dv + 15) / 16, nkh = a.heads / a.share, alike = a.share * slices, sets = a.nseq * nkh;
   const int whole_sets = sets / kXcds * kXcds, at = blockIdx.x < whole_sets * alike ? blockIdx.x : blockIdx.x - whole_sets * alike;
@@ -535,233 +578,287 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 2 : 1) void delta_scan_k
   const int turn = at / round, set = (blockIdx.x < whole_sets * alike ? turn / alike * kXcds : whole_sets) + at % round, member = turn % alike;
   const int i0 = set / nkh, kh = set % nkh, head = kh * a.share + member / slices, col0 = member % slices * 16;
   const int begin = tab.start[i0], end = tab.end[i0], nchunk = tab.chunk[i0 + 1] - tab.chunk[i0], first = tab.chunk[i0];
-  const size_t st = ((size_t)tab.seq[i0] * a.heads + head) * a.dk * a.dv;
-  const float* const from = i0 == 0 && tab.ahead ? a.state_out : a.state;
+  const size_t nall = tab.chunk[a.nseq];
   const bool mine = col0 + c < a.dv;
   const int col = mine ? col0 + c : a.dv - 1;
-  const int row0 = w * 16 + g * 4, at_row = (w >> 1) * 32 + g * 8 + (w & 1) * 4, d0 = w * (ST * 16) + g * 4;  // the lane's rows of a chunk, in R, of S[0]
+  constexpr size_t head_step = In::bytes, key_step = key_bytes(KS * 32, NK);
+  const char* here = heads + (head * nall + first) * head_step;  // of the chunk that is requested next
+  const int row0 = w * 16 + g * 4, quad0 = row0 + (c & 3);       // the lane's rows of a chunk; the one of which it requests factors
+  const uint32_t limits_at = In::bounds + (lane & 7) * 4;
+  if (wave < 4) {
+    __builtin_amdgcn_s_setprio(2);
+    const char* own = keys + (kh * nall + first) * key_step;
+    const uint32_t own_at = (w * KS * NK * 64 + lane) * 16;
+    h8 Kf[KS][NK], Qf[KS][NK];
+    auto load_step = [&](const char* p, h8 (&f)[KS][NK], int ks) {
+      const h8* const q = reinterpret_cast<const h8*>(behind(p, own_at));
+#pragma unroll
+      for (int n = 0; n < NK; n++) f[ks][n] = q[(ks * NK + n) * 64];
+    };
+    auto load_own = [&](const char* p, h8 (&f)[KS][NK]) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) load_step(p, f, ks);
+    };
+    constexpr size_t queries = (size_t)4 * KS * NK * 64 * 16;  // behind the keys
+    const size_t st = ((size_t)tab.seq[i0] * a.heads + head) * a.dk * a.dv;
+    const float* const from = i0 == 0 && tab.ahead ? a.state_out : a.state;
+    const int d0 = w * (ST * 16) + g * 4, at_row = (w >> 1) * 32 + g * 8 + (w & 1) * 4;  // the lane's rows of S[0], of R
+    const uint32_t back_at = In::W + (w * ST * 2 * 2 * 64 + lane) * 16, key_at = In::rows + (kRowK * kChunk + quad0) * 4,
+                   scale_at = In::back + (d0 + (c & 3)) * 4;
+    h8 Wf[ST][2][2];
+    float key, limits, scale[ST];
+    auto load_back = [&](const char* p, int t) {
+      const h8* const q = reinterpret_cast<const h8*>(behind(p, back_at));
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+        for (int n = 0; n < 2; n++) Wf[t][ks][n] = q[((t * 2 + ks) * 2 + n) * 64];
+      scale[t] = *reinterpret_cast<const float*>(behind(p + t * 64, scale_at));
+    };
+    auto load_key = [&](const char* p) {
+      key = *reinterpret_cast<const float*>(behind(p, key_at));
+      limits = *reinterpret_cast<const float*>(behind(p, limits_at));
+    };
+    load_own(own, Kf);
+    load_key(here);
+    load_own(own + queries, Qf);
+#pragma unroll
+    for (int t = 0; t < ST; t++) load_back(here, t);
+    f32x4 S[ST];
+#pragma unroll
+    for (int t = 0; t < ST; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int d = d0 + t * 16 + r;
+        S[t][r] = d < a.dk ? from[st + (size_t)d * a.dv + col] : 0.f;
+      }
+    auto most_of_S = [&] {
+      float m = 0.f;
+#pragma unroll
+      for (int t = 0; t < ST; t++) m = larger(m, most_of(S[t]));
+      lds.most[c][w * 4 + g] = m;
+    };
+    auto most_of_all = [&] { return max_across_rows(most_of(*reinterpret_cast<const f32x4*>(&lds.most[c][g * 4]))); };
+    most_of_S();
+    lds_barrier();
+    float sbound = most_of_all();  // of the column of S; the first chunk's is its own largest value
+    lds_barrier();
+    for (int j = 0; j < nchunk; j++) {
+      const bool more = j + 1 < nchunk;
+      const float power = scale_for(magnitude(sbound)), sinv = inverse_of(power);
+#pragma unroll
+      for (int t = 0; t < ST; t++) {
+        h4 hi, lo;
+        split(S[t] * power, hi, lo);
+        *reinterpret_cast<h4*>(&lds.S[0][c][d0 + t * 16]) = hi;
+        *reinterpret_cast<h4*>(&lds.S[1][c][d0 + t * 16]) = lo;
+        if (t > 0) {
+          load_back(here, t);
+          in_order();
+        }
+      }
+      most_of_S();
+      lds_barrier();
+      h8 hi[KS], lo[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        lo[ks] = *reinterpret_cast<const h8*>(&lds.S[1][c][ks * 32 + g * 8]);
+        hi[ks] = *reinterpret_cast<const h8*>(&lds.S[0][c][ks * 32 + g * 8]);
+      }
+      const float vm = lds.cols[c][0], keep = lds.cols[c][1];
+      f32x4 bv = *reinterpret_cast<const f32x4*>(lds.bv[j & 1][w][lane]), kf = of_quad(key);
+      const float sm = most_of_all();
+      f32x4 s[4];  // hi and lo apart, and both in two sums: a product waits for the one ahead of it
+#pragma unroll
+      for (int k = 0; k < 4; k++) s[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        s[ks & 1] = mfma_h(Kf[ks][0], lo[ks], s[ks & 1]);
+        s[2 + (ks & 1)] = mfma_h(Kf[ks][0], hi[ks], s[2 + (ks & 1)]);
+        if constexpr (NK == 2) s[ks & 1] = mfma_h(Kf[ks][1], hi[ks], s[ks & 1]);
+      }
+      f32x4 q[2];
+      q[0] = q[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      own = more ? own + key_step : own;
+      here = more ? here + head_step : here;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        in_order();
+        load_step(own, Kf, ks);
+        q[0] = mfma_h(Qf[ks][0], lo[ks], q[0]);
+        q[1] = mfma_h(Qf[ks][0], hi[ks], q[1]);
+        if constexpr (NK == 2) q[0] = mfma_h(Qf[ks][1], hi[ks], q[0]);
+      }
+      in_order();
+      load_own(own + queries, Qf);
+      const float rpower = scale_for(magnitude(__builtin_fmaf(of_lane<0>(limits), sm, vm))), rinv = inverse_of(rpower);
+      sbound = __builtin_fmaf(of_lane<3>(limits) + of_lane<2>(limits), sm, of_lane<1>(limits) * vm);
+      kf *= sinv * rpower;
+      bv *= rpower;
+      f32x4 R;
+#pragma unroll
+      for (int r = 0; r < 4; r++) R[r] = __builtin_fmaf(-kf[r], (s[2][r] + s[3][r]) + (s[0][r] + s[1][r]), bv[r]);
+      h4 rhi, rlo;
+      split(R, rhi, rlo);
+      *reinterpret_cast<h4*>(&lds.R[0][c][at_row]) = rhi;
+      *reinterpret_cast<h4*>(&lds.R[1][c][at_row]) = rlo;
+      load_key(here);
+      lds_barrier();
+      h8 rh[2], rl[2];
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++) {
+        rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][ks * 32 + g * 8]);
+        rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][ks * 32 + g * 8]);
+      }
+      *reinterpret_cast<f32x4*>(lds.qs[w][lane]) = (q[1] + q[0]) * sinv;
+      if (w == 0 && g == 0) lds.rinv[c] = rinv;
+      f32x4 rw[ST], ws[ST][2];
+#pragma unroll
+      for (int t = 0; t < ST; t++) {
+        rw[t] = of_quad(scale[t]) * rinv;
+        S[t] *= keep;
+      }
+#pragma unroll
+      for (int t = 0; t < ST; t++) {
+        ws[t][0] = ws[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 2; ks++) {
+          ws[t][0] = mfma_h(Wf[t][ks][0], rl[ks], ws[t][0]);
+          ws[t][1] = mfma_h(Wf[t][ks][0], rh[ks], ws[t][1]);
+          ws[t][0] = mfma_h(Wf[t][ks][1], rh[ks], ws[t][0]);
+        }
+      }
+      in_order();
+      load_back(here, 0);
+#pragma unroll
+      for (int t = 0; t < ST; t++) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) S[t][r] = __builtin_fmaf(rw[t][r], ws[t][1][r] + ws[t][0][r], S[t][r]);
+      }
+    }
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < ST; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int d = d0 + t * 16 + r;
+        if (mine && d < a.dk) a.state_out[st + (size_t)d * a.dv + col] = S[t][r];
+      }
+    return;
+  }
   uint32_t vat[4], yat[4];  // of the lane's values in a chunk, bytes
 #pragma unroll
   for (int r = 0; r < 4; r++) {
     vat[r] = ((uint32_t)(row0 + r) * a.ldv + col) * sizeof(T);
-    yat[r] = ((uint32_t)(row0 + r) * a.ldy + col) * sizeof(T);
+    yat[r] = mine ? ((uint32_t)(row0 + r) * a.ldy + col) * sizeof(T) : ~0u;
   }
-  h8 Kf[KS][NK], Qf[KS][NK], Pf[2][2], Wf[ST][2][2];
+  const uint32_t tri_at = block_of(w, 0) * kBlockBytes + lane * 16, tri_on = w < 2 ? 0 : kBlockBytes, factor_at = In::rows + quad0 * 4;
+  h8 Pf[2][2];
   T v[4];
-  float row_factor, back_factor;
-  auto head_of = [&](int j) { return heads + ((size_t)j * a.heads + head) * In::bytes; };
-  auto keys_of = [&](int j) { return reinterpret_cast<const h8*>(keys + ((size_t)j * nkh + kh) * key_bytes(KS * 32, NK)) + lane; };
-  auto load_key = [&](const h8* p, int ks) {
-#pragma unroll
-    for (int n = 0; n < NK; n++) {
-      Kf[ks][n] = p[((w * KS + ks) * NK + n) * 64];
-      Qf[ks][n] = p[(((4 + w) * KS + ks) * NK + n) * 64];
-    }
-  };
-  auto load_back = [&](const char* p, int t) {
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-      for (int n = 0; n < 2; n++) Wf[t][ks][n] = reinterpret_cast<const h8*>(p + In::W + ((w * ST + t) * 2 + ks) * kBlockBytes)[n * 64 + lane];
-  };
+  float query, tri, beta, limits;
   auto load_tri = [&](const char* p) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ks++)
+    for (int ks = 0; ks < 2; ks++) {  // (waves 4 and 5 have one block and take it twice)
+      const h8* const q = reinterpret_cast<const h8*>(behind(p + ks * tri_on, tri_at));
 #pragma unroll
-      for (int n = 0; n < 2; n++)
-        if (2 * ks <= w) Pf[ks][n] = reinterpret_cast<const h8*>(p + block_of(w, ks) * kBlockBytes)[n * 64 + lane];
+      for (int n = 0; n < 2; n++) Pf[ks][n] = q[n * 64];
+    }
+    query = *reinterpret_cast<const float*>(behind(p + kRowQ * kChunk * 4, factor_at));
+    tri = *reinterpret_cast<const float*>(behind(p + kRowP * kChunk * 4, factor_at));
   };
-  // A lane requests a factor of each kind for the wave, and they go by LDS: four rows a lane, 16 lanes alike
-  auto load_factors = [&](const char* p) {
-    row_factor = reinterpret_cast<const float*>(p + In::rows)[g * kChunk + w * 16 + c];
-    back_factor = reinterpret_cast<const float*>(p + In::back)[w * (ST * 16) + (lane < ST * 16 ? lane : 0)];
-  };
-  auto keep_factors = [&](int buf) {
-    lds.rows[buf][w][g][c] = row_factor;
-    if (lane < ST * 16) lds.back[buf][w][lane] = back_factor;
-  };
-  auto row_factors = [&](int buf, int kind) { return *reinterpret_cast<const f32x4*>(&lds.rows[buf][w][kind][g * 4]); };
-  auto load_values = [&](int t0) {
-    const T* const p = a.v + (size_t)t0 * a.ldv + (size_t)head * a.dv;
-    const bool whole = t0 + kChunk <= end;
+  auto load_limits = [&](const char* p) { limits = *reinterpret_cast<const float*>(behind(p, limits_at)); };
+  auto load_values = [&](int t0, const char* p) {  // (behind the end: none)
+    const auto rows = rows_of(a.v + (size_t)min(t0, end) * a.ldv + (size_t)head * a.dv, end - t0, a.ldv);
 #pragma unroll
-    for (int r = 0; r < 4; r++) v[r] = whole || t0 + row0 + r < end ? *behind(p, vat[r]) : (T)0.f;
+    for (int r = 0; r < 4; r++) v[r] = load_row<T>(rows, vat[r]);
+    beta = *reinterpret_cast<const float*>(behind(p + kRowBeta * kChunk * 4, factor_at));
   };
-  auto bounds_of = [&](int j) {
-    typedef const __attribute__((address_space(4))) u32x4 constant;  // to scalar registers
-    return __builtin_bit_cast(ChunkBounds, *(constant*)(reinterpret_cast<uintptr_t>(head_of(j) + In::bounds)));
-  };
-  f32x4 S[ST], bv;
-  // b v of a chunk, and its largest value, to LDS
-  auto take_values = [&](int buf) {
-    const f32x4 rb = row_factors(buf, kRowBeta);
+  f32x4 bv;
+  auto take_values = [&](int buf) {  // b v of a chunk and its largest value, to LDS
+    const f32x4 rb = of_quad(beta);
     uint32_t m = 0;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
       bv[r] = rb[r] * (float)v[r];
       m = max(m, magnitude(bv[r]));
     }
+    *reinterpret_cast<f32x4*>(lds.bv[buf][w][lane]) = bv;
     m = max_across_rows(m);
     if (g == 0) lds.vmost[c][w] = m;
   };
-  {
-    const h8* const p = keys_of(first);
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) load_key(p, ks);
-  }
-  load_values(begin);
-  load_factors(head_of(first));
-  ChunkBounds bound = bounds_of(first);
-#pragma unroll
-  for (int t = 0; t < ST; t++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int d = d0 + t * 16 + r;
-      S[t][r] = d < a.dk ? from[st + (size_t)d * a.dv + col] : 0.f;
-    }
-  auto most_of_S = [&] {
-    float m = 0.f;
-#pragma unroll
-    for (int t = 0; t < ST; t++) m = larger(m, most_of(S[t]));
-    m = max_across_rows(m);
-    if (g == 0) lds.smost[c][w] = m;
-  };
-  most_of_S();
-  keep_factors(0);
-  load_factors(head_of(first + (nchunk > 1)));
-  take_values(0);
-  if (nchunk > 1) load_values(begin + kChunk);
-  lds_barrier();
-  float sbound = most_of(*reinterpret_cast<const f32x4*>(lds.smost[c]));  // of the column of S; the first chunk's is its own largest value
-  lds_barrier();
-  f32x4 y = {0.f, 0.f, 0.f, 0.f}, before = y;  // of the chunk before: its P R and what is to be added; stored while the next one's products run
-  f32x4 yp = y;
-  int spoilt = kChunk;
-  float rinv = 0.f;
-  auto finish = [&](int t0, int buf) {
-    const f32x4 rp = row_factors(buf, kRowP);
-#pragma unroll
-    for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(rp[r], rinv * yp[r], before[r]);
-    if (__ballot(spoilt < kChunk)) {
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-        if (row0 + r >= spoilt) y[r] = __builtin_nanf("");
-    }
-    T* const p = a.y + (size_t)t0 * a.ldy + (size_t)head * a.dv;
-    const bool whole = t0 + kChunk <= end;
-    if (mine) {
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-        if (whole || t0 + row0 + r < end) *behind(p, yat[r]) = (T)y[r];
-    }
-  };
-  for (int j = 0; j < nchunk; j++) {
-    const int t0 = begin + j * kChunk, next = first + min(j + 1, nchunk - 1), buf = j & 1;
-    const char* const here = head_of(first + j);
-    // S to LDS, and its largest values; this chunk's W and P on their way
-    const float power = scale_for(magnitude(sbound)), sinv = inverse_of(power);
-#pragma unroll
-    for (int t = 0; t < ST; t++) {
-      h4 hi, lo;
-      split(S[t] * power, hi, lo);
-      *reinterpret_cast<h4*>(&lds.S[0][c][d0 + t * 16]) = hi;
-      *reinterpret_cast<h4*>(&lds.S[1][c][d0 + t * 16]) = lo;
-      load_back(here, t);
-      in_order();
-    }
-    most_of_S();
-    load_tri(here);
-    lds_barrier();
-    // [K; Q] S, in sums of their own: a product waits for the one ahead of it
-    const h8* const kp = keys_of(next);
-    f32x4 s[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) s[k] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    h8 hi[KS], lo[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      hi[ks] = *reinterpret_cast<const h8*>(&lds.S[0][c][ks * 32 + g * 8]);
-      lo[ks] = *reinterpret_cast<const h8*>(&lds.S[1][c][ks * 32 + g * 8]);
-    }
+  int spoilt = kChunk;  // of the column, the first row of which something is not finite
+  // What belongs to b v of a chunk, to LDS
+  auto hand_over = [&](const char* p, int t0, int buf) {
     const u32x4 mv = *reinterpret_cast<const u32x4*>(lds.vmost[c]);
-    const float sm = most_of(*reinterpret_cast<const f32x4*>(lds.smost[c]));
-    const f32x4 rk = row_factors(buf, kRowK), rq = row_factors(buf, kRowQ);
-    in_order();
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      s[0] = mfma_h(Kf[ks][0], lo[ks], s[0]);
-      s[1] = mfma_h(Kf[ks][0], hi[ks], s[1]);
-      if constexpr (NK == 2) s[0] = mfma_h(Kf[ks][1], hi[ks], s[0]);
-    }
-    if (j > 0) finish(t0 - kChunk, buf ^ 1);
-    in_order();
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++) {
-      s[2] = mfma_h(Qf[ks][0], lo[ks], s[2]);
-      s[3] = mfma_h(Qf[ks][0], hi[ks], s[3]);
-      if constexpr (NK == 2) s[2] = mfma_h(Qf[ks][1], hi[ks], s[2]);
-    }
-    // R, to LDS
-    const int bad = bound.bad;  // the first row of which something is not finite; of a column:
-    spoilt = bad;
-    uint32_t vm = max(max(mv[0], mv[1]), max(mv[2], mv[3]));
-    if (__ballot(vm >= kNotFinite)) {  // seldom: every wave looks for the first such value itself
-      if (vm >= kNotFinite) {
-        const float* const b = reinterpret_cast<const float*>(here + In::rows) + kRowBeta * kChunk;
-        vm = 0;
+    uint32_t m = max(max(mv[0], mv[1]), max(mv[2], mv[3]));
+    spoilt = (int)__float_as_uint(of_lane<4>(limits));
+    if (__ballot(m >= kNotFinite)) {  // seldom: every wave looks for the first such value itself
+      if (m >= kNotFinite) {
+        const float* const b = reinterpret_cast<const float*>(p + In::rows) + kRowBeta * kChunk;
+        m = 0;
         for (int r = min(end - t0, kChunk) - 1; r >= 0; r--) {
-          const uint32_t m = magnitude(b[r] * (float)a.v[(size_t)(t0 + r) * a.ldv + (size_t)head * a.dv + col]);
-          if (m >= kNotFinite) spoilt = min(spoilt, r);
-          else vm = max(vm, m);
+          const uint32_t x = magnitude(b[r] * (float)a.v[(size_t)(t0 + r) * a.ldv + (size_t)head * a.dv + col]);
+          if (x >= kNotFinite) spoilt = min(spoilt, r);
+          else m = max(m, x);
         }
 #pragma unroll
         for (int r = 0; r < 4; r++)
           if (magnitude(bv[r]) >= kNotFinite) bv[r] = 0.f;
+        *reinterpret_cast<f32x4*>(lds.bv[buf][w][lane]) = bv;
       }
     }
-    const float rbound = __builtin_fmaf(bound.key, sm, __uint_as_float(vm)), rpower = scale_for(magnitude(rbound)), keep = bound.keep;
-    rinv = inverse_of(rpower);
-    sbound = __builtin_fmaf(keep, sm, bound.back * rbound);
-    {
-      const f32x4 ks_ = s[1] + s[0];
-      f32x4 R;
-#pragma unroll
-      for (int r = 0; r < 4; r++) R[r] = (bv[r] - rk[r] * (sinv * ks_[r])) * rpower;
-      h4 rhi, rlo;
-      split(R, rhi, rlo);
-      *reinterpret_cast<h4*>(&lds.R[0][c][at_row]) = rhi;
-      *reinterpret_cast<h4*>(&lds.R[1][c][at_row]) = rlo;
+    if (w == 0 && g == 0) {
+      lds.cols[c][0] = __uint_as_float(m);
+      lds.cols[c][1] = spoilt < kChunk ? __builtin_nanf("") : of_lane<3>(limits);
     }
+  };
+  const char* ahead = nchunk > 1 ? here + head_step : here;  // the next chunk's
+  load_values(begin, here);
+  load_limits(here);
+  load_tri(here);
+  take_values(0);
+  load_values(begin + kChunk, ahead);
+  lds_barrier();
+  hand_over(here, begin, 0);
+  load_limits(ahead);
+  lds_barrier();
+  // Of the chunk before: its P R, its rows' factors, its first row that is not finite.  Its y is made while the next one's K S is.
+  f32x4 yp = {0.f, 0.f, 0.f, 0.f}, yt = yp, yq = yp;
+  int none = kChunk;
+  auto finish = [&](int t0, int nrows) {
+    const f32x4 qs = *reinterpret_cast<const f32x4*>(lds.qs[w][lane]);
+    const float rinv = lds.rinv[c];
+    f32x4 y;
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) load_key(kp, ks);
+    for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(yt[r], rinv * yp[r], yq[r] * qs[r]);
+    if (__ballot(none < kChunk)) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        if (row0 + r >= none) y[r] = __builtin_nanf("");
+    }
+    const auto rows = rows_of(a.y + (size_t)t0 * a.ldy + (size_t)head * a.dv, nrows, a.ldy);
+#pragma unroll
+    for (int r = 0; r < 4; r++) store_row<T>(rows, yat[r], (T)y[r]);
+  };
+  int t0 = begin;
+  for (int j = 0; j < nchunk; j++, t0 += kChunk) {
+    const char* const far = j + 2 < nchunk ? ahead + head_step : ahead;
     lds_barrier();
-    // [W; P] R
+    take_values(~j & 1);
+    load_values(t0 + 2 * kChunk, far);
+    finish(j ? t0 - kChunk : t0, j ? kChunk : 0);  // (a chunk with another one behind it is whole)
+    lds_barrier();
     h8 rh[2], rl[2];
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
-      rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][ks * 32 + g * 8]);
       rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][ks * 32 + g * 8]);
+      rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][ks * 32 + g * 8]);
     }
-    f32x4 rw[ST], ws[ST][2], p[2];
-#pragma unroll
-    for (int t = 0; t < ST; t++) {
-      rw[t] = *reinterpret_cast<const f32x4*>(&lds.back[buf][w][t * 16 + g * 4]);
-      ws[t][0] = ws[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    }
+    none = spoilt;
+    hand_over(ahead, t0 + kChunk, ~j & 1);  // (behind the last chunk: nobody's)
+    load_limits(far);
+    f32x4 p[2];
     p[0] = p[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    const f32x4 qs = s[3] + s[2];
-#pragma unroll
-    for (int r = 0; r < 4; r++) before[r] = rq[r] * (sinv * qs[r]);
-    keep_factors(buf ^ 1);
-    in_order();
-#pragma unroll
-    for (int t = 0; t < ST; t++)
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        ws[t][0] = mfma_h(Wf[t][ks][0], rl[ks], ws[t][0]);
-        ws[t][1] = mfma_h(Wf[t][ks][0], rh[ks], ws[t][1]);
-        ws[t][0] = mfma_h(Wf[t][ks][1], rh[ks], ws[t][0]);
-      }
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
       if (2 * ks > w) break;
@@ -769,31 +866,14 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 2 : 1) void delta_scan_k
       p[1] = mfma_h(Pf[ks][0], rh[ks], p[1]);
       p[0] = mfma_h(Pf[ks][1], rh[ks], p[0]);
     }
-    bound = bounds_of(next);
-    take_values(buf ^ 1);
-    if (j + 2 < nchunk) load_values(t0 + 2 * kChunk);
-    load_factors(head_of(first + min(j + 2, nchunk - 1)));
-#pragma unroll
-    for (int t = 0; t < ST; t++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) S[t][r] = __builtin_fmaf(rw[t][r], rinv * (ws[t][1][r] + ws[t][0][r]), keep * S[t][r]);
-    if (__ballot(spoilt < kChunk)) {
-      const float nan = __builtin_nanf("");
-      if (spoilt < kChunk) {
-#pragma unroll
-        for (int t = 0; t < ST; t++) S[t] = (f32x4){nan, nan, nan, nan};
-      }
-    }
+    yq = of_quad(query);
+    yt = of_quad(tri);
+    load_tri(ahead);
     yp = p[1] + p[0];
+    ahead = far;
   }
-  finish(begin + (nchunk - 1) * kChunk, (nchunk - 1) & 1);
-#pragma unroll
-  for (int t = 0; t < ST; t++)
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int d = d0 + t * 16 + r;
-      if (mine && d < a.dk) a.state_out[st + (size_t)d * a.dv + col] = S[t][r];
-    }
+  lds_barrier();
+  finish(t0 - kChunk, end - (t0 - kChunk));
 }
 
 // ---------------------------------------------------------------------------
@@ -824,7 +904,7 @@ static int chunk_launch(const DeltaArgs<T>& a, const DeltaTable& tab, char* keys
     hipLaunchKernelGGL((delta_prep_kernel<T, KS>), dim3(chunks, a.heads), dim3(256), 0, st, a, tab, keys, heads);
     if (int rc = check_launch("delta_seq")) return rc;
   }
-  hipLaunchKernelGGL((delta_scan_kernel<T, KS>), dim3(a.nseq * a.heads * slices), dim3(256), 0, st, a, tab, keys, heads);
+  hipLaunchKernelGGL((delta_scan_kernel<T, KS>), dim3(a.nseq * a.heads * slices), dim3(512), 0, st, a, tab, keys, heads);
   return check_launch("delta_seq");
 }
 
