@@ -513,13 +513,18 @@ __device__ __forceinline__ void lds_barrier() {
 
 template <class T, int KS>
 struct ScanLds {
-  h1 S[2][16][KS * 32 + 8], R[2][16][kChunk + 8];  // [column][row], hi and lo; R's rows as the blocks of P and W have their columns
+  h1 S[2][16][KS * 32], R[2][16][kChunk];          // [column][row: see place], hi and lo; R's rows as the blocks of P and W have their columns
   float bv[2][4][64][4];                           // b v of this chunk and the next one, of the lanes of waves 0 to 3
   float qs[4][64][4];                              // Q S, of their lanes
-  float most[16][16];                              // of S, of each lane's rows
+  float most[16][20];                              // of S, of each lane's rows
   uint32_t vmost[16][4];                           // of b v of the next chunk (as bits, which tell what is not finite)
   float cols[16][2], rinv[16];                     // of each column: the largest b v, the decay of the chunk (or NaN: see spoilt); R's inverse power
 };
+
+// Where the eight rows from 8 b on of column c are in S (64 rows and more) and R: rows of 16 bytes, 16 of which are on all banks, change places
+// so that the 16 columns' ones of the same b are, and those of any b that the lanes of a read mix
+template <int ROWS>
+__device__ __forceinline__ int place(int c, int b) { return (b ^ (ROWS == 64 ? c >> 1 : c)) * 8; }
 
 // An element `off` bytes behind a uniform address (or the compiler adds the two ahead of the loop, and keeps 64 bits a lane)
 template <class T>
@@ -602,7 +607,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
     constexpr size_t queries = (size_t)4 * KS * NK * 64 * 16;  // behind the keys
     const size_t st = ((size_t)tab.seq[i0] * a.heads + head) * a.dk * a.dv;
     const float* const from = i0 == 0 && tab.ahead ? a.state_out : a.state;
-    const int d0 = w * (ST * 16) + g * 4, at_row = (w >> 1) * 32 + g * 8 + (w & 1) * 4;  // the lane's rows of S[0], of R
+    const int d0 = w * (ST * 16) + g * 4, at_row = place<kChunk>(c, (w >> 1) * 4 + g) + (w & 1) * 4;  // the lane's rows of S[0], of R
     const uint32_t back_at = In::W + (w * ST * 2 * 2 * 64 + lane) * 16, key_at = In::rows + (kRowK * kChunk + quad0) * 4,
                    scale_at = In::back + (d0 + (c & 3)) * 4;
     h8 Wf[ST][2][2];
@@ -650,8 +655,9 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
       for (int t = 0; t < ST; t++) {
         h4 hi, lo;
         split(S[t] * power, hi, lo);
-        *reinterpret_cast<h4*>(&lds.S[0][c][d0 + t * 16]) = hi;
-        *reinterpret_cast<h4*>(&lds.S[1][c][d0 + t * 16]) = lo;
+        const int to = place<KS * 32>(c, (d0 + t * 16) / 8) + (g & 1) * 4;
+        *reinterpret_cast<h4*>(&lds.S[0][c][to]) = hi;
+        *reinterpret_cast<h4*>(&lds.S[1][c][to]) = lo;
         if (t > 0) {
           load_back(here, t);
           in_order();
@@ -662,8 +668,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
       h8 hi[KS], lo[KS];
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        lo[ks] = *reinterpret_cast<const h8*>(&lds.S[1][c][ks * 32 + g * 8]);
-        hi[ks] = *reinterpret_cast<const h8*>(&lds.S[0][c][ks * 32 + g * 8]);
+        lo[ks] = *reinterpret_cast<const h8*>(&lds.S[1][c][place<KS * 32>(c, ks * 4 + g)]);
+        hi[ks] = *reinterpret_cast<const h8*>(&lds.S[0][c][place<KS * 32>(c, ks * 4 + g)]);
       }
       const float vm = lds.cols[c][0], keep = lds.cols[c][1];
       f32x4 bv = *reinterpret_cast<const f32x4*>(lds.bv[j & 1][w][lane]), kf = of_quad(key);
@@ -707,8 +713,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
       h8 rh[2], rl[2];
 #pragma unroll
       for (int ks = 0; ks < 2; ks++) {
-        rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][ks * 32 + g * 8]);
-        rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][ks * 32 + g * 8]);
+        rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][place<kChunk>(c, ks * 4 + g)]);
+        rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][place<kChunk>(c, ks * 4 + g)]);
       }
       *reinterpret_cast<f32x4*>(lds.qs[w][lane]) = (q[1] + q[0]) * sinv;
       if (w == 0 && g == 0) lds.rinv[c] = rinv;
@@ -851,8 +857,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
     h8 rh[2], rl[2];
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
-      rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][ks * 32 + g * 8]);
-      rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][ks * 32 + g * 8]);
+      rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][place<kChunk>(c, ks * 4 + g)]);
+      rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][place<kChunk>(c, ks * 4 + g)]);
     }
     none = spoilt;
     hand_over(ahead, t0 + kChunk, ~j & 1);  // (behind the last chunk: nobody's)

@@ -425,7 +425,8 @@ int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int co
  *   y[t][h] = scale S^T q
  * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (up to 88 is computed; minus infinity
  * forgets).  q and k are rows of key_heads * key_dim, v and y of heads * value_dim, dt and beta of heads.  state
- * [.][heads][key_dim][value_dim] fp32.  Dimensions 1 to 256, up to 65535 heads; heads * value_dim and key_heads * key_dim up to 2^24. */
+ * [.][heads][key_dim][value_dim] fp32.  Dimensions 1 to 256, up to 65535 heads; heads * value_dim, key_heads * key_dim
+ * and pitches up to 2^23. */
 typedef struct frhip_delta {
   const float *A, *dt_bias;
   int32_t heads, key_heads, key_dim, value_dim;

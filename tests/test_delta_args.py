@@ -31,7 +31,7 @@ def delta(seq=True, p=None, **kw):
 
 @pytest.mark.parametrize("seq", [True, False])
 @pytest.mark.parametrize("kw,code", [
-    (dict(n=-1), ESHAPE), (dict(ldq=63), ESHAPE), (dict(ldk=63), ESHAPE), (dict(ldv=63), ESHAPE), (dict(lddt=3), ESHAPE), (dict(ldbeta=3), ESHAPE),
+    (dict(n=-1), ESHAPE), (dict(ldq=63), ESHAPE), (dict(ldq=(1 << 23) + 1), ESHAPE), (dict(ldy=(1 << 23) + 1), ESHAPE), (dict(ldk=63), ESHAPE), (dict(ldv=63), ESHAPE), (dict(lddt=3), ESHAPE), (dict(ldbeta=3), ESHAPE),
     (dict(ldy=63), ESHAPE), (dict(q=None), EINVAL), (dict(k=None), EINVAL), (dict(v=None), EINVAL), (dict(dt=None), EINVAL), (dict(beta=None), EINVAL),
     (dict(state=None), EINVAL), (dict(out=None), EINVAL), (dict(y=None), EINVAL), (dict(dtype=fr.U8), EINVAL), (dict(q=3 * A + 1), EINVAL), (dict(state=8 * A + 2), EINVAL),
     (dict(y=3 * A), EINVAL), (dict(y=4 * A + 2), EINVAL), (dict(y=5 * A), EINVAL), (dict(y=6 * A), EINVAL), (dict(y=7 * A + 2), EINVAL), (dict(y=8 * A), EINVAL),
