@@ -1,4 +1,4 @@
-// Sums over groups of neighbouring lanes, of a wave and of a workgroup, in fp32: every lane of the group gets the sum, whose order is fixed.
+// Sums over groups of lanes of a wave, in fp32: every lane of the group gets the sum, whose order is fixed.
 #pragma once
 
 #include "device_utils.h"
@@ -38,23 +38,6 @@ __device__ __forceinline__ float stride_sum(float v) {
   if constexpr (STEP <= 16) v = add_across_16(v);
   if constexpr (STEP <= 32) v = add_across_32(v);
   return v;
-}
-
-// Over LANES lanes, up to a workgroup of LANES threads where they are more than a wave: then all threads call it, and `red` is LANES / 64 floats of LDS
-// that were last read ahead of a barrier (callers take turns between two)
-template <int LANES>
-__device__ __forceinline__ float group_sum(float v, float* red) {
-  if constexpr (LANES <= 64) {
-    return lane_sum<LANES>(v);
-  } else {
-    v = lane_sum<64>(v);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float t = red[0];
-#pragma unroll
-    for (int i = 1; i < LANES / 64; i++) t += red[i];
-    return t;
-  }
 }
 
 }  // namespace frhip

@@ -6,6 +6,7 @@
 // A norm is v / sqrt(mean v^2 + eps), of v itself or of v less its mean.  Both are bound by memory: every element once in and once out.  A row (a
 // head of it) lies in the registers of a group of lanes, which sums its squares there; the mean is taken out ahead of them, so that
 // a large one costs no digits.
+#include <algorithm>
 #include <cstring>
 
 #include "activations.h"
@@ -28,9 +29,39 @@ struct Norm {
   int kind;
 };
 
-// Of n elements over LANES lanes, group g of a lane begins at (g LANES + lane) 8; what is behind them is zero and stays so
+// A lane's eight elements as they are in memory, the first n - at of a row's from `at` on
+template <class T>
+struct Raw {
+  typedef T any __attribute__((ext_vector_type(kNormLanes), aligned(sizeof(T))));
+  any v;
+  __device__ __forceinline__ void load(const T* row, int at, int n) {
+    if (n - at >= kNormLanes) {
+      v = *reinterpret_cast<const any*>(row + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kNormLanes; i++) v[i] = at + i < n ? row[at + i] : (T)0.f;
+    }
+  }
+};
+
+// The sum over a row's lanes: LANES of them, up to a wave, or (0) the workgroup's
+template <int LANES>
+__device__ __forceinline__ float row_sum(float v, float* red) {
+  if constexpr (LANES > 0) {
+    return lane_sum<LANES>(v);
+  } else {
+    v = lane_sum<64>(v);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float t = red[0];
+    for (int i = 1; i < (int)blockDim.x / 64; i++) t += red[i];
+    return t;
+  }
+}
+
+// Of n elements, group g of a lane begins at `at` + g `step`; what is behind them is zero and stays so
 template <int LANES, int G>
-__device__ __forceinline__ void normalise(float (&v)[G][kNormLanes], int at, int n, int kind, float eps, float (*red)[16], int& turn) {
+__device__ __forceinline__ void normalise(float (&v)[G][kNormLanes], int at, int step, int n, int kind, float eps, float (*red)[16], int& turn) {
   const float inv = 1.0f / (float)n;
   if (kind == FRHIP_NORM_MEAN) {
     float s = 0.f;
@@ -38,19 +69,19 @@ __device__ __forceinline__ void normalise(float (&v)[G][kNormLanes], int at, int
     for (int g = 0; g < G; g++)
 #pragma unroll
       for (int i = 0; i < kNormLanes; i++) s += v[g][i];
-    const float mean = group_sum<LANES>(s, red[turn]) * inv;
+    const float mean = row_sum<LANES>(s, red[turn]) * inv;
     turn ^= 1;
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
-      for (int i = 0; i < kNormLanes; i++) v[g][i] = at + g * LANES * kNormLanes + i < n ? v[g][i] - mean : 0.f;
+      for (int i = 0; i < kNormLanes; i++) v[g][i] = at + g * step + i < n ? v[g][i] - mean : 0.f;
   }
   float s = 0.f;
 #pragma unroll
   for (int g = 0; g < G; g++)
 #pragma unroll
     for (int i = 0; i < kNormLanes; i++) s = __builtin_fmaf(v[g][i], v[g][i], s);
-  const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(group_sum<LANES>(s, red[turn]), inv, eps));
+  const float r = __builtin_amdgcn_rsqf(__builtin_fmaf(row_sum<LANES>(s, red[turn]), inv, eps));
   turn ^= 1;
 #pragma unroll
   for (int g = 0; g < G; g++)
@@ -58,19 +89,19 @@ __device__ __forceinline__ void normalise(float (&v)[G][kNormLanes], int at, int
     for (int i = 0; i < kNormLanes; i++) v[g][i] *= r;
 }
 
-template <int LANES, int G, class T>
-__device__ __forceinline__ void load_row(float (&v)[G][kNormLanes], const T* p, int at, int n) {
+template <int G, class T>
+__device__ __forceinline__ void load_row(float (&v)[G][kNormLanes], const T* p, int at, int step, int n) {
 #pragma unroll
   for (int g = 0; g < G; g++) {
-    const int c = at + g * LANES * kNormLanes;
+    const int c = at + g * step;
     load_group<T, kNormLanes>(v[g], p + (c < n ? c : 0), n - c);
   }
 }
-template <int LANES, int G, class T>
-__device__ __forceinline__ void store_row(T* p, const float (&v)[G][kNormLanes], int at, int n) {
+template <int G, class T>
+__device__ __forceinline__ void store_row(T* p, const float (&v)[G][kNormLanes], int at, int step, int n) {
 #pragma unroll
   for (int g = 0; g < G; g++) {
-    const int c = at + g * LANES * kNormLanes;
+    const int c = at + g * step;
     if (c < n) store_group<T, kNormLanes>(p + c, v[g], n - c);
   }
 }
@@ -98,24 +129,26 @@ struct GateArgs {
   int shift;  // 2^shift neighbouring groups of a workgroup take neighbouring heads, the others further rows
 };
 
-// blockIdx.x: heads, blockIdx.y, and so on by gridDim.y: rows.  A group keeps its head, and so the head's parameters.
+// blockIdx.x: heads, blockIdx.y, and so on by gridDim.y: rows.  A group of LANES lanes (0: the workgroup) keeps its head, and so the head's parameters.
+// 4096 rows of 32 heads of 128 of binary16: 20.4 us, 4.9 TB/s, as a large copy has.
 template <class T, int LANES, int G>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_gate_kernel(GateArgs<T> a) {
-  constexpr int GROUPS = LANES > 256 ? 1 : 256 / LANES;
+__global__ __launch_bounds__(LANES ? 256 : 1024) void norm_gate_kernel(GateArgs<T> a) {
+  constexpr int GROUPS = LANES ? 256 / (LANES ? LANES : 1) : 1;
   __shared__ float red[2][16];
-  const int group = GROUPS == 1 ? 0 : threadIdx.x / LANES, at = (threadIdx.x % LANES) * kNormLanes, n = a.dim;
+  const int lanes = LANES ? LANES : blockDim.x, group = LANES ? threadIdx.x / lanes : 0, at = (threadIdx.x - group * lanes) * kNormLanes, n = a.dim;
+  const int grid_step = lanes * kNormLanes;
   const int head = (blockIdx.x << a.shift) + (group & ((1 << a.shift) - 1)), step = GROUPS >> a.shift;
-  if (head >= a.heads) return;  // more than a wave has one head, and stays together
+  if (head >= a.heads) return;  // a workgroup that has one head stays together
   const size_t c0 = (size_t)head * n;
   float w[G][kNormLanes], b[G][kNormLanes];
-  if (a.norm.w) load_row<LANES, G>(w, a.norm.w + c0, at, n);
-  if (a.norm.b) load_row<LANES, G>(b, a.norm.b + c0, at, n);
+  if (a.norm.w) load_row<G>(w, a.norm.w + c0, at, grid_step, n);
+  if (a.norm.b) load_row<G>(b, a.norm.b + c0, at, grid_step, n);
   int turn = 0;
   for (int row = blockIdx.y * step + (group >> a.shift); row < a.rows; row += gridDim.y * step) {
     float v[G][kNormLanes], z[G][kNormLanes];
-    load_row<LANES, G>(v, a.x + (size_t)row * a.ldx + c0, at, n);
-    if (a.z) load_row<LANES, G>(z, a.z + (size_t)row * a.ldz + c0, at, n);
-    normalise<LANES, G>(v, at, n, a.norm.kind, a.norm.eps, red, turn);
+    load_row<G>(v, a.x + (size_t)row * a.ldx + c0, at, grid_step, n);
+    if (a.z) load_row<G>(z, a.z + (size_t)row * a.ldz + c0, at, grid_step, n);
+    normalise<LANES, G>(v, at, grid_step, n, a.norm.kind, a.norm.eps, red, turn);
 #pragma unroll
     for (int g = 0; g < G; g++)
 #pragma unroll
@@ -124,20 +157,20 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_gate_kernel(Ga
         if (a.norm.b) v[g][i] += b[g][i];
       }
     if (a.z) times_act<sizeof(T) == 4, G>(v, z, a.act);
-    store_row<LANES, G>(a.y + (size_t)row * a.ldy + c0, v, at, n);
+    store_row<G>(a.y + (size_t)row * a.ldy + c0, v, at, grid_step, n);
   }
 }
 
 template <class T, int LANES, int G>
 static int gate_launch(GateArgs<T> a, hipStream_t st) {
-  constexpr int GROUPS = LANES > 256 ? 1 : 256 / LANES;
+  constexpr int GROUPS = LANES ? 256 / (LANES ? LANES : 1) : 1;
+  const int threads = LANES ? 256 : std::min(1024, ((a.dim - 1) / kNormLanes / 64 + 1) * 64);
   a.shift = 0;
   while ((1 << a.shift) < GROUPS && (1 << a.shift) < a.heads) a.shift++;
   const int step = GROUPS >> a.shift, blocks = (a.heads - 1) / (1 << a.shift) + 1;
-  // rows over about eight workgroups a compute unit, so that a group's parameters serve several of them
-  const int want = compute_units() * 8 / blocks + 1, most = (a.rows - 1) / step + 1;
-  const int lim = most < want ? most : want;
-  hipLaunchKernelGGL((norm_gate_kernel<T, LANES, G>), dim3(blocks, lim < 65535 ? lim : 65535), dim3(LANES > 256 ? LANES : 256), 0, st, a);
+  // rows over about 32 waves a compute unit, so that a group's parameters serve several of them
+  const int want = compute_units() * std::max(1, 2048 / threads) / blocks + 1, most = (a.rows - 1) / step + 1;
+  hipLaunchKernelGGL((norm_gate_kernel<T, LANES, G>), dim3(blocks, std::min(std::min(want, most), 65535)), dim3(threads), 0, st, a);
   return check_launch("norm_gate");
 }
 
@@ -148,10 +181,8 @@ static int gate_run(const GateArgs<T>& a, hipStream_t st) {
   if (n <= 128) return gate_launch<T, 16, 1>(a, st);
   if (n <= 256) return gate_launch<T, 32, 1>(a, st);
   if (n <= 512) return gate_launch<T, 64, 1>(a, st);
-  if (n <= 2048) return gate_launch<T, 256, 1>(a, st);
-  if (n <= 4096) return gate_launch<T, 256, 2>(a, st);
-  if (n <= 8192) return gate_launch<T, 1024, 1>(a, st);
-  return gate_launch<T, 1024, 4>(a, st);
+  if (n <= 8192) return gate_launch<T, 0, 1>(a, st);
+  return gate_launch<T, 0, 4>(a, st);
 }
 
 // ---------------------------------------------------------------------------
@@ -169,72 +200,89 @@ struct ResidualArgs {
   float scale;
 };
 
-// A row a group of lanes; blockIdx.x, and so on by gridDim.x: the rows
-template <class S, class T, int LANES, int G>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void norm_residual_kernel(ResidualArgs<S, T> a) {
-  constexpr int GROUPS = LANES > 256 ? 1 : 256 / LANES;
-  constexpr bool HOLD = G <= 2 && LANES <= 256;  // the parameters stay in registers from row to row where there is room for them
+// A row of at most 512 elements a wave (WIDE: a workgroup, G groups of eight a thread); blockIdx.x, and so on by gridDim.x: the rows.  A row's
+// loads go out ahead of the sums of the row before.
+// 4096 rows of 2560, two norms, a gate, a stream in fp32: 35 us, 4.2 TB/s; about thirteen workgroups of five waves a compute unit (six: 37).
+template <class S, class T, int G, bool WIDE>
+__global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(ResidualArgs<S, T> a) {
   constexpr bool FINE = sizeof(S) == 4 || sizeof(T) == 4;
+  constexpr int GROUPS = WIDE ? 1 : 4;
   __shared__ float red[2][16];
-  const int group = GROUPS == 1 ? 0 : threadIdx.x / LANES, at = (threadIdx.x % LANES) * kNormLanes, n = a.cols;
-  float aw[G][kNormLanes], ab[G][kNormLanes], bw[G][kNormLanes], bb[G][kNormLanes], ch[G][kNormLanes];
-  auto parameters = [&] {
-    if (a.after.w) load_row<LANES, G>(aw, a.after.w, at, n);
-    if (a.after.b) load_row<LANES, G>(ab, a.after.b, at, n);
-    if (a.before.w) load_row<LANES, G>(bw, a.before.w, at, n);
-    if (a.before.b) load_row<LANES, G>(bb, a.before.b, at, n);
-    if (a.channels) load_row<LANES, G>(ch, a.channels, at, n);
+  const int group = WIDE ? 0 : threadIdx.x / 64, lanes = WIDE ? blockDim.x : 64, at = (WIDE ? threadIdx.x : threadIdx.x & 63) * kNormLanes, n = a.cols;
+  const int step = lanes * kNormLanes;
+  constexpr bool AHEAD = G == 1;  // rows of more than 8192 have no registers to spare
+  // f(i, parameter) for the lane's eight of group g.  (In registers from row to row they cost as many waves as they save: 41 us instead of 37.)
+  auto with = [&](const float* params, int g, auto f) {
+    if (!params) return;
+    const int c = at + g * step;
+    float p[kNormLanes];
+    load_group<float, kNormLanes>(p, params + (c < n ? c : 0), n - c);
+#pragma unroll
+    for (int i = 0; i < kNormLanes; i++) f(i, p[i]);
   };
-  if constexpr (HOLD) parameters();
+  Raw<S> xr[G];
+  Raw<T> br[G], gr[G];
+  const int first = blockIdx.x * GROUPS + group, stride = gridDim.x * GROUPS;
+  auto request = [&](int row) {
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+      const int c = at + g * step;
+      if (a.block) br[g].load(a.block + (size_t)row * a.ldb, c, n);
+      if (a.gate) gr[g].load(a.gate + (size_t)row * a.ldg, c, n);
+      xr[g].load(a.x + (size_t)row * a.ldx, c, n);
+    }
+  };
+  if (AHEAD && first < a.rows) request(first);
   int turn = 0;
-  for (int row = blockIdx.x * GROUPS + group; row < a.rows; row += gridDim.x * GROUPS) {
+  for (int row = first; row < a.rows; row += stride) {
+    if (!AHEAD) request(row);
     float h[G][kNormLanes], v[G][kNormLanes], z[G][kNormLanes];
-    if (a.block) load_row<LANES, G>(v, a.block + (size_t)row * a.ldb, at, n);
-    if (a.block && a.gate) load_row<LANES, G>(z, a.gate + (size_t)row * a.ldg, at, n);
-    load_row<LANES, G>(h, a.x + (size_t)row * a.ldx, at, n);
-    if constexpr (!HOLD) parameters();
+#pragma unroll
+    for (int g = 0; g < G; g++)
+#pragma unroll
+      for (int i = 0; i < kNormLanes; i++) {
+        h[g][i] = (float)xr[g].v[i];
+        v[g][i] = a.block ? (float)br[g].v[i] : 0.f;
+        z[g][i] = a.gate ? (float)gr[g].v[i] : 0.f;
+      }
+    if (AHEAD && a.rows - row > stride) request(row + stride);
     if (a.block) {
       if (a.after.kind != FRHIP_NORM_NONE) {
-        normalise<LANES, G>(v, at, n, a.after.kind, a.after.eps, red, turn);
+        normalise<WIDE ? 0 : 64, G>(v, at, step, n, a.after.kind, a.after.eps, red, turn);
 #pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-          for (int i = 0; i < kNormLanes; i++) {
-            if (a.after.w) v[g][i] *= aw[g][i];
-            if (a.after.b) v[g][i] += ab[g][i];
-          }
+        for (int g = 0; g < G; g++) {
+          with(a.after.w, g, [&](int i, float p) { v[g][i] *= p; });
+          with(a.after.b, g, [&](int i, float p) { v[g][i] += p; });
+        }
       }
       if (a.gate) times_act<FINE, G>(v, z, a.act);
 #pragma unroll
-      for (int g = 0; g < G; g++)
+      for (int g = 0; g < G; g++) {
+        with(a.channels, g, [&](int i, float p) { v[g][i] *= p; });
 #pragma unroll
-        for (int i = 0; i < kNormLanes; i++) {
-          if (a.channels) v[g][i] *= ch[g][i];
-          h[g][i] = __builtin_fmaf(a.scale, v[g][i], h[g][i]);
-        }
+        for (int i = 0; i < kNormLanes; i++) h[g][i] = __builtin_fmaf(a.scale, v[g][i], h[g][i]);
+      }
     }
-    if (a.h) store_row<LANES, G>(a.h + (size_t)row * a.ldh, h, at, n);
+    if (a.h) store_row<G>(a.h + (size_t)row * a.ldh, h, at, step, n);
     if (a.y) {
       if (a.before.kind != FRHIP_NORM_NONE) {
-        normalise<LANES, G>(h, at, n, a.before.kind, a.before.eps, red, turn);
+        normalise<WIDE ? 0 : 64, G>(h, at, step, n, a.before.kind, a.before.eps, red, turn);
 #pragma unroll
-        for (int g = 0; g < G; g++)
-#pragma unroll
-          for (int i = 0; i < kNormLanes; i++) {
-            if (a.before.w) h[g][i] *= bw[g][i];
-            if (a.before.b) h[g][i] += bb[g][i];
-          }
+        for (int g = 0; g < G; g++) {
+          with(a.before.w, g, [&](int i, float p) { h[g][i] *= p; });
+          with(a.before.b, g, [&](int i, float p) { h[g][i] += p; });
+        }
       }
-      store_row<LANES, G>(a.y + (size_t)row * a.ldy, h, at, n);
+      store_row<G>(a.y + (size_t)row * a.ldy, h, at, step, n);
     }
   }
 }
 
-template <class S, class T, int LANES, int G>
+template <class S, class T, int G, bool WIDE>
 static int residual_launch(const ResidualArgs<S, T>& a, hipStream_t st) {
-  constexpr int GROUPS = LANES > 256 ? 1 : 256 / LANES;
-  const int want = compute_units() * 8, most = (a.rows - 1) / GROUPS + 1;
-  hipLaunchKernelGGL((norm_residual_kernel<S, T, LANES, G>), dim3(most < want ? most : want), dim3(LANES > 256 ? LANES : 256), 0, st, a);
+  const int groups = (a.cols - 1) / kNormLanes + 1, threads = WIDE ? std::min(1024, (groups + 63) / 64 * 64) : 256;
+  const int per = WIDE ? 1 : 4, want = compute_units() * std::max(1, 4096 / threads), most = (a.rows - 1) / per + 1;
+  hipLaunchKernelGGL((norm_residual_kernel<S, T, G, WIDE>), dim3(std::min(want, most)), dim3(threads), 0, st, a);
   return check_launch("norm_residual");
 }
 
@@ -260,11 +308,10 @@ static int residual_run(const frhip_block_norm& p, int rows, const void* x, int 
   a.ldy = ldy;
   a.act = p.gate_act;
   a.scale = p.scale;
-  if (p.cols <= 512) return residual_launch<S, T, 64, 1>(a, st);
-  if (p.cols <= 2048) return residual_launch<S, T, 256, 1>(a, st);
-  if (p.cols <= 4096) return residual_launch<S, T, 256, 2>(a, st);
-  if (p.cols <= 8192) return residual_launch<S, T, 1024, 1>(a, st);
-  return residual_launch<S, T, 1024, 4>(a, st);
+  if (p.cols <= 512) return residual_launch<S, T, 1, false>(a, st);
+  if (p.cols <= 8192) return residual_launch<S, T, 1, true>(a, st);
+  if (p.cols <= 16384) return residual_launch<S, T, 2, true>(a, st);
+  return residual_launch<S, T, 4, true>(a, st);
 }
 
 // ---------------------------------------------------------------------------
