@@ -53,6 +53,8 @@ __device__ __forceinline__ float finite_rate(float r) { return r < -__FLT_MAX__ 
 
 // The form by chunks, host side: its scratch for T rows, and prompts of a call by it (indices into start; in any order)
 size_t delta_chunk_bytes(const frhip_delta& p, int elem, int T);
+// Whether prompts, some of them of kDeltaChunkLeast rows, have no more chunks than one pair of launches for T rows takes
+bool delta_chunks_fit(const frhip_delta& p, int elem, const int32_t* start, int nseq, int T);
 template <class T>
 int delta_chunk_run(const DeltaArgs<T>& a, const int* seqs, int nseq, const int32_t* start, int rows, void* workspace, hipStream_t st);
 

@@ -586,6 +586,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
   const size_t nall = tab.chunk[a.nseq];
   const bool mine = col0 + c < a.dv;
   const int col = mine ? col0 + c : a.dv - 1;
+  if (nchunk == 0) {  // no rows: the state as it was
+    const float* const from = a.state;
+    const size_t st = ((size_t)tab.seq[i0] * a.heads + head) * a.dk * a.dv;
+    for (int d = wave * 4 + g; d < a.dk; d += 32)
+      if (mine) a.state_out[st + (size_t)d * a.dv + col] = from[st + (size_t)d * a.dv + col];
+    return;
+  }
   constexpr size_t head_step = In::bytes, key_step = key_bytes(KS * 32, NK);
   const char* here = heads + (head * nall + first) * head_step;  // of the chunk that is requested next
   const int row0 = w * 16 + g * 4, quad0 = row0 + (c & 3);       // the lane's rows of a chunk; the one of which it requests factors
@@ -891,7 +898,7 @@ static size_t chunk_bytes(int heads, int key_heads, int dk, int parts) {
   const int ks = key_steps(dk), head = ks == 2 ? HeadLayout<2>::bytes : ks == 4 ? HeadLayout<4>::bytes : HeadLayout<8>::bytes;
   return (size_t)heads * head + (size_t)key_heads * key_bytes(ks * 32, parts);
 }
-// Chunks of a pair of launches: prompts have kDeltaChunkLeast rows at least, so there are no more chunks than rows / kDeltaChunkLeast + 1
+// Chunks of a pair of launches.  Prompts of kDeltaChunkLeast rows and more have rows / kDeltaChunkLeast + 1 at most.
 static size_t most_chunks(size_t per, int T) {
   const size_t by_rows = (size_t)T / kDeltaChunkLeast + 1, by_bytes = std::max<size_t>(kPassBytes / per, 16);
   return std::min(by_rows, by_bytes);
@@ -901,6 +908,17 @@ size_t delta_chunk_bytes(const frhip_delta& p, int elem, int T) {
   if (T < kDeltaChunkLeast) return 0;
   const size_t per = chunk_bytes(p.heads, p.key_heads, p.key_dim, elem == 4 ? 2 : 1);
   return most_chunks(per, T) * per;
+}
+
+bool delta_chunks_fit(const frhip_delta& p, int elem, const int32_t* start, int nseq, int T) {
+  size_t chunks = 0;
+  int longest = 0;
+  for (int i = 0; i < nseq; i++) {
+    const int len = start[i + 1] - start[i];
+    longest = std::max(longest, len);
+    chunks += len ? (len - 1) / kChunk + 1 : 0;
+  }
+  return longest >= kDeltaChunkLeast && chunks <= most_chunks(chunk_bytes(p.heads, p.key_heads, p.key_dim, elem == 4 ? 2 : 1), T);
 }
 
 template <class T, int KS>
@@ -930,7 +948,7 @@ int delta_chunk_run(const DeltaArgs<T>& args, const int* seqs, int nseq, const i
     tab.ahead = done > 0;
     size_t left = most;
     while (i < nseq && left > 0 && a.nseq < together) {
-      const int s = seqs[i], len = start[s + 1] - start[s], chunks = (len - 1) / kChunk + 1 - done;
+      const int s = seqs[i], len = start[s + 1] - start[s], chunks = (len ? (len - 1) / kChunk + 1 : 0) - done;
       const int now = (size_t)chunks < left ? chunks : (int)left;
       tab.start[a.nseq] = start[s] + done * kChunk;
       tab.end[a.nseq] = now == chunks ? start[s + 1] : tab.start[a.nseq] + now * kChunk;
