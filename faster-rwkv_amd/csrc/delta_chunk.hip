@@ -253,8 +253,9 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
     for (int n = 0; n < NK; n++) *reinterpret_cast<h8*>(&lds.K[n][row][ks * 32 + g * 8]) = K.f[ks][n];
   if (g == 0) {
     const float nan = __builtin_nanf("");
-    lds.fk[row] = K.finite ? K.factor(a.eps) : nan;
-    lds.fq[row] = (Q.finite ? Q.factor(a.eps) : nan) * a.scale;
+    const bool real = row < len;  // (of no row, and with a.eps zero, there is no length)
+    lds.fk[row] = !real ? 0.f : K.finite ? K.factor(a.eps) : nan;
+    lds.fq[row] = !real ? 0.f : (Q.finite ? Q.factor(a.eps) : nan) * a.scale;
     lds.length[row] = __builtin_sqrtf(K.squares * (KS * 32));  // not below the sum of the row's magnitudes
   }
   if (head % a.share == 0) {
