@@ -14,7 +14,7 @@ namespace frhip {
 constexpr int kMostDim = 256;         // of a key, of a value
 constexpr int kMostHeads = 65535;     // a launch's second dimension
 constexpr int kMostPitch = 1 << 23;   // of rows: the bytes of a chunk of them, 64, stay in 32 bits
-constexpr int kDeltaChunkLeast = 17;  // rows of a prompt, at least, that goes chunk by chunk
+constexpr int kDeltaChunkLeast = 21;  // rows of a prompt, at least, that goes chunk by chunk
 
 template <class T>
 struct DeltaArgs {

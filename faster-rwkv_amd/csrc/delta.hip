@@ -16,19 +16,22 @@ namespace frhip {
 
 // ---------------------------------------------------------------------------
 // Token by token.  A wave has CL x 4 columns of a head, and CL lanes of a row of S: lane l has its columns 4 (l % CL) and the R keys from R (l / CL) on.
-// Bound by memory where there are many sequences of one token: the states once in and once out.
+// Bound by memory where there are many sequences of one token, the states once in and once out: 64 of 32 heads 128 x 128 in 55 us, 4.9 TB/s.  A prompt's
+// tokens are bound by the instructions of its waves, of which a compute unit has few: so sums over rows of lanes leave each with a column of its own, whose
+// value and result it works out, the lengths are a wave's scalars, and 64 tokens' gates are evaluated at once, a lane each.
 // ---------------------------------------------------------------------------
-// R elements as they are in memory, the first n of them
-template <class T, int R>
+// R elements as they are in memory, the first n of them.  WHOLE: all or none, and p can be read in either case
+template <class T, int R, bool WHOLE>
 struct RawRow {
   static constexpr int P = R < kGroup<T> ? R : kGroup<T>;
   typedef T any __attribute__((ext_vector_type(P), aligned(sizeof(T))));
   any v[R / P];
   __device__ __forceinline__ void load(const T* p, int n) {
-    if (n >= R) {
+    if (WHOLE || n >= R) {
 #pragma unroll
       for (int k = 0; k < R / P; k++) v[k] = *reinterpret_cast<const any*>(p + k * P);
-    } else {
+    }
+    if (!WHOLE && n < R) {
 #pragma unroll
       for (int i = 0; i < R; i++) v[i / P][i % P] = i < n ? p[i] : (T)0.f;
     }
@@ -36,26 +39,59 @@ struct RawRow {
   __device__ __forceinline__ float operator[](int i) const { return (float)v[i / P][i % P]; }
 };
 
-template <class T, int CL, int R, bool ONE>
+// Two values' sums of each lane's and the one's 32 (16) away: the first value's in the even halves (rows), the second one's in the odd ones
+__device__ __forceinline__ float halves_sum(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float rows_sum(float x, float y) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Value j's sum over the lanes that share lane % CL, in row j of 16 lanes
+template <int CL>
+__device__ __forceinline__ float sum_by_row(float v0, float v1, float v2, float v3) {
+  float v = rows_sum(halves_sum(v0, v2), halves_sum(v1, v3));
+  v += dpp_mov<0x128>(v);  // row_ror:8
+  if constexpr (CL == 4) v += dpp_mov<0x124>(v);
+  return v;
+}
+// What the four rows of lanes have, to all of them
+__device__ __forceinline__ void of_rows(float v, float (&to)[4]) {
+  const uint32_t u = __float_as_uint(v);
+  const auto h = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(h[0], h[0], false, false), hi = __builtin_amdgcn_permlane16_swap(h[1], h[1], false, false);
+  to[0] = __uint_as_float(lo[0]);
+  to[1] = __uint_as_float(lo[1]);
+  to[2] = __uint_as_float(hi[0]);
+  to[3] = __uint_as_float(hi[1]);
+}
+__device__ __forceinline__ float lane_of(float v, int lane) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane)); }
+
+template <class T, int CL, int R, bool ONE, bool WHOLE>
 __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, DeltaTable tab) {
   constexpr int W = 4 * CL;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slices = (a.dv + W - 1) / W, unit = blockIdx.x * 4 + wave;
   if (unit >= a.heads * slices) return;  // whole waves; nothing here waits for another one
-  const int head = unit / slices, kh = head / a.share, c = (unit - head * slices) * W + (lane % CL) * 4, d0 = lane / CL * R;
+  const int head = unit / slices, kh = head / a.share, c = (unit - head * slices) * W + (lane % CL) * 4, d0 = lane / CL * R, col = c + lane / 16;
   const int nc = a.dv - c, nd = a.dk - d0;
+  const bool mine = (lane & 15) < CL && col < a.dv;
   const float rate = a.A ? finite_rate(a.A[head]) : 1.f, bias = a.dt_bias ? a.dt_bias[head] : 0.f;
-  const size_t kat = (size_t)kh * a.dk + (nd > 0 ? d0 : 0), vat = (size_t)head * a.dv + (nc > 0 ? c : 0);
+  const size_t kat = (size_t)kh * a.dk + (nd > 0 ? d0 : 0), vat = (size_t)head * a.dv + (col < a.dv ? col : 0);
   const int nseq = ONE ? a.rows : a.nseq;
-  RawRow<T, R> qr, kr;
-  RawRow<T, 4> vr;
-  T dt, beta;
+  RawRow<T, R, WHOLE> qr, kr;
+  T vr;
+  float keeps, writes;  // of this token, or of 64 tokens, a lane each
   auto request = [&](int t) {
     kr.load(a.k + (size_t)t * a.ldk + kat, nd);
     qr.load(a.q + (size_t)t * a.ldq + kat, nd);
-    vr.load(a.v + (size_t)t * a.ldv + vat, nc);
-    dt = a.dt[(size_t)t * a.lddt + head];
-    beta = a.beta[(size_t)t * a.ldbeta + head];
+    vr = a.v[(size_t)t * a.ldv + vat];
+  };
+  auto gates = [&](int t) {
+    const float dt = (float)a.dt[(size_t)t * a.lddt + head], raw = (float)a.beta[(size_t)t * a.ldbeta + head];
+    keeps = decay_f(log_decay(a, dt, rate, bias));
+    writes = a.sigmoid ? sigmoid_f<true>(raw) : raw;
   };
   for (int i = blockIdx.y; i < nseq; i += gridDim.y) {
     const size_t st = ((size_t)(ONE ? i : tab.seq[i]) * a.heads + head) * a.dk * a.dv + c;
@@ -64,17 +100,18 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, DeltaTa
     float S[R][4];
 #pragma unroll
     for (int r = 0; r < R; r++) load_group<float, 4>(S[r], a.state + st + (size_t)(r < nd ? d0 + r : 0) * a.dv, r < nd ? nc : 0);
+    if (ONE) gates(begin);
     for (int t = begin; t < end; t++) {
-      float q[R], k[R], v[4];
+      const int nth = (t - begin) & 63;
+      if (!ONE && nth == 0) gates(min(t + lane, end - 1));
+      float q[R], k[R];
 #pragma unroll
       for (int r = 0; r < R; r++) {
-        q[r] = qr[r];
-        k[r] = kr[r];
+        q[r] = !WHOLE || nd > 0 ? qr[r] : 0.f;
+        k[r] = !WHOLE || nd > 0 ? kr[r] : 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < 4; j++) v[j] = vr[j];
-      const float g = log_decay(a, (float)dt, rate, bias), raw = (float)beta, keep = decay_f(g), b = a.sigmoid ? sigmoid_f<true>(raw) : raw;
-      if (!ONE && t + 1 < end) request(t + 1);  // on its way while this one is worked on
+      const float v = (float)vr, keep = ONE ? keeps : lane_of(keeps, nth), b = ONE ? writes : lane_of(writes, nth);
+      if (!ONE) request(min(t + 1, end - 1));  // on its way while this one is worked on
       float kk = 0.f, qq = 0.f, qk = 0.f, kS[4] = {}, qS[4] = {};
 #pragma unroll
       for (int r = 0; r < R; r++) {
@@ -87,23 +124,20 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, DeltaTa
           qS[j] = __builtin_fmaf(q[r], S[r][j], qS[j]);
         }
       }
-      qk = stride_sum<CL>(qk);
+      const float sums = sum_by_row<CL>(kk, qq, qk, qq), ks = sum_by_row<CL>(kS[0], kS[1], kS[2], kS[3]), qs = sum_by_row<CL>(qS[0], qS[1], qS[2], qS[3]);
       float kn = 1.f, qn = a.scale;
       if (a.eps >= 0.f) {
-        kn = __builtin_amdgcn_rsqf(stride_sum<CL>(kk) + a.eps);
-        qn = __builtin_amdgcn_rsqf(stride_sum<CL>(qq) + a.eps) * a.scale;
+        kn = __builtin_amdgcn_rsqf(lane_of(sums, 0) + a.eps);
+        qn = __builtin_amdgcn_rsqf(lane_of(sums, 16) + a.eps) * a.scale;
       }
-      float u[4], o[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        u[j] = b * (v[j] - keep * kn * stride_sum<CL>(kS[j]));
-        o[j] = qn * __builtin_fmaf(keep, stride_sum<CL>(qS[j]), qk * kn * u[j]);
-      }
+      const float u = kn * (b * (v - keep * kn * ks));
+      float to[4];
+      of_rows(u, to);
 #pragma unroll
       for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) S[r][j] = __builtin_fmaf(k[r] * kn, u[j], keep * S[r][j]);
-      if (lane < CL && nc > 0) store_group<T, 4>(a.y + (size_t)t * a.ldy + vat, o, nc);
+        for (int j = 0; j < 4; j++) S[r][j] = __builtin_fmaf(k[r], to[j], keep * S[r][j]);
+      if (mine) a.y[(size_t)t * a.ldy + vat] = (T)(qn * __builtin_fmaf(keep, qs, lane_of(sums, 32) * u));
     }
 #pragma unroll
     for (int r = 0; r < R; r++)
@@ -114,16 +148,21 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, DeltaTa
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
-template <class T, int CL, bool ONE>
-static int step_launch(const DeltaArgs<T>& a, const DeltaTable& tab, int nseq, hipStream_t st) {
+template <class T, int CL, bool ONE, bool WHOLE>
+static int step_launch_of(const DeltaArgs<T>& a, const DeltaTable& tab, int nseq, hipStream_t st) {
   const int slices = (a.dv + 4 * CL - 1) / (4 * CL), units = a.heads * slices;
   const dim3 grid((units + 3) / 4, nseq < 65535 ? nseq : 65535);
   const int rows = (a.dk + 64 / CL - 1) / (64 / CL);  // keys of a lane
-  if (rows <= 4) hipLaunchKernelGGL((delta_step_kernel<T, CL, 4, ONE>), grid, dim3(256), 0, st, a, tab);
-  else if (rows <= 8) hipLaunchKernelGGL((delta_step_kernel<T, CL, 8, ONE>), grid, dim3(256), 0, st, a, tab);
-  else if (rows <= 16) hipLaunchKernelGGL((delta_step_kernel<T, CL, 16, ONE>), grid, dim3(256), 0, st, a, tab);
-  else hipLaunchKernelGGL((delta_step_kernel<T, CL, 32, ONE>), grid, dim3(256), 0, st, a, tab);
+  if (rows <= 4) hipLaunchKernelGGL((delta_step_kernel<T, CL, 4, ONE, WHOLE>), grid, dim3(256), 0, st, a, tab);
+  else if (rows <= 8) hipLaunchKernelGGL((delta_step_kernel<T, CL, 8, ONE, WHOLE>), grid, dim3(256), 0, st, a, tab);
+  else if (rows <= 16) hipLaunchKernelGGL((delta_step_kernel<T, CL, 16, ONE, WHOLE>), grid, dim3(256), 0, st, a, tab);
+  else if constexpr (CL == 8) hipLaunchKernelGGL((delta_step_kernel<T, CL, 32, ONE, WHOLE>), grid, dim3(256), 0, st, a, tab);
   return check_launch("delta");
+}
+template <class T, int CL, bool ONE>
+static int step_launch(const DeltaArgs<T>& a, const DeltaTable& tab, int nseq, hipStream_t st) {
+  const int rows = (a.dk + 64 / CL - 1) / (64 / CL), part = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 32;
+  return a.dk % part == 0 && a.dv % 4 == 0 ? step_launch_of<T, CL, ONE, true>(a, tab, nseq, st) : step_launch_of<T, CL, ONE, false>(a, tab, nseq, st);
 }
 
 static int delta_check_params(const frhip_delta* p) {
@@ -214,6 +253,22 @@ static int delta_one_run(const frhip_delta& p, const DeltaCall& c, int rows, hip
   return step_launch<T, 8, true>(a, none, rows, st);
 }
 
+// Rows, at least, of the prompts of a call that go chunk by chunk.  Either form's time (us), 32 heads 128 x 128, by the rows of each prompt:
+//   one prompt    8: 9 / 17   16: 13 / 16   20: 16 / 16   32: 23 / 17   64: 42 / 17
+//   16 prompts    8: 22 / 77  16: 35 / 77   32: 60 / 77   48: 85 / 78   64: 110 / 78
+// A chunk of few rows costs what a whole one does, which counts where there are more of them than compute units to work on them.  For the same reason short
+// prompts join long ones if they are few: launches that are there anyway take them for nothing (nine prompts of 24 heads 64 x 64, four of them of 31 rows at
+// most: 62 -> 45 us).
+static int chunk_least(const frhip_delta& p, const int32_t* start, int n, int elem, int rows) {
+  const long long each = (long long)p.heads * ((p.value_dim + 15) / 16), room = 2LL * compute_units();  // workgroups
+  int some = 0;
+  for (int i = 0; i < n; i++) some += start[i + 1] - start[i] >= kDeltaChunkLeast;
+  const int least = some * each <= room ? kDeltaChunkLeast : 2 * kDeltaChunkLeast;
+  int below = 0;
+  for (int i = 0; i < n; i++) below += start[i + 1] - start[i] < least;
+  return below < n && below * each <= room && delta_chunks_fit(p, elem, start, n, rows) ? 0 : least;
+}
+
 template <class T>
 static int delta_seq_run(const frhip_delta& p, const DeltaCall& c, int nseq, const int32_t* start, void* workspace, hipStream_t st) {
   DeltaArgs<T> a = delta_args<T>(p, c);
@@ -225,10 +280,8 @@ static int delta_seq_run(const frhip_delta& p, const DeltaCall& c, int nseq, con
     a.state_out = c.state_out + (size_t)s0 * per;
     DeltaTable tab;
     memset(&tab, 0, sizeof(tab));
-    int many[kSeqTable], nmany = 0, least = kDeltaChunkLeast;
-    // Where some go chunk by chunk in any case, so do the short ones, if the scratch has room: a launch less (nine prompts, of 1, 2 and no rows too:
-    // 52 -> 47 us)
-    if (delta_chunks_fit(p, sizeof(T), start + s0, n, rows)) least = 0;
+    const int least = chunk_least(p, start + s0, n, sizeof(T), rows);
+    int many[kSeqTable], nmany = 0;
     a.nseq = 0;
     for (int i = 0; i < n; i++) {
       const int from = start[s0 + i], to = start[s0 + i + 1];
@@ -245,7 +298,7 @@ static int delta_seq_run(const frhip_delta& p, const DeltaCall& c, int nseq, con
       return lx != ly ? lx > ly : x < y;
     });
     if (a.nseq)
-      if (int rc = step_launch<T, 8, false>(a, tab, a.nseq, st)) return rc;
+      if (int rc = step_launch<T, 4, false>(a, tab, a.nseq, st)) return rc;
     if (nmany)
       if (int rc = delta_chunk_run<T>(a, many, nmany, start + s0, rows, workspace, st)) return rc;
   }
