@@ -100,21 +100,34 @@ struct KeyTile {
   h8 f[KS][kParts<T>];
   float squares, power;
   bool finite;
+  typedef T any8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  any8 v[KS];  // as it is in memory
+
+  // All requests of a row go out together: of whole groups they have no branches, where the compiler waits for what is on its way
+  __device__ __forceinline__ void request(const T* rows, size_t ld, int row0, int nrows, int dk) {
+    const int lane = threadIdx.x & 63, row = row0 + (lane & 15), d0 = (lane >> 4) * 8;
+    const T* const p = rows + (size_t)(row < nrows ? row : 0) * ld;
+    if (dk % 8 == 0) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) v[ks] = *reinterpret_cast<const any8*>(p + (ks * 32 + d0 < dk ? ks * 32 + d0 : 0));
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[ks][i] = ks * 32 + d0 + i < dk ? p[ks * 32 + d0 + i] : (T)0.f;
+    }
+  }
 
   template <bool SCALED>
-  __device__ __forceinline__ void load(const T* rows, size_t ld, int row0, int nrows, int dk) {
-    const int lane = threadIdx.x & 63, row = row0 + (lane & 15), d0 = (lane >> 4) * 8;
-    const bool there = row < nrows;
-    const T* const p = rows + (size_t)(there ? row : 0) * ld;
+  __device__ __forceinline__ void take(int row0, int nrows, int dk) {
+    const int lane = threadIdx.x & 63, d0 = (lane >> 4) * 8;
+    const bool there = row0 + (lane & 15) < nrows;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+      if (!there || ks * 32 + d0 >= dk) v[ks] = (any8){};
     squares = 0.f;
     if constexpr (kParts<T> == 2) {
-      float v[KS][8];
       uint32_t top = 0;
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const int d = ks * 32 + d0;
-        load_group<T, 8>(v[ks], p + (d < dk ? d : 0), there ? dk - d : 0);
-      }
 #pragma unroll
       for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -136,19 +149,8 @@ struct KeyTile {
         }
       squares = add_across_32(add_across_16(squares));
     } else {
-      typedef h1 any8 __attribute__((ext_vector_type(8), aligned(2)));
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const int d = ks * 32 + d0, n = there ? dk - d : 0;
-        h8 x = {};
-        if (n >= 8) {
-          x = *reinterpret_cast<const any8*>(p + d);
-        } else if (n > 0) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) x[i] = i < n ? p[d + i] : (h1)0.f;
-        }
-        f[ks][0] = x;
-      }
+      for (int ks = 0; ks < KS; ks++) f[ks][0] = v[ks];
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) squares = dot8acc(f[ks][0], f[ks][0], squares);
       squares = add_across_32(add_across_16(squares));
@@ -235,18 +237,20 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
   char* const out = heads + ((size_t)head * gridDim.x + cj) * Out::bytes;  // a head's chunks one behind the other: pages stay
   const int row = w * 16 + c, r0 = w * 16 + g * 4;  // the lane's row of an operand, the first one of results
   KeyTile<T, KS> K, Q;
-  K.template load<true>(a.k + (size_t)t0 * a.ldk + (size_t)kh * a.dk, a.ldk, w * 16, len, a.dk);
-  Q.template load<false>(a.q + (size_t)t0 * a.ldq + (size_t)kh * a.dk, a.ldq, w * 16, len, a.dk);
+  K.request(a.k + (size_t)t0 * a.ldk + (size_t)kh * a.dk, a.ldk, w * 16, len, a.dk);
+  Q.request(a.q + (size_t)t0 * a.ldq + (size_t)kh * a.dk, a.ldq, w * 16, len, a.dk);
   const bool there = lane < len;  // wave 0: a lane a row
-  float rate = 1.f, bias = 0.f, dt = 0.f, raw = 0.f;
+  float rate = 1.f, bias = 0.f;
+  T dt = (T)0.f, raw = (T)0.f;
   if (w == 0) {
-    if (a.A) rate = finite_rate(a.A[head]);
+    const int t = t0 + min(lane, len - 1);
+    dt = a.dt[(size_t)t * a.lddt + head];
+    raw = a.beta[(size_t)t * a.ldbeta + head];
+    if (a.A) rate = a.A[head];
     if (a.dt_bias) bias = a.dt_bias[head];
-    if (there) {
-      dt = (float)a.dt[(size_t)(t0 + lane) * a.lddt + head];
-      raw = (float)a.beta[(size_t)(t0 + lane) * a.ldbeta + head];
-    }
   }
+  K.template take<true>(w * 16, len, a.dk);
+  Q.template take<false>(w * 16, len, a.dk);
 #pragma unroll
   for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -285,8 +289,8 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
     }
   }
   if (w == 0) {
-    const float lg = log_decay(a, dt, rate, bias), fk = lds.fk[lane];
-    float b = there ? (a.sigmoid ? sigmoid_f<true>(raw) : raw) : 0.f;
+    const float lg = log_decay(a, (float)dt, finite_rate(rate), bias), fk = lds.fk[lane];
+    float b = there ? (a.sigmoid ? sigmoid_f<true>((float)raw) : (float)raw) : 0.f;
     const unsigned long long off = __ballot(there && (magnitude(fk) >= kNotFinite || magnitude(b) >= kNotFinite || !(lg < __builtin_inff())));
     const int bad = off ? __builtin_ctzll(off) : kChunk;
     double G = there && lane < bad ? (double)__builtin_fmaxf(lg, kLeastLog) : 0.0;
