@@ -224,6 +224,7 @@ struct PrepLds {
 };
 
 // blockIdx.x: a chunk, blockIdx.y: a head.  Wave w has the rows 16 w to 16 w + 15 of K, Q, L and P, those columns of T, and a quarter of W; wave 0 the gates.
+// 4096 rows of 32 heads 128 x 128 of binary16: 42 us, four workgroups a compute unit (LDS), bound by instructions: 1500 of vectors a wave, half of the cycles.
 template <class T, int KS>
 __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 ? 2 : 1) void delta_prep_kernel(DeltaArgs<T> a, DeltaTable tab, char* keys, char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;
@@ -574,6 +575,9 @@ __device__ __forceinline__ float of_lane(float f) { return __uint_as_float(__bui
 //   |R| <= max |b v| + key max |S|,   key = max_i |b_i a_i0| |k_i|_1
 //   |S'| <= a_C0 max |S| + back max |b v| + both max |S|,   back = max_d sum_i |W_di|,   both = max_d sum_i |W_di| |b_i a_i0| |k_i|_1
 // They may be 2^16 too high before a pair holds a column's largest value to less than fp32 does.
+//
+// 4096 rows of 32 heads 128 x 128 of binary16: 111 us, 1.7 a chunk, 140 where operands and rows come from memory.  Of these the dependent steps take 60 by
+// themselves; 76 KB of operands a chunk add 39, at 45 bytes a cycle and compute unit, rows of v and y ten.
 template <class T, int KS>
 __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;  // ST: tiles of 16 rows of S of a wave

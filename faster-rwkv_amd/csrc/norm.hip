@@ -202,7 +202,7 @@ struct ResidualArgs {
 
 // A row of at most 512 elements a wave (WIDE: a workgroup, G groups of eight a thread); blockIdx.x, and so on by gridDim.x: the rows.  A row's
 // loads go out ahead of the sums of the row before.
-// 4096 rows of 2560, two norms, a gate, a stream in fp32: 35 us, 4.2 TB/s; about thirteen workgroups of five waves a compute unit (six: 37).
+// 4096 rows of 2560, two norms, a gate, a stream in fp32: 35 us, 4.2 TB/s; twelve workgroups of five waves a compute unit (six: 37).
 template <class S, class T, int G, bool WIDE>
 __global__ __launch_bounds__(WIDE ? 1024 : 256) void norm_residual_kernel(ResidualArgs<S, T> a) {
   constexpr bool FINE = sizeof(S) == 4 || sizeof(T) == 4;

@@ -423,8 +423,10 @@ int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int co
  *   q, k = q[t], k[t] / sqrt(sum of their squares + norm_eps)      (norm_eps negative: as they are)
  *   S = a S + b k (v[t][h] - a S^T k)^T
  *   y[t][h] = scale S^T q
- * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (up to 88 is computed; minus infinity
- * forgets).  q and k are rows of key_heads * key_dim, v and y of heads * value_dim, dt and beta of heads.  state
+ * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (where some are, their sums over up to
+ * 64 rows are computed up to 88; minus infinity forgets).  The largest element of a q or k lies between 1e-15 and 1e15, or it is zero (their
+ * squares are fp32); norm_eps zero makes 0 / 0 of a vector of zeros.  What is not finite stays in its column of S (a value), its head (a key,
+ * dt, beta) or its row of y (a query), from its token on, where results are not finite either.  q and k are rows of key_heads * key_dim, v and y of heads * value_dim, dt and beta of heads.  state
  * [.][heads][key_dim][value_dim] fp32.  Dimensions 1 to 256, up to 65535 heads; heads * value_dim, key_heads * key_dim
  * and pitches up to 2^23. */
 typedef struct frhip_delta {
@@ -436,13 +438,15 @@ typedef struct frhip_delta {
 int frhip_delta_one(const frhip_delta *p, int rows, const void *q, int ldq, const void *k, int ldk, const void *v, int ldv, const void *dt, int lddt,
                     const void *beta, int ldbeta, const float *state, float *state_out, void *y, int ldy, int dtype, frhip_stream s);
 /* Scratch of frhip_delta_seq for T rows in nseq prompts: bytes (may be 0), 16-byte aligned, owned by the caller; calls that can
- * run at the same time need one each.  One for more rows serves fewer, in however many prompts. */
+ * run at the same time need one each.  One for more rows serves fewer, in however many prompts.  The same call gives
+ * the same bits; beside other prompts a prompt may go by the other of two forms (token by token, 64 rows at once), whose roundings differ. */
 size_t frhip_delta_workspace_bytes(const frhip_delta *p, int nseq, int T);
 int frhip_delta_seq(const frhip_delta *p, int nseq, const int32_t *seq_start, const void *q, int ldq, const void *k, int ldk, const void *v, int ldv,
                     const void *dt, int lddt, const void *beta, int ldbeta, const float *state, float *state_out, void *y, int ldy, int dtype,
                     void *workspace, frhip_stream s);
 
-/* Norms: v / sqrt(mean of v^2 + eps), FRHIP_NORM_MEAN of v less its mean.  Evaluated in fp32 (so are the squares), rounded once. */
+/* Norms: v / sqrt(mean of v^2 + eps), FRHIP_NORM_MEAN of v less its mean.  Evaluated in fp32, rounded once.  So are the squares: values of a row are
+ * below 1e18, and where eps is zero some are above 1e-18 (a row of zeros is 0 / 0 then). */
 #define FRHIP_NORM_NONE 0
 #define FRHIP_NORM_RMS 1
 #define FRHIP_NORM_MEAN 2
