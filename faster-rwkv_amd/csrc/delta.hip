@@ -173,6 +173,7 @@ static int delta_check_params(const frhip_delta* p) {
   if ((long long)p->heads * p->value_dim > kMostPitch || (long long)p->key_heads * p->key_dim > kMostPitch)
     return set_error(FRHIP_ESHAPE, "delta: a row may have up to 2^23 elements");
   if (off_grid(4, {p->A, p->dt_bias})) return set_error(FRHIP_EINVAL, "delta: pointer not aligned to its element");
+  if (!(p->norm_eps < 3e38f)) return set_error(FRHIP_EINVAL, "delta: norm_eps must be a number, or negative");
   return 0;
 }
 

@@ -63,3 +63,14 @@ def test_a_workspace_for_more_rows_serves_fewer(heads, key_heads, dk, dv):
     p = params(heads=heads, key_heads=key_heads, dk=dk, dv=dv)
     sizes = [fr.lib().frhip_delta_workspace_bytes(p, n, T) for T in [*range(600), 4096, 100000, 1 << 28] for n in (1, 200)]
     assert sizes == sorted(sizes) and sizes[0::2] == sizes[1::2]
+
+
+@pytest.mark.parametrize("seq", [True, False])
+@pytest.mark.parametrize("eps", [float("nan"), float("inf")])
+def test_an_eps_that_is_no_number(eps, seq):
+    assert delta(seq, p=dict(eps=eps)) == EINVAL
+
+
+def test_a_workspace_that_is_not_there_or_off_its_grid():
+    for ws in (None, 11 * A + 8):
+        assert delta(at=starts(0, 100), ws=ws, q=3 * A, k=13 * A) == EINVAL
