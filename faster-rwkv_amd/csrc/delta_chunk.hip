@@ -8,9 +8,11 @@
 // P and W do not depend on S: a first launch finds them for all chunks at once; a second one walks the chunks of a prompt, a head and 16 columns of S
 // a workgroup, with two products a chunk that wait for each other: [K; Q] S and [W; P] R.
 //
-// The products multiply binary16 with fp32 sums.  What is fp32 goes in as a pair hi + lo, 22 bits and more, scaled by a power of two: rows of W and P, of q
-// and k where they are fp32, columns of S and R.  Rows of k go in as they are but for a power of two, binary16 exactly, those of q as they are, and their
-// lengths are made good behind the products.
+// The products multiply binary16 with fp32 sums.  What is fp32 goes in as a pair hi + lo, scaled by a power of two: rows of W and P, of q
+// and k where they are fp32, columns of S and R.  Where a row or column has decays in it (W, P, R, S) lo goes in times 2^11, in sums of its own: a pair is
+// 22 bits and more of what is within 2^29 of the largest, and off by 2^-51 of that below it (without the 2^11, 2^18 and 2^-40).  Where rows of R are so far below
+// their column's bound that results would show it, they go token by token (see the scan).
+// Rows of k go in as they are but for a power of two, those of q as they are, and their lengths are made good behind the products.
 #include <algorithm>
 #include <climits>
 #include <cstring>
@@ -30,7 +32,7 @@ constexpr float kLeastLog = -1e4f;  // of a row's decay, which is zero there; su
 constexpr int kBlockBytes = 2 * 64 * 16;
 __device__ __forceinline__ constexpr int block_of(int tile, int ks) { return (tile == 3 ? 4 : tile) + ks; }  // of P; its tiles 0 and 1 have one
 constexpr int kTriBytes = 6 * kBlockBytes;
-enum { kRowBeta, kRowK, kRowQ, kRowP, kRowKinds };
+enum { kRowBeta, kRowK, kRowQ, kRowP, kRowKeep, kRowKinds };  // kRowKeep: a row's own decay; -1 for none, or from what is not finite on
 struct ChunkBounds {
   float key, back, both;  // see the scan
   float keep;             // the decay of the whole chunk
@@ -66,10 +68,12 @@ __device__ __forceinline__ uint32_t max_across_rows(uint32_t v) {
   const auto s = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   return max((uint32_t)s[0], (uint32_t)s[1]);
 }
-// A power of two that takes what is not above `bound` (its bits, sign off) below 2^15, and its reciprocal.  For no bound that is finite: any
+constexpr int kLoBits = 11;
+constexpr float kLoUp = 1 << kLoBits, kLoDown = 1.f / kLoUp;
+// A power of two (kLoUp times which is a number) that takes what is not above `bound` (its bits, sign off) below 2^15, and its reciprocal.  For no bound that is finite: any
 __device__ __forceinline__ float scale_for(uint32_t bound) {
   const int field = 268 - (int)(bound >> 23);
-  return __uint_as_float((uint32_t)min(field, 253) << 23);
+  return __uint_as_float((uint32_t)min(field, 253 - kLoBits) << 23);
 }
 __device__ __forceinline__ float inverse_of(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
@@ -180,6 +184,23 @@ struct KeyTile {
   }
 };
 
+// Values as hi + lo 2^-kLoBits, from 2^kLoBits times them
+__device__ __forceinline__ void split_far(const f32x4& up, h4& hi, h4& lo) {
+  f32x4 v = up * kLoDown;
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    asm("" : "+v"(v[i]), "+v"(v[i + 1]));  // (or the compiler finds hi twice, by itself and for lo)
+    const h2 h = __builtin_convertvector((f32x2){v[i], v[i + 1]}, h2);
+    hi[i] = h[0], hi[i + 1] = h[1];
+    lo[i] = (h1)__builtin_fmaf((float)h[0], -kLoUp, up[i]);
+    lo[i + 1] = (h1)__builtin_fmaf((float)h[1], -kLoUp, up[i + 1]);
+  }
+}
+__device__ __forceinline__ float join(float hi, float lo) { return __builtin_fmaf(lo, kLoDown, hi); }
+__device__ __forceinline__ f32x4 join(const f32x4& hi, const f32x4& lo) {
+  return (f32x4){join(hi[0], lo[0]), join(hi[1], lo[1]), join(hi[2], lo[2]), join(hi[3], lo[3])};
+}
+
 constexpr int kLd = kChunk + 4;  // of an fp32 matrix in LDS: 16 rows, 16 bytes each, are on all banks
 constexpr int kLdT = kChunk + 8;
 
@@ -190,12 +211,13 @@ __device__ __forceinline__ h4 read_columns(const h1* p) {
   return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(void*)p));
 }
 
-// Operands of a block and its row's power, of two tiles of results whose rows are its columns
+// Operands of a block, of its row's power, of two tiles of results whose rows are its columns
 __device__ __forceinline__ void store_block(char* to, const f32x4& a, const f32x4& b, float power) {
   const int lane = threadIdx.x & 63;
+  const float up = power * kLoUp;
   h4 h[2], l[2];
-  split(a * power, h[0], l[0]);
-  split(b * power, h[1], l[1]);
+  split_far(a * up, h[0], l[0]);
+  split_far(b * up, h[1], l[1]);
   reinterpret_cast<h8*>(to)[lane] = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
   reinterpret_cast<h8*>(to)[64 + lane] = __builtin_shufflevector(l[0], l[1], 0, 1, 2, 3, 4, 5, 6, 7);
 }
@@ -309,6 +331,7 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
     rows[kRowBeta * kChunk] = b;
     rows[kRowK * kChunk] = key;
     rows[kRowQ * kChunk] = lds.fq[lane] * from;
+    rows[kRowKeep * kChunk] = there && lane < bad ? decay_f(lg) : -1.f;
     const float reach = __builtin_fabsf(key) * lds.length[lane], bkey = max_across_rows(most_of_16(reach));
     lds.length[lane] = reach;
     if (lane == 63) {
@@ -509,6 +532,8 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
 // ---------------------------------------------------------------------------
 // Second launch: the chunks of a prompt one after another
 // ---------------------------------------------------------------------------
+constexpr float kLeastSize = 0x1p-15f * kLoUp;  // see the scan
+
 // LDS alone: loads that are on their way to registers stay on it
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -525,6 +550,8 @@ struct ScanLds {
   float most[16][20];                              // of S, of each lane's rows
   uint32_t vmost[16][4];                           // of b v of the next chunk (as bits, which tell what is not finite)
   float cols[16][2], rinv[16];                     // of each column: the largest b v, the decay of the chunk (or NaN: see spoilt); R's inverse power
+  float sums[2][5][16][4];                         // of a row that goes token by token and the next one, of waves 0 to 3
+  int gone[4], far;                                // rows that go token by token; the last chunk that has rows of R or columns of S far below their bounds
 };
 
 // Where the eight rows from 8 b on of column c are in S (64 rows and more) and R: rows of 16 bytes, 16 of which are on all banks, change places
@@ -559,6 +586,9 @@ __device__ __forceinline__ void store_row(__amdgpu_buffer_rsrc_t rows, uint32_t 
   else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), rows, at, 0, 0);
 }
 
+// The lane, found anew: where it is seldom needed, so that nothing that is made of it stays in registers until then
+__device__ __forceinline__ int this_lane() { return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+
 // Four rows' factors of the one that each lane of a quad requested
 __device__ __forceinline__ f32x4 of_quad(float f) { return (f32x4){dpp_mov<0x00>(f), dpp_mov<0x55>(f), dpp_mov<0xAA>(f), dpp_mov<0xFF>(f)}; }
 template <int LANE>
@@ -574,12 +604,20 @@ __device__ __forceinline__ float of_lane(float f) { return __uint_as_float(__bui
 // The powers of two by which columns are scaled come from bounds, of S ahead of its values (without waiting for the other waves' ones):
 //   |R| <= max |b v| + key max |S|,   key = max_i |b_i a_i0| |k_i|_1
 //   |S'| <= a_C0 max |S| + back max |b v| + both max |S|,   back = max_d sum_i |W_di|,   both = max_d sum_i |W_di| |b_i a_i0| |k_i|_1
-// They may be 2^16 too high before a pair holds a column's largest value to less than fp32 does.
+// They may be 2^27 too high before a pair holds a column's largest value to less than fp32 does.
+//
+// The 64 rows of a column of R share a power, so one that is 2^-s of the bound is off by 2^(s - 51) of itself, and by as much in the results of a row is what
+// W's and P's pairs make of those ahead of it.  It shows where nothing of a row's own size stands behind it: ahead of a value that is far above the others, and
+// behind one (or a state) that has been forgotten.  So a row i whose size, the largest a_ij max(|R_j|, |b_j v_j|) of the rows up to it, is below 2^-29 of the bound or
+// so, and all ahead of it, go token by token from S (far_rows, walk); others are off by 2^-20 of their size at most for each row that is at the bound,
+// no more than fp32's roundings of 64 products.  So do all rows of a chunk whose S is 2^27 and more below its bound, which is too high where a value was
+// forgotten in the chunk before.  Only chunks with a row of R that is that low look for them, hardly any of a layer's ordinary values (without the 2^11
+// it would be one in some hundred); a look takes 1 us, a row 0.8 to 2.6 (64 to 256 keys).
 //
 // 4096 rows of 32 heads 128 x 128 of binary16: 111 us, 1.7 a chunk, 140 where operands and rows come from memory.  Of these the dependent steps take 60 by
 // themselves; 76 KB of operands a chunk add 39, at 45 bytes a cycle and compute unit, rows of v and y ten.
 template <class T, int KS>
-__global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
+__global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;  // ST: tiles of 16 rows of S of a wave
   typedef ScanLds<T, KS> Lds;
   typedef HeadLayout<KS> In;
@@ -595,6 +633,10 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
   const size_t nall = tab.chunk[a.nseq];
   const bool mine = col0 + c < a.dv;
   const int col = mine ? col0 + c : a.dv - 1;
+  // Whether rows of chunk j are far below their bounds, behind the barrier behind R; and how many go token by token, behind two more
+  auto is_far = [](int seen, int j) { return __builtin_expect(__builtin_amdgcn_readfirstlane(seen) == j, 0); };  // lds.far
+  auto gone_of = [&] { return max(max(__builtin_amdgcn_readfirstlane(lds.gone[0]), __builtin_amdgcn_readfirstlane(lds.gone[1])),
+                                  max(__builtin_amdgcn_readfirstlane(lds.gone[2]), __builtin_amdgcn_readfirstlane(lds.gone[3]))); };
   if (nchunk == 0) {  // no rows: the state as it was
     const float* const from = a.state;
     const size_t st = ((size_t)tab.seq[i0] * a.heads + head) * a.dk * a.dv;
@@ -646,6 +688,116 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
 #pragma unroll
     for (int t = 0; t < ST; t++) load_back(here, t);
     f32x4 S[ST];
+    auto most_of_S = [&] {
+      float m = 0.f;
+#pragma unroll
+      for (int t = 0; t < ST; t++) m = larger(m, most_of(S[t]));
+      lds.most[c][w * 4 + g] = m;
+    };
+    // How many rows of chunk j, up to the last one that must, are to go token by token; all of them if a lane says so.  What a row is off by is carried on like its size, and grows with decays
+    // that do.  A lane's rows are taken together, then the wave's, then those of all four.
+    auto far_rows = [&](int j, const f32x4& size, bool every, int len) {
+      const int lane = this_lane(), c = lane & 15, g = lane >> 4;
+      const f32x4 keep = *reinterpret_cast<const f32x4*>(heads + (head * nall + first + j) * head_step + In::rows + (kRowKeep * kChunk + w * 16 + g * 4) * 4);
+      float s[4], o[4], k[4];  // of its rows by themselves: size, what they are off by, and what is left of a size ahead of them
+      auto of_row = [&](int r) { return keep[r] < 0.f ? __builtin_inff() : size[r]; };
+      s[0] = of_row(0), o[0] = 1.f, k[0] = keep[0];
+#pragma unroll
+      for (int r = 1; r < 4; r++) s[r] = larger(of_row(r), keep[r] * s[r - 1]), o[r] = larger(1.f, keep[r] * o[r - 1]), k[r] = keep[r] * k[r - 1];
+      float S1 = s[3], O1 = o[3], K1 = k[3];
+#pragma unroll
+      for (int m = 16; m < 64; m *= 2) {
+        const float sm = __shfl_up(S1, m), om = __shfl_up(O1, m), km = __shfl_up(K1, m);
+        if (lane >= m) S1 = larger(S1, K1 * sm), O1 = larger(O1, K1 * om), K1 *= km;
+      }
+      f32x4* const waves = reinterpret_cast<f32x4*>(&lds.sums[0][0][0][0]);
+      if (g == 3) waves[w * 16 + c] = (f32x4){S1, O1, K1, 0.f};
+      float sa = __shfl_up(S1, 16), oa = __shfl_up(O1, 16), ka = __shfl_up(K1, 16);  // of the rows ahead of the lane's: in the wave
+      if (g == 0) sa = oa = 0.f, ka = 1.f;
+      lds_barrier();
+      float sb = 0.f, ob = 1.f;  // and in those before
+      for (int i = 0; i < w; i++) {
+        const f32x4 m = waves[i * 16 + c];
+        sb = larger(m[0], m[2] * sb), ob = larger(m[1], m[2] * ob);
+      }
+      sa = larger(sa, ka * sb), oa = larger(oa, ka * ob);
+      int rows = __ballot(every) ? len : 0;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float z = larger(s[r], k[r] * sa);
+        const unsigned long long off = __ballot(z > 0.f && z < kLeastSize * larger(o[r], k[r] * oa));
+        if (off) rows = max(rows, w * 16 + (63 - __builtin_clzll(off)) / 16 * 4 + r + 1);
+      }
+      lds.gone[w] = rows;
+      lds_barrier();
+      return gone_of();
+    };
+    // The first rows of chunk j token by token, y and, in LDS, S: each wave has its rows of S, whose sums meet there.  In few registers, and loops that are not
+    // unrolled: what counts is that the chunks that do not come here are not held up.
+    auto state_of = [&](int lane) { return reinterpret_cast<float*>(&lds.S[0][0][0]) + (w * (ST * 16) + (lane >> 4) * 4) * 16 + (lane & 15); };  // [row][column]
+    auto walk = [&](int j, int rows) {
+      const int lane = this_lane(), c = lane & 15, g = lane >> 4, d0 = w * (ST * 16) + g * 4, col = min(col0 + c, a.dv - 1);
+      float* const state = state_of(lane);
+      const float* const factors = reinterpret_cast<const float*>(heads + (head * nall + first + j) * head_step + In::rows);
+      const float keeps = factors[kRowKeep * kChunk + lane], writes = factors[kRowBeta * kChunk + lane];
+#pragma unroll
+      for (int t = 0; t < ST; t++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) state[(t * 16 + r) * 16] = S[t][r];
+#pragma clang loop unroll(disable)
+      for (int i = 0; i < rows; i++) {
+        const size_t t = (size_t)begin + j * kChunk + i;
+        const T* const kr = a.k + t * a.ldk + (size_t)kh * a.dk;
+        const T* const qr = a.q + t * a.ldq + (size_t)kh * a.dk;
+        const float v = (float)a.v[t * a.ldv + (size_t)head * a.dv + col];
+        const float keep = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(keeps), i)), b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(writes), i));
+        float sum[5] = {};  // k k, q q, q k, k S, q S
+#pragma clang loop unroll(disable)
+        for (int e = 0; e < ST * 16; e += 16) {
+          T k[4], q[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const int d = min(d0 + e + r, a.dk - 1);
+            k[r] = kr[d], q[r] = qr[d];
+          }
+#pragma unroll
+          for (int r = 0; r < 4; r++) {
+            const float x = d0 + e + r < a.dk ? (float)k[r] : 0.f, y = d0 + e + r < a.dk ? (float)q[r] : 0.f, s = state[(e + r) * 16];
+            sum[0] = __builtin_fmaf(x, x, sum[0]);
+            sum[1] = __builtin_fmaf(y, y, sum[1]);
+            sum[2] = __builtin_fmaf(y, x, sum[2]);
+            sum[3] = __builtin_fmaf(x, s, sum[3]);
+            sum[4] = __builtin_fmaf(y, s, sum[4]);
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < 5; n++) {
+          const float all = add_across_32(add_across_16(sum[n]));
+          if (g == 0) lds.sums[i & 1][n][c][w] = all;  // the next row's go elsewhere: a barrier a row
+        }
+        lds_barrier();
+#pragma unroll
+        for (int n = 0; n < 5; n++) {
+          const f32x4 m = *reinterpret_cast<const f32x4*>(lds.sums[i & 1][n][c]);
+          sum[n] = (m[0] + m[1]) + (m[2] + m[3]);
+        }
+        float kn = 1.f, qn = a.scale;
+        if (a.eps >= 0.f) {
+          kn = __builtin_amdgcn_rsqf(sum[0] + a.eps);
+          qn = __builtin_amdgcn_rsqf(sum[1] + a.eps) * a.scale;
+        }
+        const float u = kn * (b * (v - keep * kn * sum[3]));
+#pragma clang loop unroll(disable)
+        for (int e = 0; e < ST * 16; e += 16) {
+          T k[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) k[r] = kr[min(d0 + e + r, a.dk - 1)];
+#pragma unroll
+          for (int r = 0; r < 4; r++) state[(e + r) * 16] = __builtin_fmaf(d0 + e + r < a.dk ? (float)k[r] : 0.f, u, keep * state[(e + r) * 16]);
+        }
+        if (w == 0 && g == 0 && col0 + c < a.dv) a.y[t * a.ldy + (size_t)head * a.dv + col] = (T)(qn * __builtin_fmaf(keep, sum[4], sum[2] * u));
+      }
+    };
 #pragma unroll
     for (int t = 0; t < ST; t++)
 #pragma unroll
@@ -653,24 +805,32 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
         const int d = d0 + t * 16 + r;
         S[t][r] = d < a.dk ? from[st + (size_t)d * a.dv + col] : 0.f;
       }
-    auto most_of_S = [&] {
-      float m = 0.f;
-#pragma unroll
-      for (int t = 0; t < ST; t++) m = larger(m, most_of(S[t]));
-      lds.most[c][w * 4 + g] = m;
-    };
     auto most_of_all = [&] { return max_across_rows(most_of(*reinterpret_cast<const f32x4*>(&lds.most[c][g * 4]))); };
     most_of_S();
+    if (threadIdx.x == 0) lds.far = -1;
     lds_barrier();
     float sbound = most_of_all();  // of the column of S; the first chunk's is its own largest value
     lds_barrier();
+    const int last = end - begin - (nchunk - 1) * kChunk;  // rows of the last chunk
+    auto sizes_of = [&](const f32x4& R, const f32x4& bv) {  // of the lane's rows
+      f32x4 size;
+#pragma unroll
+      for (int r = 0; r < 4; r++) size[r] = larger(__builtin_fabsf(R[r]), __builtin_fabsf(bv[r]));
+      return size;
+    };
+    auto sizes_there = [&](f32x4 size) {  // rows behind the last one have none that is too small
+      asm volatile("");  // (a branch: a row's selects would be made of every chunk)
+#pragma unroll
+      for (int r = 0; r < 4; r++) size[r] = row0 + r < last ? size[r] : __builtin_inff();
+      return size;
+    };
     for (int j = 0; j < nchunk; j++) {
       const bool more = j + 1 < nchunk;
-      const float power = scale_for(magnitude(sbound)), sinv = inverse_of(power);
+      const float power = scale_for(magnitude(sbound)), sinv = inverse_of(power), sup = power * kLoUp;
 #pragma unroll
       for (int t = 0; t < ST; t++) {
         h4 hi, lo;
-        split(S[t] * power, hi, lo);
+        split_far(S[t] * sup, hi, lo);
         const int to = place<KS * 32>(c, (d0 + t * 16) / 8) + (g & 1) * 4;
         *reinterpret_cast<h4*>(&lds.S[0][c][to]) = hi;
         *reinterpret_cast<h4*>(&lds.S[1][c][to]) = lo;
@@ -687,7 +847,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
         lo[ks] = *reinterpret_cast<const h8*>(&lds.S[1][c][place<KS * 32>(c, ks * 4 + g)]);
         hi[ks] = *reinterpret_cast<const h8*>(&lds.S[0][c][place<KS * 32>(c, ks * 4 + g)]);
       }
-      const float vm = lds.cols[c][0], keep = lds.cols[c][1];
+      const float vm = lds.cols[c][0];
+      float keep = lds.cols[c][1];
       f32x4 bv = *reinterpret_cast<const f32x4*>(lds.bv[j & 1][w][lane]), kf = of_quad(key);
       const float sm = most_of_all();
       f32x4 s[4];  // hi and lo apart, and both in two sums: a product waits for the one ahead of it
@@ -697,8 +858,15 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
       for (int ks = 0; ks < KS; ks++) {
         s[ks & 1] = mfma_h(Kf[ks][0], lo[ks], s[ks & 1]);
         s[2 + (ks & 1)] = mfma_h(Kf[ks][0], hi[ks], s[2 + (ks & 1)]);
-        if constexpr (NK == 2) s[ks & 1] = mfma_h(Kf[ks][1], hi[ks], s[ks & 1]);
+        if constexpr (NK == 2) s[2 + (ks & 1)] = mfma_h(Kf[ks][1], hi[ks], s[2 + (ks & 1)]);
       }
+      const float reach = __builtin_fmaf(of_lane<0>(limits), sm, vm), rpower = scale_for(magnitude(reach)), rup = rpower * kLoUp;
+      float rinv = inverse_of(rpower);
+      sbound = __builtin_fmaf(of_lane<3>(limits) + of_lane<2>(limits), sm, of_lane<1>(limits) * vm);
+      kf *= sinv * rup;
+      bv *= rup;
+      // A row's least size: none is below that of a column of zeros, all are where S is not zero but more than 2^27 below its bound
+      const float least = magnitude(sm * sup) - 1 < magnitude(0.5f) - 1 ? __builtin_inff() : reach * (rup * (kLeastSize * 0x1p-26f));
       f32x4 q[2];
       q[0] = q[1] = (f32x4){0.f, 0.f, 0.f, 0.f};
       own = more ? own + key_step : own;
@@ -709,37 +877,33 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
         load_step(own, Kf, ks);
         q[0] = mfma_h(Qf[ks][0], lo[ks], q[0]);
         q[1] = mfma_h(Qf[ks][0], hi[ks], q[1]);
-        if constexpr (NK == 2) q[0] = mfma_h(Qf[ks][1], hi[ks], q[0]);
+        if constexpr (NK == 2) q[1] = mfma_h(Qf[ks][1], hi[ks], q[1]);
       }
       in_order();
       load_own(own + queries, Qf);
-      const float rpower = scale_for(magnitude(__builtin_fmaf(of_lane<0>(limits), sm, vm))), rinv = inverse_of(rpower);
-      sbound = __builtin_fmaf(of_lane<3>(limits) + of_lane<2>(limits), sm, of_lane<1>(limits) * vm);
-      kf *= sinv * rpower;
-      bv *= rpower;
       f32x4 R;
 #pragma unroll
-      for (int r = 0; r < 4; r++) R[r] = __builtin_fmaf(-kf[r], (s[2][r] + s[3][r]) + (s[0][r] + s[1][r]), bv[r]);
+      for (int r = 0; r < 4; r++) R[r] = __builtin_fmaf(-kf[r], join(s[2][r] + s[3][r], s[0][r] + s[1][r]), bv[r]);
       h4 rhi, rlo;
-      split(R, rhi, rlo);
+      split_far(R, rhi, rlo);
       *reinterpret_cast<h4*>(&lds.R[0][c][at_row]) = rhi;
       *reinterpret_cast<h4*>(&lds.R[1][c][at_row]) = rlo;
+      f32x4 size = sizes_of(R, bv);
+      if (!more) size = sizes_there(size);
+      if (__builtin_expect(__ballot(__builtin_fminf(__builtin_fminf(size[0], size[1]), __builtin_fminf(size[2], size[3])) < least) != 0, 0)) lds.far = j;
       load_key(here);
       lds_barrier();
+      const int seen = lds.far;
       h8 rh[2], rl[2];
 #pragma unroll
       for (int ks = 0; ks < 2; ks++) {
         rl[ks] = *reinterpret_cast<const h8*>(&lds.R[1][c][place<kChunk>(c, ks * 4 + g)]);
         rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][place<kChunk>(c, ks * 4 + g)]);
       }
-      *reinterpret_cast<f32x4*>(lds.qs[w][lane]) = (q[1] + q[0]) * sinv;
+      in_order();
+      *reinterpret_cast<f32x4*>(lds.qs[w][lane]) = join(q[1], q[0]) * sinv;
       if (w == 0 && g == 0) lds.rinv[c] = rinv;
       f32x4 rw[ST], ws[ST][2];
-#pragma unroll
-      for (int t = 0; t < ST; t++) {
-        rw[t] = of_quad(scale[t]) * rinv;
-        S[t] *= keep;
-      }
 #pragma unroll
       for (int t = 0; t < ST; t++) {
         ws[t][0] = ws[t][1] = (f32x4){0.f, 0.f, 0.f, 0.f};
@@ -750,12 +914,42 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
           ws[t][0] = mfma_h(Wf[t][ks][1], rh[ks], ws[t][0]);
         }
       }
+      if (is_far(seen, j)) {
+        const int lane = this_lane(), c = lane & 15, at = place<kChunk>(c, (w >> 1) * 4 + (lane >> 4)) + (w & 1) * 4;
+        const h4 hi = *reinterpret_cast<const h4*>(&lds.R[0][c][at]), lo = *reinterpret_cast<const h4*>(&lds.R[1][c][at]);
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds.bv[j & 1][w][lane]) * (inverse_of(rinv) * kLoUp);
+        f32x4 Rj;  // what has become zero in a pair may have been less than nothing else is
+#pragma unroll
+        for (int r = 0; r < 4; r++) Rj[r] = larger(__builtin_fabsf(join((float)hi[r], (float)lo[r]) * kLoUp), 0x1p-60f);
+        f32x4 size = sizes_of(Rj, v);
+        const bool some = least > 0.f && most_of_all() < __builtin_inff();  // not a column of zeros, and finite
+        if (!some) size = (f32x4){} + __builtin_inff();
+        const int len = more ? kChunk : last, gone = far_rows(j, size, some && least == __builtin_inff(), len);
+        if (gone > 0) walk(j, gone);
+        if (gone == len) {  // S is that behind the chunk, to which nothing is left to add
+#pragma unroll
+          for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) S[t][r] = state_of(lane)[(t * 16 + r) * 16];
+          if (keep == keep) keep = 1.f;
+          rinv = 0.f;
+          most_of_S();
+        }
+        lds_barrier();
+        if (gone == len) sbound = most_of_all();
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // all that is on its way: what follows need not wait for more than it does without this
+      }
+#pragma unroll
+      for (int t = 0; t < ST; t++) {
+        rw[t] = of_quad(scale[t]) * rinv;
+        S[t] *= keep;
+      }
       in_order();
       load_back(here, 0);
 #pragma unroll
       for (int t = 0; t < ST; t++) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) S[t][r] = __builtin_fmaf(rw[t][r], ws[t][1][r] + ws[t][0][r], S[t][r]);
+        for (int r = 0; r < 4; r++) S[t][r] = __builtin_fmaf(rw[t][r], join(ws[t][1][r], ws[t][0][r]), S[t][r]);
       }
     }
     lds_barrier();
@@ -846,7 +1040,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
   lds_barrier();
   // Of the chunk before: its P R, its rows' factors, its first row that is not finite.  Its y is made while the next one's K S is.
   f32x4 yp = {0.f, 0.f, 0.f, 0.f}, yt = yp, yq = yp;
-  int none = kChunk;
+  int none = kChunk, gone = 0;  // gone: rows that went token by token, whose y is there
   auto finish = [&](int t0, int nrows) {
     const f32x4 qs = *reinterpret_cast<const f32x4*>(lds.qs[w][lane]);
     const float rinv = lds.rinv[c];
@@ -860,7 +1054,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
     }
     const auto rows = rows_of(a.y + (size_t)t0 * a.ldy + (size_t)head * a.dv, nrows, a.ldy);
 #pragma unroll
-    for (int r = 0; r < 4; r++) store_row<T>(rows, yat[r], (T)y[r]);
+    for (int r = 0; r < 4; r++) store_row<T>(rows, row0 + r < gone ? ~0u : yat[r], (T)y[r]);
   };
   int t0 = begin;
   for (int j = 0; j < nchunk; j++, t0 += kChunk) {
@@ -891,8 +1085,15 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(DeltaArgs<T> a, DeltaTa
     yq = of_quad(query);
     yt = of_quad(tri);
     load_tri(ahead);
-    yp = p[1] + p[0];
+    yp = join(p[1], p[0]);
     ahead = far;
+    gone = 0;
+    if (is_far(lds.far, j)) {  // the same barriers as waves 0 to 3
+      lds_barrier();
+      lds_barrier();
+      gone = gone_of();
+      for (int i = 0; i <= gone; i++) lds_barrier();
+    }
   }
   lds_barrier();
   finish(t0 - kChunk, end - (t0 - kChunk));
