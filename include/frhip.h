@@ -424,7 +424,7 @@ int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int co
  *   S = a S + b k (v[t][h] - a S^T k)^T
  *   y[t][h] = scale S^T q
  * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (where some are, their sums over up to
- * 64 rows are computed up to 88; minus infinity forgets).  The largest element of a q or k lies between 1e-15 and 1e15, or it is zero (their
+ * 64 rows may reach 80, and what grows with them stays in fp32; minus infinity forgets).  The largest element of a q or k lies between 1e-15 and 1e15, or it is zero (their
  * squares are fp32); norm_eps zero makes 0 / 0 of a vector of zeros.  A result is as exact as an fp32 sum of its own terms, whatever values, states and
  * decays the rows around it have, S^T k and S^T q relative to the largest element of their column of S, and of keys as they are (norm_eps negative) those
  * whose lengths are within 2^24 of each other in any 64 rows.  What is not finite stays in its column of S (a value), its head (a key,
