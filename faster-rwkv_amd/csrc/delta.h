@@ -37,11 +37,8 @@ struct DeltaTable {
   int ahead;                             // the first one goes on from what an earlier launch left in state_out
 };
 
-// exp(g) for the logarithm of a decay: below -120 it is zero in fp32, above 88 it stays there
-__device__ __forceinline__ float decay_f(float g) {
-  const float a = exp_neg_fine(__builtin_fmaxf(__builtin_fminf(-g, 120.f), -88.f));
-  return g == g ? a : g;
-}
+// exp(g) for the logarithm of a decay, which is a number: below -120 it is zero in fp32, above 88 it stays there
+__device__ __forceinline__ float decay_f(float g) { return exp_neg_fine(__builtin_fmaxf(__builtin_fminf(-g, 120.f), -88.f)); }
 
 // The logarithm of a row's decay.  A rate of minus infinity stays a number (times a step of width zero it keeps the state).
 template <class T>

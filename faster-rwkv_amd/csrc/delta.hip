@@ -90,7 +90,8 @@ __global__ __launch_bounds__(256) void delta_step_kernel(DeltaArgs<T> a, DeltaTa
   };
   auto gates = [&](int t) {
     const float dt = (float)a.dt[(size_t)t * a.lddt + head], raw = (float)a.beta[(size_t)t * a.ldbeta + head];
-    keeps = decay_f(log_decay(a, dt, rate, bias));
+    const float log = log_decay(a, dt, rate, bias);
+    keeps = log < __builtin_inff() ? decay_f(log) : __builtin_nanf("");  // one that grows without end is no number, as chunk by chunk
     writes = a.sigmoid ? sigmoid_f<true>(raw) : raw;
   };
   for (int i = blockIdx.y; i < nseq; i += gridDim.y) {
