@@ -447,8 +447,8 @@ int frhip_delta_seq(const frhip_delta *p, int nseq, const int32_t *seq_start, co
                     const void *dt, int lddt, const void *beta, int ldbeta, const float *state, float *state_out, void *y, int ldy, int dtype,
                     void *workspace, frhip_stream s);
 
-/* Norms: v / sqrt(mean of v^2 + eps), FRHIP_NORM_MEAN of v less its mean.  Evaluated in fp32, rounded once.  So are the squares: values of a row are
- * below 1e18, and where eps is zero some are above 1e-18 (a row of zeros is 0 / 0 then). */
+/* Norms: v / sqrt(mean of v^2 + eps), FRHIP_NORM_MEAN of v less its mean.  Evaluated in fp32, rounded once.  So are the sums of squares, of up to 2^15:
+ * values of a row are up to 1e17, and where eps is zero some are above 1e-16 (a row of zeros is 0 / 0 then). */
 #define FRHIP_NORM_NONE 0
 #define FRHIP_NORM_RMS 1
 #define FRHIP_NORM_MEAN 2
