@@ -4,7 +4,6 @@
 //
 // with q and k divided by their length.  S is [key][value] and its columns do not mix: a column of S, v and y is a recurrence of its own.
 #include <algorithm>
-#include <climits>
 #include <cstring>
 
 #include "delta.h"

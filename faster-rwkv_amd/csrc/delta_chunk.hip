@@ -14,7 +14,6 @@
 // their column's bound that results would show it, they go token by token (see the scan).
 // Rows of k go in as they are but for a power of two, those of q as they are, and their lengths are made good behind the products.
 #include <algorithm>
-#include <climits>
 #include <cstring>
 
 #include "delta.h"

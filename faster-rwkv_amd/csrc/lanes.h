@@ -30,14 +30,4 @@ __device__ __forceinline__ float lane_sum(float v) {
   return v;
 }
 
-// Over the lanes of a wave that share lane % STEP, STEP 4 to 64: the lanes of a row of 16 by rotations, then the rows
-template <int STEP>
-__device__ __forceinline__ float stride_sum(float v) {
-  if constexpr (STEP <= 4) v += dpp_mov<0x124>(v);  // row_ror:4
-  if constexpr (STEP <= 8) v += dpp_mov<0x128>(v);  // row_ror:8
-  if constexpr (STEP <= 16) v = add_across_16(v);
-  if constexpr (STEP <= 32) v = add_across_32(v);
-  return v;
-}
-
 }  // namespace frhip
