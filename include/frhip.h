@@ -425,12 +425,12 @@ int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int co
  *   y[t][h] = scale S^T q
  * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (where some are, their sums over up to
  * 64 rows may reach 80, and what grows with them stays in fp32; minus infinity forgets).  The largest element of a q or k lies between 1e-15 and 1e15, or it is zero (their
- * squares are fp32); norm_eps zero makes 0 / 0 of a vector of zeros.  A result is as exact as an fp32 sum of its own terms, whatever values, states and
- * decays the rows around it have, S^T k and S^T q relative to the largest element of their column of S, and of keys as they are (norm_eps negative) those
- * whose lengths are within 2^24 of each other in any 64 rows.  What is not finite stays in its column of S (a value, a state), its head (a key, b,
- * a logarithm of a decay that is plus infinity or no number) or its row of y (a query), from its token on, where results are not finite either.  q and k are rows of key_heads * key_dim, v and y of heads * value_dim, dt and beta of heads.  state
- * [.][heads][key_dim][value_dim] fp32.  Dimensions 1 to 256, up to 65535 heads; heads * value_dim, key_heads * key_dim
- * and pitches up to 2^23. */
+ * squares are fp32); norm_eps zero makes 0 / 0 of a vector of zeros.  A result is as exact as an fp32 sum of its own terms, products of q, k and columns
+ * of S relative to the lengths of these, whatever values, states and decays the rows around it have (of keys as they are, norm_eps negative: if their
+ * lengths are within 2^24 of each other in any 64 rows).  What is not finite stays in its column of S (a value, a state), its head (a key, b, a logarithm of a
+ * decay that is plus infinity or no number) or its row of y (a query), from its token on, where results are not finite either.  q and k are rows of
+ * key_heads * key_dim, v and y of heads * value_dim, dt and beta of heads.  state [.][heads][key_dim][value_dim] fp32.  Dimensions 1 to 256, up to 65535
+ * heads; heads * value_dim, key_heads * key_dim and pitches up to 2^23. */
 typedef struct frhip_delta {
   const float *A, *dt_bias;
   int32_t heads, key_heads, key_dim, value_dim;
