@@ -693,9 +693,9 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
       for (int t = 0; t < ST; t++) m = larger(m, most_of(S[t]));
       lds.most[c][w * 4 + g] = m;
     };
-    // How many rows of chunk j, up to the last one that must, are to go token by token; all of them if a lane says so.  What a row is off by is carried on like its size, and grows with decays
-    // that do.  A lane's rows are taken together, then the wave's, then those of all four.
-    auto far_rows = [&](int j, const f32x4& size, bool every, int len) {
+    // How many rows of chunk j, up to the last one that must, are to go token by token.  What a row is off by is carried on like its size, and grows with
+    // decays that do.  A lane's rows are taken together, then the wave's, then those of all four.
+    auto far_rows = [&](int j, const f32x4& size) {
       const int lane = this_lane(), c = lane & 15, g = lane >> 4;
       const f32x4 keep = *reinterpret_cast<const f32x4*>(heads + (head * nall + first + j) * head_step + In::rows + (kRowKeep * kChunk + w * 16 + g * 4) * 4);
       float s[4], o[4], k[4];  // of its rows by themselves: size, what they are off by, and what is left of a size ahead of them
@@ -720,7 +720,7 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
         sb = larger(m[0], m[2] * sb), ob = larger(m[1], m[2] * ob);
       }
       sa = larger(sa, ka * sb), oa = larger(oa, ka * ob);
-      int rows = __ballot(every) ? len : 0;
+      int rows = 0;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const float z = larger(s[r], k[r] * sa);
@@ -749,7 +749,8 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
         const T* const kr = a.k + t * a.ldk + (size_t)kh * a.dk;
         const T* const qr = a.q + t * a.ldq + (size_t)kh * a.dk;
         const float v = (float)a.v[t * a.ldv + (size_t)head * a.dv + col];
-        const float keep = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(keeps), i)), b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(writes), i));
+        const float keep = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(keeps), i));
+        const float b = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(writes), i));
         float sum[5] = {};  // k k, q q, q k, k S, q S
 #pragma clang loop unroll(disable)
         for (int e = 0; e < ST * 16; e += 16) {
@@ -922,8 +923,8 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
         for (int r = 0; r < 4; r++) Rj[r] = larger(__builtin_fabsf(join((float)hi[r], (float)lo[r]) * kLoUp), 0x1p-60f);
         f32x4 size = sizes_of(Rj, v);
         const bool some = least > 0.f && most_of_all() < __builtin_inff();  // not a column of zeros, and finite
-        if (!some) size = (f32x4){} + __builtin_inff();
-        const int len = more ? kChunk : last, gone = far_rows(j, size, some && least == __builtin_inff(), len);
+        if (!some || least == __builtin_inff()) size = (f32x4){} + (some ? 0x1p-60f : __builtin_inff());
+        const int len = more ? kChunk : last, gone = far_rows(j, size);
         if (gone > 0) walk(j, gone);
         if (gone == len) {  // S is that behind the chunk, to which nothing is left to add
 #pragma unroll

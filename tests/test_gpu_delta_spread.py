@@ -94,3 +94,44 @@ def test_keys_as_they_are_whose_lengths_are_far_apart(dtype, by, turned):
         if turned:
             x[2][::2] *= np.asarray(1 / by, x[2].dtype)
     delta_case(2, 1, 64, 32, [100, 3], dtype, norm=False, change=far)
+
+
+@pytest.mark.parametrize("name", ["dt", "k", "v", None])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_what_is_not_finite_in_a_chunk_whose_state_is_far_below_its_bound(dtype, name):
+    """A value 2^28 above the others is forgotten: the next 64 rows' state is far below what it might have been.  One of them is not finite"""
+    shape, row = (4, 2, 64, 32), 90  # the last head
+
+    def far(x, rates, biases, S):
+        keep_all(x, [(AT + 1, -np.inf)])
+        size = 2.0 ** -14 if dtype == "f16" else 1.0
+        x[2][:] = np.sign(np.asarray(x[2], np.float64) + 1e-30) * size
+        x[2][GUARD + AT] *= np.asarray(2.0 ** 28, np.float64).astype(np.float32)
+        x[4][:] = 9
+        S[:] = 0
+
+    def spoil(x, rates, biases, S):
+        far(x, rates, biases, S)
+        if name == "dt":
+            x[3][GUARD + row, 3] = np.nan
+        elif name == "k":
+            x[1][GUARD + row, 64 + 5] = np.inf  # of heads 2 and 3
+        else:
+            x[2][GUARD + row, 3 * 32 + 7] = np.nan
+    run = dict(dtype=dtype, softplus=0, A=False, bias=False)
+    if name is None:
+        delta_case(*shape, [150], change=far, **run)
+        return
+
+    def look(y, left, starts, x, S0):
+        return y[starts[0]:starts[1]].reshape(150, 4, 32).astype(np.float32), left[0]
+    (clean, want), (y, S) = (delta_case(*shape, [150], change=c, check=look, **run) for c in (far, spoil))
+    ybad, Sbad = np.zeros(y.shape, bool), np.zeros(S.shape, bool)
+    if name == "dt":
+        ybad[row:, 3] = Sbad[3] = True
+    elif name == "k":
+        ybad[row:, 2:] = Sbad[2:] = True
+    else:
+        ybad[row:, 3, 7] = Sbad[3, :, 7] = True
+    assert np.isfinite(clean).all() and np.array_equal(y[~ybad], clean[~ybad]) and np.array_equal(S[~Sbad], want[~Sbad])
+    assert not np.isfinite(y[ybad]).any() and not np.isfinite(S[Sbad]).any()
