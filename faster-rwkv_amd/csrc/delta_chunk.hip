@@ -245,7 +245,7 @@ struct PrepLds {
 };
 
 // blockIdx.x: a chunk, blockIdx.y: a head.  Wave w has the rows 16 w to 16 w + 15 of K, Q, L and P, those columns of T, and a quarter of W; wave 0 the gates.
-// 4096 rows of 32 heads 128 x 128 of binary16: 42 us, four workgroups a compute unit (LDS), bound by instructions: 1500 of vectors a wave, half of the cycles.
+// 4096 rows of 32 heads 128 x 128 of binary16: 45 us, four workgroups a compute unit (LDS), bound by instructions: 1470 of vectors a wave, 60 % of the cycles.
 template <class T, int KS>
 __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 ? 2 : 1) void delta_prep_kernel(DeltaArgs<T> a, DeltaTable tab, char* keys, char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 
 // ---------------------------------------------------------------------------
 // Second launch: the chunks of a prompt one after another
 // ---------------------------------------------------------------------------
-constexpr float kLeastSize = 0x1p-15f * kLoUp;  // see the scan
+constexpr float kLeastSize = 0x1p-12f * kLoUp;  // see the scan
 
 // LDS alone: loads that are on their way to registers stay on it
 __device__ __forceinline__ void lds_barrier() {
@@ -607,14 +607,14 @@ __device__ __forceinline__ float of_lane(float f) { return __uint_as_float(__bui
 //
 // The 64 rows of a column of R share a power, so one that is 2^-s of the bound is off by 2^(s - 51) of itself, and by as much in the results of a row is what
 // W's and P's pairs make of those ahead of it.  It shows where nothing of a row's own size stands behind it: ahead of a value that is far above the others, and
-// behind one (or a state) that has been forgotten.  So a row i whose size, the largest a_ij max(|R_j|, |b_j v_j|) of the rows up to it, is below 2^-29 of the bound or
-// so, and all ahead of it, go token by token from S (far_rows, walk); others are off by 2^-20 of their size at most for each row that is at the bound,
-// no more than fp32's roundings of 64 products.  So do all rows of a chunk whose S is 2^27 and more below its bound, which is too high where a value was
-// forgotten in the chunk before.  Only chunks with a row of R that is that low look for them, hardly any of a layer's ordinary values (without the 2^11
-// it would be one in some hundred); a look takes 1 us, a row 0.8 to 2.6 (64 to 256 keys).
+// behind one (or a state) that has been forgotten.  So a row i whose size, the largest a_ij max(|R_j|, |b_j v_j|) of the rows up to it, is below 2^-26 of the
+// bound or so, and all ahead of it, go token by token from S (far_rows, walk); others are off by 2^-23 of their size at most for each row that is at the bound,
+// as the roundings of 64 fp32 products are.  So do all rows of a chunk whose S is 2^27 and more below its bound, which is too high where a value was
+// forgotten in the chunk before.  Only chunks with a row of R that is that low look for them, hardly any of a layer's ordinary values (without the 2^11 it would
+// be one in some hundred); a look takes 1 us, a row 0.8 to 2.6 (64 to 256 keys).
 //
-// 4096 rows of 32 heads 128 x 128 of binary16: 111 us, 1.7 a chunk, 140 where operands and rows come from memory.  Of these the dependent steps take 60 by
-// themselves; 76 KB of operands a chunk add 39, at 45 bytes a cycle and compute unit, rows of v and y ten.
+// 4096 rows of 32 heads 128 x 128 of binary16: 107 us, 1.7 a chunk, 129 to 137 where operands and rows come from memory.  Vector instructions take 36 % of the
+// cycles, matrix ones 15 %; the rest is the latency of the dependent steps, and of 76 KB of operands a chunk.
 template <class T, int KS>
 __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;  // ST: tiles of 16 rows of S of a wave

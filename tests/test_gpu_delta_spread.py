@@ -98,15 +98,16 @@ def test_keys_as_they_are_whose_lengths_are_far_apart(dtype, by, turned):
 
 @pytest.mark.parametrize("name", ["dt", "k", "v", None])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-def test_what_is_not_finite_in_a_chunk_whose_state_is_far_below_its_bound(dtype, name):
-    """A value 2^28 above the others is forgotten: the next 64 rows' state is far below what it might have been.  One of them is not finite"""
+@pytest.mark.parametrize("above", [25, 28])
+def test_what_is_not_finite_in_a_chunk_whose_state_is_far_below_its_bound(above, dtype, name):
+    """A value far above the others is forgotten: the next 64 rows' state is far below what it might have been.  One of them is not finite"""
     shape, row = (4, 2, 64, 32), 90  # the last head
 
     def far(x, rates, biases, S):
         keep_all(x, [(AT + 1, -np.inf)])
         size = 2.0 ** -14 if dtype == "f16" else 1.0
         x[2][:] = np.sign(np.asarray(x[2], np.float64) + 1e-30) * size
-        x[2][GUARD + AT] *= np.asarray(2.0 ** 28, np.float64).astype(np.float32)
+        x[2][GUARD + AT] *= np.float32(2.0 ** above)
         x[4][:] = 9
         S[:] = 0
 
@@ -135,3 +136,15 @@ def test_what_is_not_finite_in_a_chunk_whose_state_is_far_below_its_bound(dtype,
         ybad[row:, 3, 7] = Sbad[3, :, 7] = True
     assert np.isfinite(clean).all() and np.array_equal(y[~ybad], clean[~ybad]) and np.array_equal(S[~Sbad], want[~Sbad])
     assert not np.isfinite(y[ybad]).any() and not np.isfinite(S[Sbad]).any()
+
+
+@pytest.mark.parametrize("log", [-np.inf, -22, -18, -15])
+@pytest.mark.parametrize("dtype,above", [("f16", 26), ("f32", 24), ("f32", 28), ("f32", 40)])
+def test_many_far_values_that_are_forgotten_together(dtype, above, log):
+    """As many as there are ahead of the rows that forget them: each may show in those"""
+    def far(x, rates, biases, S):
+        keep_all(x, [(40, log)])
+        x[2][:] = np.asarray(x[2], np.float64) * (2.0 ** -12 if dtype == "f16" else 1)
+        x[2][GUARD:GUARD + 40] = np.clip(np.asarray(x[2][GUARD:GUARD + 40], np.float64) * 2.0 ** above, -6e4, 6e4) if dtype == "f16" else x[2][GUARD:GUARD + 40] * np.float32(2.0 ** above)
+        S[:] = 0
+    delta_case(2, 2, 64, 32, [100], dtype, softplus=0, A=False, bias=False, change=far)
