@@ -256,7 +256,7 @@ static int delta_one_run(const frhip_delta& p, const DeltaCall& c, int rows, hip
 
 // Rows, at least, of the prompts of a call that go chunk by chunk.  Either form's time (us), 32 heads 128 x 128, by the rows of each prompt:
 //   one prompt    8: 9 / 17   16: 13 / 16   20: 16 / 16   32: 23 / 17   64: 42 / 17
-//   16 prompts    8: 22 / 77  16: 35 / 77   32: 60 / 77   48: 85 / 78   64: 110 / 78
+//   16 prompts    8: 22 / 77  16: 35 / 77   32: 60 / 77   48: 85 / 79   64: 110 / 80
 // A chunk of few rows costs what a whole one does, which counts where there are more of them than compute units to work on them.  For the same reason short
 // prompts join long ones if they are few: launches that are there anyway take them for nothing (nine prompts of 24 heads 64 x 64, four of them of 31 rows at
 // most: 62 -> 45 us).
