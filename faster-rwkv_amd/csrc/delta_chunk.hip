@@ -548,7 +548,7 @@ struct ScanLds {
   float qs[4][64][4];                              // Q S, of their lanes
   float most[16][20];                              // of S, of each lane's rows
   uint32_t vmost[16][4];                           // of b v of the next chunk (as bits, which tell what is not finite)
-  float cols[16][2], rinv[16];                     // of each column: the largest b v, the decay of the chunk (or NaN: see spoilt); R's inverse power
+  float cols[16][2], inv[16][2];                   // of each column: the largest b v, the decay of the chunk (or NaN: see spoilt); R's inverse power, S's
   float sums[2][5][16][4];                         // of a row that goes token by token and the next one, of waves 0 to 3
   int gone[4], far;                                // rows that go token by token; the last chunk that has rows of R or columns of S far below their bounds
 };
@@ -863,7 +863,8 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
       const float reach = __builtin_fmaf(of_lane<0>(limits), sm, vm), rpower = scale_for(magnitude(reach)), rup = rpower * kLoUp;
       float rinv = inverse_of(rpower);
       sbound = __builtin_fmaf(of_lane<3>(limits) + of_lane<2>(limits), sm, of_lane<1>(limits) * vm);
-      kf *= sinv * rup;
+      kf *= rup;  // (one by one: their product may be no number)
+      kf *= sinv;
       bv *= rup;
       // A row's least size: none is below that of a column of zeros, all are where S is not zero but more than 2^27 below its bound
       const float least = magnitude(sm * sup) - 1 < magnitude(0.5f) - 1 ? __builtin_inff() : reach * (rup * (kLeastSize * 0x1p-26f));
@@ -901,8 +902,8 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
         rh[ks] = *reinterpret_cast<const h8*>(&lds.R[0][c][place<kChunk>(c, ks * 4 + g)]);
       }
       in_order();
-      *reinterpret_cast<f32x4*>(lds.qs[w][lane]) = join(q[1], q[0]) * sinv;
-      if (w == 0 && g == 0) lds.rinv[c] = rinv;
+      *reinterpret_cast<f32x4*>(lds.qs[w][lane]) = join(q[1], q[0]);
+      if (w == 0 && g == 0) *reinterpret_cast<f32x2*>(lds.inv[c]) = (f32x2){rinv, sinv};
       f32x4 rw[ST], ws[ST][2];
 #pragma unroll
       for (int t = 0; t < ST; t++) {
@@ -1043,10 +1044,10 @@ __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_k
   int none = kChunk, gone = 0;  // gone: rows that went token by token, whose y is there
   auto finish = [&](int t0, int nrows) {
     const f32x4 qs = *reinterpret_cast<const f32x4*>(lds.qs[w][lane]);
-    const float rinv = lds.rinv[c];
-    f32x4 y;
+    const f32x2 inv = *reinterpret_cast<const f32x2*>(lds.inv[c]);
+    f32x4 y;  // (powers of two last: what a row of q or P has makes the other factor no larger than a result)
 #pragma unroll
-    for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(yt[r], rinv * yp[r], yq[r] * qs[r]);
+    for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(yt[r] * inv[0], yp[r], yq[r] * qs[r] * inv[1]);
     if (__ballot(none < kChunk)) {
 #pragma unroll
       for (int r = 0; r < 4; r++)
