@@ -245,7 +245,7 @@ struct PrepLds {
 };
 
 // blockIdx.x: a chunk, blockIdx.y: a head.  Wave w has the rows 16 w to 16 w + 15 of K, Q, L and P, those columns of T, and a quarter of W; wave 0 the gates.
-// 4096 rows of 32 heads 128 x 128 of binary16: 45 us, four workgroups a compute unit (LDS), bound by instructions: 1470 of vectors a wave, 60 % of the cycles.
+// 4096 rows of 32 heads 128 x 128 of binary16: 44 us, four workgroups a compute unit (LDS), bound by instructions: 1470 of vectors a wave, 60 % of the cycles.
 template <class T, int KS>
 __global__ __launch_bounds__(256, KS * kParts<T> <= 4 ? 4 : KS * kParts<T> <= 8 ? 2 : 1) void delta_prep_kernel(DeltaArgs<T> a, DeltaTable tab, char* keys, char* heads) {
   constexpr int NK = kParts<T>, ST = KS / 2;
@@ -613,7 +613,7 @@ __device__ __forceinline__ float of_lane(float f) { return __uint_as_float(__bui
 // forgotten in the chunk before.  Only chunks with a row of R that is that low look for them, hardly any of a layer's ordinary values (without the 2^11 it would
 // be one in some hundred); a look takes 1 us, a row 0.8 to 2.6 (64 to 256 keys).
 //
-// 4096 rows of 32 heads 128 x 128 of binary16: 107 us, 1.7 a chunk, 129 to 137 where operands and rows come from memory.  Vector instructions take 37 % of the
+// 4096 rows of 32 heads 128 x 128 of binary16: 109 us, 1.7 a chunk, 130 to 139 where operands and rows come from memory.  Vector instructions take 36 % of the
 // cycles, matrix ones 15 %; the rest is the latency of the dependent steps, and of 76 KB of operands a chunk.
 template <class T, int KS>
 __global__ __launch_bounds__(512, KS * kParts<T> <= 2 ? 4 : 2) void delta_scan_kernel(DeltaArgs<T> a, DeltaTable tab, const char* keys, const char* heads) {

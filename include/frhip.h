@@ -425,7 +425,7 @@ int frhip_ssm_cut(const frhip_ssm *p, int nseq, const int32_t *seq_start, int co
  *   y[t][h] = scale S^T q
  * A [heads], NULL: 1; dt_bias [heads], NULL: zero.  A dt' is the logarithm of a decay: not positive (where some are, their sums over up to
  * 64 rows may reach 80, and what grows with them stays in fp32; minus infinity forgets).  The largest element of a q or k lies between 1e-15 and 1e15, or it is zero (their
- * squares are fp32); norm_eps zero makes 0 / 0 of a vector of zeros.  A result is as exact as an fp32 sum of its own terms, products of q, k and columns
+ * squares, and their products with S ahead of the division, are fp32); norm_eps zero makes 0 / 0 of a vector of zeros.  A result is as exact as an fp32 sum of its own terms, products of q, k and columns
  * of S relative to the lengths of these, whatever values, states and decays the rows around it have (of keys as they are, norm_eps negative: if their
  * lengths are within 2^24 of each other in any 64 rows).  What is not finite stays in its column of S (a value, a state), its head (a key, b, a logarithm of a
  * decay that is plus infinity or no number) or its row of y (a query), from its token on, where results are not finite either.  q and k are rows of
